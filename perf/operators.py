@@ -2,8 +2,9 @@
 ``vllm_cpp_b200.ops.fp4_cache``.
 
 ``append``: merged ``[q | k | v]`` rows of a step are normed per head (optionally) and rotated; q goes on, k and v go into the
-cache in groups of 16 dimensions, each with an e4m3 scale (largest magnitude / 6) and e2m1 codes of value / scale. What comes
-back: q, and the keys and values that the cache now holds for these tokens.
+cache in groups of 16 dimensions, each with a scale (largest magnitude / 6) of 5 exponent and 3 mantissa bits, which are an f16's
+behind its sign, and e2m1 codes of value / scale. What comes back: q, and the keys and values that the cache now holds for these
+tokens.
 ``decode``: attention of one new token a sequence over its cached keys and values.
 ``prefill``: attention of several new tokens a sequence (prompts, portions of prompts, drafts to verify), causal from the end.
 
@@ -19,7 +20,8 @@ import torch
 own = False
 
 LEVELS = (0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0)
-FAR = -1
+MOST = 10240.0                 # largest scale: 6 times it is still an f16
+NONE = -1                      # slot of a padding row
 
 
 def _spread(n, low, high):
@@ -118,7 +120,7 @@ def _random_cache(pages, hkv, page, d, gen):
         code = mag | ((x < 0).to(torch.uint8) << 3)
         part[:, : 16 * d] = code[..., 0] | (code[..., 1] << 4)
         s = torch.randn((part.shape[0], 2 * d), generator=gen, device="cuda").mul_(0.5).exp_().mul_(0.2)
-        part[:, 16 * d:] = s.to(torch.float8_e4m3fn).view(torch.uint8)
+        part[:, 16 * d:] = _scale_bytes(s)
     return cache.view(pages, hkv, cells, 18 * d)
 
 
@@ -141,7 +143,7 @@ def prepare(case, seed):
         pages = -(-n // page) + 3
         s["cache"] = torch.zeros((pages, hkv, page // 16, 18 * d), dtype=torch.uint8, device="cuda")
         s["slots"] = torch.cat([torch.randperm(pages * page, generator=gen, device="cuda")[:n],
-                                torch.full((c["pad"],), FAR, device="cuda", dtype=torch.int64)])
+                                torch.full((c["pad"],), NONE, device="cuda", dtype=torch.int64)])
         w = (1 + 0.2 * torch.randn((2, d), generator=gen, device="cuda")).to(torch.bfloat16)
         s["q_norm"], s["k_norm"] = (w[0], w[1]) if c["norm"] else (None, None)
         s["q_out"] = torch.empty((t, hq * d), dtype=torch.bfloat16, device="cuda")
@@ -165,23 +167,34 @@ def prepare(case, seed):
 
 
 # ------------------------------------------------------------------------------------------------ the plain forms
+def _scale_bytes(s):
+    """Scales of few bits -> the bits of an f16 behind its sign, its last seven left off."""
+    return (s.half().view(torch.int16) >> 7).to(torch.uint8)
+
+
+def _scale_values(b):
+    return (b.to(torch.int16) << 7).view(torch.float16).float()
+
+
 def _codes_and_scales(x):
-    """fp32 [..., D] -> codes [..., D] (0..15), scales [..., D / 16] as e4m3."""
+    """fp32 [..., D] -> codes [..., D] (0..15), scales [..., D / 16]."""
     g = x.unflatten(-1, (-1, 16))
     six = torch.full((), 6.0, dtype=torch.float64, device=x.device)
-    scale = (g.abs().amax(-1).double() / six).float().clamp(max=448.0).to(torch.float8_e4m3fn)
-    r = g.abs().double() / scale.double()[..., None]
-    r = torch.where(scale.double()[..., None] > 0, r, torch.zeros_like(r))
+    s = g.abs().amax(-1).double() / six
+    step = torch.ldexp(torch.ones_like(s), (torch.frexp(s)[1] - 1).clamp(min=-14) - 3)
+    scale = (torch.round(s / step) * step).clamp(max=MOST)
+    r = g.abs().double() / scale[..., None]
+    r = torch.where(scale[..., None] > 0, r, torch.zeros_like(r))
     # the nearest of the levels, of two that are equally near the one with an even code
     code = ((r > 0.25).int() + (r >= 0.75).int() + (r > 1.25).int() + (r >= 1.75).int() + (r > 2.5).int() + (r >= 3.5).int()
             + (r > 5.0).int())
     code = code + 8 * torch.signbit(g).int()
-    return code.flatten(-2), scale
+    return code.flatten(-2), scale.float()
 
 
 def _values(codes, scales, levels):
-    """codes [..., D], e4m3 scales [..., D / 16] -> fp32 [..., D]."""
-    return (levels[codes.int()].unflatten(-1, (-1, 16)) * scales.float()[..., None]).flatten(-2)
+    """codes [..., D], scales [..., D / 16] -> fp32 [..., D]."""
+    return (levels[codes.int()].unflatten(-1, (-1, 16)) * scales[..., None]).flatten(-2)
 
 
 def _levels(dtype=torch.float32):
@@ -209,8 +222,8 @@ def _cells(cells, d):
     k = _unpack(cells[..., : 8 * d].unflatten(-1, (16, d // 2)))
     v = cells[..., 8 * d: 16 * d].unflatten(-1, (d // 2, 16))[..., _value_order(d), :]
     v = _unpack(v.flatten(-2).unflatten(-1, (16, d // 2)))
-    ks = cells[..., 16 * d: 17 * d].unflatten(-1, (16, d // 16)).view(torch.float8_e4m3fn)
-    vs = cells[..., 17 * d:].unflatten(-1, (d // 16, 16)).transpose(-1, -2).contiguous().view(torch.float8_e4m3fn)
+    ks = _scale_values(cells[..., 16 * d: 17 * d].unflatten(-1, (16, d // 16)))
+    vs = _scale_values(cells[..., 17 * d:].unflatten(-1, (d // 16, 16)).transpose(-1, -2))
     return _values(k, ks, levels), _values(v, vs, levels)
 
 
@@ -247,9 +260,9 @@ def _append_plain(s):
     cache[at[0][..., None], at[1][..., None], at[2][..., None], 8 * d + swapped[:, None]] = _pack(vc[used])
     group = torch.arange(d // 16, device="cuda")[None]
     cache[at[0][..., None], at[1][..., None], at[2][..., None], (16 * d + tok[:, None] * (d // 16) + group)[:, None]] = \
-        ks[used].view(torch.uint8)
+        _scale_bytes(ks[used])
     cache[at[0][..., None], at[1][..., None], at[2][..., None], (17 * d + group * 16 + tok[:, None])[:, None]] = \
-        vs[used].view(torch.uint8)
+        _scale_bytes(vs[used])
     levels = _levels()
     there = (slots >= 0)[:, None, None]
     k, v = _values(kc, ks, levels) * there, _values(vc, vs, levels) * there
@@ -343,7 +356,8 @@ def work(case):
 
 
 # ------------------------------------------------------------------------------------------ the definition, in 64 bits
-_E4M3 = [(m / 8 * 2.0 ** -6) if e == 0 else (1 + m / 8) * 2.0 ** (e - 7) for e in range(16) for m in range(8)][:127]
+_SCALES = [(m / 8 * 2.0 ** -14) if e == 0 else (1 + m / 8) * 2.0 ** (e - 15) for e in range(31) for m in range(8)]
+_USED = [v for v in _SCALES if v <= MOST]
 
 
 def _nearest(x, values):
@@ -357,7 +371,8 @@ def _nearest(x, values):
 
 def _quantised(x):
     g = x.reshape(*x.shape[:-1], -1, 16)
-    s = torch.tensor(_E4M3, dtype=torch.float64, device=x.device)[_nearest(g.abs().amax(-1) / torch.tensor(6.0, dtype=torch.float64, device=x.device), _E4M3)]
+    top = g.abs().amax(-1) / torch.tensor(6.0, dtype=torch.float64, device=x.device)
+    s = torch.tensor(_USED, dtype=torch.float64, device=x.device)[_nearest(top, _USED)]
     s = s[..., None]
     r = torch.where(s > 0, g.abs() / torch.where(s > 0, s, torch.ones_like(s)), torch.zeros_like(g))
     held = torch.tensor(LEVELS, dtype=torch.float64, device=x.device)[_nearest(r, list(LEVELS))] * s
@@ -392,8 +407,7 @@ def _held(cell, d):
         both[..., 0::2], both[..., 1::2] = level[(codes % 16).long()], level[(codes // 16).long()]
         return (both * scale.repeat_interleave(16, -1)).reshape(n * 16, d)
 
-    e4m3 = torch.tensor(_E4M3 + [math.nan], dtype=torch.float64, device=cell.device)
-    scales = e4m3[cell[:, 16 * d:].long()]
+    scales = torch.tensor(_SCALES, dtype=torch.float64, device=cell.device)[cell[:, 16 * d:].long()]
     keys = values(cell[:, : 8 * d].reshape(n, 16, d // 2), scales[:, :d].reshape(n, 16, d // 16))
     rows = torch.empty((n, 16, d // 2), dtype=torch.uint8, device=cell.device)
     for token in range(16):
