@@ -218,6 +218,46 @@ typedef struct B200BiasAttn {
   float out_scale;             // the outputs are multiplied by this
 } B200BiasAttn;
 
+// Keys and values of a step into a paged cache held in 4 bits (fp4_cache.cu): per-head RMSNorm of q and k (weights or null), rotation (cos_sin null:
+// none), q to q_out (null: in place), k and v to the cache. Rows of heads: k and v heads D apart, q heads q_head_stride apart. A slot outside the
+// cache writes nothing, a position outside the table gives NaN. Rows, weights and cache lie on 16-byte boundaries.
+typedef struct B200Fp4Append {
+  void* q;                     // bf16 [T][Hq heads]
+  const void* k;
+  const void* v;
+  void* q_out;                 // [T][Hq D]
+  long long ldq, ldk, ldv, ldo;
+  const void* positions;       // int64 [T]
+  const void* cos_sin;         // fp32 [table_rows][cos rot / 2 | sin rot / 2]
+  const void* q_norm;
+  const void* k_norm;
+  const void* slots;           // int64 [T]
+  void* cache;                 // [num_blocks][Hkv][block_size / 16][18 D]
+  long long num_blocks, table_rows;
+  int T, Hq, Hkv, D, rot, q_head_stride, block_size, neox, gemma;
+  float eps;
+} B200Fp4Append;
+
+// Attention over that cache (fp4_attn.cu). q_start null: one query a sequence (decode), else [num_reqs + 1] and causal from the end of each sequence
+// (causal 0: every query sees every key). window as in b200_attn_decode. parts: b200_fp4_attn_scratch floats, for this call alone until it is done.
+typedef struct B200Fp4Attn {
+  const void* q;
+  void* out;
+  long long ldq, ldo, ldt;
+  const void* cache;
+  long long num_blocks;
+  const void* block_table;     // int32 [num_reqs][max_blocks], rows ldt apart
+  const void* seq_lens;        // int32 [num_reqs]
+  const void* q_start;
+  const void* tile_req;        // 128-token query tiles (q_start given)
+  const void* tile_q0;
+  void* parts;
+  int max_blocks, num_reqs, total_q, num_tiles;
+  int Hq, Hkv, D, block_size;
+  int window, causal;
+  float scale, softcap;
+} B200Fp4Attn;
+
 // Latent attention (latent.cu): norms of the query and key latents, rotation of the shared key part, cache rows
 // [latent (rankp) | rotated part]. down rows: query latent | key latent at kv_col | rotated part at rot_col.
 typedef struct B200LatentPrep {
@@ -476,6 +516,12 @@ int b200_outer_norm(const B200Outer* a, int reqs, int chunks, cudaStream_t strea
 int b200_outer_fits(const B200Outer* a);
 void b200_outer_workspace(int kind, int D, int* values);
 int b200_outer_chunk(const B200Outer* a, cudaStream_t stream);
+// ---- fp4_attn.cu
+long long b200_fp4_attn_scratch(int Hq, int Hkv, int D);
+int b200_fp4_attn(const B200Fp4Attn* a, cudaStream_t stream);
+// ---- fp4_cache.cu
+int b200_fp4_append(const B200Fp4Append* a, cudaStream_t stream);
+int b200_fp4_read(const void* cache, long long num_blocks, int block_size, int Hkv, int D, const void* slots, void* k, long long ldk, void* v, long long ldv, long long n, cudaStream_t stream);
 // ---- gdn.cu
 int b200_gdn_conv1d_fwd(const void* x, long ldx, const void* w, void* conv_state, const int* qsl, const int* slots, const int* has_init, void* out, long ldo, int n_seq, int total_tokens, int C, cudaStream_t stream);
 int b200_gdn_conv1d_update(const void* x, long ldx, const void* w, void* conv_state, const int* slots, void* out, long ldo, int B, int C, cudaStream_t stream);

@@ -1,0 +1,612 @@
+// Attention over the paged cache held in 4 bits (layout: fp4_cache.cuh), for few query rows a sequence: decode, and the verification of drafts.
+//
+//   o[r] = sum_j p[r, j] v_j / sum_j p[r, j],   p[r, j] = 2^(scale log2(e) q_r . k_j - m),   m a running reference of the maximum
+//
+// The rows of a sequence that share a kv head (query tokens x heads of the group) are cut into tiles of 8 or 16. A warp takes cells of 16 keys:
+//   S^T [16 keys x rows] = K Q^T     A = keys, straight from the cell: codes to f16 (cvt.rn.f16x2.e2m1x2), times their scale, exact
+//   O^T [dims x rows]   += V^T P^T   A = values of four keys a lane; codes of two keys are merged before the conversion, so that a pair of
+//                                    f16 holds two keys of one dim and one multiplication applies both scales; B = P^T, transposed in
+//                                    registers (movmatrix)
+// Q is f16 times a power of two per row (its largest magnitude between 1 and 2), which goes back into the softmax scale.
+//
+// Work is shared out evenly whatever the lengths: the cells of all (sequence, kv head, row tile) items stand in one line, each CTA takes an equal
+// stretch of it, and its warps the cells of a stretch in turn, fetched ahead by bulk copies into a ring of their own. An item that lies in one
+// stretch is finished there; of one that was cut the parts (m, l, O) go to scratch, and a second kernel joins them.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "api.h"
+#include "fp4_cache.cuh"
+#include "sm100.cuh"
+
+namespace b200 {
+
+struct Fp4Rows {
+  const __nv_bfloat16* q;
+  long long ldq;
+  __nv_bfloat16* out;
+  long long ldo;
+  const uint8_t* cache;
+  long long num_blocks;
+  const int32_t* block_table;
+  int max_blocks;              // of a sequence
+  long long ldt;               // entries from one sequence's row of the table to the next
+  const int32_t* seq_lens;
+  const int32_t* q_start;      // null: one row a sequence
+  int num_reqs, total_q;
+  int Hkv, G, cells_per_page, window, causal, rows;   // rows: of a tile
+  float scale_log2, softcap2;
+  float* parts;                // [CTAs][2][rows * (D + 2)]
+  int* status;
+};
+
+static constexpr int kRowWarps = 8, kRowStages = 4;
+// p is at most 2^8 before its reference is raised; times 2^7 it is still an f16, and the smallest ones keep their bits.
+static constexpr float kUp = 7.f;
+
+__device__ __forceinline__ float ex2_of(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t transposed(uint32_t a) {
+  uint32_t d;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
+  return d;
+}
+__device__ __forceinline__ uint32_t mul_f16x2(uint32_t a, uint32_t b) {
+  uint32_t d;
+  asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+  return d;
+}
+// Scale bytes lo and hi (selectors of __byte_perm) of w -> f16x2.
+__device__ __forceinline__ uint32_t scales_f16x2(uint32_t w, int lo, int hi) { return __byte_perm(w, 0, 0x4040 | lo | hi << 8) << 7; }
+__device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
+  const __half2 h = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ uint32_t low_nibbles_else(uint32_t a, uint32_t b) {     // nibble 0, 2, .. of a, the others of b
+  return (a & 0x0f0f0f0fu) | (b & 0xf0f0f0f0u);
+}
+__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_u32(dst)), "l"(src),
+               "r"(bytes), "r"(smem_u32(bar))
+               : "memory");
+}
+
+// What a sequence brings: keys [first key cell, first + cells) x items (kv heads x row tiles); positions of its rows are first_pos + token.
+struct Fp4Seq {
+  int len, q_begin, q_len, first_cell, cells, tiles;
+  __device__ __forceinline__ Fp4Seq(const Fp4Rows& p, int b) {
+    q_begin = p.q_start ? min(max(p.q_start[b], 0), p.total_q) : b;
+    q_len = p.q_start ? max(min(p.q_start[b + 1], p.total_q) - q_begin, 0) : 1;
+    len = min(max(p.seq_lens[b], 0), p.max_blocks * p.cells_per_page * kCellTokens);
+    first_cell = max(0, lowest(p, len - q_len)) / kCellTokens;
+    cells = max(1, (len + kCellTokens - 1) / kCellTokens - first_cell);          // (no keys: one cell that counts as masked)
+    tiles = (q_len * p.G + p.rows - 1) / p.rows;
+  }
+  // lowest position that the query at `pos` sees
+  static __device__ __forceinline__ int lowest(const Fp4Rows& p, int pos) {
+    return p.window > 0 ? pos - p.window + 1 : p.window < 0 && pos >= 0 ? pos / -p.window * -p.window : 0;
+  }
+};
+
+// line[b] = cells in the line in front of sequence b (num_reqs + 1 entries). All threads of the block take part.
+__device__ void fp4_line(const Fp4Rows& p, uint32_t* line) {
+  __shared__ uint32_t warp_sum[32];
+  const int per = (p.num_reqs + blockDim.x - 1) / blockDim.x, b0 = min((int)threadIdx.x * per, p.num_reqs), b1 = min(b0 + per, p.num_reqs);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
+  uint32_t sum = 0;
+  for (int b = b0; b < b1; ++b) {
+    const Fp4Seq s(p, b);
+    const uint32_t n = (uint32_t)s.cells * (uint32_t)(s.tiles * p.Hkv);
+    line[b + 1] = n;
+    sum += n;
+  }
+  uint32_t x = sum;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const uint32_t y = __shfl_up_sync(0xffffffffu, x, o);
+    if (lane >= o) x += y;
+  }
+  if (lane == 31) warp_sum[warp] = x;
+  __syncthreads();
+  uint32_t before = x - sum;
+  for (int w = 0; w < warps; ++w) before += w < warp ? warp_sum[w] : 0;
+  for (int b = b0; b < b1; ++b) {
+    before += line[b + 1];
+    line[b + 1] = before;
+  }
+  if (threadIdx.x == 0) line[0] = 0;
+  __syncthreads();
+}
+__device__ __forceinline__ int fp4_find(const uint32_t* line, int n, uint32_t u) {   // the sequence that cell u is of
+  int lo = 0, hi = n - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi) >> 1;
+    if (line[mid + 1] > u) hi = mid;
+    else lo = mid + 1;
+  }
+  return lo;
+}
+// Stretches: CTA i of n has cells [total i / n, total (i + 1) / n). No more CTAs than give each warp a cell.
+__device__ __forceinline__ uint32_t fp4_ctas(uint32_t total, uint32_t grid) { return max(1u, min(grid, total / kRowWarps)); }
+__device__ __forceinline__ uint32_t fp4_begin(uint32_t total, uint32_t i, uint32_t n) { return (uint32_t)((uint64_t)total * i / n); }
+
+// A piece of an item: cells [c0, c1) of the item's n.
+struct Fp4Piece {
+  uint32_t u, u_end;           // in the line: where the piece begins, where the CTA's stretch ends
+  int b, item, c0, c1;
+  __device__ __forceinline__ void at(const Fp4Rows& p, const uint32_t* line, uint32_t from, uint32_t to) {
+    u = from;
+    u_end = to;
+    if (u >= u_end) return;
+    b = fp4_find(line, p.num_reqs, u);
+    const int n = Fp4Seq(p, b).cells;
+    const uint32_t local = u - line[b];
+    item = (int)(local / (uint32_t)n);
+    c0 = (int)(local - (uint32_t)item * n);
+    c1 = (int)min((uint32_t)n, c0 + (u_end - u));
+  }
+  __device__ __forceinline__ void next(const Fp4Rows& p, const uint32_t* line) {
+    u += c1 - c0;
+    if (u >= u_end) return;
+    ++item;
+    if (u == line[b + 1]) {
+      item = 0;
+      do ++b;
+      while (line[b + 1] == u);
+    }
+    c0 = 0;
+    c1 = (int)min((uint32_t)Fp4Seq(p, b).cells, u_end - u);
+  }
+  __device__ __forceinline__ bool more() const { return u < u_end; }
+};
+
+template <int D, int NT>
+struct Fp4RowsShape {
+  static constexpr int kRows = 8 * NT, kMT = D / 16;
+  static constexpr int kMergeTiles = kMT * NT <= 8 ? kMT : 8 / NT;                   // m-tiles of the merge buffer (32 KB)
+  static constexpr int kMergeRow = kMergeTiles * 16 + 8;                             // floats of a row in it
+  static constexpr int kRingBytes = kRowWarps * kRowStages * Fp4Cell<D>::kBytes;
+  static constexpr int kMergeBytes = kRowWarps * kRows * kMergeRow * 4;
+  static constexpr int kFixed = kRingBytes + kMergeBytes + kRowWarps * kRows * 8 + kRowWarps * kRowStages * 8;
+  static constexpr int kPart = kRows * (D + 2);                                      // floats of a part in scratch
+};
+
+template <int D, int NT>
+__global__ void __launch_bounds__(kRowWarps * 32, NT == 1 && D <= 128 ? 2 : 1) fp4_rows_kernel(Fp4Rows p) {
+  using Cell = Fp4Cell<D>;
+  using Shape = Fp4RowsShape<D, NT>;
+  constexpr int kRows = Shape::kRows, kMT = Shape::kMT, kKW = D / 32, kVW = D / 64;   // m-tiles, words of a lane's keys and values
+  extern __shared__ __align__(128) uint8_t smem[];
+  float* merge = reinterpret_cast<float*>(smem + Shape::kRingBytes);
+  float* top = reinterpret_cast<float*>(smem + Shape::kRingBytes + Shape::kMergeBytes);      // [warps][rows] m, then l
+  float* sums = top + kRowWarps * kRows;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(sums + kRowWarps * kRows);
+  uint32_t* line = reinterpret_cast<uint32_t*>(bars + kRowWarps * kRowStages);
+  const int warp = warp_index(), lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  uint8_t* ring = smem + warp * kRowStages * Cell::kBytes;
+  uint64_t* full = bars + warp * kRowStages;
+  if (lane < kRowStages) mbar_init(&full[lane], 1);
+  mbar_fence_init();
+  pdl_wait();
+  pdl_launch_dependents();
+  fp4_line(p, line);
+  const uint32_t total = line[p.num_reqs], ctas = fp4_ctas(total, gridDim.x);
+  if (blockIdx.x >= ctas) return;
+  const uint32_t from = fp4_begin(total, blockIdx.x, ctas), to = fp4_begin(total, blockIdx.x + 1, ctas);
+
+  // ---- fetching ahead: the warp's cells in their order, kRowStages of them in flight
+  Fp4Piece f;
+  f.at(p, line, from, to);
+  int fc = f.c0 + warp, fj = 32, page = 0;      // next cell; page ids of the next 32 cells, a lane each
+  uint32_t bad = 0, phase = 0, flying = 0;      // of each stage: nothing was fetched (no such page); parity of its barrier; not waited for yet
+  const auto fetch = [&](int st) {
+    while (f.more() && fc >= f.c1) {
+      f.next(p, line);
+      fc = f.c0 + warp;
+      fj = 32;
+    }
+    if (!f.more()) return;
+    const Fp4Seq s(p, f.b);
+    if (fj == 32) {
+      const int c = fc + lane * kRowWarps, pg = (s.first_cell + c) / p.cells_per_page;
+      page = c < f.c1 && pg < p.max_blocks && s.len > 0 ? p.block_table[f.b * p.ldt + pg] : -1;
+      fj = 0;
+    }
+    const int id = __shfl_sync(0xffffffffu, page, fj);
+    const bool there = id >= 0 && id < p.num_blocks;
+    bad = there ? bad & ~(1u << st) : bad | 1u << st;
+    flying |= there ? 1u << st : 0;
+    if (there && lane == 0) {
+      const int h = f.item / s.tiles, cell = (s.first_cell + fc) % p.cells_per_page;
+      mbar_expect_tx(&full[st], Cell::kBytes);
+      bulk_load(ring + st * Cell::kBytes, p.cache + (((long long)id * p.Hkv + h) * p.cells_per_page + cell) * Cell::kBytes, Cell::kBytes, &full[st]);
+    }
+    __syncwarp();
+    fc += kRowWarps;
+    ++fj;
+  };
+#pragma unroll
+  for (int st = 0; st < kRowStages; ++st) fetch(st);
+  int st = 0;
+  bool ok = true;
+
+  Fp4Piece w;
+  for (w.at(p, line, from, to); w.more(); w.next(p, line)) {
+    const Fp4Seq s(p, w.b);
+    const int h = w.item / s.tiles, r0 = (w.item - h * s.tiles) * kRows, nrows = min(kRows, s.q_len * p.G - r0);
+    const int first = s.len - s.q_len;                                           // position of the sequence's first query
+    // ---- the tile's queries: B operand, lane (g, t) has dims [t D / 4, + D / 4) of row g
+    uint32_t bq[NT][D / 16][2];
+    float mul[NT][2];                                                            // of the lane's rows 2t, 2t + 1: scores to log2 units
+    int hi[NT][2], lo[NT][2];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      const int r = r0 + nt * 8 + g, token = r / p.G, head = r - token * p.G;
+      const bool row = nt * 8 + g < nrows;
+      const __nv_bfloat16* src = p.q + (long long)(s.q_begin + token) * p.ldq + (long long)(h * p.G + head) * D + t * (D / 4);
+      float big = 0.f;
+      uint4 raw[D / 32];
+#pragma unroll
+      for (int i = 0; i < D / 32; ++i) {
+        raw[i] = row ? *reinterpret_cast<const uint4*>(src + i * 8) : make_uint4(0, 0, 0, 0);
+        const uint32_t v[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float2 x = unpack_bf16x2(v[e]);
+          big = fmaxf(big, fmaxf(fabsf(x.x), fabsf(x.y)));
+        }
+      }
+      big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 1));
+      big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 2));
+      const int e2 = min(max((int)(__float_as_uint(big) >> 23) - 127, -100), 100);
+      const float down = __uint_as_float((uint32_t)(127 - e2) << 23), up = __uint_as_float((uint32_t)(127 + e2) << 23);
+#pragma unroll
+      for (int i = 0; i < D / 32; ++i) {
+        const uint32_t v[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float2 x = unpack_bf16x2(v[e]);
+          bq[nt][2 * i + (e >> 1)][e & 1] = pack_f16x2(x.x * down, x.y * down);
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        mul[nt][e] = __shfl_sync(0xffffffffu, up, (2 * t + e) * 4) * p.scale_log2;
+        const int rr = min(nt * 8 + 2 * t + e, nrows - 1) + r0, pos = first + rr / p.G;
+        hi[nt][e] = p.causal ? pos : s.len - 1;
+        lo[nt][e] = Fp4Seq::lowest(p, pos);
+      }
+    }
+    const int tok0 = r0 / p.G, tok1 = (r0 + nrows - 1) / p.G;                    // the tile's tokens
+    const int least_hi = p.causal ? first + tok0 : s.len - 1, most_hi = p.causal ? first + tok1 : s.len - 1;
+    const int most_lo = Fp4Seq::lowest(p, first + tok1), least_lo = Fp4Seq::lowest(p, first + tok0);
+
+    float o[NT][kMT][4], m[NT][2], l[NT][2];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+      for (int i = 0; i < kMT; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[nt][i][e] = 0.f;
+      m[nt][0] = m[nt][1] = -INFINITY;
+      l[nt][0] = l[nt][1] = 0.f;
+    }
+    for (int c = w.c0 + warp; c < w.c1; c += kRowWarps) {
+      const int key0 = (s.first_cell + c) * kCellTokens;
+      const bool there = !(bad >> st & 1);
+      if (there) {
+        if (ok) ok = __all_sync(0xffffffffu, mbar_wait(&full[st], phase >> st & 1, p.status));
+        if (ok) flying &= ~(1u << st);
+        phase ^= 1u << st;
+      }
+      if (there && ok && key0 <= most_hi && key0 + kCellTokens > least_lo) {
+        const uint8_t* cell = ring + st * Cell::kBytes;
+        // S^T: rows g and g + 8 of the tile are keys 4 (g / 2) + g % 2 and two on
+        const int k0 = 4 * (g >> 1) + (g & 1);
+        uint32_t kw[2][kKW], ks[2][kKW / 2];
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          const uint8_t* row = cell + (k0 + 2 * r) * Cell::kRow + t * (D / 8);
+          const uint8_t* sc = cell + Cell::kKeyScales + (k0 + 2 * r) * Cell::kScales + t * (D / 64);
+          if constexpr (D == 64) {
+            const uint2 x = *reinterpret_cast<const uint2*>(row);
+            kw[r][0] = x.x; kw[r][1] = x.y;
+            ks[r][0] = scales_f16x2(*sc, 0, 0);
+          } else {
+#pragma unroll
+            for (int i = 0; i < kKW / 4; ++i) {
+              const uint4 x = *reinterpret_cast<const uint4*>(row + i * 16);
+              kw[r][4 * i] = x.x; kw[r][4 * i + 1] = x.y; kw[r][4 * i + 2] = x.z; kw[r][4 * i + 3] = x.w;
+              const uint32_t two = *reinterpret_cast<const uint16_t*>(sc + i * 2);
+              ks[r][2 * i] = scales_f16x2(two, 0, 0);
+              ks[r][2 * i + 1] = scales_f16x2(two, 1, 1);
+            }
+          }
+        }
+        float sc[NT][4];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) sc[nt][0] = sc[nt][1] = sc[nt][2] = sc[nt][3] = 0.f;
+#pragma unroll
+        for (int i = 0; i < kKW; ++i) {
+          uint32_t x[4], y[4];
+          cvt_e2m1x8(kw[0][i], x);
+          cvt_e2m1x8(kw[1][i], y);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            x[e] = mul_f16x2(x[e], ks[0][i >> 1]);
+            y[e] = mul_f16x2(y[e], ks[1][i >> 1]);
+          }
+          const uint32_t a0[4] = {x[0], y[0], x[1], y[1]}, a1[4] = {x[2], y[2], x[3], y[3]};
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            mma_f16(sc[nt], a0, bq[nt][2 * i][0], bq[nt][2 * i][1]);
+            mma_f16(sc[nt], a1, bq[nt][2 * i + 1][0], bq[nt][2 * i + 1][1]);
+          }
+        }
+        const bool edge = key0 + kCellTokens - 1 > least_hi || key0 < most_lo;
+        uint32_t bp[NT][2];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          float over = -INFINITY;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            float x = sc[nt][e] * mul[nt][e & 1];
+            if (p.softcap2 > 0.f) x = p.softcap2 * tanhf(x / p.softcap2);
+            if (edge) {
+              const int key = key0 + k0 + (e & 2);
+              if (key > hi[nt][e & 1] || key < lo[nt][e & 1]) x = -INFINITY;
+            }
+            sc[nt][e] = x;
+            over = fmaxf(over, x - m[nt][e & 1]);
+          }
+          // the reference is raised when a score passes it by 8 (p stays below 2^8), and at the first visible key
+          if (__any_sync(0xffffffffu, over > 8.f)) {
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              float x = fmaxf(sc[nt][e], sc[nt][e + 2]);
+#pragma unroll
+              for (int d = 4; d < 32; d <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, d));
+              x = fmaxf(x, m[nt][e]);
+              const float alpha = m[nt][e] == -INFINITY ? 0.f : ex2_of(m[nt][e] - x);
+              m[nt][e] = x;
+              l[nt][e] *= alpha;
+#pragma unroll
+              for (int i = 0; i < kMT; ++i) {
+                o[nt][i][e] *= alpha;
+                o[nt][i][e + 2] *= alpha;
+              }
+            }
+          }
+          float pr[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            pr[e] = ex2_of(sc[nt][e] - (m[nt][e & 1] == -INFINITY ? 0.f : m[nt][e & 1] - kUp));
+            l[nt][e & 1] += pr[e];
+          }
+          bp[nt][0] = transposed(pack_f16x2(pr[0], pr[1]));
+          bp[nt][1] = transposed(pack_f16x2(pr[2], pr[3]));
+        }
+        // O^T: lane (g, t) has keys 4t..4t+3 and dims [g D / 8, + D / 8); the m-tile i is its dims 2i (row g) and 2i + 1 (row g + 8)
+        uint32_t vw[4][kVW];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const uint8_t* at = cell + Cell::kValues + (((4 * t + j) * Cell::kRow + g * (D / 16)) ^ (32 * t));
+          if constexpr (D == 64) {
+            vw[j][0] = *reinterpret_cast<const uint32_t*>(at);
+          } else if constexpr (D == 128) {
+            const uint2 x = *reinterpret_cast<const uint2*>(at);
+            vw[j][0] = x.x; vw[j][1] = x.y;
+          } else {
+            const uint4 x = *reinterpret_cast<const uint4*>(at);
+            vw[j][0] = x.x; vw[j][1] = x.y; vw[j][2] = x.z; vw[j][3] = x.w;
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < kVW; ++i) {
+          const int group = (g * (D / 8) + 8 * i) / 16;
+          uint32_t scales = *reinterpret_cast<const uint32_t*>(cell + Cell::kValueScales + group * kCellTokens + 4 * t);
+          if (edge) {              // what lies behind the sequence or before every window may be anything: NaN times 0 too
+            const int key = key0 + 4 * t;
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              if (key + j >= s.len || key + j < least_lo) scales &= ~(0xffu << (8 * j));
+          }
+          const uint32_t s01 = scales_f16x2(scales, 0, 1), s23 = scales_f16x2(scales, 2, 3);
+          uint32_t e01[4], d01[4], e23[4], d23[4];             // even dims, odd dims of key pairs
+          cvt_e2m1x8(low_nibbles_else(vw[0][i], vw[1][i] << 4), e01);
+          cvt_e2m1x8(low_nibbles_else(vw[0][i] >> 4, vw[1][i]), d01);
+          cvt_e2m1x8(low_nibbles_else(vw[2][i], vw[3][i] << 4), e23);
+          cvt_e2m1x8(low_nibbles_else(vw[2][i] >> 4, vw[3][i]), d23);
+#pragma unroll
+          for (int y = 0; y < 4; ++y) {
+            const uint32_t a[4] = {mul_f16x2(e01[y], s01), mul_f16x2(d01[y], s01), mul_f16x2(e23[y], s23), mul_f16x2(d23[y], s23)};
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) mma_f16(o[nt][4 * i + y], a, bp[nt][0], bp[nt][1]);
+          }
+        }
+      }
+      __syncwarp();
+      if (ok) fetch(st);
+      if (++st == kRowStages) st = 0;
+    }
+    // ---- the warps' parts of the piece together
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        float x = l[nt][e];
+#pragma unroll
+        for (int d = 4; d < 32; d <<= 1) x += __shfl_xor_sync(0xffffffffu, x, d);
+        if (g == 0) {
+          top[warp * kRows + nt * 8 + 2 * t + e] = m[nt][e];
+          sums[warp * kRows + nt * 8 + 2 * t + e] = x;
+        }
+      }
+    __syncthreads();
+    float scale[NT][2];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        float x = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < kRowWarps; ++i) x = fmaxf(x, top[i * kRows + nt * 8 + 2 * t + e]);
+        scale[nt][e] = m[nt][e] == -INFINITY ? 0.f : ex2_of(m[nt][e] - x);
+      }
+    const bool whole = w.c0 == 0 && w.c1 == s.cells;
+    float* part = p.parts + ((size_t)blockIdx.x * 2 + (w.c0 == 0)) * Shape::kPart;
+    constexpr int kMC = Shape::kMergeTiles, kMR = Shape::kMergeRow;
+#pragma unroll
+    for (int i0 = 0; i0 < kMT; i0 += kMC) {
+      if (i0) __syncthreads();
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int i = 0; i < kMC; ++i)
+#pragma unroll
+          for (int e = 0; e < 2; ++e)
+            *reinterpret_cast<float2*>(merge + (warp * kRows + nt * 8 + 2 * t + e) * kMR + (i * 8 + g) * 2) =
+                make_float2(o[nt][i0 + i][e] * scale[nt][e], o[nt][i0 + i][e + 2] * scale[nt][e]);
+      __syncthreads();
+      for (int x = threadIdx.x; x < nrows * kMC * 8; x += kRowWarps * 32) {
+        const int i = x % kMC, gg = x / kMC % 8, r = x / (kMC * 8), d = gg * (D / 8) + 2 * (i0 + i);
+        float a = 0.f, b = 0.f, mx = -INFINITY, sum = 0.f;
+#pragma unroll
+        for (int y = 0; y < kRowWarps; ++y) {
+          const float2 v = *reinterpret_cast<const float2*>(merge + (y * kRows + r) * kMR + (i * 8 + gg) * 2);
+          a += v.x;
+          b += v.y;
+          mx = fmaxf(mx, top[y * kRows + r]);
+        }
+#pragma unroll
+        for (int y = 0; y < kRowWarps; ++y)
+          sum += top[y * kRows + r] == -INFINITY ? 0.f : sums[y * kRows + r] * ex2_of(top[y * kRows + r] - mx);
+        if (whole) {
+          const int token = (r0 + r) / p.G, head = r0 + r - token * p.G;
+          const float inv = sum == 0.f ? 0.f : 1.f / sum;
+          *reinterpret_cast<uint32_t*>(p.out + (long long)(s.q_begin + token) * p.ldo + (long long)(h * p.G + head) * D + d) =
+              pack_bf16x2(a * inv, b * inv);
+        } else {
+          *reinterpret_cast<float2*>(part + r * D + d) = make_float2(a, b);
+          if (d == 0) {
+            part[kRows * D + 2 * r] = mx;
+            part[kRows * D + 2 * r + 1] = sum;
+          }
+        }
+      }
+    }
+    __syncthreads();             // (top, sums and the buffer are written again)
+  }
+  // a wait ran out: what is still on its way to the ring gets the same time again before the CTA gives its memory up
+  for (int i = 0; i < kRowStages && !ok; ++i)
+    if (flying >> i & 1) mbar_wait(&full[i], phase >> i & 1, p.status);
+}
+
+// Joins the parts of items that the ends of stretches cut. Block i looks at the line where stretch i + 1 begins; the first cut of an item is the
+// one that joins it: part 1 of the CTA that begins it, part 0 of those behind.
+template <int D, int NT>
+__global__ void __launch_bounds__(256) fp4_join_kernel(Fp4Rows p, int grid) {
+  using Shape = Fp4RowsShape<D, NT>;
+  constexpr int kRows = Shape::kRows;
+  extern __shared__ uint32_t line[];
+  pdl_wait();
+  pdl_launch_dependents();
+  fp4_line(p, line);
+  const uint32_t total = line[p.num_reqs], ctas = fp4_ctas(total, grid), i = blockIdx.x;
+  if (i + 1 >= ctas) return;
+  const uint32_t u = fp4_begin(total, i + 1, ctas);
+  const int b = fp4_find(line, p.num_reqs, u);
+  const Fp4Seq s(p, b);
+  const uint32_t local = u - line[b], item = local / (uint32_t)s.cells, begin = line[b] + item * s.cells;
+  if (begin == u || fp4_begin(total, i, ctas) > begin) return;
+  const uint32_t last = (uint32_t)(((uint64_t)(begin + s.cells) * ctas - 1) / total);         // the CTA that has the item's last cell
+  const int h = item / s.tiles, r0 = (int)(item - h * s.tiles) * kRows, nrows = min(kRows, s.q_len * p.G - r0);
+  for (int x = threadIdx.x; x < nrows * (D / 4); x += 256) {
+    const int r = x / (D / 4), d = x % (D / 4) * 4;
+    float mx = -INFINITY;
+    for (uint32_t c = i; c <= last; ++c) mx = fmaxf(mx, p.parts[((size_t)c * 2 + (c == i)) * Shape::kPart + kRows * D + 2 * r]);
+    float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+    float sum = 0.f;
+#pragma unroll 4
+    for (uint32_t c = i; c <= last; ++c) {
+      const float* part = p.parts + ((size_t)c * 2 + (c == i)) * Shape::kPart;
+      const float2 ml = *reinterpret_cast<const float2*>(part + kRows * D + 2 * r);
+      const float4 v = *reinterpret_cast<const float4*>(part + r * D + d);
+      const float f = ml.x == -INFINITY ? 0.f : ex2_of(ml.x - mx);
+      sum += ml.y * f;
+      a.x += v.x * f; a.y += v.y * f; a.z += v.z * f; a.w += v.w * f;
+    }
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    const int token = (r0 + r) / p.G, head = r0 + r - token * p.G;
+    *reinterpret_cast<uint2*>(p.out + (long long)(s.q_begin + token) * p.ldo + (long long)(h * p.G + head) * D + d) =
+        make_uint2(pack_bf16x2(a.x * inv, a.y * inv), pack_bf16x2(a.z * inv, a.w * inv));
+  }
+}
+
+static constexpr int kMostReqs = 8192;         // (the line of a step is in shared memory)
+
+template <int D, int NT>
+static int launch_rows(Fp4Rows p, int grid, cudaStream_t stream) {
+  using Shape = Fp4RowsShape<D, NT>;
+  p.rows = Shape::kRows;
+  const size_t smem = Shape::kFixed + (size_t)(p.num_reqs + 1) * 4;
+  static PerDeviceOnce once;
+  if (once.first()) {
+    cudaFuncSetAttribute(fp4_rows_kernel<D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape::kFixed + (kMostReqs + 1) * 4);
+  }
+  if (launch_pdl(fp4_rows_kernel<D, NT>, dim3(grid), dim3(kRowWarps * 32), smem, stream, p) != cudaSuccess) return -2;
+  return launch_pdl(fp4_join_kernel<D, NT>, dim3(grid), dim3(256), (size_t)(p.num_reqs + 1) * 4, stream, p, grid) == cudaSuccess ? 0 : -2;
+}
+
+}  // namespace b200
+
+using namespace b200;
+
+static int fp4_tile_rows(int G, int D) { return G > 8 && D <= 128 ? 16 : 8; }
+static int fp4_grid(int rows, int D) { return b200_num_sms() * (rows == 8 && D <= 128 ? 2 : 1); }
+
+// Floats of scratch that b200_fp4_attn needs (B200Fp4Attn.parts).
+extern "C" long long b200_fp4_attn_scratch(int Hq, int Hkv, int D) {
+  if (Hkv <= 0 || Hq % Hkv) return -1;
+  const int rows = 16;
+  return (long long)b200_num_sms() * 2 * 2 * rows * (D + 2);
+}
+
+extern "C" int b200_fp4_attn(const B200Fp4Attn* a, cudaStream_t stream) {
+  if (a->num_reqs <= 0 || a->total_q <= 0) return 0;
+  if ((a->D != 64 && a->D != 128 && a->D != 256) || a->Hkv <= 0 || a->Hq <= 0 || a->Hq % a->Hkv || a->block_size <= 0 ||
+      a->block_size % kCellTokens || a->num_blocks <= 0 || a->max_blocks <= 0)
+    return -1;
+  const uintptr_t bits = (uintptr_t)a->q | (uintptr_t)a->out | (uintptr_t)a->cache | (uintptr_t)((a->ldq | a->ldo) * 2);
+  if ((bits & 15) || !a->q || !a->out || !a->cache || !a->block_table || !a->seq_lens || !a->parts) return -1;
+  if (a->num_reqs > kMostReqs) return -4;
+  const int G = a->Hq / a->Hkv;
+  // cells of the whole line in 31 bits, whatever the lengths
+  if ((double)a->max_blocks * (a->block_size / kCellTokens) * a->Hkv * ((double)a->total_q * G / 8 + a->num_reqs) > 2147483647.0) return -4;
+  if ((double)a->max_blocks * a->block_size > 2147483647.0) return -4;
+  Fp4Rows p;
+  p.q = (const __nv_bfloat16*)a->q; p.ldq = a->ldq;
+  p.out = (__nv_bfloat16*)a->out; p.ldo = a->ldo;
+  p.cache = (const uint8_t*)a->cache; p.num_blocks = a->num_blocks;
+  p.block_table = (const int32_t*)a->block_table; p.max_blocks = a->max_blocks; p.ldt = a->ldt;
+  p.seq_lens = (const int32_t*)a->seq_lens; p.q_start = (const int32_t*)a->q_start;
+  p.num_reqs = a->num_reqs; p.total_q = a->total_q;
+  p.Hkv = a->Hkv; p.G = G; p.cells_per_page = a->block_size / kCellTokens;
+  p.window = a->window; p.causal = a->causal;
+  p.scale_log2 = a->scale * 1.4426950408889634f;
+  p.softcap2 = a->softcap * 1.4426950408889634f;
+  p.parts = (float*)a->parts;
+  p.status = device_status_word();
+  const int rows = a->q_start && a->D <= 128 ? 16 : fp4_tile_rows(G, a->D), grid = fp4_grid(rows, a->D);
+  if (a->D == 64) return rows == 8 ? launch_rows<64, 1>(p, grid, stream) : launch_rows<64, 2>(p, grid, stream);
+  if (a->D == 128) return rows == 8 ? launch_rows<128, 1>(p, grid, stream) : launch_rows<128, 2>(p, grid, stream);
+  return launch_rows<256, 1>(p, grid, stream);
+}

@@ -1,0 +1,256 @@
+// Keys and values into a paged cache held in 4 bits, and back (layout: fp4_cache.cuh).
+//
+// append:  y = rope(norm(x)) for q and k heads, v as it is; q goes on in bf16, rounded once; k and v in groups of 16 dims
+//            s = max |y| / 6,   code = e2m1(y / s)   (both rounded to nearest, ties to even; s = 0: all codes 0)
+//          Sums, rotation and quotients are fp32, and keys are not rounded to bf16 on the way to their codes. Values past 6 * 10240
+//          (infinities too) saturate, a NaN makes its group NaN.
+// read:    code * s for the given slots, exact in bf16.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "api.h"
+#include "fp4_cache.cuh"
+#include "sm100.cuh"
+
+namespace b200 {
+
+// Eight values -> eight codes, the first in the lowest nibble.
+__device__ __forceinline__ uint32_t e2m1_of(const float (&r)[8]) {
+  uint32_t w;
+  asm("{\n\t.reg .b8 b0, b1, b2, b3;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 b0, %2, %1;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 b1, %4, %3;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 b2, %6, %5;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 b3, %8, %7;\n\t"
+      "mov.b32 %0, {b0, b1, b2, b3};\n\t}\n"
+      : "=r"(w)
+      : "f"(r[0]), "f"(r[1]), "f"(r[2]), "f"(r[3]), "f"(r[4]), "f"(r[5]), "f"(r[6]), "f"(r[7]));
+  return w;
+}
+
+__device__ __forceinline__ void unpack_bf16x8(const uint4& v, float (&x)[8]) {
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const float2 f = unpack_bf16x2(w[k]);
+    x[2 * k] = f.x;
+    x[2 * k + 1] = f.y;
+  }
+}
+
+// A lane has 8 dims (16 bytes) of a head, so a head is D / 8 lanes and a group of 16 dims two neighbours. A warp takes PASSES times
+// the heads that its lanes hold, all of one token, whose position, slot, cos and sin are fetched once behind the heads' loads.
+template <int D, int PASSES>
+__global__ void __launch_bounds__(128) fp4_append_kernel(B200Fp4Append p) {
+  using Cell = Fp4Cell<D>;
+  constexpr int kLanes = D / 8, kHeads = 32 / kLanes;
+  __shared__ float exchange[4][256];
+  pdl_wait();
+  pdl_launch_dependents();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, l = lane % kLanes, side = lane / kLanes;
+  const int nheads = p.Hq + 2 * p.Hkv, v0 = p.Hq + p.Hkv, parts = (nheads + kHeads * PASSES - 1) / (kHeads * PASSES);
+  const uint32_t gw = blockIdx.x * 4 + warp;                     // (T * parts < 2^31)
+  const int t = (int)(gw / (uint32_t)parts), h0 = (int)(gw - (uint32_t)t * parts) * (kHeads * PASSES);
+  if (t >= p.T) return;
+  const __nv_bfloat16* qrow = (const __nv_bfloat16*)p.q + (size_t)t * p.ldq;
+  const __nv_bfloat16* krow = (const __nv_bfloat16*)p.k + (size_t)t * p.ldk;
+  const __nv_bfloat16* vrow = (const __nv_bfloat16*)p.v + (size_t)t * p.ldv;
+  uint4 raw[PASSES];
+#pragma unroll
+  for (int i = 0; i < PASSES; ++i) {
+    const int h = h0 + i * kHeads + side;
+    if (h < nheads)
+      raw[i] = *reinterpret_cast<const uint4*>((h < p.Hq ? qrow + (size_t)h * p.q_head_stride : h < v0 ? krow + (h - p.Hq) * D
+                                                                                                  : vrow + (h - v0) * D) + l * 8);
+  }
+  const int rot = p.cos_sin ? p.rot : 0, half = rot >> 1;
+  float c[8], s[8];                                             // y = x c + partner s
+#pragma unroll
+  for (int e = 0; e < 8; ++e) { c[e] = 1.f; s[e] = 0.f; }
+  if (rot && h0 < v0) {
+    const int64_t at = ((const int64_t*)p.positions)[t];
+    const bool there = at >= 0 && at < p.table_rows;
+    const float* cs = (const float*)p.cos_sin + (there ? at : 0) * rot;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const int d = l * 8 + e;
+      if (d < rot) {
+        const int j = p.neox ? (d < half ? d : d - half) : d >> 1;
+        const bool minus = p.neox ? d < half : !(d & 1);
+        c[e] = there ? cs[j] : __int_as_float(0x7fffffff);       // a position outside the table: NaN
+        s[e] = minus ? -cs[half + j] : cs[half + j];
+      }
+    }
+  }
+  uint8_t* cell = nullptr;                                      // the token's cell of kv head 0
+  int token = 0;
+  if (h0 + kHeads * PASSES > p.Hq) {
+    const int64_t slot = ((const int64_t*)p.slots)[t];
+    if (slot >= 0 && slot < p.num_blocks * p.block_size) {
+      const int64_t blk = (slot >> 31) == 0 ? (int64_t)((uint32_t)slot / (uint32_t)p.block_size) : slot / p.block_size;
+      const int off = (int)(slot - blk * p.block_size);
+      cell = (uint8_t*)p.cache + (blk * p.Hkv * (p.block_size / kCellTokens) + off / kCellTokens) * Cell::kBytes;
+      token = off % kCellTokens;
+    }
+  }
+  const size_t head_bytes = (size_t)(p.block_size / kCellTokens) * Cell::kBytes;
+  const float g = p.gemma ? 1.f : 0.f;
+#pragma unroll
+  for (int i = 0; i < PASSES; ++i) {
+    const int h = h0 + i * kHeads + side;
+    if (h0 + i * kHeads >= nheads) break;                       // (the warp stays together: shuffles)
+    float x[8];
+    unpack_bf16x8(raw[i], x);
+    const bool is_q = h < p.Hq, is_v = h >= v0;
+    if (p.q_norm || p.k_norm) {
+      float ss = 0.f;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) ss += x[e] * x[e];
+#pragma unroll
+      for (int o = kLanes / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+      const __nv_bfloat16* w = (const __nv_bfloat16*)(is_q ? p.q_norm : p.k_norm);
+      if (w && !is_v) {
+        float wf[8];
+        unpack_bf16x8(*reinterpret_cast<const uint4*>(w + l * 8), wf);
+        const float inv = rsqrtf(ss / (float)D + p.eps);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = x[e] * inv * (wf[e] + g);
+      }
+    }
+    float y[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) y[e] = x[e];
+    if (rot && h0 + i * kHeads < v0) {                          // (the same for the warp: a q or k head among its heads)
+      float other[8];
+      if (!p.neox) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) other[e] = x[e ^ 1];
+      } else if (!(half & 7)) {
+        const int partner = lane + (l * 8 < half ? half / 8 : l * 8 < rot ? -half / 8 : 0);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) other[e] = __shfl_sync(0xffffffffu, x[e], partner);
+      } else {
+        float* b = exchange[warp];
+        __syncwarp();
+#pragma unroll
+        for (int e = 0; e < 8; ++e) b[lane * 8 + e] = x[e];
+        __syncwarp();
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const int d = l * 8 + e;
+          other[e] = d < rot ? b[side * D + (d < half ? d + half : d - half)] : 0.f;
+        }
+      }
+      if (!is_v) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) y[e] = l * 8 + e < rot ? x[e] * c[e] + other[e] * s[e] : x[e];
+      }
+    }
+    uint32_t top = 0;                                           // of |y|, as bits: a NaN is above infinity
+#pragma unroll
+    for (int e = 0; e < 8; ++e) top = max(top, __float_as_uint(y[e]) & 0x7fffffffu);
+    top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+    if (h >= nheads) continue;
+    if (is_q) {
+      __nv_bfloat16* dst = p.q_out ? (__nv_bfloat16*)p.q_out + (size_t)t * p.ldo + h * D
+                                   : (__nv_bfloat16*)p.q + (size_t)t * p.ldq + (size_t)h * p.q_head_stride;
+      *reinterpret_cast<uint4*>(dst + l * 8) = make_uint4(pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3]), pack_bf16x2(y[4], y[5]),
+                                                          pack_bf16x2(y[6], y[7]));
+      continue;
+    }
+    if (!cell) continue;
+    const uint8_t scale = fp4_scale_byte(__fdiv_rn(__uint_as_float(top), 6.f));
+    const float sf = fp4_scale_value(scale);
+    float r[8];
+    // (a true quotient: values of few bits lie between two codes exactly, and there a reciprocal decides by its own rounding)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) r[e] = sf == 0.f ? 0.f : __fdiv_rn(y[e], sf);
+    const uint32_t codes = e2m1_of(r);
+    uint8_t* dst = cell + (size_t)(is_v ? h - v0 : h - p.Hq) * head_bytes;
+    if (is_v) {
+      *reinterpret_cast<uint32_t*>(dst + Cell::value_at(token, l * 4)) = codes;
+      if (!(l & 1)) dst[Cell::kValueScales + (l >> 1) * kCellTokens + token] = scale;
+    } else {
+      *reinterpret_cast<uint32_t*>(dst + token * Cell::kRow + l * 4) = codes;
+      if (!(l & 1)) dst[Cell::kKeyScales + token * Cell::kScales + (l >> 1)] = scale;
+    }
+  }
+}
+
+// A lane turns 8 codes into 16 bytes of bf16.
+template <int D>
+__global__ void __launch_bounds__(128) fp4_read_kernel(const uint8_t* __restrict__ cache, long long num_blocks, int block_size, int Hkv,
+                                                       const int64_t* __restrict__ slots, __nv_bfloat16* __restrict__ k, long long ldk,
+                                                       __nv_bfloat16* __restrict__ v, long long ldv, long long n) {
+  using Cell = Fp4Cell<D>;
+  pdl_wait();
+  pdl_launch_dependents();
+  const long long i = blockIdx.x * 128ll + threadIdx.x;
+  const int l = (int)(i % (D / 8));
+  const long long th = i / (D / 8);
+  const long long t = th / (2 * Hkv);
+  if (t >= n) return;
+  const int h2 = (int)(th - t * (2 * Hkv)), kv = h2 >= Hkv, h = h2 - kv * Hkv;
+  const int64_t slot = slots[t];
+  uint32_t o[4] = {0, 0, 0, 0};
+  if (slot >= 0 && slot < num_blocks * block_size) {
+    const int64_t blk = (slot >> 31) == 0 ? (int64_t)((uint32_t)slot / (uint32_t)block_size) : slot / block_size;
+    const int off = (int)(slot - blk * block_size), token = off % kCellTokens;
+    const uint8_t* cell = cache + ((blk * Hkv + h) * (block_size / kCellTokens) + off / kCellTokens) * (long long)Cell::kBytes;
+    const uint32_t codes = *reinterpret_cast<const uint32_t*>(cell + (kv ? Cell::value_at(token, l * 4) : token * Cell::kRow + l * 4));
+    const float s = fp4_scale_value(cell[kv ? Cell::kValueScales + (l >> 1) * kCellTokens + token
+                                          : Cell::kKeyScales + token * Cell::kScales + (l >> 1)]);
+    uint32_t f16[4];
+    cvt_e2m1x8(codes, f16);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float2 f = __half22float2(*reinterpret_cast<__half2*>(&f16[e]));
+      o[e] = pack_bf16x2(f.x * s, f.y * s);
+    }
+  }
+  *reinterpret_cast<uint4*>((kv ? v + t * ldv : k + t * ldk) + h * D + l * 8) = make_uint4(o[0], o[1], o[2], o[3]);
+}
+
+template <int D>
+static int launch_append(const B200Fp4Append& p, cudaStream_t stream) {
+  constexpr int kHeads = 32 / (D / 8);
+  const int nheads = p.Hq + 2 * p.Hkv;
+  const auto go = [&](auto kernel, int passes) {
+    const long long warps = (long long)p.T * ((nheads + kHeads * passes - 1) / (kHeads * passes));
+    if (warps >= (1ll << 31)) return -4;
+    return launch_pdl(kernel, dim3((unsigned)((warps + 3) / 4)), dim3(128), 0, stream, p) == cudaSuccess ? 0 : -2;
+  };
+  return go(fp4_append_kernel<D, 1>, 1);
+}
+
+}  // namespace b200
+
+using namespace b200;
+
+static bool fp4_cache_ok(int D, int block_size, int Hkv, long long num_blocks) {
+  return (D == 64 || D == 128 || D == 256) && block_size > 0 && block_size % kCellTokens == 0 && Hkv > 0 && num_blocks > 0;
+}
+
+extern "C" int b200_fp4_append(const B200Fp4Append* a, cudaStream_t stream) {
+  if (a->T <= 0) return 0;
+  if (!fp4_cache_ok(a->D, a->block_size, a->Hkv, a->num_blocks) || a->Hq < 0 || !a->k || !a->v || !a->slots || !a->cache || (a->Hq && !a->q))
+    return -1;
+  if (a->cos_sin && (!a->positions || a->rot < 0 || a->rot > a->D || (a->rot & 1))) return -1;
+  const uintptr_t bits = (uintptr_t)a->q | (uintptr_t)a->k | (uintptr_t)a->v | (uintptr_t)a->q_out | (uintptr_t)a->q_norm |
+                         (uintptr_t)a->k_norm | (uintptr_t)a->cache | (uintptr_t)((a->ldq | a->ldk | a->ldv | a->ldo | a->q_head_stride) * 2);
+  if (bits & 15) return -1;
+  return a->D == 64 ? launch_append<64>(*a, stream) : a->D == 128 ? launch_append<128>(*a, stream) : launch_append<256>(*a, stream);
+}
+
+extern "C" int b200_fp4_read(const void* cache, long long num_blocks, int block_size, int Hkv, int D, const void* slots, void* k, long long ldk,
+                             void* v, long long ldv, long long n, cudaStream_t stream) {
+  if (n <= 0) return 0;
+  if (!fp4_cache_ok(D, block_size, Hkv, num_blocks) || (((uintptr_t)cache | (uintptr_t)k | (uintptr_t)v | (uintptr_t)((ldk | ldv) * 2)) & 15)) return -1;
+  const long long blocks = (n * 2 * Hkv * (D / 8) + 127) / 128;
+  if (blocks >= (1ll << 31)) return -4;
+  const auto go = [&](auto kernel) {
+    return launch_pdl(kernel, dim3((unsigned)blocks), dim3(128), 0, stream, (const uint8_t*)cache, num_blocks, block_size, Hkv,
+                      (const int64_t*)slots, (__nv_bfloat16*)k, ldk, (__nv_bfloat16*)v, ldv, n) == cudaSuccess ? 0 : -2;
+  };
+  return D == 64 ? go(fp4_read_kernel<64>) : D == 128 ? go(fp4_read_kernel<128>) : go(fp4_read_kernel<256>);
+}

@@ -1,0 +1,317 @@
+"""A paged KV cache held in 4 bits: what writes it, what reads it back, and the attention over it.
+
+A layer's cache is uint8 ``[num_blocks, kv heads, block_size / 16, 18 * head_dim]`` (:func:`alloc`), 9 bits for 2 bytes of a bf16
+cache; slots and block tables are those of the bf16 cache. Groups of 16 neighbouring head dimensions share a scale,
+``s = max |x| / 6`` in 5 exponent and 3 mantissa bits (the upper half of an f16 behind its sign), and hold codes ``e2m1(x / s)``, both
+rounded to nearest, ties to even. Code times scale is exact in bf16. Magnitudes past 6 * 10240 saturate, a NaN makes its group NaN. Within the last dimension, 16 tokens:
+key codes ``[16, D / 2]`` (the even dimension in the low nibble), value codes ``[16, D / 2]`` whose 16-byte piece ``n`` lies at
+``n ^ 2 (token // 4)``, key scales ``[16, D / 16]``, value scales ``[D / 16, 16]``.
+
+head_dim 64, 128 or 256; block_size a multiple of 16; bf16 queries, keys and values in rows on 16-byte boundaries. The ``ref_*``
+functions restate the operators in plain PyTorch (any device).
+"""
+from __future__ import annotations
+
+import ctypes
+import math
+from typing import Optional
+
+import torch
+
+from . import _lib, reference
+from ._lib import check, lib, ptr, stream_ptr
+from .validate import OpArgumentError, validate
+
+CELL = 16                      # tokens of a cell
+LEVELS = (0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0)
+MOST_SCALE = 10240.0           # (6 times it is still an f16)
+BF16 = torch.bfloat16
+
+_P, _L, _I, _F = ctypes.c_void_p, ctypes.c_longlong, ctypes.c_int, ctypes.c_float
+
+
+class AppendArgs(ctypes.Structure):
+    _fields_ = [("q", _P), ("k", _P), ("v", _P), ("q_out", _P), ("ldq", _L), ("ldk", _L), ("ldv", _L), ("ldo", _L),
+                ("positions", _P), ("cos_sin", _P), ("q_norm", _P), ("k_norm", _P), ("slots", _P), ("cache", _P),
+                ("num_blocks", _L), ("table_rows", _L), ("T", _I), ("Hq", _I), ("Hkv", _I), ("D", _I), ("rot", _I),
+                ("q_head_stride", _I), ("block_size", _I), ("neox", _I), ("gemma", _I), ("eps", _F)]
+
+
+class AttnArgs(ctypes.Structure):
+    _fields_ = [("q", _P), ("out", _P), ("ldq", _L), ("ldo", _L), ("ldt", _L), ("cache", _P), ("num_blocks", _L),
+                ("block_table", _P), ("seq_lens", _P), ("q_start", _P), ("tile_req", _P), ("tile_q0", _P), ("parts", _P),
+                ("max_blocks", _I), ("num_reqs", _I), ("total_q", _I), ("num_tiles", _I), ("Hq", _I), ("Hkv", _I), ("D", _I),
+                ("block_size", _I), ("window", _I), ("causal", _I), ("scale", _F), ("softcap", _F)]
+
+
+_declared = False
+
+
+def _declare():
+    global _declared
+    if _declared:
+        return
+    _lib.declare("b200_fp4_append", [ctypes.POINTER(AppendArgs), _P], _I)
+    _lib.declare("b200_fp4_read", [_P, _L, _I, _I, _I, _P, _P, _L, _P, _L, _L, _P], _I)
+    _lib.declare("b200_fp4_attn", [ctypes.POINTER(AttnArgs), _P], _I)
+    _lib.declare("b200_fp4_attn_scratch", [_I, _I, _I], _L)
+    lib()
+    _declared = True
+
+
+def bytes_per_block(num_kv_heads: int, block_size: int, head_dim: int) -> int:
+    return num_kv_heads * (block_size // CELL) * 18 * head_dim
+
+
+def alloc(num_blocks: int, num_kv_heads: int, block_size: int, head_dim: int, device) -> torch.Tensor:
+    """The zeroed cache of a layer."""
+    if head_dim not in (64, 128, 256) or block_size <= 0 or block_size % CELL:
+        raise OpArgumentError("fp4_cache.alloc", "head_dim is 64, 128 or 256 and block_size a multiple of 16",
+                              f"head_dim={head_dim}, block_size={block_size}")
+    return torch.zeros((num_blocks, num_kv_heads, block_size // CELL, 18 * head_dim), dtype=torch.uint8, device=device)
+
+
+def shape_of(cache: torch.Tensor) -> tuple[int, int, int, int]:
+    """(num_blocks, kv heads, block_size, head_dim) of a cache."""
+    n, h, c, b = cache.shape
+    return n, h, c * CELL, b // 18
+
+
+def _launch(device: torch.device, call, what: str) -> None:
+    """Launches on the current stream of the tensors' device, whichever device is current."""
+    if device.index == torch._C._cuda_getDevice():
+        check(call(stream_ptr()), what)
+    else:
+        with torch.cuda.device(device):
+            check(call(stream_ptr()), what)
+
+
+def append(qkv: torch.Tensor, positions: Optional[torch.Tensor], cos_sin: Optional[torch.Tensor], cache: torch.Tensor,
+           slots: torch.Tensor, *, num_q_heads: int, rot_dim: Optional[int] = None, neox: bool = True,
+           q_norm: Optional[torch.Tensor] = None, k_norm: Optional[torch.Tensor] = None, eps: float = 1e-6, gemma: bool = False,
+           q_out: Optional[torch.Tensor] = None, q_head_stride: Optional[int] = None,
+           offsets: Optional[tuple[int, int, int]] = None) -> None:
+    """Per-head RMSNorm of q and k (weights bf16 ``[D]``, optional) and rotation of merged ``[T, q | k | v]`` rows; q in place or to
+    ``q_out`` ``[T, Hq * D]``, k and v into the cache. ``cos_sin``: fp32 ``[positions, cos | sin]`` (None: no rotation), ``rot_dim``
+    its width, pairs half of it apart (``neox``) or neighbours. ``offsets``: columns where q, k and v begin; ``q_head_stride``:
+    columns between q heads. The slots of a call differ; slots outside the cache (-1) write nothing, and a position
+    outside the table makes its row NaN. The k and v columns of ``qkv`` stay as they are."""
+    a = AppendArgs()
+    a.num_blocks, a.Hkv, a.block_size, D = shape_of(cache) if cache.dim() == 4 else (0, 0, 0, 0)
+    hs = D if q_head_stride is None else q_head_stride
+    if offsets is None:
+        offsets = (0, num_q_heads * D, (num_q_heads + a.Hkv) * D)
+    rot = (D if cos_sin is None else cos_sin.shape[1]) if rot_dim is None else rot_dim
+    validate("fp4_append", qkv=qkv, cache=cache, slots=slots, positions=positions, cos_sin=cos_sin, q_norm=q_norm, k_norm=k_norm,
+             q_out=q_out, num_q_heads=num_q_heads, rot_dim=rot, q_head_stride=hs, offsets=offsets)
+    _declare()
+    at = qkv.data_ptr()
+    a.q, a.k, a.v = at + 2 * offsets[0], at + 2 * offsets[1], at + 2 * offsets[2]
+    a.ldq = a.ldk = a.ldv = qkv.stride(0)
+    if q_out is not None:
+        a.q_out, a.ldo = q_out.data_ptr(), q_out.stride(0)
+    if cos_sin is not None:
+        a.positions, a.cos_sin, a.table_rows, a.rot = positions.data_ptr(), cos_sin.data_ptr(), cos_sin.shape[0], rot
+    a.q_norm, a.k_norm, a.slots, a.cache = ptr(q_norm), ptr(k_norm), slots.data_ptr(), cache.data_ptr()
+    a.T, a.Hq, a.D, a.q_head_stride, a.neox, a.gemma, a.eps = qkv.shape[0], num_q_heads, D, hs, neox, gemma, eps
+    _launch(qkv.device, lambda s: lib().b200_fp4_append(ctypes.byref(a), s), "fp4_append")
+
+
+def write(k: torch.Tensor, v: torch.Tensor, cache: torch.Tensor, slots: torch.Tensor) -> None:
+    """Keys and values ``[n, Hkv * D]`` (or ``[n, Hkv, D]``) that are normed and rotated already, into the cache. What :func:`read`
+    gave comes back to the same values, but for groups whose scale was below 2^-14 or that had saturated."""
+    k, v = k.flatten(1), v.flatten(1)
+    validate("fp4_write", k=k, v=v, cache=cache, slots=slots)
+    _declare()
+    a = AppendArgs()
+    a.num_blocks, a.Hkv, a.block_size, a.D = shape_of(cache)
+    a.k, a.v, a.ldk, a.ldv = k.data_ptr(), v.data_ptr(), k.stride(0), v.stride(0)
+    a.slots, a.cache, a.T, a.eps = slots.data_ptr(), cache.data_ptr(), k.shape[0], 1.0
+    _launch(k.device, lambda s: lib().b200_fp4_append(ctypes.byref(a), s), "fp4_write")
+
+
+def read(cache: torch.Tensor, slots: torch.Tensor, k: Optional[torch.Tensor] = None,
+         v: Optional[torch.Tensor] = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """Keys and values bf16 ``[n, Hkv, D]`` that the cache holds for ``slots`` (int64 ``[n]``); zeros for slots outside the cache."""
+    validate("fp4_read", cache=cache, slots=slots, k=k, v=v)
+    _declare()
+    nb, H, bs, D = shape_of(cache)
+    n = slots.numel()
+    k = torch.empty((n, H, D), dtype=BF16, device=cache.device) if k is None else k
+    v = torch.empty((n, H, D), dtype=BF16, device=cache.device) if v is None else v
+    _launch(cache.device, lambda s: lib().b200_fp4_read(cache.data_ptr(), nb, bs, H, D, slots.data_ptr(), k.data_ptr(), k.stride(0),
+                                                        v.data_ptr(), v.stride(0), n, s), "fp4_read")
+    return k, v
+
+
+_scratch_floats: dict = {}
+
+
+def scratch(device: torch.device, num_q_heads: int, num_kv_heads: int, head_dim: int) -> torch.Tensor:
+    """What ``decode`` and ``prefill`` take as ``tmp``: parts of sequences that several CTAs share. Calls that may run at the same time
+    (streams, graphs replayed side by side) need one each."""
+    key = (device.index, num_q_heads, num_kv_heads, head_dim)
+    n = _scratch_floats.get(key)
+    if n is None:
+        _declare()
+        with torch.cuda.device(device):
+            n = _scratch_floats[key] = lib().b200_fp4_attn_scratch(num_q_heads, num_kv_heads, head_dim)
+    return torch.empty(n, dtype=torch.float32, device=device)
+
+
+def _attend(op, q, cache, block_table, seq_lens, q_start, tile_req, tile_q0, scale, out, softcap, window, causal, tmp):
+    if out is None and q.is_cuda:
+        out = torch.empty((q.shape[0], q.shape[1]), dtype=q.dtype, device=q.device)
+    validate(op, q=q, cache=cache, block_table=block_table, seq_lens=seq_lens, q_start=q_start, tile_req=tile_req, tile_q0=tile_q0,
+             out=out, softcap=softcap, tmp=tmp)
+    _declare()
+    a = AttnArgs()
+    a.num_blocks, a.Hkv, a.block_size, D = shape_of(cache)
+    a.Hq, a.D = q.shape[1] // D, D
+    a.q, a.ldq, a.out, a.ldo, a.cache = q.data_ptr(), q.stride(0), out.data_ptr(), out.stride(0), cache.data_ptr()
+    a.block_table, a.ldt, a.max_blocks = block_table.data_ptr(), block_table.stride(0), block_table.shape[1]
+    a.seq_lens, a.total_q = seq_lens.data_ptr(), q.shape[0]
+    if q_start is None:
+        a.num_reqs = q.shape[0]
+    else:
+        a.q_start, a.num_reqs = q_start.data_ptr(), min(q_start.numel() - 1, block_table.shape[0], seq_lens.numel())
+        a.tile_req, a.tile_q0, a.num_tiles = tile_req.data_ptr(), tile_q0.data_ptr(), tile_req.numel()
+    a.window, a.causal, a.scale, a.softcap = window, causal, scale, softcap
+    if tmp is None:
+        tmp = scratch(q.device, a.Hq, a.Hkv, D)
+    a.parts = tmp.data_ptr()
+    _launch(q.device, lambda s: lib().b200_fp4_attn(ctypes.byref(a), s), op)
+    return out
+
+
+def decode(q: torch.Tensor, cache: torch.Tensor, *, block_table: torch.Tensor, seq_lens: torch.Tensor, scale: float,
+           out: Optional[torch.Tensor] = None, softcap: float = 0.0, window: int = 0,
+           tmp: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Attention of one query row a sequence, ``q`` ``[B, Hq * D]``, at its last position. ``seq_lens`` int32 ``[B]`` counts the row's own
+    key; 0: zeros come out. ``window`` as in :func:`vllm_cpp_b200.ops.attn_decode`; entries of ``block_table`` outside the cache count as
+    masked keys. ``tmp``: :func:`scratch`, allocated if not given."""
+    return _attend("fp4_decode", q, cache, block_table, seq_lens, None, None, None, scale, out, softcap, window, True, tmp)
+
+
+def prefill(q: torch.Tensor, cache: torch.Tensor, *, block_table: torch.Tensor, seq_lens: torch.Tensor, q_start: torch.Tensor,
+            tile_req: torch.Tensor, tile_q0: torch.Tensor, scale: float, out: Optional[torch.Tensor] = None, softcap: float = 0.0,
+            window: int = 0, causal: bool = True, tmp: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Attention of the query rows ``q_start[r]..q_start[r + 1]`` of each sequence, the last of its ``seq_lens[r]`` positions.
+    ``tile_req`` / ``tile_q0`` list their 128-row tiles, as in :func:`vllm_cpp_b200.ops.attn_prefill`. Rows outside every
+    sequence stay as they are."""
+    return _attend("fp4_prefill", q, cache, block_table, seq_lens, q_start, tile_req, tile_q0, scale, out, softcap, window, causal, tmp)
+
+
+# ------------------------------------------------------------------------------ restatements
+def scale_values(b: torch.Tensor) -> torch.Tensor:
+    """Scale bytes as fp32."""
+    return (b.to(torch.int16) << 7).view(torch.float16).float()
+
+
+def ref_quantize(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """``x`` ``[..., D]`` -> codes ``[..., D]``, scale bytes ``[..., D / 16]``, both uint8."""
+    g = x.float().unflatten(-1, (-1, 16))
+    top = g.abs().amax(-1)                                       # (a NaN stays one)
+    s = (top / torch.full_like(top, 6.0)).clamp(max=MOST_SCALE)
+    step = torch.ldexp(torch.ones_like(s), (torch.frexp(s)[1] - 1).clamp(min=-14) - 3)
+    scale = ((torch.round(s / step) * step).half().view(torch.int16) >> 7).to(torch.uint8)
+    scale = torch.where(s.isnan(), torch.full_like(scale, 0xff), scale)
+    s = scale_values(scale)[..., None]
+    r = torch.where(s == 0, torch.zeros_like(g), g.abs() / s)
+    code = sum((r > b if i % 2 == 0 else r >= b).to(torch.uint8) for i, b in enumerate((0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0)))
+    return (code | torch.signbit(g).to(torch.uint8) << 3).flatten(-2), scale
+
+
+def _value_order(D: int, device) -> torch.Tensor:
+    """Where 16-byte piece n of a cell's value codes lies."""
+    n = torch.arange(D // 2, device=device)
+    return n ^ (2 * (n // (D // 32) // 4))
+
+
+def ref_write(k: torch.Tensor, v: torch.Tensor, cache: torch.Tensor, slots: torch.Tensor) -> None:
+    nb, H, bs, D = shape_of(cache)
+    ok = (slots >= 0) & (slots < nb * bs)
+    slot = slots[ok]
+    b, c, t = slot // bs, slot % bs // CELL, slot % CELL
+    kc, ks = ref_quantize(k[ok].reshape(-1, H, D))
+    vc, vs = ref_quantize(v[ok].reshape(-1, H, D))
+    order = _value_order(D, cache.device).view(CELL, D // 32)
+    row, groups = torch.arange(D // 2, device=cache.device), torch.arange(D // 16, device=cache.device)
+    cells = cache.permute(0, 2, 1, 3)                            # [blocks, cells, heads, bytes]
+    for i in range(slot.numel()):
+        cell, tok = cells[b[i], c[i]], int(t[i])
+        cell[:, tok * (D // 2) + row] = kc[i, :, 0::2] | kc[i, :, 1::2] << 4
+        cell[:, 8 * D + order[tok][row // 16] * 16 + row % 16] = vc[i, :, 0::2] | vc[i, :, 1::2] << 4
+        cell[:, 16 * D + tok * (D // 16) + groups] = ks[i]
+        cell[:, 17 * D + groups * CELL + tok] = vs[i]
+
+
+def ref_append(qkv, positions, cos_sin, cache, slots, *, num_q_heads, rot_dim=None, neox=True, q_norm=None, k_norm=None, eps=1e-6,
+               gemma=False, q_out=None, q_head_stride=None, offsets=None) -> None:
+    nb, H, bs, D = shape_of(cache)
+    T, hs = qkv.shape[0], D if q_head_stride is None else q_head_stride
+    o = (0, num_q_heads * D, (num_q_heads + H) * D) if offsets is None else offsets
+    rot = 0 if cos_sin is None else cos_sin.shape[1] if rot_dim is None else rot_dim
+    q = torch.stack([qkv[:, o[0] + i * hs: o[0] + i * hs + D] for i in range(num_q_heads)], 1).float() if num_q_heads else None
+    k, v = (qkv[:, o[i]: o[i] + H * D].reshape(T, H, D).float() for i in (1, 2))
+
+    def turned(x, w):
+        if w is not None:
+            x = x * torch.rsqrt(x.pow(2).mean(-1, keepdim=True) + eps) * (w.float() + float(gemma))
+        if not rot:
+            return x
+        inside = (positions >= 0) & (positions < cos_sin.shape[0])
+        cs = cos_sin[torch.where(inside, positions, 0)]
+        cs = torch.where(inside[:, None], cs, torch.full_like(cs, math.nan))
+        return reference.apply_rope(x, cs[:, : rot // 2], cs[:, rot // 2:], rot, neox)
+    k = turned(k, k_norm)
+    if num_q_heads:
+        q = turned(q, q_norm).to(qkv.dtype)
+        if q_out is not None:
+            q_out[:T, : num_q_heads * D] = q.flatten(1)
+        else:
+            for i in range(num_q_heads):
+                qkv[:, o[0] + i * hs: o[0] + i * hs + D] = q[:, i]
+    ref_write(k, v, cache, slots)
+
+
+def ref_expand(cache: torch.Tensor) -> torch.Tensor:
+    """The cache as bf16 ``[num_blocks, 2, block_size, Hkv, D]`` (exact)."""
+    nb, H, bs, D = shape_of(cache)
+    levels = torch.tensor(LEVELS + tuple(-x for x in LEVELS), device=cache.device)
+
+    def values(codes, scales):                                   # [..., 16, D / 2], [..., 16, D / 16] bytes
+        both = levels[torch.stack([codes & 15, codes >> 4], -1).flatten(-2).int()]
+        return (both.unflatten(-1, (-1, 16)) * scale_values(scales)[..., None]).flatten(-2)
+    k = values(cache[..., : 8 * D].unflatten(-1, (CELL, D // 2)), cache[..., 16 * D: 17 * D].unflatten(-1, (CELL, D // 16)))
+    vc = cache[..., 8 * D: 16 * D].unflatten(-1, (D // 2, 16))[..., _value_order(D, cache.device), :]
+    v = values(vc.flatten(-2).unflatten(-1, (CELL, D // 2)), cache[..., 17 * D:].unflatten(-1, (D // 16, CELL)).transpose(-1, -2))
+    both = torch.stack([k, v], 1)                                # [nb, 2, H, cells, 16, D]
+    return both.flatten(3, 4).transpose(2, 3).contiguous().to(BF16)
+
+
+def ref_read(cache: torch.Tensor, slots: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    nb, H, bs, D = shape_of(cache)
+    ok = (slots >= 0) & (slots < nb * bs)
+    at = torch.where(ok, slots, 0)
+    blocks, where = torch.unique(at // bs, return_inverse=True)
+    held = ref_expand(cache[blocks])
+    k, v = held[where, 0, at % bs], held[where, 1, at % bs]
+    zero = torch.zeros((), dtype=BF16, device=cache.device)
+    return torch.where(ok[:, None, None], k, zero), torch.where(ok[:, None, None], v, zero)
+
+
+def ref_attention(q, cache, *, block_table, seq_lens, q_start, scale, softcap=0.0, window=0, causal=True) -> torch.Tensor:
+    """:func:`prefill` (and, with ``q_start`` 0, 1, 2.., :func:`decode`) over the pages that the sequences use; their table entries lie
+    inside the cache."""
+    nb, H, bs, D = shape_of(cache)
+    used = [int(-(-int(n) // bs)) for n in seq_lens]
+    ids = torch.cat([block_table[r, :n] for r, n in enumerate(used)] or [block_table.new_zeros(0)]).long()
+    blocks, where = torch.unique(ids, return_inverse=True)
+    table = torch.zeros((len(used), max(used, default=0) or 1), dtype=torch.int32, device=cache.device)
+    at = 0
+    for r, n in enumerate(used):
+        table[r, :n] = where[at: at + n].int()
+        at += n
+    kv = ref_expand(cache[blocks]) if blocks.numel() else ref_expand(cache[:1])
+    return reference.paged_attention(q, kv, table, seq_lens, q_start, q.shape[1] // D, H, D, bs, scale, softcap, window, causal)

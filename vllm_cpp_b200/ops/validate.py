@@ -95,6 +95,96 @@ RULES: dict[str, list] = {
 }
 
 
+def _fp4_cache(cache, **_) -> bool:
+    return cache.dim() == 4 and cache.dtype == torch.uint8 and cache.is_contiguous() and cache.shape[3] in (64 * 18, 128 * 18, 256 * 18) \
+        and cache.shape[2] > 0 and cache.data_ptr() % 16 == 0
+
+
+def _on_gpu(*tensors) -> bool:
+    """All of them (None apart) on one GPU."""
+    dev = {t.device for t in tensors if t is not None}
+    return len(dev) == 1 and next(iter(dev)).type == "cuda"
+
+
+def _ids(t, dtype, n) -> bool:
+    return t.dtype == dtype and t.dim() == 1 and t.numel() >= n and t.is_contiguous()
+
+
+def _bf16_rows(t) -> bool:
+    return t.dim() == 2 and t.dtype == BF16 and (t.shape[0] <= 1 or _rows16(t)) and (t.shape[1] <= 1 or t.stride(1) == 1) and t.data_ptr() % 16 == 0
+
+
+_FP4_CACHE = ("cache is uint8 [blocks, kv heads, block_size / 16, 18 head_dim], contiguous, head_dim 64, 128 or 256", _fp4_cache)
+_FP4_ATTN = [
+    _FP4_CACHE,
+    ("q is [rows, Hq * head_dim] bf16 with rows on 16-byte boundaries, Hq a multiple of the kv heads", lambda q, cache, **_: _bf16_rows(q)
+     and q.shape[1] > 0 and q.shape[1] % (cache.shape[3] // 18 * cache.shape[1]) == 0),
+    ("out is like q and apart from it", lambda q, out, **_: _bf16_rows(out) and out.shape == q.shape and (
+        q.numel() == 0 or out.data_ptr() != q.data_ptr())),
+    ("block_table is int32 [sequences, pages], rows contiguous", lambda block_table, **_: block_table.dtype == torch.int32
+     and block_table.dim() == 2 and block_table.shape[1] > 0 and (block_table.shape[1] == 1 or block_table.stride(1) == 1)),
+    ("softcap is not negative", lambda softcap, **_: softcap >= 0),
+    ("tmp is fp32 and large enough", lambda q, cache, tmp=None, **_: tmp is None or (
+        tmp.dtype == torch.float32 and tmp.is_contiguous() and tmp.numel() >= _fp4_scratch(q, cache))),
+    ("all tensors are on one GPU", lambda q, cache, block_table, seq_lens, out, q_start=None, tile_req=None, tile_q0=None, tmp=None, **_:
+     _on_gpu(q, cache, block_table, seq_lens, out, q_start, tile_req, tile_q0, tmp)),
+]
+
+
+def _fp4_scratch(q, cache) -> int:
+    from ._lib import lib
+    D = cache.shape[3] // 18
+    return lib().b200_fp4_attn_scratch(q.shape[1] // D, cache.shape[1], D)
+
+
+RULES.update({
+    "fp4_append": [
+        _FP4_CACHE,
+        ("qkv is [T, columns] bf16 with rows on 16-byte boundaries", lambda qkv, **_: _bf16_rows(qkv)),
+        ("q, k and v lie inside the rows, their columns multiples of 8", lambda qkv, cache, num_q_heads, q_head_stride, offsets, **_:
+         num_q_heads >= 0 and all(o >= 0 and o % 8 == 0 for o in (*offsets, q_head_stride)) and max(
+             offsets[0] + (num_q_heads - 1) * q_head_stride + cache.shape[3] // 18 if num_q_heads else 0,
+             max(offsets[1:]) + cache.shape[1] * (cache.shape[3] // 18)) <= qkv.shape[1]),
+        ("slots is int64 [T]", lambda qkv, slots, **_: _ids(slots, torch.int64, qkv.shape[0])),
+        ("cos_sin is fp32 [positions, rot_dim] with positions int64 [T], rot_dim even and at most head_dim",
+         lambda qkv, cache, cos_sin, positions, rot_dim, **_: cos_sin is None or (
+             cos_sin.dtype == torch.float32 and cos_sin.dim() == 2 and cos_sin.is_contiguous() and cos_sin.shape[0] > 0
+             and cos_sin.shape[1] == rot_dim and rot_dim % 2 == 0 and 0 < rot_dim <= cache.shape[3] // 18
+             and positions is not None and _ids(positions, torch.int64, qkv.shape[0]))),
+        ("norm weights are bf16 [head_dim] on 16-byte boundaries", lambda cache, q_norm, k_norm, **_: all(
+            w is None or (w.dtype == BF16 and w.is_contiguous() and w.numel() == cache.shape[3] // 18 and w.data_ptr() % 16 == 0)
+            for w in (q_norm, k_norm))),
+        ("q_out is [T, Hq * head_dim] bf16 with rows on 16-byte boundaries", lambda qkv, cache, num_q_heads, q_out, **_: q_out is None or (
+            _bf16_rows(q_out) and q_out.shape[0] >= qkv.shape[0] and q_out.shape[1] == num_q_heads * (cache.shape[3] // 18))),
+        ("all tensors are on one GPU", lambda qkv, cache, slots, positions, cos_sin, q_norm, k_norm, q_out, **_:
+         _on_gpu(qkv, cache, slots, positions, cos_sin, q_norm, k_norm, q_out)),
+    ],
+    "fp4_write": [
+        _FP4_CACHE,
+        ("k and v are [n, kv heads * head_dim] bf16 with rows on 16-byte boundaries", lambda k, v, cache, **_: all(
+            _bf16_rows(x) and x.shape[1] == cache.shape[1] * (cache.shape[3] // 18) for x in (k, v)) and k.shape == v.shape),
+        ("slots is int64 [n]", lambda k, slots, **_: _ids(slots, torch.int64, k.shape[0])),
+        ("all tensors are on one GPU", lambda k, v, cache, slots, **_: _on_gpu(k, v, cache, slots)),
+    ],
+    "fp4_read": [
+        _FP4_CACHE,
+        ("slots is int64 [n]", lambda slots, **_: _ids(slots, torch.int64, 0)),
+        ("k and v are bf16 [n, kv heads, head_dim], contiguous", lambda cache, slots, k=None, v=None, **_: all(
+            x is None or (x.dtype == BF16 and x.is_contiguous() and x.data_ptr() % 16 == 0
+                          and tuple(x.shape) == (slots.numel(), cache.shape[1], cache.shape[3] // 18)) for x in (k, v))),
+        ("all tensors are on one GPU", lambda cache, slots, k=None, v=None, **_: _on_gpu(cache, slots, k, v)),
+    ],
+    "fp4_decode": _FP4_ATTN + [
+        ("block_table and seq_lens (int32) have a row for each of q", lambda q, block_table, seq_lens, **_:
+         block_table.shape[0] >= q.shape[0] and _ids(seq_lens, torch.int32, q.shape[0])),
+    ],
+    "fp4_prefill": _FP4_ATTN + [
+        ("q_start, seq_lens, tile_req and tile_q0 are int32", lambda seq_lens, q_start, tile_req, tile_q0, **_: _ids(q_start, torch.int32, 1)
+         and _ids(seq_lens, torch.int32, 0) and _ids(tile_req, torch.int32, 0) and _ids(tile_q0, torch.int32, tile_req.numel())),
+    ],
+})
+
+
 def validate(op: str, **args) -> None:
     """Raises :class:`OpArgumentError` for the first rule of ``op`` the arguments break."""
     for rule, ok in RULES[op]:
