@@ -977,6 +977,9 @@ class EngineArgs:
     # "auto": the checkpoint's type (bf16). "float32": weights, activations, cache and products in
     # 32 bits, for the models that support it
     dtype: str = "auto"
+    # "auto": the KV cache in the activations' type. "fp4": in 4 bits (ops/fp4_cache.py), 3.56 times the tokens in the same memory,
+    # for the models that name it in KV_CACHE_DTYPES (head_dim 64, 128 or 256, block_size a multiple of 16)
+    kv_cache_dtype: str = "auto"
     # logits rows per step for positions asked for with LLM.score_positions (besides the sampled ones)
     max_score_rows: int = 0
     seed: int = 0

@@ -80,9 +80,13 @@ class LLM:
             if args.dtype not in cls.DTYPES:
                 raise ValueError(f"{cfg.architecture} runs in {', '.join(cls.DTYPES)}, not in {args.dtype}")
             cfg.dtype = args.dtype
+        if args.kv_cache_dtype not in cls.KV_CACHE_DTYPES:
+            raise ValueError(f"{cfg.architecture} holds its KV cache in {', '.join(cls.KV_CACHE_DTYPES)}, not in {args.kv_cache_dtype}")
         if args.max_score_rows and par.tensor_parallel_size > 1:
             raise ValueError("scored positions need the whole vocabulary on one rank")
         self.model = cls(cfg, device=device, parallel=par, comm=self.comm, max_position=max_len)
+        if args.kv_cache_dtype != "auto":
+            self.model.set_kv_cache_dtype(args.kv_cache_dtype, args.block_size)
         if torch.device(device).type == "cpu" and args.cpu_backend == "native":
             from ..models.backend import CpuNativeBackend
             self.model.be = CpuNativeBackend(device)

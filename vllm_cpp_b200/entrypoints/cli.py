@@ -17,6 +17,7 @@ def main(argv=None) -> int:
     ap.add_argument("--prompt-ids", default=None, metavar="ID,ID,...",
                     help="token ids instead of text (models without a tokenizer); prints the generated ids")
     ap.add_argument("--dtype", default="auto", choices=["auto", "bfloat16", "float32"])
+    ap.add_argument("--kv-cache-dtype", default="auto", choices=["auto", "fp4"])
     ap.add_argument("--max-tokens", type=int, default=64)
     ap.add_argument("--temperature", type=float, default=0.0)
     ap.add_argument("--top-p", type=float, default=1.0)
@@ -40,7 +41,7 @@ def main(argv=None) -> int:
     from ..engine import LLM, SamplingParams
     from .async_llm import AsyncLLM
     llm = LLM(EngineArgs(model=a.model, tokenizer=a.tokenizer, device=a.device, max_model_len=a.max_model_len,
-                         max_num_seqs=1, dtype=a.dtype))
+                         max_num_seqs=1, dtype=a.dtype, kv_cache_dtype=a.kv_cache_dtype))
     kw = dict(temperature=a.temperature, top_p=a.top_p, top_k=a.top_k, max_tokens=a.max_tokens)
     if a.seed is not None:
         kw["seed"] = a.seed

@@ -45,6 +45,10 @@ REGISTRY: list[AttentionBackend] = [
                      and v_head_dim % 8 == 0 and v_head_dim <= 256 and _pages_tile(block_size, 128)),
     AttentionBackend("any-size-bias-decode", "decode", "bias", 1, "b200_bias_attn_decode", lambda **_: True),
     AttentionBackend("any-size-bias-prefill", "prefill", "bias", 1, "b200_bias_attn_prefill", lambda **_: True),
+    AttentionBackend("mma-fp4-decode", "decode", "fp4", 0, "b200_fp4_attn",
+                     lambda head_dim, block_size, **_: head_dim in (64, 128, 256) and block_size % 16 == 0),
+    AttentionBackend("mma-fp4-prefill", "prefill", "fp4", 1, "b200_fp4_attn",
+                     lambda head_dim, block_size, **_: head_dim in (64, 128, 256) and block_size % 16 == 0),
     AttentionBackend("mla-absorbed-decode", "decode", "mla", 0, "b200_mla_decode",
                      lambda num_heads, block_size, **_: 1 <= num_heads <= 16 and _pages_tile(block_size, 128)),
     AttentionBackend("mla-expanded-prefill", "prefill", "mla", 0, "b200_attn_prefill (head_dim 256 over expanded K/V)",
@@ -74,7 +78,7 @@ def select(phase: str, kind: str = "paged", *, exclude: tuple = (), **features) 
     return None
 
 
-def describe(cfg, block_size: int) -> dict:
+def describe(cfg, block_size: int, kv_cache_dtype: str = "auto") -> dict:
     """Backends a model configuration resolves to, per layer kind and phase."""
     out = {}
     if getattr(cfg, "kv_lora_rank", 0):
@@ -82,7 +86,8 @@ def describe(cfg, block_size: int) -> dict:
                       for p in ("decode", "prefill")}
     else:
         group = max(1, cfg.num_heads // max(1, cfg.num_kv_heads))
-        out["paged"] = {p: getattr(select(p, "paged", head_dim=cfg.head_dim, group=group, block_size=block_size),
+        kind = "fp4" if kv_cache_dtype == "fp4" else "paged"
+        out[kind] = {p: getattr(select(p, kind, head_dim=cfg.head_dim, group=group, block_size=block_size),
                                    "name", None) for p in ("decode", "prefill")}
     if getattr(cfg, "layer_types", None) and "linear_attention" in cfg.layer_types:
         out["gdn"] = {p: getattr(select(p, "gdn"), "name", None) for p in ("decode", "prefill")}

@@ -252,6 +252,11 @@ class CpuBackend(FusedLinearMixin):
     def rope_kv(self, qkv, positions, table, *, num_q_heads, num_kv_heads, head_dim, rot_dim,
                 neox, q_norm, k_norm, eps, gemma, slot_mapping, kv_cache, block_size,
                 q_head_stride=None, offsets=None):
+        if kv_cache is not None and kv_cache.dtype == torch.uint8:
+            from ..ops import fp4_cache
+            return fp4_cache.ref_append(qkv, positions, table, kv_cache, slot_mapping, num_q_heads=num_q_heads, rot_dim=rot_dim,
+                                        neox=neox, q_norm=q_norm, k_norm=k_norm, eps=eps, gemma=gemma, q_head_stride=q_head_stride,
+                                        offsets=offsets)
         q, k, v = ref.rope_kv(qkv, positions, table, num_q_heads, num_kv_heads, head_dim, rot_dim,
                               neox, q_norm, k_norm, eps, gemma)
         T = qkv.shape[0]
@@ -261,9 +266,14 @@ class CpuBackend(FusedLinearMixin):
 
     def attention(self, q, kv_cache, ctx, group, *, num_q_heads, num_kv_heads, head_dim,
                   block_size, scale, out=None, softcap=0.0, window=0):
-        y = ref.paged_attention(q, kv_cache, ctx.block_table[group], ctx.seq_lens,
-                                ctx.query_start, num_q_heads, num_kv_heads, head_dim, block_size,
-                                scale, softcap, window)
+        if kv_cache.dtype == torch.uint8:
+            from ..ops import fp4_cache
+            y = fp4_cache.ref_attention(q, kv_cache, block_table=ctx.block_table[group], seq_lens=ctx.seq_lens,
+                                        q_start=ctx.query_start, scale=scale, softcap=softcap, window=window)
+        else:
+            y = ref.paged_attention(q, kv_cache, ctx.block_table[group], ctx.seq_lens,
+                                    ctx.query_start, num_q_heads, num_kv_heads, head_dim, block_size,
+                                    scale, softcap, window)
         if out is not None:
             out.copy_(y)
             return out
@@ -438,18 +448,19 @@ class CpuNativeBackend(CpuBackend):
     def rope_kv(self, qkv, positions, table, *, num_q_heads, num_kv_heads, head_dim, rot_dim,
                 neox, q_norm, k_norm, eps, gemma, slot_mapping, kv_cache, block_size,
                 q_head_stride=None, offsets=None):
-        if qkv.dtype != torch.bfloat16 or q_head_stride is not None or offsets is not None:
+        if qkv.dtype != torch.bfloat16 or q_head_stride is not None or offsets is not None or \
+                (kv_cache is not None and kv_cache.dtype == torch.uint8):
             return super().rope_kv(qkv, positions, table, num_q_heads=num_q_heads, num_kv_heads=num_kv_heads,
                                    head_dim=head_dim, rot_dim=rot_dim, neox=neox, q_norm=q_norm, k_norm=k_norm,
                                    eps=eps, gemma=gemma, slot_mapping=slot_mapping, kv_cache=kv_cache,
-                                   block_size=block_size)
+                                   block_size=block_size, q_head_stride=q_head_stride, offsets=offsets)
         self.n.rope_kv(qkv, positions, table, num_q_heads=num_q_heads, num_kv_heads=num_kv_heads,
                        head_dim=head_dim, rot_dim=rot_dim, neox=neox, q_norm=q_norm, k_norm=k_norm, eps=eps,
                        gemma=gemma, slot_mapping=slot_mapping, kv_cache=kv_cache, block_size=block_size)
 
     def attention(self, q, kv_cache, ctx, group, *, num_q_heads, num_kv_heads, head_dim,
                   block_size, scale, out=None, softcap=0.0, window=0):
-        if q.dtype != torch.bfloat16 or q.stride(-1) != 1:
+        if q.dtype != torch.bfloat16 or q.stride(-1) != 1 or kv_cache.dtype == torch.uint8:
             return super().attention(q, kv_cache, ctx, group, num_q_heads=num_q_heads, num_kv_heads=num_kv_heads,
                                      head_dim=head_dim, block_size=block_size, scale=scale, out=out,
                                      softcap=softcap, window=window)
@@ -616,6 +627,10 @@ class GpuBackend(FusedLinearMixin):
     def rope_kv(self, qkv, positions, table, *, num_q_heads, num_kv_heads, head_dim, rot_dim,
                 neox, q_norm, k_norm, eps, gemma, slot_mapping, kv_cache, block_size,
                 q_head_stride=None, offsets=None):
+        if kv_cache is not None and kv_cache.dtype == torch.uint8:
+            from ..ops import fp4_cache
+            return fp4_cache.append(qkv, positions, table, kv_cache, slot_mapping, num_q_heads=num_q_heads, rot_dim=rot_dim, neox=neox,
+                                    q_norm=q_norm, k_norm=k_norm, eps=eps, gemma=gemma, q_head_stride=q_head_stride, offsets=offsets)
         self.ops.rope_kv(qkv, positions, table, num_q_heads=num_q_heads,
                          num_kv_heads=num_kv_heads, head_dim=head_dim, rot_dim=rot_dim, neox=neox,
                          q_norm=q_norm, k_norm=k_norm, eps=eps, gemma=gemma,
@@ -630,6 +645,17 @@ class GpuBackend(FusedLinearMixin):
             out = torch.empty((T, num_q_heads * head_dim), dtype=q.dtype, device=q.device)
         nd = ctx.num_decodes
         bt = ctx.block_table[group]
+        if kv_cache.dtype == torch.uint8:
+            from ..ops import fp4_cache
+            common = dict(scale=scale, softcap=softcap, window=window, tmp=ctx.extra.get("decode_tmp"))
+            if nd > 0:
+                fp4_cache.decode(q[:nd], kv_cache, block_table=bt[:nd], seq_lens=ctx.seq_lens[:nd], out=out[:nd], **common)
+            if ctx.num_prefills > 0:
+                P = ctx.num_prefills
+                fp4_cache.prefill(q[nd:], kv_cache, block_table=bt[nd: nd + P], seq_lens=ctx.seq_lens[nd: nd + P],
+                                  q_start=ctx.prefill_q_start[: P + 1], tile_req=ctx.tile_req[:ctx.num_tiles],
+                                  tile_q0=ctx.tile_q0[:ctx.num_tiles], out=out[nd:], **common)
+            return out
         if nd > 0:
             self.ops.attn_decode(q[:nd], kv_cache, block_table=bt[:nd], seq_lens=ctx.seq_lens[:nd],
                                  num_q_heads=num_q_heads, num_kv_heads=num_kv_heads,

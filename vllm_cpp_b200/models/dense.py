@@ -27,6 +27,8 @@ ACT_KIND = {"silu": 0, "gelu_tanh": 1, "gelu_pytorch_tanh": 1, "gelu": 2}
 
 class DenseModel:
     DTYPES = ("bfloat16",)         # types the family's kernels run in (EngineArgs.dtype)
+    KV_CACHE_DTYPES = ("auto", "fp4")   # what its KV cache may be held in (EngineArgs.kv_cache_dtype)
+    kv_cache_dtype = "auto"
 
     def __init__(self, cfg: ModelConfig, device="cuda", parallel: ParallelConfig | None = None,
                  comm=None, max_position: int | None = None):
@@ -270,11 +272,36 @@ class DenseModel:
             groups.append((chunked, s))
         return groups
 
+    def set_kv_cache_dtype(self, name: str, block_size: int) -> None:
+        """Before the cache is sized and allocated. "fp4": the back end appends to and attends over the 4-bit cache by its type
+        (uint8); blocks run op by op, as the native layer entries write bf16."""
+        if name not in self.KV_CACHE_DTYPES:
+            raise ValueError(f"kv_cache_dtype {name!r} is none of {', '.join(self.KV_CACHE_DTYPES)}")
+        if name == "fp4":
+            if self.D not in (64, 128, 256) or block_size % 16:
+                raise ValueError(f"a 4-bit KV cache needs head_dim 64, 128 or 256 and a block_size in multiples of 16, not {self.D} and "
+                                 f"{block_size}")
+            self.native_layers = False
+            self.decode_workspace = self._fp4_workspace
+        self.kv_cache_dtype = name
+
+    def _fp4_workspace(self, batch: int, max_seq_len: int, block_size: int):
+        """(splits, scratch) of a decode batch as the runner keeps them: one scratch for all steps, which follow one another."""
+        if getattr(self, "_fp4_scratch", None) is None:
+            from ..ops import fp4_cache
+            self._fp4_scratch = fp4_cache.scratch(self.device, self.hq, self.hkv, self.D)
+        return 1, self._fp4_scratch
+
     def alloc_kv_cache(self, num_blocks: int, block_size: int):
         self.block_size = block_size
-        self.kv_caches = [torch.zeros((num_blocks, 2, block_size, self.hkv, self.D),
-                                      dtype=self.dtype, device=self.device)
-                          for _ in range(self.cfg.num_layers)]
+        if self.kv_cache_dtype == "fp4":
+            from ..ops import fp4_cache
+            self.kv_caches = [fp4_cache.alloc(num_blocks, self.hkv, block_size, self.D, self.device)
+                              for _ in range(self.cfg.num_layers)]
+        else:
+            self.kv_caches = [torch.zeros((num_blocks, 2, block_size, self.hkv, self.D),
+                                          dtype=self.dtype, device=self.device)
+                              for _ in range(self.cfg.num_layers)]
         self.layer_group = [0] * self.cfg.num_layers
         for gi, (layers, _) in enumerate(self.kv_cache_groups(block_size)):
             for l in layers:
@@ -282,6 +309,9 @@ class DenseModel:
         return self.kv_caches
 
     def kv_bytes_per_block(self, block_size: int) -> int:
+        if self.kv_cache_dtype == "fp4":
+            from ..ops import fp4_cache
+            return self.cfg.num_layers * fp4_cache.bytes_per_block(self.hkv, block_size, self.D)
         return self.cfg.num_layers * 2 * block_size * self.hkv * self.D * 2
 
     def weight_bytes(self) -> int:
@@ -496,6 +526,8 @@ class DenseModel:
         c = self.cfg
         if self.device.type != "cuda" or self.tp > 1 or type(self).forward is not DenseModel.forward:
             return False
+        if self.kv_cache_dtype != "auto":
+            return False
         if os.environ.get("B200_NATIVE_LAYERS", "1") == "0":      # debugging: keep the per-op path
             return False
         if (c.post_norm or c.sandwich_norm or c.attention_bias or c.mlp_bias or c.sliding_window
@@ -594,6 +626,8 @@ class DenseModel:
         """The fused tensor-parallel stack has a native entry for the plain pre-norm block with one
         KV-cache group (the same configurations as the one-GPU native entry)."""
         c = self.cfg
+        if self.kv_cache_dtype != "auto":
+            return False
         if os.environ.get("B200_NATIVE_LAYERS", "1") == "0" or type(self)._forward_tp_fused is not \
                 DenseModel._forward_tp_fused:
             return False

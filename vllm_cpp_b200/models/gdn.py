@@ -30,6 +30,8 @@ def _round_up(a, b):
 
 
 class Qwen35Model(DenseModel):
+    KV_CACHE_DTYPES = ("auto",)
+
     def __init__(self, cfg: ModelConfig, device="cuda", parallel: ParallelConfig | None = None,
                  comm=None, max_position: int | None = None):
         super().__init__(cfg, device, parallel, comm, max_position)

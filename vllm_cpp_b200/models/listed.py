@@ -34,6 +34,7 @@ def pad_heads(t: torch.Tensor, heads: int, padded: int, axis: int = 0) -> torch.
 
 class ListedModel(DenseModel):
     DTYPES = ("bfloat16", "float32")
+    KV_CACHE_DTYPES = ("auto",)
 
     def __init__(self, cfg: ModelConfig, device="cuda", parallel: ParallelConfig | None = None,
                  comm=None, max_position: int | None = None):

@@ -27,6 +27,8 @@ from .moe import MoeModel
 
 
 class DeepseekV2Model(MoeModel):
+    KV_CACHE_DTYPES = ("auto",)
+
     def __init__(self, cfg: ModelConfig, device="cuda", parallel: ParallelConfig | None = None,
                  comm=None, max_position: int | None = None):
         c = cfg

@@ -276,6 +276,8 @@ class MoeModel(DenseModel):
     def _native_attn_ok(self) -> bool:
         """The plain attention block on one GPU with bf16 projections, as the native entry takes it."""
         c = self.cfg
+        if self.kv_cache_dtype != "auto":
+            return False
         if self.device.type != "cuda" or self.tp > 1 or self.ep > 1 or os.environ.get("B200_NATIVE_LAYERS", "1") == "0":
             return False
         if (c.post_norm or c.sandwich_norm or c.attention_bias or c.sliding_window or c.attention_chunk_size or c.gemma_norm

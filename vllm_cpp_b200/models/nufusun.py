@@ -39,6 +39,7 @@ def _padded(t: torch.Tensor, *shape: int) -> torch.Tensor:
 
 class NufusunModel(DenseModel):
     DTYPES = ("bfloat16", "float32")
+    KV_CACHE_DTYPES = ("auto",)
 
     def __init__(self, cfg: ModelConfig, device="cuda", parallel: ParallelConfig | None = None,
                  comm=None, max_position: int | None = None):

@@ -17,6 +17,7 @@ from typing import Sequence
 import torch
 
 from .. import _engine as E
+from ..ops import fp4_cache
 
 lm = E.lmcache
 
@@ -37,7 +38,9 @@ class LMCacheStore:
     def __init__(self, url: str, model_name: str, kv_caches: Sequence[torch.Tensor], block_size: int,
                  chunk_size: int = 256, world_size: int = 1, worker_id: int = 0, connect: bool = True,
                  hash_algo: str = "blake3"):
-        """``kv_caches``: one ``[num_blocks, 2, block_size, Hkv, D]`` tensor per attention layer."""
+        """``kv_caches``: one ``[num_blocks, 2, block_size, Hkv, D]`` tensor per attention layer, or one 4-bit cache
+        (``ops/fp4_cache.py``): its keys and values travel as the bf16 values they stand for, under a model name of their own,
+        and come back to the same codes."""
         host, port = parse_url(url)
         self.client = lm.RemoteClient(host, port)
         if connect:
@@ -52,9 +55,15 @@ class LMCacheStore:
         self.kv_caches = list(kv_caches)
         self.block_size, self.chunk_size = block_size, chunk_size
         c = self.kv_caches[0]
-        self.hidden = c.shape[3] * c.shape[4]
-        self.dtype = _DTYPES[c.dtype]
-        self.elem = c.element_size()
+        self.fp4 = c.dtype == torch.uint8
+        if self.fp4:
+            _, h, _, d = fp4_cache.shape_of(c)
+            self.hidden, self.dtype, self.elem = h * d, _DTYPES[torch.bfloat16], 2
+            self.model_name = f"{model_name}+fp4kv"
+        else:
+            self.hidden = c.shape[3] * c.shape[4]
+            self.dtype = _DTYPES[c.dtype]
+            self.elem = c.element_size()
         self.stats = {"put_chunks": 0, "hit_chunks": 0, "miss_chunks": 0}
 
     # ------------------------------------------------------------------ keys
@@ -77,6 +86,11 @@ class LMCacheStore:
         slots = self._slots(block_ids, start, end)
         k_planes, v_planes = [], []
         for cache in self.kv_caches:
+            if self.fp4:
+                read = fp4_cache.read if cache.is_cuda else fp4_cache.ref_read
+                for x, planes in zip(read(cache, slots.to(cache.device)), (k_planes, v_planes)):
+                    planes.append(bytes(x.cpu().contiguous().view(torch.uint8).numpy().tobytes()))
+                continue
             nb, _, bs, h, d = cache.shape
             flat = cache.view(nb, 2, bs, h * d)
             idx = slots.to(cache.device)
@@ -89,6 +103,11 @@ class LMCacheStore:
     def _scatter(self, block_ids, start, end, k_planes, v_planes):
         slots = self._slots(block_ids, start, end)
         for cache, kb, vb in zip(self.kv_caches, k_planes, v_planes):
+            if self.fp4:
+                k, v = (torch.frombuffer(bytearray(b), dtype=torch.uint8).view(torch.bfloat16).view(end - start, self.hidden).to(cache.device)
+                        for b in (kb, vb))
+                (fp4_cache.write if cache.is_cuda else fp4_cache.ref_write)(k, v, cache, slots.to(cache.device))
+                continue
             nb, _, bs, h, d = cache.shape
             k = torch.frombuffer(bytearray(kb), dtype=torch.uint8).view(cache.dtype).view(end - start, h, d)
             v = torch.frombuffer(bytearray(vb), dtype=torch.uint8).view(cache.dtype).view(end - start, h, d)
