@@ -239,7 +239,8 @@ typedef struct B200Fp4Append {
 } B200Fp4Append;
 
 // Attention over that cache (fp4_attn.cu). q_start null: one query a sequence (decode), else [num_reqs + 1] and causal from the end of each sequence
-// (causal 0: every query sees every key). window as in b200_attn_decode. parts: b200_fp4_attn_scratch floats, for this call alone until it is done.
+// (causal 0: every query sees every key) and with its 128-token query tiles. window as in b200_attn_decode, scale > 0. parts: b200_fp4_attn_scratch
+// floats, for this call alone until it is done. At most 8192 sequences and 8000 tiles.
 typedef struct B200Fp4Attn {
   const void* q;
   void* out;
@@ -249,7 +250,7 @@ typedef struct B200Fp4Attn {
   const void* block_table;     // int32 [num_reqs][max_blocks], rows ldt apart
   const void* seq_lens;        // int32 [num_reqs]
   const void* q_start;
-  const void* tile_req;        // 128-token query tiles (q_start given)
+  const void* tile_req;
   const void* tile_q0;
   void* parts;
   int max_blocks, num_reqs, total_q, num_tiles;
@@ -517,7 +518,7 @@ int b200_outer_fits(const B200Outer* a);
 void b200_outer_workspace(int kind, int D, int* values);
 int b200_outer_chunk(const B200Outer* a, cudaStream_t stream);
 // ---- fp4_attn.cu
-long long b200_fp4_attn_scratch(int Hq, int Hkv, int D);
+long long b200_fp4_attn_scratch(int D, int prefill);
 int b200_fp4_attn(const B200Fp4Attn* a, cudaStream_t stream);
 // ---- fp4_cache.cu
 int b200_fp4_append(const B200Fp4Append* a, cudaStream_t stream);

@@ -1,4 +1,5 @@
-// Attention over the paged cache held in 4 bits (layout: fp4_cache.cuh), for few query rows a sequence: decode, and the verification of drafts.
+// Attention over the paged cache held in 4 bits (layout: fp4_cache.cuh), for few query rows a sequence: decode, and the verification of drafts. Also
+// the entry point for both kernels; sequences of many rows go to fp4_prefill.cu.
 //
 //   o[r] = sum_j p[r, j] v_j / sum_j p[r, j],   p[r, j] = 2^(scale log2(e) q_r . k_j - m),   m a running reference of the maximum
 //
@@ -9,46 +10,16 @@
 //                                    registers (movmatrix)
 // Q is f16 times a power of two per row (its largest magnitude between 1 and 2), which goes back into the softmax scale.
 //
-// Work is shared out evenly whatever the lengths: the cells of all (sequence, kv head, row tile) items stand in one line, each CTA takes an equal
-// stretch of it, and its warps the cells of a stretch in turn, fetched ahead by bulk copies into a ring of their own. An item that lies in one
-// stretch is finished there; of one that was cut the parts (m, l, O) go to scratch, and a second kernel joins them.
-#include <cuda_bf16.h>
-#include <cuda_fp16.h>
-
+// Work is shared out evenly whatever the lengths (fp4_work.cuh). The warps of a CTA take the cells of a piece in turn, fetched ahead by bulk copies
+// into a ring of their own. An item that lies in one stretch is finished there; of one that was cut the parts (m, l, O) go to scratch, and a second
+// kernel joins them.
 #include "api.h"
-#include "fp4_cache.cuh"
-#include "sm100.cuh"
+#include "fp4_work.cuh"
 
 namespace b200 {
 
-struct Fp4Rows {
-  const __nv_bfloat16* q;
-  long long ldq;
-  __nv_bfloat16* out;
-  long long ldo;
-  const uint8_t* cache;
-  long long num_blocks;
-  const int32_t* block_table;
-  int max_blocks;              // of a sequence
-  long long ldt;               // entries from one sequence's row of the table to the next
-  const int32_t* seq_lens;
-  const int32_t* q_start;      // null: one row a sequence
-  int num_reqs, total_q;
-  int Hkv, G, cells_per_page, window, causal, rows;   // rows: of a tile
-  float scale_log2, softcap2;
-  float* parts;                // [CTAs][2][rows * (D + 2)]
-  int* status;
-};
-
 static constexpr int kRowWarps = 8, kRowStages = 4;
-// p is at most 2^8 before its reference is raised; times 2^7 it is still an f16, and the smallest ones keep their bits.
-static constexpr float kUp = 7.f;
 
-__device__ __forceinline__ float ex2_of(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
 __device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
@@ -59,17 +30,6 @@ __device__ __forceinline__ uint32_t transposed(uint32_t a) {
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
   return d;
 }
-__device__ __forceinline__ uint32_t mul_f16x2(uint32_t a, uint32_t b) {
-  uint32_t d;
-  asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
-  return d;
-}
-// Scale bytes lo and hi (selectors of __byte_perm) of w -> f16x2.
-__device__ __forceinline__ uint32_t scales_f16x2(uint32_t w, int lo, int hi) { return __byte_perm(w, 0, 0x4040 | lo | hi << 8) << 7; }
-__device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
-  const __half2 h = __floats2half2_rn(lo, hi);
-  return *reinterpret_cast<const uint32_t*>(&h);
-}
 __device__ __forceinline__ uint32_t low_nibbles_else(uint32_t a, uint32_t b) {     // nibble 0, 2, .. of a, the others of b
   return (a & 0x0f0f0f0fu) | (b & 0xf0f0f0f0u);
 }
@@ -79,95 +39,6 @@ __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t b
                : "memory");
 }
 
-// What a sequence brings: keys [first key cell, first + cells) x items (kv heads x row tiles); positions of its rows are first_pos + token.
-struct Fp4Seq {
-  int len, q_begin, q_len, first_cell, cells, tiles;
-  __device__ __forceinline__ Fp4Seq(const Fp4Rows& p, int b) {
-    q_begin = p.q_start ? min(max(p.q_start[b], 0), p.total_q) : b;
-    q_len = p.q_start ? max(min(p.q_start[b + 1], p.total_q) - q_begin, 0) : 1;
-    len = min(max(p.seq_lens[b], 0), p.max_blocks * p.cells_per_page * kCellTokens);
-    first_cell = max(0, lowest(p, len - q_len)) / kCellTokens;
-    cells = max(1, (len + kCellTokens - 1) / kCellTokens - first_cell);          // (no keys: one cell that counts as masked)
-    tiles = (q_len * p.G + p.rows - 1) / p.rows;
-  }
-  // lowest position that the query at `pos` sees
-  static __device__ __forceinline__ int lowest(const Fp4Rows& p, int pos) {
-    return p.window > 0 ? pos - p.window + 1 : p.window < 0 && pos >= 0 ? pos / -p.window * -p.window : 0;
-  }
-};
-
-// line[b] = cells in the line in front of sequence b (num_reqs + 1 entries). All threads of the block take part.
-__device__ void fp4_line(const Fp4Rows& p, uint32_t* line) {
-  __shared__ uint32_t warp_sum[32];
-  const int per = (p.num_reqs + blockDim.x - 1) / blockDim.x, b0 = min((int)threadIdx.x * per, p.num_reqs), b1 = min(b0 + per, p.num_reqs);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
-  uint32_t sum = 0;
-  for (int b = b0; b < b1; ++b) {
-    const Fp4Seq s(p, b);
-    const uint32_t n = (uint32_t)s.cells * (uint32_t)(s.tiles * p.Hkv);
-    line[b + 1] = n;
-    sum += n;
-  }
-  uint32_t x = sum;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const uint32_t y = __shfl_up_sync(0xffffffffu, x, o);
-    if (lane >= o) x += y;
-  }
-  if (lane == 31) warp_sum[warp] = x;
-  __syncthreads();
-  uint32_t before = x - sum;
-  for (int w = 0; w < warps; ++w) before += w < warp ? warp_sum[w] : 0;
-  for (int b = b0; b < b1; ++b) {
-    before += line[b + 1];
-    line[b + 1] = before;
-  }
-  if (threadIdx.x == 0) line[0] = 0;
-  __syncthreads();
-}
-__device__ __forceinline__ int fp4_find(const uint32_t* line, int n, uint32_t u) {   // the sequence that cell u is of
-  int lo = 0, hi = n - 1;
-  while (lo < hi) {
-    const int mid = (lo + hi) >> 1;
-    if (line[mid + 1] > u) hi = mid;
-    else lo = mid + 1;
-  }
-  return lo;
-}
-// Stretches: CTA i of n has cells [total i / n, total (i + 1) / n). No more CTAs than give each warp a cell.
-__device__ __forceinline__ uint32_t fp4_ctas(uint32_t total, uint32_t grid) { return max(1u, min(grid, total / kRowWarps)); }
-__device__ __forceinline__ uint32_t fp4_begin(uint32_t total, uint32_t i, uint32_t n) { return (uint32_t)((uint64_t)total * i / n); }
-
-// A piece of an item: cells [c0, c1) of the item's n.
-struct Fp4Piece {
-  uint32_t u, u_end;           // in the line: where the piece begins, where the CTA's stretch ends
-  int b, item, c0, c1;
-  __device__ __forceinline__ void at(const Fp4Rows& p, const uint32_t* line, uint32_t from, uint32_t to) {
-    u = from;
-    u_end = to;
-    if (u >= u_end) return;
-    b = fp4_find(line, p.num_reqs, u);
-    const int n = Fp4Seq(p, b).cells;
-    const uint32_t local = u - line[b];
-    item = (int)(local / (uint32_t)n);
-    c0 = (int)(local - (uint32_t)item * n);
-    c1 = (int)min((uint32_t)n, c0 + (u_end - u));
-  }
-  __device__ __forceinline__ void next(const Fp4Rows& p, const uint32_t* line) {
-    u += c1 - c0;
-    if (u >= u_end) return;
-    ++item;
-    if (u == line[b + 1]) {
-      item = 0;
-      do ++b;
-      while (line[b + 1] == u);
-    }
-    c0 = 0;
-    c1 = (int)min((uint32_t)Fp4Seq(p, b).cells, u_end - u);
-  }
-  __device__ __forceinline__ bool more() const { return u < u_end; }
-};
-
 template <int D, int NT>
 struct Fp4RowsShape {
   static constexpr int kRows = 8 * NT, kMT = D / 16;
@@ -176,13 +47,13 @@ struct Fp4RowsShape {
   static constexpr int kRingBytes = kRowWarps * kRowStages * Fp4Cell<D>::kBytes;
   static constexpr int kMergeBytes = kRowWarps * kRows * kMergeRow * 4;
   static constexpr int kFixed = kRingBytes + kMergeBytes + kRowWarps * kRows * 8 + kRowWarps * kRowStages * 8;
-  static constexpr int kPart = kRows * (D + 2);                                      // floats of a part in scratch
 };
 
 template <int D, int NT>
-__global__ void __launch_bounds__(kRowWarps * 32, NT == 1 && D <= 128 ? 2 : 1) fp4_rows_kernel(Fp4Rows p) {
+__global__ void __launch_bounds__(kRowWarps * 32, NT == 1 && D <= 128 ? 2 : 1) fp4_rows_kernel(Fp4Attn p, float* parts) {
   using Cell = Fp4Cell<D>;
   using Shape = Fp4RowsShape<D, NT>;
+  using Seq = Fp4Seq<Shape::kRows>;
   constexpr int kRows = Shape::kRows, kMT = Shape::kMT, kKW = D / 32, kVW = D / 64;   // m-tiles, words of a lane's keys and values
   extern __shared__ __align__(128) uint8_t smem[];
   float* merge = reinterpret_cast<float*>(smem + Shape::kRingBytes);
@@ -197,13 +68,13 @@ __global__ void __launch_bounds__(kRowWarps * 32, NT == 1 && D <= 128 ? 2 : 1) f
   mbar_fence_init();
   pdl_wait();
   pdl_launch_dependents();
-  fp4_line(p, line);
-  const uint32_t total = line[p.num_reqs], ctas = fp4_ctas(total, gridDim.x);
+  fp4_line<Seq>(p, line);
+  const uint32_t total = line[p.num_reqs], ctas = fp4_ctas(total, gridDim.x, kRowWarps);
   if (blockIdx.x >= ctas) return;
-  const uint32_t from = fp4_begin(total, blockIdx.x, ctas), to = fp4_begin(total, blockIdx.x + 1, ctas);
+  const uint32_t from = fp4_begin<Seq>(p, line, total, blockIdx.x, ctas), to = fp4_begin<Seq>(p, line, total, blockIdx.x + 1, ctas);
 
   // ---- fetching ahead: the warp's cells in their order, kRowStages of them in flight
-  Fp4Piece f;
+  Fp4Piece<Seq> f;
   f.at(p, line, from, to);
   int fc = f.c0 + warp, fj = 32, page = 0;      // next cell; page ids of the next 32 cells, a lane each
   uint32_t bad = 0, phase = 0, flying = 0;      // of each stage: nothing was fetched (no such page); parity of its barrier; not waited for yet
@@ -214,10 +85,9 @@ __global__ void __launch_bounds__(kRowWarps * 32, NT == 1 && D <= 128 ? 2 : 1) f
       fj = 32;
     }
     if (!f.more()) return;
-    const Fp4Seq s(p, f.b);
     if (fj == 32) {
-      const int c = fc + lane * kRowWarps, pg = (s.first_cell + c) / p.cells_per_page;
-      page = c < f.c1 && pg < p.max_blocks && s.len > 0 ? p.block_table[f.b * p.ldt + pg] : -1;
+      const int c = fc + lane * kRowWarps, pg = (f.e.begin + c) / p.cells_per_page;
+      page = c < f.c1 && pg < p.max_blocks && f.e.len > 0 ? p.block_table[f.b * p.ldt + pg] : -1;
       fj = 0;
     }
     const int id = __shfl_sync(0xffffffffu, page, fj);
@@ -225,7 +95,7 @@ __global__ void __launch_bounds__(kRowWarps * 32, NT == 1 && D <= 128 ? 2 : 1) f
     bad = there ? bad & ~(1u << st) : bad | 1u << st;
     flying |= there ? 1u << st : 0;
     if (there && lane == 0) {
-      const int h = f.item / s.tiles, cell = (s.first_cell + fc) % p.cells_per_page;
+      const int h = f.item / f.e.tiles, cell = (f.e.begin + fc) % p.cells_per_page;
       mbar_expect_tx(&full[st], Cell::kBytes);
       bulk_load(ring + st * Cell::kBytes, p.cache + (((long long)id * p.Hkv + h) * p.cells_per_page + cell) * Cell::kBytes, Cell::kBytes, &full[st]);
     }
@@ -238,11 +108,10 @@ __global__ void __launch_bounds__(kRowWarps * 32, NT == 1 && D <= 128 ? 2 : 1) f
   int st = 0;
   bool ok = true;
 
-  Fp4Piece w;
+  Fp4Piece<Seq> w;
   for (w.at(p, line, from, to); w.more(); w.next(p, line)) {
-    const Fp4Seq s(p, w.b);
-    const int h = w.item / s.tiles, r0 = (w.item - h * s.tiles) * kRows, nrows = min(kRows, s.q_len * p.G - r0);
-    const int first = s.len - s.q_len;                                           // position of the sequence's first query
+    const Seq& s = w.e;
+    const int h = w.item / s.tiles, r0 = (w.item - h * s.tiles) * kRows, nrows = min(kRows, s.rows - r0), first = s.first;
     // ---- the tile's queries: B operand, lane (g, t) has dims [t D / 4, + D / 4) of row g
     uint32_t bq[NT][D / 16][2];
     float mul[NT][2];                                                            // of the lane's rows 2t, 2t + 1: scores to log2 units
@@ -251,7 +120,7 @@ __global__ void __launch_bounds__(kRowWarps * 32, NT == 1 && D <= 128 ? 2 : 1) f
     for (int nt = 0; nt < NT; ++nt) {
       const int r = r0 + nt * 8 + g, token = r / p.G, head = r - token * p.G;
       const bool row = nt * 8 + g < nrows;
-      const __nv_bfloat16* src = p.q + (long long)(s.q_begin + token) * p.ldq + (long long)(h * p.G + head) * D + t * (D / 4);
+      const __nv_bfloat16* src = p.q + (long long)(s.token0 + token) * p.ldq + (long long)(h * p.G + head) * D + t * (D / 4);
       float big = 0.f;
       uint4 raw[D / 32];
 #pragma unroll
@@ -282,12 +151,12 @@ __global__ void __launch_bounds__(kRowWarps * 32, NT == 1 && D <= 128 ? 2 : 1) f
         mul[nt][e] = __shfl_sync(0xffffffffu, up, (2 * t + e) * 4) * p.scale_log2;
         const int rr = min(nt * 8 + 2 * t + e, nrows - 1) + r0, pos = first + rr / p.G;
         hi[nt][e] = p.causal ? pos : s.len - 1;
-        lo[nt][e] = Fp4Seq::lowest(p, pos);
+        lo[nt][e] = fp4_lowest(p, pos);
       }
     }
     const int tok0 = r0 / p.G, tok1 = (r0 + nrows - 1) / p.G;                    // the tile's tokens
     const int least_hi = p.causal ? first + tok0 : s.len - 1, most_hi = p.causal ? first + tok1 : s.len - 1;
-    const int most_lo = Fp4Seq::lowest(p, first + tok1), least_lo = Fp4Seq::lowest(p, first + tok0);
+    const int most_lo = fp4_lowest(p, first + tok1), least_lo = fp4_lowest(p, first + tok0);
 
     float o[NT][kMT][4], m[NT][2], l[NT][2];
 #pragma unroll
@@ -300,7 +169,7 @@ __global__ void __launch_bounds__(kRowWarps * 32, NT == 1 && D <= 128 ? 2 : 1) f
       l[nt][0] = l[nt][1] = 0.f;
     }
     for (int c = w.c0 + warp; c < w.c1; c += kRowWarps) {
-      const int key0 = (s.first_cell + c) * kCellTokens;
+      const int key0 = (s.begin + c) * kCellTokens;
       const bool there = !(bad >> st & 1);
       if (there) {
         if (ok) ok = __all_sync(0xffffffffu, mbar_wait(&full[st], phase >> st & 1, p.status));
@@ -461,8 +330,8 @@ __global__ void __launch_bounds__(kRowWarps * 32, NT == 1 && D <= 128 ? 2 : 1) f
         for (int i = 0; i < kRowWarps; ++i) x = fmaxf(x, top[i * kRows + nt * 8 + 2 * t + e]);
         scale[nt][e] = m[nt][e] == -INFINITY ? 0.f : ex2_of(m[nt][e] - x);
       }
-    const bool whole = w.c0 == 0 && w.c1 == s.cells;
-    float* part = p.parts + ((size_t)blockIdx.x * 2 + (w.c0 == 0)) * Shape::kPart;
+    const bool whole = w.whole();
+    float* part = parts + fp4_part<Seq, D>(blockIdx.x, w.part());
     constexpr int kMC = Shape::kMergeTiles, kMR = Shape::kMergeRow;
 #pragma unroll
     for (int i0 = 0; i0 < kMT; i0 += kMC) {
@@ -492,7 +361,7 @@ __global__ void __launch_bounds__(kRowWarps * 32, NT == 1 && D <= 128 ? 2 : 1) f
         if (whole) {
           const int token = (r0 + r) / p.G, head = r0 + r - token * p.G;
           const float inv = sum == 0.f ? 0.f : 1.f / sum;
-          *reinterpret_cast<uint32_t*>(p.out + (long long)(s.q_begin + token) * p.ldo + (long long)(h * p.G + head) * D + d) =
+          *reinterpret_cast<uint32_t*>(p.out + (long long)(s.token0 + token) * p.ldo + (long long)(h * p.G + head) * D + d) =
               pack_bf16x2(a * inv, b * inv);
         } else {
           *reinterpret_cast<float2*>(part + r * D + d) = make_float2(a, b);
@@ -510,103 +379,86 @@ __global__ void __launch_bounds__(kRowWarps * 32, NT == 1 && D <= 128 ? 2 : 1) f
     if (flying >> i & 1) mbar_wait(&full[i], phase >> i & 1, p.status);
 }
 
-// Joins the parts of items that the ends of stretches cut. Block i looks at the line where stretch i + 1 begins; the first cut of an item is the
-// one that joins it: part 1 of the CTA that begins it, part 0 of those behind.
-template <int D, int NT>
-__global__ void __launch_bounds__(256) fp4_join_kernel(Fp4Rows p, int grid) {
-  using Shape = Fp4RowsShape<D, NT>;
-  constexpr int kRows = Shape::kRows;
+// Parts of the row kernel's items, then those of the tile kernel's, each by a block of its own.
+template <int D, int ROWS>
+__global__ void __launch_bounds__(256) fp4_join_kernel(Fp4Attn p, const float* row_parts, int row_grid, const float* tile_parts, int tile_grid) {
   extern __shared__ uint32_t line[];
   pdl_wait();
   pdl_launch_dependents();
-  fp4_line(p, line);
-  const uint32_t total = line[p.num_reqs], ctas = fp4_ctas(total, grid), i = blockIdx.x;
-  if (i + 1 >= ctas) return;
-  const uint32_t u = fp4_begin(total, i + 1, ctas);
-  const int b = fp4_find(line, p.num_reqs, u);
-  const Fp4Seq s(p, b);
-  const uint32_t local = u - line[b], item = local / (uint32_t)s.cells, begin = line[b] + item * s.cells;
-  if (begin == u || fp4_begin(total, i, ctas) > begin) return;
-  const uint32_t last = (uint32_t)(((uint64_t)(begin + s.cells) * ctas - 1) / total);         // the CTA that has the item's last cell
-  const int h = item / s.tiles, r0 = (int)(item - h * s.tiles) * kRows, nrows = min(kRows, s.q_len * p.G - r0);
-  for (int x = threadIdx.x; x < nrows * (D / 4); x += 256) {
-    const int r = x / (D / 4), d = x % (D / 4) * 4;
-    float mx = -INFINITY;
-    for (uint32_t c = i; c <= last; ++c) mx = fmaxf(mx, p.parts[((size_t)c * 2 + (c == i)) * Shape::kPart + kRows * D + 2 * r]);
-    float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-    float sum = 0.f;
-#pragma unroll 4
-    for (uint32_t c = i; c <= last; ++c) {
-      const float* part = p.parts + ((size_t)c * 2 + (c == i)) * Shape::kPart;
-      const float2 ml = *reinterpret_cast<const float2*>(part + kRows * D + 2 * r);
-      const float4 v = *reinterpret_cast<const float4*>(part + r * D + d);
-      const float f = ml.x == -INFINITY ? 0.f : ex2_of(ml.x - mx);
-      sum += ml.y * f;
-      a.x += v.x * f; a.y += v.y * f; a.z += v.z * f; a.w += v.w * f;
-    }
-    const float inv = sum == 0.f ? 0.f : 1.f / sum;
-    const int token = (r0 + r) / p.G, head = r0 + r - token * p.G;
-    *reinterpret_cast<uint2*>(p.out + (long long)(s.q_begin + token) * p.ldo + (long long)(h * p.G + head) * D + d) =
-        make_uint2(pack_bf16x2(a.x * inv, a.y * inv), pack_bf16x2(a.z * inv, a.w * inv));
-  }
+  if ((int)blockIdx.x < row_grid)
+    fp4_join<Fp4Seq<ROWS>, D>(p, row_parts, line, blockIdx.x, row_grid, kRowWarps);
+  else if constexpr (D <= 128)
+    fp4_join<Fp4Tile, D>(p, tile_parts, line, blockIdx.x - row_grid, tile_grid, kTileLeast);
 }
 
-static constexpr int kMostReqs = 8192;         // (the line of a step is in shared memory)
+static constexpr int kMostReqs = 8192, kMostTiles = 8000;         // (the line of a step is in shared memory)
 
 template <int D, int NT>
-static int launch_rows(Fp4Rows p, int grid, cudaStream_t stream) {
+static int launch_attn(const Fp4Attn& p, bool rows, bool tiles, float* parts, cudaStream_t stream) {
   using Shape = Fp4RowsShape<D, NT>;
-  p.rows = Shape::kRows;
-  const size_t smem = Shape::kFixed + (size_t)(p.num_reqs + 1) * 4;
-  static PerDeviceOnce once;
-  if (once.first()) {
-    cudaFuncSetAttribute(fp4_rows_kernel<D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape::kFixed + (kMostReqs + 1) * 4);
+  using Seq = Fp4Seq<Shape::kRows>;
+  const int row_grid = rows ? b200_num_sms() * (NT == 1 && D <= 128 ? 2 : 1) : 0, tile_grid = tiles ? fp4_tile_grid() : 0;
+  float* tile_parts = parts + (size_t)row_grid * 2 * Seq::kRows * (D + 2);
+  if (rows) {
+    static PerDeviceOnce once;
+    if (once.first())
+      cudaFuncSetAttribute(fp4_rows_kernel<D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape::kFixed + (kMostReqs + 1) * 4);
+    if (launch_pdl(fp4_rows_kernel<D, NT>, dim3(row_grid), dim3(kRowWarps * 32), Shape::kFixed + (size_t)(p.num_reqs + 1) * 4, stream, p, parts) !=
+        cudaSuccess)
+      return -2;
   }
-  if (launch_pdl(fp4_rows_kernel<D, NT>, dim3(grid), dim3(kRowWarps * 32), smem, stream, p) != cudaSuccess) return -2;
-  return launch_pdl(fp4_join_kernel<D, NT>, dim3(grid), dim3(256), (size_t)(p.num_reqs + 1) * 4, stream, p, grid) == cudaSuccess ? 0 : -2;
+  if (tiles)
+    if (const int rc = launch_fp4_tiles(p, D, tile_parts, stream)) return rc;
+  const size_t line = (size_t)((rows ? p.num_reqs : 0) > (tiles ? p.num_tiles : 0) ? p.num_reqs : tiles ? p.num_tiles : 0) * 4 + 4;
+  return launch_pdl(fp4_join_kernel<D, Shape::kRows>, dim3(row_grid + tile_grid), dim3(256), line, stream, p, (const float*)parts, row_grid,
+                    (const float*)tile_parts, tile_grid) == cudaSuccess ? 0 : -2;
 }
 
 }  // namespace b200
 
 using namespace b200;
 
-static int fp4_tile_rows(int G, int D) { return G > 8 && D <= 128 ? 16 : 8; }
-static int fp4_grid(int rows, int D) { return b200_num_sms() * (rows == 8 && D <= 128 ? 2 : 1); }
-
 // Floats of scratch that b200_fp4_attn needs (B200Fp4Attn.parts).
-extern "C" long long b200_fp4_attn_scratch(int Hq, int Hkv, int D) {
-  if (Hkv <= 0 || Hq % Hkv) return -1;
-  const int rows = 16;
-  return (long long)b200_num_sms() * 2 * 2 * rows * (D + 2);
+extern "C" long long b200_fp4_attn_scratch(int D, int prefill) {
+  const long long sms = b200_num_sms();
+  return (sms * 2 * 16 * 2 + (prefill && D <= 128 ? (long long)fp4_tile_grid() * 2 * Fp4Tile::kRows : 0)) * (D + 2);
 }
 
 extern "C" int b200_fp4_attn(const B200Fp4Attn* a, cudaStream_t stream) {
   if (a->num_reqs <= 0 || a->total_q <= 0) return 0;
   if ((a->D != 64 && a->D != 128 && a->D != 256) || a->Hkv <= 0 || a->Hq <= 0 || a->Hq % a->Hkv || a->block_size <= 0 ||
-      a->block_size % kCellTokens || a->num_blocks <= 0 || a->max_blocks <= 0)
+      a->block_size % kCellTokens || a->num_blocks <= 0 || a->max_blocks <= 0 || !(a->scale > 0.f))
     return -1;
-  const uintptr_t bits = (uintptr_t)a->q | (uintptr_t)a->out | (uintptr_t)a->cache | (uintptr_t)((a->ldq | a->ldo) * 2);
-  if ((bits & 15) || !a->q || !a->out || !a->cache || !a->block_table || !a->seq_lens || !a->parts) return -1;
-  if (a->num_reqs > kMostReqs) return -4;
+  const uintptr_t bits = (uintptr_t)a->q | (uintptr_t)a->out | (uintptr_t)a->cache | (uintptr_t)a->parts | (uintptr_t)((a->ldq | a->ldo) * 2);
+  if ((bits & 15) || !a->q || !a->out || !a->cache || !a->block_table || !a->seq_lens || !a->parts || (a->q_start && (!a->tile_req || !a->tile_q0)))
+    return -1;
+  if (a->num_reqs > kMostReqs || a->num_tiles > kMostTiles) return -4;
   const int G = a->Hq / a->Hkv;
   // cells of the whole line in 31 bits, whatever the lengths
   if ((double)a->max_blocks * (a->block_size / kCellTokens) * a->Hkv * ((double)a->total_q * G / 8 + a->num_reqs) > 2147483647.0) return -4;
   if ((double)a->max_blocks * a->block_size > 2147483647.0) return -4;
-  Fp4Rows p;
+  Fp4Attn p;
   p.q = (const __nv_bfloat16*)a->q; p.ldq = a->ldq;
   p.out = (__nv_bfloat16*)a->out; p.ldo = a->ldo;
   p.cache = (const uint8_t*)a->cache; p.num_blocks = a->num_blocks;
   p.block_table = (const int32_t*)a->block_table; p.max_blocks = a->max_blocks; p.ldt = a->ldt;
   p.seq_lens = (const int32_t*)a->seq_lens; p.q_start = (const int32_t*)a->q_start;
-  p.num_reqs = a->num_reqs; p.total_q = a->total_q;
+  p.tile_req = (const int32_t*)a->tile_req; p.tile_q0 = (const int32_t*)a->tile_q0;
+  p.num_reqs = a->num_reqs; p.total_q = a->total_q; p.num_tiles = a->q_start ? a->num_tiles : 0;
   p.Hkv = a->Hkv; p.G = G; p.cells_per_page = a->block_size / kCellTokens;
   p.window = a->window; p.causal = a->causal;
   p.scale_log2 = a->scale * 1.4426950408889634f;
   p.softcap2 = a->softcap * 1.4426950408889634f;
-  p.parts = (float*)a->parts;
   p.status = device_status_word();
-  const int rows = a->q_start && a->D <= 128 ? 16 : fp4_tile_rows(G, a->D), grid = fp4_grid(rows, a->D);
-  if (a->D == 64) return rows == 8 ? launch_rows<64, 1>(p, grid, stream) : launch_rows<64, 2>(p, grid, stream);
-  if (a->D == 128) return rows == 8 ? launch_rows<128, 1>(p, grid, stream) : launch_rows<128, 2>(p, grid, stream);
-  return launch_rows<256, 1>(p, grid, stream);
+  // Which sequences go to which kernel. Both are launched where the lengths, which only the device knows, may call for both.
+  static constexpr int kFew = 64;
+  const bool tensor = a->D <= 128 && a->q_start && p.num_tiles > 0, long_one = tensor && (long long)a->total_q * G > kFew;
+  bool rows = true, tiles = long_one;
+  p.few = long_one ? kFew : 0x7fffffff;
+  if (long_one && a->num_reqs == 1) { rows = false; p.few = -1; }
+  float* parts = (float*)a->parts;
+  const bool two = a->D <= 128 && (a->q_start ? G > 4 || a->total_q > a->num_reqs : G > 8);      // row tiles of 16
+  if (a->D == 64) return two ? launch_attn<64, 2>(p, rows, tiles, parts, stream) : launch_attn<64, 1>(p, rows, tiles, parts, stream);
+  if (a->D == 128) return two ? launch_attn<128, 2>(p, rows, tiles, parts, stream) : launch_attn<128, 1>(p, rows, tiles, parts, stream);
+  return launch_attn<256, 1>(p, rows, tiles, parts, stream);
 }

@@ -1,0 +1,491 @@
+// Attention over the paged cache held in 4 bits, for many query rows a sequence (prompts and portions of prompts), on tcgen05 / tensor memory.
+//
+// A CTA works on 256 rows (query tokens x heads of a group: neighbouring rows share their keys, whatever the group) as two halves of 128 over tiles
+// of 128 keys:
+//   S(t) = Q(t) K^T,   P(t) = 2^(S - m + 7),   O(t) += P(t) V
+// Keys and values are expanded to f16 on the way to shared memory, by four warps that read codes and scales straight from the cache's cells and
+// write the 128-byte swizzled tiles that the matrix instructions take (keys with dims contiguous, values the same: their operand is MN-major). A tile
+// is expanded once for 256 rows. Q is f16 times a power of two per row, which goes back into the softmax scale. While the softmax of one half
+// runs, the tensor pipe works on the other, in the order of issue of the bf16 kernel for two heads (attn_prefill.cu):
+//   P(t, j) written and V(j) there   ->  O(t) += P(t, j) V(j), then, with K(j+1) there, S(t) = Q(t) K(j+1)^T
+// P goes back to tensor memory over its scores. The work of a call is shared out evenly among one CTA an SM (fp4_work.cuh): long and short
+// prompts, early and late tiles of a causal prompt, a portion of few tokens after a long context.
+//
+// Tensor memory (512 columns): S0 | S1 | O0 | O1; P(t) is the first 64 columns of S(t).
+// Warps (512 threads): 0 issues MMAs and holds tensor memory; 4..7 and 8..11 softmax and output of half 0 and 1, a thread a row; 12..15 expand, a
+// thread a key. Registers move from the first and the last warpgroup to the two of the softmax.
+#include "api.h"
+#include "fp4_work.cuh"
+
+namespace b200 {
+
+static constexpr int kFRing = 4;
+static constexpr int kRegsIssue = 40, kRegsSoftmax = 184, kRegsExpand = 96;
+
+__host__ __device__ constexpr uint32_t umma_idesc_f16(int m, int n, int b_mn) {
+  return (1u << 4) | ((uint32_t)b_mn << 16) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
+}
+template <int N>
+__device__ __forceinline__ void regs_inc() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N>
+__device__ __forceinline__ void regs_dec() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
+
+template <int D>
+struct Fp4TileShape {
+  static constexpr int kHalves = D / 64;                    // 64-dim halves of an operand tile
+  static constexpr int kPlane = 128 * 128;                  // 128 rows of 64 dims
+  static constexpr int kSlot = kHalves * kPlane;
+  static constexpr int kLine = (2 + kFRing) * kSlot;        // Q of both halves, the ring, then the line
+};
+
+struct alignas(8) Fp4TileBars {
+  uint64_t q_full[2], kv_full[kFRing], kv_empty[kFRing], s_full[2], p_first[2], p_full[2], pv_done[2];
+  uint32_t tmem_base;
+};
+
+// What a piece has for its two halves: `rows` of the tile's 256 exist, key tiles [c0, c1) of the item are seen by any of them.
+struct Fp4TilePiece {
+  int h, r0, rows, halves, k0, n, first;       // k0: first key of the piece's first tile, n: tiles
+  __device__ __forceinline__ Fp4TilePiece(const Fp4Attn& p, const Fp4Piece<Fp4Tile>& w) {
+    const Fp4Tile& e = w.e;
+    h = w.item / e.tiles;
+    r0 = (w.item - h * e.tiles) * Fp4Tile::kRows;
+    rows = min(Fp4Tile::kRows, e.rows - r0);
+    halves = rows > 128 ? 2 : 1;
+    first = e.first;
+    const int low = max(0, fp4_lowest(p, first + r0 / p.G)), high = min(p.causal ? first + (r0 + rows - 1) / p.G : e.len - 1, e.len - 1);
+    const int t0 = max(e.begin + w.c0, low / kTileKeys), t1 = min(e.begin + w.c1, high < 0 ? 0 : high / kTileKeys + 1);
+    k0 = t0 * kTileKeys;
+    n = max(0, t1 - t0);
+  }
+};
+
+template <int D>
+__global__ void __launch_bounds__(512, 1) fp4_tiles_kernel(Fp4Attn p, float* parts) {
+  using Cell = Fp4Cell<D>;
+  using Shape = Fp4TileShape<D>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  __shared__ Fp4TileBars bars;
+  __shared__ uint32_t no_page[4][4];                            // key tiles in turn: keys of a warp of expanders that have no page
+  __shared__ Fp4Piece<Fp4Tile> held[16];                        // each warp's piece, out of the registers of its loop over tiles
+  uint8_t* sQ = smem;
+  uint8_t* ring = smem + 2 * Shape::kSlot;
+  uint32_t* line = reinterpret_cast<uint32_t*>(smem + Shape::kLine);
+  const int warp = warp_index(), lane = threadIdx.x & 31, group = warp >> 2;
+  if (threadIdx.x == 0) {
+    for (int t = 0; t < 2; ++t) {
+      mbar_init(&bars.q_full[t], 4);
+      mbar_init(&bars.s_full[t], 1);
+      mbar_init(&bars.p_first[t], 4);
+      mbar_init(&bars.p_full[t], 4);
+      mbar_init(&bars.pv_done[t], 1);
+    }
+    for (int i = 0; i < kFRing; ++i) {
+      mbar_init(&bars.kv_full[i], 4);
+      mbar_init(&bars.kv_empty[i], 1);
+    }
+    mbar_fence_init();
+  }
+  if (warp == 0) {
+    tmem_alloc(&bars.tmem_base, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  tc_fence_after_sync();
+  const uint32_t tmem = bars.tmem_base;
+  pdl_wait();
+  pdl_launch_dependents();
+  fp4_line<Fp4Tile>(p, line);
+  const uint32_t total = line[p.num_tiles], ctas = fp4_ctas(total, gridDim.x, kTileLeast);
+  const bool mine = blockIdx.x < ctas;
+  const uint32_t from = mine ? fp4_begin<Fp4Tile>(p, line, total, blockIdx.x, ctas) : 0;
+  const uint32_t to = mine ? fp4_begin<Fp4Tile>(p, line, total, blockIdx.x + 1, ctas) : 0;
+  Fp4Piece<Fp4Tile>& w = held[warp];
+  const auto begin = [&] {
+    Fp4Piece<Fp4Tile> x;
+    x.at(p, line, from, to);
+    if (lane == 0) w = x;
+    __syncwarp();
+  };
+  const auto next = [&] {
+    Fp4Piece<Fp4Tile> x = w;
+    x.next(p, line);
+    __syncwarp();
+    if (lane == 0) w = x;
+    __syncwarp();
+  };
+
+  if (group == 0) {
+    regs_dec<kRegsIssue>();
+    if (warp == 0) {
+      constexpr uint32_t idesc_qk = umma_idesc_f16(128, kTileKeys, 0), idesc_pv = umma_idesc_f16(128, D, 1);
+      const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0), q_addr = smem_u32(sQ), ring_addr = smem_u32(ring);
+      uint32_t sq = 0, pieces[2] = {0, 0}, count[2] = {0, 0};    // ring items, pieces and tiles of each half so far
+      bool ok = true;
+      for (begin(); w.more() && ok; next()) {
+        const Fp4TilePiece x(p, w);
+        const int n = x.n, halves = x.halves;
+        if (n == 0) continue;
+        const auto qk = [&](int t, uint32_t slot, bool last) {      // S(t) = Q(t) K^T
+          if (elect_one()) {
+#pragma unroll
+            for (int kk = 0; kk < D / 16; ++kk)
+              umma_bf16_ss(tm + t * 128, umma_desc_k_sw128(q_addr + t * Shape::kSlot + (kk / 4) * Shape::kPlane + (kk % 4) * 32, 1024),
+                           umma_desc_k_sw128(ring_addr + slot * Shape::kSlot + (kk / 4) * Shape::kPlane + (kk % 4) * 32, 1024), idesc_qk, kk != 0);
+            umma_commit(&bars.s_full[t]);
+            if (last) umma_commit(&bars.kv_empty[slot]);
+          }
+          __syncwarp();
+        };
+        const auto wait_kv = [&](uint32_t i) { return mbar_wait_warp(&bars.kv_full[i % kFRing], (i / kFRing) & 1, p.status); };
+        if (!(ok = wait_kv(sq))) break;
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          if (t >= halves || !ok) continue;
+          if (!(ok = mbar_wait_warp(&bars.q_full[t], pieces[t] & 1, p.status))) continue;
+          ++pieces[t];
+          tc_fence_after_sync();
+          qk(t, sq % kFRing, t == halves - 1);
+        }
+        for (int j = 0; j < n && ok; ++j) {
+          const uint32_t iv = sq + 2 * j + 1, ik = iv + 1, slot = iv % kFRing;
+          const uint64_t vd = umma_desc_mn_sw128(ring_addr + slot * Shape::kSlot, Shape::kPlane, 1024);
+          if (!(ok = wait_kv(iv))) break;
+#pragma unroll
+          for (int t = 0; t < 2; ++t) {
+            if (t >= halves || !ok) continue;
+            const uint32_t phase = count[t] & 1;
+            ++count[t];
+            if (!(ok = mbar_wait_warp(&bars.p_first[t], phase, p.status))) continue;
+            tc_fence_after_sync();
+            if (elect_one()) {
+#pragma unroll
+              for (int kk = 0; kk < kTileKeys / 32; ++kk)
+                umma_bf16_ts(tm + 256 + t * 128, tm + t * 128 + kk * 8, vd + kk * (2048 >> 4), idesc_pv, (j | kk) != 0);
+            }
+            __syncwarp();
+            if (!(ok = mbar_wait_warp(&bars.p_full[t], phase, p.status))) continue;
+            tc_fence_after_sync();
+            if (elect_one()) {
+#pragma unroll
+              for (int kk = kTileKeys / 32; kk < kTileKeys / 16; ++kk)
+                umma_bf16_ts(tm + 256 + t * 128, tm + t * 128 + kk * 8, vd + kk * (2048 >> 4), idesc_pv, 1);
+              if (t == halves - 1) umma_commit(&bars.kv_empty[slot]);
+              if (j == n - 1) umma_commit(&bars.pv_done[t]);
+            }
+            __syncwarp();
+            if (j + 1 < n) {
+              if (t == 0) {
+                if (!(ok = wait_kv(ik))) continue;
+                tc_fence_after_sync();
+              }
+              qk(t, ik % kFRing, t == halves - 1);
+            }
+          }
+        }
+        sq += 2 * n;
+      }
+    }
+  } else if (group == 3) {
+    // ---------------- expanders: thread r has key r of a tile ----------------
+    regs_dec<kRegsExpand>();
+    const int r = threadIdx.x & 127, token = r % kCellTokens;
+    const long long head_bytes = (long long)p.cells_per_page * Cell::kBytes;
+    uint32_t sq = 0, tiles = 0;
+    bool ok = true;
+    for (begin(); w.more() && ok; next()) {
+      const Fp4TilePiece x(p, w);
+      if (x.n == 0) continue;
+      const int32_t* table = p.block_table + w.e.req * p.ldt;
+      const int low = max(0, fp4_lowest(p, x.first + x.r0 / p.G));
+      const auto page_of = [&](int j) {                          // -1: none; -2: not a key that any row sees
+        const int pos = x.k0 + j * kTileKeys + r;
+        return pos >= low && pos < w.e.len ? max(-1, table[pos / (p.cells_per_page * kCellTokens)]) : -2;
+      };
+      const auto cell_of = [&](int j, int page) -> const uint8_t* {
+        const int cell = (x.k0 + j * kTileKeys + r) / kCellTokens % p.cells_per_page;
+        return page >= 0 && page < p.num_blocks ? p.cache + ((long long)page * p.Hkv + x.h) * head_bytes + (long long)cell * Cell::kBytes : nullptr;
+      };
+      uint4 code[D / 32];
+      uint32_t scale[D / 64];
+      const auto load = [&](const uint8_t* cell, int kv) {
+#pragma unroll
+        for (int i = 0; i < D / 32; ++i) code[i] = make_uint4(0, 0, 0, 0);
+#pragma unroll
+        for (int i = 0; i < D / 64; ++i) scale[i] = 0;
+        if (!cell) return;
+#pragma unroll
+        for (int i = 0; i < D / 32; ++i)
+          code[i] = *reinterpret_cast<const uint4*>(cell + (kv ? Cell::value_at(token, i * 16) : token * Cell::kRow + i * 16));
+        if (kv) {
+#pragma unroll
+          for (int i = 0; i < D / 16; ++i) scale[i / 4] |= (uint32_t)cell[Cell::kValueScales + i * kCellTokens + token] << (i % 4 * 8);
+        } else {
+#pragma unroll
+          for (int i = 0; i < D / 64; ++i) scale[i] = reinterpret_cast<const uint32_t*>(cell + Cell::kKeyScales + token * Cell::kScales)[i];
+        }
+      };
+      int page = page_of(0);
+      const uint8_t* cell = cell_of(0, page);
+      load(cell, 0);
+      for (int i = 0; i < 2 * x.n; ++i, ++sq) {
+        const int j = i >> 1, kv = i & 1;
+        const uint32_t slot = sq % kFRing;
+        const bool none = page != -2 && cell == nullptr;
+        uint4 c[D / 32];
+        uint32_t s[D / 64];
+#pragma unroll
+        for (int k = 0; k < D / 32; ++k) c[k] = code[k];
+#pragma unroll
+        for (int k = 0; k < D / 64; ++k) s[k] = scale[k];
+        // the next item's loads, and in front of a key tile's the page
+        if (kv == 0) {
+          load(cell, 1);
+          if (j + 1 < x.n) page = page_of(j + 1);
+        } else if (j + 1 < x.n) {
+          cell = cell_of(j + 1, page);
+          load(cell, 0);
+        }
+        if (!(ok = __all_sync(0xffffffffu, mbar_wait(&bars.kv_empty[slot], ((sq / kFRing) & 1) ^ 1, p.status)))) break;
+        if (kv == 0) {
+          const uint32_t mask = __ballot_sync(0xffffffffu, none);
+          if (lane == 0) no_page[tiles % 4][warp & 3] = mask;
+          ++tiles;
+        }
+        uint8_t* row = ring + slot * Shape::kSlot + r * 128;
+#pragma unroll
+        for (int k = 0; k < D / 32; ++k) {
+          const uint32_t word[4] = {c[k].x, c[k].y, c[k].z, c[k].w};
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int g = 2 * k + (e >> 1), piece = 4 * k + e;                   // scale, 16 bytes of the row
+            const uint32_t sc = scales_f16x2(s[g / 4], g % 4, g % 4);
+            uint32_t v[4];
+            cvt_e2m1x8(word[e], v);
+            *reinterpret_cast<uint4*>(row + (piece / 8) * Shape::kPlane + (((piece % 8) ^ (r & 7)) << 4)) =
+                make_uint4(mul_f16x2(v[0], sc), mul_f16x2(v[1], sc), mul_f16x2(v[2], sc), mul_f16x2(v[3], sc));
+          }
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bars.kv_full[slot]);
+      }
+    }
+  } else {
+    // ---------------- softmax and output: thread r has row r of half t ----------------
+    regs_inc<kRegsSoftmax>();
+    const int t = group - 1, quarter = warp & 3, r = quarter * 32 + lane;
+    const uint32_t lane_off = (uint32_t)(quarter * 32) << 16;
+    const uint32_t s_addr = tmem + t * 128 + lane_off, o_addr = tmem + 256 + t * 128 + lane_off;
+    uint32_t pieces = 0, count = 0, tiles = 0;
+    bool ok = true;
+    for (begin(); w.more() && ok; next()) {
+      const Fp4TilePiece x(p, w);
+      if (t >= x.halves) {
+        tiles += x.n;
+        continue;
+      }
+      const int n = x.n, k0 = x.k0;
+      int hi, lo;
+      float sc = p.scale_log2, m = -INFINITY, l = 0.f;
+      {
+        const int token = (x.r0 + min(t * 128 + r, x.rows - 1)) / p.G, pos = x.first + token;
+        hi = min(p.causal ? pos : w.e.len - 1, w.e.len - 1);
+        lo = fp4_lowest(p, pos);
+      }
+      if (n > 0) {
+        // ---- the row's query (every product of the piece before is done: its last scores have been read)
+        const bool row = t * 128 + r < x.rows;
+        const int rr = x.r0 + min(t * 128 + r, x.rows - 1), token = rr / p.G, head = x.h * p.G + rr - token * p.G;
+        const uint4* src = reinterpret_cast<const uint4*>(p.q + (long long)(w.e.token0 + token) * p.ldq + (long long)head * D);
+        uint4 raw[D / 8];
+        float big = 0.f;
+#pragma unroll
+        for (int i = 0; i < D / 8; ++i) raw[i] = row ? src[i] : make_uint4(0, 0, 0, 0);
+#pragma unroll
+        for (int i = 0; i < D / 8; ++i) {
+          const uint32_t v[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float2 f = unpack_bf16x2(v[e]);
+            big = fmaxf(big, fmaxf(fabsf(f.x), fabsf(f.y)));
+          }
+        }
+        const int e2 = min(max((int)(__float_as_uint(big) >> 23) - 127, -100), 100);
+        const float down = __uint_as_float((uint32_t)(127 - e2) << 23);
+        sc *= __uint_as_float((uint32_t)(127 + e2) << 23);
+        uint8_t* dst = sQ + t * Shape::kSlot + r * 128;
+#pragma unroll
+        for (int i = 0; i < D / 8; ++i) {
+          const uint32_t v[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+          uint32_t f16[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float2 f = unpack_bf16x2(v[e]);
+            f16[e] = pack_f16x2(f.x * down, f.y * down);
+          }
+          *reinterpret_cast<uint4*>(dst + (i / 8) * Shape::kPlane + (((i % 8) ^ (r & 7)) << 4)) = make_uint4(f16[0], f16[1], f16[2], f16[3]);
+        }
+        fence_proxy_async_smem();
+        tc_fence_before_sync();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bars.q_full[t]);
+      }
+      for (int j = 0; j < n; ++j, ++count, ++tiles) {
+        ok = __all_sync(0xffffffffu, mbar_wait(&bars.s_full[t], count & 1, p.status));
+        if (!ok) break;
+        tc_fence_after_sync();
+        uint32_t s[kTileKeys];
+#pragma unroll
+        for (int c = 0; c < kTileKeys / 32; ++c) tmem_ld_32x32b_x32(s_addr + c * 32, s + c * 32);
+        tmem_ld_wait();
+        const int kbase = k0 + j * kTileKeys;
+        if (p.softcap2 > 0.f) {                                  // (scores in units of the cap from here on)
+          const float in = sc / p.softcap2;
+#pragma unroll
+          for (int i = 0; i < kTileKeys; ++i) s[i] = __float_as_uint(tanhf(__uint_as_float(s[i]) * in));
+        }
+        const float to_log2 = p.softcap2 > 0.f ? p.softcap2 : sc;
+        if (kbase + kTileKeys - 1 > hi || kbase < lo) {
+#pragma unroll
+          for (int i = 0; i < kTileKeys; ++i)
+            if (kbase + i > hi || kbase + i < lo) s[i] = 0xff800000u;       // -inf
+        }
+        const volatile uint32_t* gone = no_page[tiles % 4];
+        const uint32_t g0 = gone[0], g1 = gone[1], g2 = gone[2], g3 = gone[3];
+        if (g0 | g1 | g2 | g3) {
+#pragma unroll
+          for (int i = 0; i < kTileKeys; ++i)
+            if ((i < 32 ? g0 : i < 64 ? g1 : i < 96 ? g2 : g3) >> (i & 31) & 1) s[i] = 0xff800000u;
+        }
+        float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+        for (int i = 0; i < kTileKeys; i += 4)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) mx[e] = fmaxf(mx[e], __uint_as_float(s[i + e]));
+        const float tile_max = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * to_log2;
+        float alpha = 1.f;
+        bool rescale = false;
+        if (tile_max > m + 8.f) {          // also the first finite tile: m == -inf
+          if (m != -INFINITY) {
+            alpha = ex2_of(m - tile_max);
+            rescale = j > 0;
+          }
+          m = tile_max;
+        }
+        const float off = m == -INFINITY ? 0.f : kUp - m;
+        // O is at rest: S(j) is issued right behind P V(j - 1), by the same elected lane, and a commit covers all that its thread has issued before
+        if (__any_sync(0xffffffffu, rescale)) {
+#pragma unroll 1
+          for (int c = 0; c < D / 16; ++c) {
+            uint32_t o[16];
+            tmem_ld_32x32b_x16(o_addr + c * 16, o);
+            tmem_ld_wait();
+#pragma unroll
+            for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+            tmem_st_32x32b_x16(o_addr + c * 16, o);
+          }
+        }
+        const uint64_t sc2 = pack_f32x2(to_log2, to_log2), off2 = pack_f32x2(off, off);
+        uint64_t sum2[2] = {0, 0};
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          uint32_t pk[16];
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            float a, b;
+            unpack_f32x2(fma_f32x2(pack_b32x2(s[c * 32 + 2 * i], s[c * 32 + 2 * i + 1]), sc2, off2), a, b);
+            a = ex2_of(a);
+            b = ex2_of(b);
+            sum2[i & 1] = add_f32x2(sum2[i & 1], pack_f32x2(a, b));
+            pk[i] = pack_f16x2(a, b);
+          }
+          tmem_st_32x32b_x16(s_addr + c * 16, pk);
+          if (c == 1) {                  // P V of the first half of the keys may start
+            tmem_st_wait();
+            tc_fence_before_sync();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&bars.p_first[t]);
+          }
+        }
+        float sum[4];
+        unpack_f32x2(sum2[0], sum[0], sum[1]);
+        unpack_f32x2(sum2[1], sum[2], sum[3]);
+        l = l * alpha + ((sum[0] + sum[1]) + (sum[2] + sum[3]));
+        tmem_st_wait();
+        tc_fence_before_sync();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bars.p_full[t]);
+      }
+      if (!ok) break;
+      if (n > 0) {
+        ok = __all_sync(0xffffffffu, mbar_wait(&bars.pv_done[t], pieces & 1, p.status));
+        if (!ok) break;
+        ++pieces;
+        tc_fence_after_sync();
+      }
+      const Fp4TilePiece y(p, w);
+      const bool row = t * 128 + r < y.rows, whole = w.whole();
+      const int rr = y.r0 + min(t * 128 + r, y.rows - 1), token = rr / p.G, head = y.h * p.G + rr - token * p.G;
+      const float inv = l == 0.f ? 0.f : 1.f / l;
+      float* part = parts + fp4_part<Fp4Tile, D>(blockIdx.x, w.part());
+      __nv_bfloat16* dst = p.out + (long long)(w.e.token0 + token) * p.ldo + (long long)head * D;
+#pragma unroll
+      for (int c = 0; c < D / 32; ++c) {
+        uint32_t o[32];
+        if (n > 0) {
+          tmem_ld_32x32b_x32(o_addr + c * 32, o);   // (whole warp)
+          tmem_ld_wait();
+        } else {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) o[i] = 0;
+        }
+        if (row && whole) {
+#pragma unroll
+          for (int i = 0; i < 32; i += 8) {
+            uint32_t v[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] = pack_bf16x2(__uint_as_float(o[i + 2 * e]) * inv, __uint_as_float(o[i + 2 * e + 1]) * inv);
+            *reinterpret_cast<uint4*>(dst + c * 32 + i) = make_uint4(v[0], v[1], v[2], v[3]);
+          }
+        } else if (row) {
+#pragma unroll
+          for (int i = 0; i < 32; i += 4)
+            *reinterpret_cast<uint4*>(part + (t * 128 + r) * D + c * 32 + i) = make_uint4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+        }
+      }
+      if (row && !whole) *reinterpret_cast<float2*>(part + Fp4Tile::kRows * D + 2 * (t * 128 + r)) = make_float2(m, l);
+    }
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  tc_fence_after_sync();
+  if (warp == 0) tmem_dealloc(tmem, 512);
+}
+
+int fp4_tile_grid() { return b200_num_sms(); }
+
+template <int D>
+static int launch_tiles(const Fp4Attn& p, float* parts, cudaStream_t stream) {
+  const size_t smem = 1024 + Fp4TileShape<D>::kLine + (size_t)(p.num_tiles + 1) * 4;
+  static PerDeviceOnce once;
+  static std::atomic<int> regs{0};
+  if (once.first()) {
+    cudaFuncAttributes attr;
+    if (cudaFuncGetAttributes(&attr, fp4_tiles_kernel<D>) != cudaSuccess) return -2;
+    if (cudaFuncSetAttribute(fp4_tiles_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, 1024 + Fp4TileShape<D>::kLine + 8001 * 4) != cudaSuccess)
+      return -2;
+    regs = attr.numRegs;
+  }
+  // a warpgroup waits without limit for registers that the launch did not bring
+  if (4 * regs < kRegsIssue + 2 * kRegsSoftmax + kRegsExpand) return -2;
+  return launch_pdl(fp4_tiles_kernel<D>, dim3(fp4_tile_grid()), dim3(512), smem, stream, p, parts) == cudaSuccess ? 0 : -2;
+}
+
+int launch_fp4_tiles(const Fp4Attn& p, int D, float* parts, cudaStream_t stream) {
+  return D == 64 ? launch_tiles<64>(p, parts, stream) : launch_tiles<128>(p, parts, stream);
+}
+
+}  // namespace b200

@@ -158,6 +158,7 @@ def test_refusals_without_a_gpu():
     refused("block_table", C.decode, q, cache, **{**good, "block_table": table.long()})
     refused("block_table", C.decode, q, cache, **{**good, "block_table": table[:, :0]})
     refused("softcap", C.decode, q, cache, softcap=-1.0, **good)
+    refused("scale is positive", C.decode, q, cache, **{**good, "scale": 0.0})
     tiles = dict(q_start=torch.zeros(4, dtype=torch.int32), tile_req=slots.int(), tile_q0=slots.int())
     refused("one GPU", C.prefill, q, cache, **tiles, **good)
     qkv = torch.zeros((3, 640), dtype=torch.bfloat16)

@@ -215,6 +215,14 @@ PREFILL = [
     ([400, 31], [77, 31], 4, 2, 128, 32, 0, 0.0, False),
     ([400, 31], [77, 31], 6, 2, 256, 32, 50, 0.0, True),
     ([3000] * 9, [4, 5, 6, 1, 2, 3, 4, 5, 6], 32, 8, 128, 32, 0, 0.0, True),
+    ([5000], [70], 32, 8, 128, 32, 0, 0.0, True),                        # few rows after a long context: every item is cut
+    ([5000], [70], 4, 1, 64, 16, 0, 0.0, True),
+    ([260, 3, 2000, 17], [130, 3, 5, 17], 24, 4, 128, 32, 0, 0.0, True), # sequences of both kernels
+    ([130 + i for i in range(40)], [65 + i for i in range(40)], 8, 4, 128, 16, 0, 0.0, True),
+    ([4000], [4000], 16, 2, 128, 32, 0, 0.0, True),
+    ([4000, 500], [2048, 129], 8, 8, 64, 128, 700, 0.0, True),
+    ([1300, 200], [900, 200], 16, 1, 128, 32, 0, 15.0, False),
+    ([3000], [1500], 5, 1, 128, 16, -512, 0.0, True),
 ]
 
 
@@ -263,6 +271,27 @@ def test_queries_before_the_first_key_and_pages_outside_the_cache():
     for r, slots in ((0, list(range(16, 32)) + list(range(48, 61))), (2, list(range(32, 48)) + list(range(48, 64)))):
         k, v = C.ref_read(cache, torch.tensor(slots))
         F.check_attention(out[r].view(1, Hq, D), *F.attention(q[r].view(1, Hq, D), k, v, len(slots), 0.1, 0.0, 0))
+
+
+def test_pages_outside_the_cache_under_many_rows():
+    Hq, Hkv, D, bs, n = 4, 2, 128, 16, 700
+    gen = _gen(4)
+    cache = F.random_cache(60, Hkv, bs, D, gen)
+    table = torch.randperm(60, generator=gen)[: n // bs + 1].int()[None]
+    gone = [3, 4, 17, 30]
+    table[0, gone] = torch.tensor([-1, 60, 1 << 30, -(1 << 31)], dtype=torch.int32)
+    q = torch.randn((n, Hq * D), generator=gen).to(torch.bfloat16)
+    req, q0 = _tiles([n])
+    out = C.prefill(q.to(DEV), cache.to(DEV), block_table=table.to(DEV), seq_lens=torch.tensor([n], dtype=torch.int32, device=DEV),
+                    q_start=torch.tensor([0, n], dtype=torch.int32, device=DEV), tile_req=req, tile_q0=q0, scale=0.1).cpu()
+    pos = torch.arange(n)
+    there = ~torch.isin(pos // bs, torch.tensor(gone))
+    k, v = C.ref_read(cache, table[0].long().clamp(0, 59)[pos // bs] * bs + pos % bs)
+    for first in (0, 47, 48, 79, 80, 300, 699):                          # a row at a time, over the keys that it has
+        seen = there & (pos <= first)
+        want = F.attention(q[first].view(1, Hq, D), k[seen], v[seen], int(seen.sum()), 0.1, 0.0, 0)
+        F.check_attention(out[first].view(1, Hq, D), *want)
+    assert _status() == 0
 
 
 def test_values_of_every_size():

@@ -289,7 +289,7 @@ class DenseModel:
         """(splits, scratch) of a decode batch as the runner keeps them: one scratch for all steps, which follow one another."""
         if getattr(self, "_fp4_scratch", None) is None:
             from ..ops import fp4_cache
-            self._fp4_scratch = fp4_cache.scratch(self.device, self.hq, self.hkv, self.D)
+            self._fp4_scratch = fp4_cache.scratch(self.device, self.D)
         return 1, self._fp4_scratch
 
     def alloc_kv_cache(self, num_blocks: int, block_size: int):

@@ -54,7 +54,7 @@ def _declare():
     _lib.declare("b200_fp4_append", [ctypes.POINTER(AppendArgs), _P], _I)
     _lib.declare("b200_fp4_read", [_P, _L, _I, _I, _I, _P, _P, _L, _P, _L, _L, _P], _I)
     _lib.declare("b200_fp4_attn", [ctypes.POINTER(AttnArgs), _P], _I)
-    _lib.declare("b200_fp4_attn_scratch", [_I, _I, _I], _L)
+    _lib.declare("b200_fp4_attn_scratch", [_I, _I], _L)
     lib()
     _declared = True
 
@@ -147,23 +147,27 @@ def read(cache: torch.Tensor, slots: torch.Tensor, k: Optional[torch.Tensor] = N
 _scratch_floats: dict = {}
 
 
-def scratch(device: torch.device, num_q_heads: int, num_kv_heads: int, head_dim: int) -> torch.Tensor:
-    """What ``decode`` and ``prefill`` take as ``tmp``: parts of sequences that several CTAs share. Calls that may run at the same time
-    (streams, graphs replayed side by side) need one each."""
-    key = (device.index, num_q_heads, num_kv_heads, head_dim)
+def scratch_floats(device: torch.device, head_dim: int, prefill: bool) -> int:
+    key = (device.index, head_dim, prefill)
     n = _scratch_floats.get(key)
     if n is None:
         _declare()
         with torch.cuda.device(device):
-            n = _scratch_floats[key] = lib().b200_fp4_attn_scratch(num_q_heads, num_kv_heads, head_dim)
-    return torch.empty(n, dtype=torch.float32, device=device)
+            n = _scratch_floats[key] = lib().b200_fp4_attn_scratch(head_dim, prefill)
+    return n
+
+
+def scratch(device: torch.device, head_dim: int, prefill: bool = True) -> torch.Tensor:
+    """What ``decode`` and (with ``prefill``) ``prefill`` take as ``tmp``: parts of sequences that several CTAs share. Calls that may
+    run at the same time (streams, graphs replayed side by side) need one each."""
+    return torch.empty(scratch_floats(device, head_dim, prefill), dtype=torch.float32, device=device)
 
 
 def _attend(op, q, cache, block_table, seq_lens, q_start, tile_req, tile_q0, scale, out, softcap, window, causal, tmp):
     if out is None and q.is_cuda:
         out = torch.empty((q.shape[0], q.shape[1]), dtype=q.dtype, device=q.device)
     validate(op, q=q, cache=cache, block_table=block_table, seq_lens=seq_lens, q_start=q_start, tile_req=tile_req, tile_q0=tile_q0,
-             out=out, softcap=softcap, tmp=tmp)
+             out=out, scale=scale, softcap=softcap, tmp=tmp)
     _declare()
     a = AttnArgs()
     a.num_blocks, a.Hkv, a.block_size, D = shape_of(cache)
@@ -178,7 +182,7 @@ def _attend(op, q, cache, block_table, seq_lens, q_start, tile_req, tile_q0, sca
         a.tile_req, a.tile_q0, a.num_tiles = tile_req.data_ptr(), tile_q0.data_ptr(), tile_req.numel()
     a.window, a.causal, a.scale, a.softcap = window, causal, scale, softcap
     if tmp is None:
-        tmp = scratch(q.device, a.Hq, a.Hkv, D)
+        tmp = scratch(q.device, D, q_start is not None)
     a.parts = tmp.data_ptr()
     _launch(q.device, lambda s: lib().b200_fp4_attn(ctypes.byref(a), s), op)
     return out

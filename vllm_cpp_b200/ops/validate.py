@@ -123,18 +123,18 @@ _FP4_ATTN = [
         q.numel() == 0 or out.data_ptr() != q.data_ptr())),
     ("block_table is int32 [sequences, pages], rows contiguous", lambda block_table, **_: block_table.dtype == torch.int32
      and block_table.dim() == 2 and block_table.shape[1] > 0 and (block_table.shape[1] == 1 or block_table.stride(1) == 1)),
-    ("softcap is not negative", lambda softcap, **_: softcap >= 0),
-    ("tmp is fp32 and large enough", lambda q, cache, tmp=None, **_: tmp is None or (
-        tmp.dtype == torch.float32 and tmp.is_contiguous() and tmp.numel() >= _fp4_scratch(q, cache))),
+    ("scale is positive and softcap is not negative", lambda scale, softcap, **_: scale > 0 and softcap >= 0),
+    ("tmp is fp32 and large enough", lambda cache, q_start=None, tmp=None, **_: tmp is None or (
+        tmp.dtype == torch.float32 and tmp.is_contiguous() and tmp.data_ptr() % 16 == 0
+        and tmp.numel() >= _fp4_scratch(cache, q_start is not None))),
     ("all tensors are on one GPU", lambda q, cache, block_table, seq_lens, out, q_start=None, tile_req=None, tile_q0=None, tmp=None, **_:
      _on_gpu(q, cache, block_table, seq_lens, out, q_start, tile_req, tile_q0, tmp)),
 ]
 
 
-def _fp4_scratch(q, cache) -> int:
-    from ._lib import lib
-    D = cache.shape[3] // 18
-    return lib().b200_fp4_attn_scratch(q.shape[1] // D, cache.shape[1], D)
+def _fp4_scratch(cache, prefill) -> int:
+    from .fp4_cache import scratch_floats
+    return scratch_floats(cache.device, cache.shape[3] // 18, prefill)
 
 
 RULES.update({
