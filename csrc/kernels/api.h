@@ -238,6 +238,16 @@ typedef struct B200Fp4Append {
   float eps;
 } B200Fp4Append;
 
+// What that cache holds for n slots, as bf16; zeros for slots outside it.
+typedef struct B200Fp4Read {
+  const void* cache;
+  const void* slots;           // int64 [n]
+  void* k;                     // [n][Hkv][D]
+  void* v;
+  long long num_blocks, n;
+  int block_size, Hkv, D;
+} B200Fp4Read;
+
 // Attention over that cache (fp4_attn.cu). q_start null: one query a sequence (decode), else [num_reqs + 1] and causal from the end of each sequence
 // (causal 0: every query sees every key) and with its 128-token query tiles. window as in b200_attn_decode, scale > 0. parts: b200_fp4_attn_scratch
 // floats, for this call alone until it is done. At most 8192 sequences and 8000 tiles.
@@ -522,7 +532,7 @@ long long b200_fp4_attn_scratch(int D, int prefill);
 int b200_fp4_attn(const B200Fp4Attn* a, cudaStream_t stream);
 // ---- fp4_cache.cu
 int b200_fp4_append(const B200Fp4Append* a, cudaStream_t stream);
-int b200_fp4_read(const void* cache, long long num_blocks, int block_size, int Hkv, int D, const void* slots, void* k, long long ldk, void* v, long long ldv, long long n, cudaStream_t stream);
+int b200_fp4_read(const B200Fp4Read* a, cudaStream_t stream);
 // ---- gdn.cu
 int b200_gdn_conv1d_fwd(const void* x, long ldx, const void* w, void* conv_state, const int* qsl, const int* slots, const int* has_init, void* out, long ldo, int n_seq, int total_tokens, int C, cudaStream_t stream);
 int b200_gdn_conv1d_update(const void* x, long ldx, const void* w, void* conv_state, const int* slots, void* out, long ldo, int B, int C, cudaStream_t stream);

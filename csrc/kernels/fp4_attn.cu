@@ -379,16 +379,19 @@ __global__ void __launch_bounds__(kRowWarps * 32, NT == 1 && D <= 128 ? 2 : 1) f
     if (flying >> i & 1) mbar_wait(&full[i], phase >> i & 1, p.status);
 }
 
-// Parts of the row kernel's items, then those of the tile kernel's, each by a block of its own.
+// Parts of the row kernel's items, each by a block of its own, then those of the tile kernel's, each by kTileShares.
+static constexpr int kTileShares = 8;
 template <int D, int ROWS>
 __global__ void __launch_bounds__(256) fp4_join_kernel(Fp4Attn p, const float* row_parts, int row_grid, const float* tile_parts, int tile_grid) {
   extern __shared__ uint32_t line[];
   pdl_wait();
   pdl_launch_dependents();
-  if ((int)blockIdx.x < row_grid)
-    fp4_join<Fp4Seq<ROWS>, D>(p, row_parts, line, blockIdx.x, row_grid, kRowWarps);
-  else if constexpr (D <= 128)
-    fp4_join<Fp4Tile, D>(p, tile_parts, line, blockIdx.x - row_grid, tile_grid, kTileLeast);
+  if ((int)blockIdx.x < row_grid) {
+    fp4_join<Fp4Seq<ROWS>, D>(p, row_parts, line, blockIdx.x, row_grid, kRowWarps, 0, 1);
+  } else if constexpr (D <= 128) {
+    const int i = blockIdx.x - row_grid;
+    fp4_join<Fp4Tile, D>(p, tile_parts, line, i / kTileShares, tile_grid, kTileLeast, i % kTileShares, kTileShares);
+  }
 }
 
 static constexpr int kMostReqs = 8192, kMostTiles = 8000;         // (the line of a step is in shared memory)
@@ -410,7 +413,7 @@ static int launch_attn(const Fp4Attn& p, bool rows, bool tiles, float* parts, cu
   if (tiles)
     if (const int rc = launch_fp4_tiles(p, D, tile_parts, stream)) return rc;
   const size_t line = (size_t)((rows ? p.num_reqs : 0) > (tiles ? p.num_tiles : 0) ? p.num_reqs : tiles ? p.num_tiles : 0) * 4 + 4;
-  return launch_pdl(fp4_join_kernel<D, Shape::kRows>, dim3(row_grid + tile_grid), dim3(256), line, stream, p, (const float*)parts, row_grid,
+  return launch_pdl(fp4_join_kernel<D, Shape::kRows>, dim3(row_grid + tile_grid * kTileShares), dim3(256), line, stream, p, (const float*)parts, row_grid,
                     (const float*)tile_parts, tile_grid) == cudaSuccess ? 0 : -2;
 }
 

@@ -177,38 +177,40 @@ __global__ void __launch_bounds__(128) fp4_append_kernel(B200Fp4Append p) {
   }
 }
 
-// A lane turns 8 codes into 16 bytes of bf16.
+// A lane turns 8 codes into 16 bytes of bf16. A block has one token, or as many as its threads have room for.
 template <int D>
-__global__ void __launch_bounds__(128) fp4_read_kernel(const uint8_t* __restrict__ cache, long long num_blocks, int block_size, int Hkv,
-                                                       const int64_t* __restrict__ slots, __nv_bfloat16* __restrict__ k, long long ldk,
-                                                       __nv_bfloat16* __restrict__ v, long long ldv, long long n) {
+__global__ void __launch_bounds__(256) fp4_read_kernel(B200Fp4Read p, int tokens) {
   using Cell = Fp4Cell<D>;
   pdl_wait();
   pdl_launch_dependents();
-  const long long i = blockIdx.x * 128ll + threadIdx.x;
-  const int l = (int)(i % (D / 8));
-  const long long th = i / (D / 8);
-  const long long t = th / (2 * Hkv);
-  if (t >= n) return;
-  const int h2 = (int)(th - t * (2 * Hkv)), kv = h2 >= Hkv, h = h2 - kv * Hkv;
-  const int64_t slot = slots[t];
-  uint32_t o[4] = {0, 0, 0, 0};
-  if (slot >= 0 && slot < num_blocks * block_size) {
-    const int64_t blk = (slot >> 31) == 0 ? (int64_t)((uint32_t)slot / (uint32_t)block_size) : slot / block_size;
-    const int off = (int)(slot - blk * block_size), token = off % kCellTokens;
-    const uint8_t* cell = cache + ((blk * Hkv + h) * (block_size / kCellTokens) + off / kCellTokens) * (long long)Cell::kBytes;
-    const uint32_t codes = *reinterpret_cast<const uint32_t*>(cell + (kv ? Cell::value_at(token, l * 4) : token * Cell::kRow + l * 4));
-    const float s = fp4_scale_value(cell[kv ? Cell::kValueScales + (l >> 1) * kCellTokens + token
-                                          : Cell::kKeyScales + token * Cell::kScales + (l >> 1)]);
-    uint32_t f16[4];
-    cvt_e2m1x8(codes, f16);
+  const int per = 2 * p.Hkv * (D / 8);                          // lanes of a token
+  const int local = tokens > 1 ? threadIdx.x / per : 0, first = threadIdx.x - local * per;
+  const long long t = (long long)blockIdx.x * tokens + local;
+  if (local >= tokens || t >= p.n) return;
+  const int64_t slot = ((const int64_t*)p.slots)[t];
+  const bool there = slot >= 0 && slot < p.num_blocks * p.block_size;
+  const int64_t blk = !there ? 0 : (slot >> 31) == 0 ? (int64_t)((uint32_t)slot / (uint32_t)p.block_size) : slot / p.block_size;
+  const int off = there ? (int)(slot - blk * p.block_size) : 0, token = off % kCellTokens, cells = p.block_size / kCellTokens;
+  const uint8_t* cell0 = (const uint8_t*)p.cache + (blk * p.Hkv * cells + off / kCellTokens) * Cell::kBytes;
+  for (int i = first; i < per; i += 256) {
+    const int l = i % (D / 8), h2 = i / (D / 8), kv = h2 >= p.Hkv, h = h2 - kv * p.Hkv;
+    uint32_t o[4] = {0, 0, 0, 0};
+    if (there) {
+      const uint8_t* cell = cell0 + (size_t)h * cells * Cell::kBytes;
+      const uint32_t codes = *reinterpret_cast<const uint32_t*>(cell + (kv ? Cell::value_at(token, l * 4) : token * Cell::kRow + l * 4));
+      const float s = fp4_scale_value(cell[kv ? Cell::kValueScales + (l >> 1) * kCellTokens + token
+                                              : Cell::kKeyScales + token * Cell::kScales + (l >> 1)]);
+      uint32_t f16[4];
+      cvt_e2m1x8(codes, f16);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const float2 f = __half22float2(*reinterpret_cast<__half2*>(&f16[e]));
-      o[e] = pack_bf16x2(f.x * s, f.y * s);
+      for (int e = 0; e < 4; ++e) {
+        const float2 f = __half22float2(*reinterpret_cast<__half2*>(&f16[e]));
+        o[e] = pack_bf16x2(f.x * s, f.y * s);
+      }
     }
+    __nv_bfloat16* dst = (__nv_bfloat16*)(kv ? p.v : p.k) + (t * p.Hkv + h) * D + l * 8;
+    *reinterpret_cast<uint4*>(dst) = make_uint4(o[0], o[1], o[2], o[3]);
   }
-  *reinterpret_cast<uint4*>((kv ? v + t * ldv : k + t * ldk) + h * D + l * 8) = make_uint4(o[0], o[1], o[2], o[3]);
 }
 
 template <int D>
@@ -220,7 +222,8 @@ static int launch_append(const B200Fp4Append& p, cudaStream_t stream) {
     if (warps >= (1ll << 31)) return -4;
     return launch_pdl(kernel, dim3((unsigned)((warps + 3) / 4)), dim3(128), 0, stream, p) == cudaSuccess ? 0 : -2;
   };
-  return go(fp4_append_kernel<D, 1>, 1);
+  // many tokens: a warp takes four times the heads of a token, so that position, slot, cos and sin are fetched once for them
+  return (long long)p.T * nheads > 4096 * kHeads ? go(fp4_append_kernel<D, 4>, 4) : go(fp4_append_kernel<D, 1>, 1);
 }
 
 }  // namespace b200
@@ -242,15 +245,16 @@ extern "C" int b200_fp4_append(const B200Fp4Append* a, cudaStream_t stream) {
   return a->D == 64 ? launch_append<64>(*a, stream) : a->D == 128 ? launch_append<128>(*a, stream) : launch_append<256>(*a, stream);
 }
 
-extern "C" int b200_fp4_read(const void* cache, long long num_blocks, int block_size, int Hkv, int D, const void* slots, void* k, long long ldk,
-                             void* v, long long ldv, long long n, cudaStream_t stream) {
-  if (n <= 0) return 0;
-  if (!fp4_cache_ok(D, block_size, Hkv, num_blocks) || (((uintptr_t)cache | (uintptr_t)k | (uintptr_t)v | (uintptr_t)((ldk | ldv) * 2)) & 15)) return -1;
-  const long long blocks = (n * 2 * Hkv * (D / 8) + 127) / 128;
+extern "C" int b200_fp4_read(const B200Fp4Read* a, cudaStream_t stream) {
+  if (a->n <= 0) return 0;
+  if (!fp4_cache_ok(a->D, a->block_size, a->Hkv, a->num_blocks) || (((uintptr_t)a->cache | (uintptr_t)a->k | (uintptr_t)a->v) & 15) || !a->slots ||
+      !a->cache || !a->k || !a->v)
+    return -1;
+  const int per = 2 * a->Hkv * (a->D / 8), tokens = per < 256 ? 256 / per : 1;
+  const long long blocks = (a->n + tokens - 1) / tokens;
   if (blocks >= (1ll << 31)) return -4;
   const auto go = [&](auto kernel) {
-    return launch_pdl(kernel, dim3((unsigned)blocks), dim3(128), 0, stream, (const uint8_t*)cache, num_blocks, block_size, Hkv,
-                      (const int64_t*)slots, (__nv_bfloat16*)k, ldk, (__nv_bfloat16*)v, ldv, n) == cudaSuccess ? 0 : -2;
+    return launch_pdl(kernel, dim3((unsigned)blocks), dim3(256), 0, stream, *a, tokens) == cudaSuccess ? 0 : -2;
   };
-  return D == 64 ? go(fp4_read_kernel<64>) : D == 128 ? go(fp4_read_kernel<128>) : go(fp4_read_kernel<256>);
+  return a->D == 64 ? go(fp4_read_kernel<64>) : a->D == 128 ? go(fp4_read_kernel<128>) : go(fp4_read_kernel<256>);
 }

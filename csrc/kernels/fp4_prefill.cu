@@ -54,7 +54,7 @@ struct Fp4TilePiece {
     halves = rows > 128 ? 2 : 1;
     first = e.first;
     const int low = max(0, fp4_lowest(p, first + r0 / p.G)), high = min(p.causal ? first + (r0 + rows - 1) / p.G : e.len - 1, e.len - 1);
-    const int t0 = max(e.begin + w.c0, low / kTileKeys), t1 = min(e.begin + w.c1, high < 0 ? 0 : high / kTileKeys + 1);
+    const int t0 = max(e.begin + w.from(), low / kTileKeys), t1 = min(e.begin + w.to(), high < 0 ? 0 : high / kTileKeys + 1);
     k0 = t0 * kTileKeys;
     n = max(0, t1 - t0);
   }
@@ -281,10 +281,23 @@ __global__ void __launch_bounds__(512, 1) fp4_tiles_kernel(Fp4Attn p, float* par
     const uint32_t s_addr = tmem + t * 128 + lane_off, o_addr = tmem + 256 + t * 128 + lane_off;
     uint32_t pieces = 0, count = 0, tiles = 0;
     bool ok = true;
-    for (begin(); w.more() && ok; next()) {
+    uint4 raw[D / 8];
+    const auto query = [&](const Fp4Piece<Fp4Tile>& w) {         // the row's query of a piece, on its way
+      const Fp4TilePiece x(p, w);
+      const int rr = x.r0 + t * 128 + r, token = rr / p.G, head = x.h * p.G + rr - token * p.G;
+      const uint4* src = reinterpret_cast<const uint4*>(p.q + (long long)(w.e.token0 + token) * p.ldq + (long long)head * D);
+      const bool row = x.n > 0 && t * 128 + r < x.rows;
+#pragma unroll
+      for (int i = 0; i < D / 8; ++i) raw[i] = row ? src[i] : make_uint4(0, 0, 0, 0);
+    };
+    begin();
+    if (w.more()) query(w);
+    while (w.more() && ok) {
       const Fp4TilePiece x(p, w);
       if (t >= x.halves) {
         tiles += x.n;
+        next();
+        if (w.more()) query(w);
         continue;
       }
       const int n = x.n, k0 = x.k0;
@@ -297,13 +310,7 @@ __global__ void __launch_bounds__(512, 1) fp4_tiles_kernel(Fp4Attn p, float* par
       }
       if (n > 0) {
         // ---- the row's query (every product of the piece before is done: its last scores have been read)
-        const bool row = t * 128 + r < x.rows;
-        const int rr = x.r0 + min(t * 128 + r, x.rows - 1), token = rr / p.G, head = x.h * p.G + rr - token * p.G;
-        const uint4* src = reinterpret_cast<const uint4*>(p.q + (long long)(w.e.token0 + token) * p.ldq + (long long)head * D);
-        uint4 raw[D / 8];
         float big = 0.f;
-#pragma unroll
-        for (int i = 0; i < D / 8; ++i) raw[i] = row ? src[i] : make_uint4(0, 0, 0, 0);
 #pragma unroll
         for (int i = 0; i < D / 8; ++i) {
           const uint32_t v[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
@@ -420,18 +427,21 @@ __global__ void __launch_bounds__(512, 1) fp4_tiles_kernel(Fp4Attn p, float* par
         if (lane == 0) mbar_arrive(&bars.p_full[t]);
       }
       if (!ok) break;
+      const Fp4Piece<Fp4Tile> now = w;
+      const Fp4TilePiece y(p, now);
+      next();
+      if (w.more()) query(w);
       if (n > 0) {
         ok = __all_sync(0xffffffffu, mbar_wait(&bars.pv_done[t], pieces & 1, p.status));
         if (!ok) break;
         ++pieces;
         tc_fence_after_sync();
       }
-      const Fp4TilePiece y(p, w);
-      const bool row = t * 128 + r < y.rows, whole = w.whole();
+      const bool row = t * 128 + r < y.rows, whole = now.whole();
       const int rr = y.r0 + min(t * 128 + r, y.rows - 1), token = rr / p.G, head = y.h * p.G + rr - token * p.G;
       const float inv = l == 0.f ? 0.f : 1.f / l;
-      float* part = parts + fp4_part<Fp4Tile, D>(blockIdx.x, w.part());
-      __nv_bfloat16* dst = p.out + (long long)(w.e.token0 + token) * p.ldo + (long long)head * D;
+      float* part = parts + fp4_part<Fp4Tile, D>(blockIdx.x, now.part());
+      __nv_bfloat16* dst = p.out + (long long)(now.e.token0 + token) * p.ldo + (long long)head * D;
 #pragma unroll
       for (int c = 0; c < D / 32; ++c) {
         uint32_t o[32];

@@ -1,6 +1,7 @@
 // How attention over the 4-bit cache is shared out, for both of its kernels. An entry (a sequence, or a tile of 128 query tokens) has items (kv head,
 // row tile) that all read the same number of key cells. The cells of all items of all entries stand in one line, each CTA takes an equal stretch of
-// it, and the parts of items that the ends of stretches cut are joined afterwards.
+// it, and the parts of items that the ends of stretches cut are joined afterwards. What an item costs besides its cells (queries, output) stands in
+// the line as kStart cells in front of them: without, the CTAs that get the short items of a causal prompt's beginning finish last.
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -68,7 +69,7 @@ struct Fp4Span {
 // An entry's token0 is the query row of its first row, first that one's position, rows = tokens x G.
 template <int ROWS>
 struct Fp4Seq {                // cells of 16 keys, row tiles of ROWS
-  static constexpr int kRows = ROWS, kSnap = 0;
+  static constexpr int kRows = ROWS, kStart = 0, kSnap = 0;
   int req, len, token0, rows, first, begin, cells, tiles;       // begin: first cell of the sequence that any row sees
   static __device__ __forceinline__ int count(const Fp4Attn& p) { return p.num_reqs; }
   __device__ __forceinline__ Fp4Seq() {}
@@ -81,14 +82,14 @@ struct Fp4Seq {                // cells of 16 keys, row tiles of ROWS
     if (rows > p.few) rows = 0;
     first = len - s.q_len;
     begin = max(0, fp4_lowest(p, first)) / kCellTokens;
-    cells = max(1, (len + kCellTokens - 1) / kCellTokens - begin);          // (no keys: one cell that counts as masked)
+    cells = kStart + max(1, (len + kCellTokens - 1) / kCellTokens - begin);          // (no keys: one cell that counts as masked)
     tiles = (rows + ROWS - 1) / ROWS;
   }
 };
 
 static constexpr int kTileKeys = 128, kTileTokens = 128;
 struct Fp4Tile {               // tiles of 128 keys, row tiles of 256
-  static constexpr int kRows = 256, kSnap = 8;
+  static constexpr int kRows = 256, kStart = 3, kSnap = 8;
   int req, len, token0, rows, first, begin, cells, tiles;       // begin: first key tile that any row sees
   static __device__ __forceinline__ int count(const Fp4Attn& p) { return p.num_tiles; }
   __device__ __forceinline__ Fp4Tile() {}
@@ -102,7 +103,7 @@ struct Fp4Tile {               // tiles of 128 keys, row tiles of 256
     first = len - s.q_len + q0;
     begin = max(0, fp4_lowest(p, first)) / kTileKeys;
     const int last = min(p.causal ? first + tokens - 1 : len - 1, len - 1);
-    cells = max(1, (last < 0 ? 0 : last / kTileKeys + 1) - begin);
+    cells = kStart + max(1, (last < 0 ? 0 : last / kTileKeys + 1) - begin);
     tiles = (rows + kRows - 1) / kRows;
   }
 };
@@ -146,8 +147,8 @@ __device__ __forceinline__ int fp4_find(const uint32_t* line, int n, uint32_t u)
   }
   return lo;
 }
-// Stretches: CTA i of `ctas` begins at cell total i / ctas; where that falls into an item of at most kSnap cells, at the nearer end of the item.
-// (Short items are not worth a part in scratch; and as a longer item is cut exactly where the unmoved line says, the join finds its parts.)
+// Stretches: CTA i of `ctas` begins at cell total i / ctas; where that falls into an item of at most kSnap cells, at the nearer end of the item, and
+// where it falls among the first kStart or on the first cell behind them, at the item's beginning. (Short items are not worth a part in scratch.)
 __device__ __forceinline__ uint32_t fp4_ctas(uint32_t total, uint32_t grid, int least) { return max(1u, min(grid, total / least)); }
 template <class Entry>
 __device__ __forceinline__ uint32_t fp4_begin(const Fp4Attn& p, const uint32_t* line, uint32_t total, uint32_t i, uint32_t ctas) {
@@ -155,10 +156,10 @@ __device__ __forceinline__ uint32_t fp4_begin(const Fp4Attn& p, const uint32_t* 
   if (Entry::kSnap == 0 || u == 0 || u >= total) return u;
   const int b = fp4_find(line, Entry::count(p), u);
   const uint32_t n = Entry(p, b).cells, off = (u - line[b]) % n;
-  return n <= Entry::kSnap ? u - off + (2 * off >= n ? n : 0) : u;
+  return n <= Entry::kSnap + Entry::kStart ? u - off + (2 * off >= n ? n : 0) : off <= Entry::kStart ? u - off : u;
 }
 
-// A piece of an item: cells [c0, c1) of the e.cells that it has.
+// A piece of an item: cells [c0, c1) of the e.cells that it has, kStart among them.
 template <class Entry>
 struct Fp4Piece {
   uint32_t u, u_end;           // in the line: where the piece begins, where the CTA's stretch ends
@@ -189,6 +190,8 @@ struct Fp4Piece {
     c1 = (int)min((uint32_t)e.cells, u_end - u);
   }
   __device__ __forceinline__ bool more() const { return u < u_end; }
+  __device__ __forceinline__ int from() const { return max(0, c0 - Entry::kStart); }             // without those
+  __device__ __forceinline__ int to() const { return max(0, c1 - Entry::kStart); }
   __device__ __forceinline__ bool whole() const { return c0 == 0 && c1 == e.cells; }
   // Of the two parts that a CTA has in scratch: 1 for an item that it begins, 0 for one that it goes on with.
   __device__ __forceinline__ int part() const { return c0 == 0; }
@@ -199,9 +202,10 @@ template <class Entry, int D>
 __device__ __forceinline__ size_t fp4_part(uint32_t cta, int part) { return ((size_t)cta * 2 + part) * (Entry::kRows * (D + 2)); }
 
 // Joins the parts of cut items. Block i looks at the line where stretch i + 1 begins; the first cut of an item is the one that joins it: part 1 of the
-// CTA that begins it, part 0 of those behind.
+// CTA that begins it, part 0 of those behind. `share` of `shares` blocks takes every shares-th 4 dims.
 template <class Entry, int D>
-__device__ __forceinline__ void fp4_join(const Fp4Attn& p, const float* parts, uint32_t* line, uint32_t i, uint32_t grid, int least) {
+__device__ __forceinline__ void fp4_join(const Fp4Attn& p, const float* parts, uint32_t* line, uint32_t i, uint32_t grid, int least, int share,
+                                         int shares) {
   constexpr int kRows = Entry::kRows;
   fp4_line<Entry>(p, line);
   const int entries = Entry::count(p);
@@ -215,7 +219,7 @@ __device__ __forceinline__ void fp4_join(const Fp4Attn& p, const float* parts, u
   if (begin == u || fp4_begin<Entry>(p, line, total, i, ctas) > begin) return;
   const uint32_t last = (uint32_t)(((uint64_t)(begin + e.cells) * ctas - 1) / total);         // the CTA that has the item's last cell
   const int h = item / e.tiles, r0 = (int)(item - h * e.tiles) * kRows, nrows = min(kRows, e.rows - r0);
-  for (int x = threadIdx.x; x < nrows * (D / 4); x += blockDim.x) {
+  for (int x = threadIdx.x + share * blockDim.x; x < nrows * (D / 4); x += shares * blockDim.x) {
     const int r = x / (D / 4), d = x % (D / 4) * 4;
     float mx = -INFINITY;
     for (uint32_t c = i; c <= last; ++c) mx = fmaxf(mx, parts[fp4_part<Entry, D>(c, c == i) + kRows * D + 2 * r]);

@@ -19,7 +19,7 @@ from typing import Optional
 import torch
 
 from . import _lib, reference
-from ._lib import check, lib, ptr, stream_ptr
+from ._lib import check, lib, stream_ptr
 from .validate import OpArgumentError, validate
 
 CELL = 16                      # tokens of a cell
@@ -44,18 +44,24 @@ class AttnArgs(ctypes.Structure):
                 ("block_size", _I), ("window", _I), ("causal", _I), ("scale", _F), ("softcap", _F)]
 
 
+class ReadArgs(ctypes.Structure):
+    _fields_ = [("cache", _P), ("slots", _P), ("k", _P), ("v", _P), ("num_blocks", _L), ("n", _L), ("block_size", _I), ("Hkv", _I),
+                ("D", _I)]
+
+
 _declared = False
+_append = _read = _attn = None      # the library's entry points
 
 
 def _declare():
-    global _declared
+    global _declared, _append, _read, _attn
     if _declared:
         return
-    _lib.declare("b200_fp4_append", [ctypes.POINTER(AppendArgs), _P], _I)
-    _lib.declare("b200_fp4_read", [_P, _L, _I, _I, _I, _P, _P, _L, _P, _L, _L, _P], _I)
-    _lib.declare("b200_fp4_attn", [ctypes.POINTER(AttnArgs), _P], _I)
+    for name, args in (("b200_fp4_append", AppendArgs), ("b200_fp4_read", ReadArgs), ("b200_fp4_attn", AttnArgs)):
+        _lib.declare(name, [ctypes.POINTER(args), _P], _I)
     _lib.declare("b200_fp4_attn_scratch", [_I, _I], _L)
-    lib()
+    l = lib()
+    _append, _read, _attn = l.b200_fp4_append, l.b200_fp4_read, l.b200_fp4_attn
     _declared = True
 
 
@@ -77,13 +83,13 @@ def shape_of(cache: torch.Tensor) -> tuple[int, int, int, int]:
     return n, h, c * CELL, b // 18
 
 
-def _launch(device: torch.device, call, what: str) -> None:
-    """Launches on the current stream of the tensors' device, whichever device is current."""
-    if device.index == torch._C._cuda_getDevice():
-        check(call(stream_ptr()), what)
+def _launch(t: torch.Tensor, call, args, what: str) -> None:
+    """On the current stream of the device of ``t``, whichever device is current."""
+    if t.get_device() == torch._C._cuda_getDevice():
+        check(call(args, stream_ptr()), what)
     else:
-        with torch.cuda.device(device):
-            check(call(stream_ptr()), what)
+        with torch.cuda.device(t.device):
+            check(call(args, stream_ptr()), what)
 
 
 def append(qkv: torch.Tensor, positions: Optional[torch.Tensor], cos_sin: Optional[torch.Tensor], cache: torch.Tensor,
@@ -96,25 +102,53 @@ def append(qkv: torch.Tensor, positions: Optional[torch.Tensor], cos_sin: Option
     its width, pairs half of it apart (``neox``) or neighbours. ``offsets``: columns where q, k and v begin; ``q_head_stride``:
     columns between q heads. The slots of a call differ; slots outside the cache (-1) write nothing, and a position
     outside the table makes its row NaN. The k and v columns of ``qkv`` stay as they are."""
-    a = AppendArgs()
-    a.num_blocks, a.Hkv, a.block_size, D = shape_of(cache) if cache.dim() == 4 else (0, 0, 0, 0)
+    nb, H, bs, D = shape_of(cache) if cache.dim() == 4 else (0, 0, 0, 0)
     hs = D if q_head_stride is None else q_head_stride
     if offsets is None:
-        offsets = (0, num_q_heads * D, (num_q_heads + a.Hkv) * D)
+        offsets = (0, num_q_heads * D, (num_q_heads + H) * D)
     rot = (D if cos_sin is None else cos_sin.shape[1]) if rot_dim is None else rot_dim
-    validate("fp4_append", qkv=qkv, cache=cache, slots=slots, positions=positions, cos_sin=cos_sin, q_norm=q_norm, k_norm=k_norm,
-             q_out=q_out, num_q_heads=num_q_heads, rot_dim=rot, q_head_stride=hs, offsets=offsets)
+    # (the rules of ops.validate for the plain call of a model's layer, in a fraction of their time)
+    try:
+        (T, cols), dev, (n,) = qkv.shape, qkv.get_device(), slots.shape
+        ok = (dev >= 0 and dev == cache.get_device() == slots.get_device() and D in (64, 128, 256) and cache.shape[3] == 18 * D
+              and bs > 0 and cache.dtype is torch.uint8 and cache.is_contiguous() and qkv.dtype is BF16 and qkv.stride(1) == 1
+              and slots.dtype is torch.int64 and slots.is_contiguous() and n >= T and hs == D and num_q_heads >= 0
+              and offsets == (0, num_q_heads * D, (num_q_heads + H) * D) and cols >= (num_q_heads + 2 * H) * D
+              and (qkv.data_ptr() | cache.data_ptr() | 2 * qkv.stride(0)) % 16 == 0)
+        if ok and cos_sin is not None:
+            rows, width = cos_sin.shape
+            ok = (cos_sin.dtype is torch.float32 and cos_sin.is_contiguous() and width == rot and rows > 0 and 0 < rot <= D and rot % 2 == 0
+                  and positions.dtype is torch.int64 and positions.is_contiguous() and positions.dim() == 1 and positions.numel() >= T
+                  and dev == cos_sin.get_device() == positions.get_device())
+        if ok and q_out is not None:
+            ok = (q_out.dtype is BF16 and q_out.get_device() == dev and q_out.dim() == 2 and q_out.stride(1) == 1 and q_out.shape[0] >= T
+                  and q_out.shape[1] == num_q_heads * D and (q_out.data_ptr() | 2 * q_out.stride(0)) % 16 == 0)
+        for w in (q_norm, k_norm):
+            if ok and w is not None:
+                ok = w.dtype is BF16 and w.get_device() == dev and w.numel() == D and w.is_contiguous() and w.data_ptr() % 16 == 0
+    except (TypeError, ValueError, AttributeError):
+        ok = False
+    if not ok:
+        validate("fp4_append", qkv=qkv, cache=cache, slots=slots, positions=positions, cos_sin=cos_sin, q_norm=q_norm, k_norm=k_norm,
+                 q_out=q_out, num_q_heads=num_q_heads, rot_dim=rot, q_head_stride=hs, offsets=offsets)
+        T = qkv.shape[0]
     _declare()
+    a = AppendArgs()
     at = qkv.data_ptr()
     a.q, a.k, a.v = at + 2 * offsets[0], at + 2 * offsets[1], at + 2 * offsets[2]
-    a.ldq = a.ldk = a.ldv = qkv.stride(0)
+    if T > 1:                      # (the stride of a single row says nothing)
+        a.ldq = a.ldk = a.ldv = qkv.stride(0)
     if q_out is not None:
-        a.q_out, a.ldo = q_out.data_ptr(), q_out.stride(0)
+        a.q_out, a.ldo = q_out.data_ptr(), q_out.stride(0) if T > 1 else 0
     if cos_sin is not None:
         a.positions, a.cos_sin, a.table_rows, a.rot = positions.data_ptr(), cos_sin.data_ptr(), cos_sin.shape[0], rot
-    a.q_norm, a.k_norm, a.slots, a.cache = ptr(q_norm), ptr(k_norm), slots.data_ptr(), cache.data_ptr()
-    a.T, a.Hq, a.D, a.q_head_stride, a.neox, a.gemma, a.eps = qkv.shape[0], num_q_heads, D, hs, neox, gemma, eps
-    _launch(qkv.device, lambda s: lib().b200_fp4_append(ctypes.byref(a), s), "fp4_append")
+    if q_norm is not None:
+        a.q_norm = q_norm.data_ptr()
+    if k_norm is not None:
+        a.k_norm = k_norm.data_ptr()
+    a.num_blocks, a.Hkv, a.block_size, a.slots, a.cache = nb, H, bs, slots.data_ptr(), cache.data_ptr()
+    a.T, a.Hq, a.D, a.q_head_stride, a.neox, a.gemma, a.eps = T, num_q_heads, D, hs, neox, gemma, eps
+    _launch(qkv, _append, a, "fp4_append")
 
 
 def write(k: torch.Tensor, v: torch.Tensor, cache: torch.Tensor, slots: torch.Tensor) -> None:
@@ -125,22 +159,28 @@ def write(k: torch.Tensor, v: torch.Tensor, cache: torch.Tensor, slots: torch.Te
     _declare()
     a = AppendArgs()
     a.num_blocks, a.Hkv, a.block_size, a.D = shape_of(cache)
-    a.k, a.v, a.ldk, a.ldv = k.data_ptr(), v.data_ptr(), k.stride(0), v.stride(0)
+    a.k, a.v, a.ldk, a.ldv = k.data_ptr(), v.data_ptr(), *((k.stride(0), v.stride(0)) if k.shape[0] > 1 else (0, 0))
     a.slots, a.cache, a.T, a.eps = slots.data_ptr(), cache.data_ptr(), k.shape[0], 1.0
-    _launch(k.device, lambda s: lib().b200_fp4_append(ctypes.byref(a), s), "fp4_write")
+    _launch(k, _append, a, "fp4_write")
 
 
 def read(cache: torch.Tensor, slots: torch.Tensor, k: Optional[torch.Tensor] = None,
          v: Optional[torch.Tensor] = None) -> tuple[torch.Tensor, torch.Tensor]:
     """Keys and values bf16 ``[n, Hkv, D]`` that the cache holds for ``slots`` (int64 ``[n]``); zeros for slots outside the cache."""
-    validate("fp4_read", cache=cache, slots=slots, k=k, v=v)
+    nb, H, bs, D = shape_of(cache) if cache.dim() == 4 else (0, 0, 0, 0)
+    if not (k is None and v is None and cache.get_device() >= 0 and slots.get_device() == cache.get_device() and D in (64, 128, 256)
+            and cache.shape[3] == 18 * D and bs > 0 and cache.dtype is torch.uint8 and cache.is_contiguous() and cache.data_ptr() % 16 == 0
+            and slots.dtype is torch.int64 and slots.dim() == 1 and slots.is_contiguous()):
+        validate("fp4_read", cache=cache, slots=slots, k=k, v=v)
     _declare()
-    nb, H, bs, D = shape_of(cache)
-    n = slots.numel()
-    k = torch.empty((n, H, D), dtype=BF16, device=cache.device) if k is None else k
-    v = torch.empty((n, H, D), dtype=BF16, device=cache.device) if v is None else v
-    _launch(cache.device, lambda s: lib().b200_fp4_read(cache.data_ptr(), nb, bs, H, D, slots.data_ptr(), k.data_ptr(), k.stride(0),
-                                                        v.data_ptr(), v.stride(0), n, s), "fp4_read")
+    a = ReadArgs()
+    a.num_blocks, a.Hkv, a.block_size, a.D = nb, H, bs, D
+    n = a.n = slots.numel()
+    if k is None or v is None:
+        both = torch.empty((2, n, H, D), dtype=BF16, device=cache.device)
+        k, v = both[0] if k is None else k, both[1] if v is None else v
+    a.cache, a.slots, a.k, a.v = cache.data_ptr(), slots.data_ptr(), k.data_ptr(), v.data_ptr()
+    _launch(cache, _read, a, "fp4_read")
     return k, v
 
 
@@ -148,7 +188,7 @@ _scratch_floats: dict = {}
 
 
 def scratch_floats(device: torch.device, head_dim: int, prefill: bool) -> int:
-    key = (device.index, head_dim, prefill)
+    key = (device.index, head_dim, bool(prefill))
     n = _scratch_floats.get(key)
     if n is None:
         _declare()
@@ -163,28 +203,55 @@ def scratch(device: torch.device, head_dim: int, prefill: bool = True) -> torch.
     return torch.empty(scratch_floats(device, head_dim, prefill), dtype=torch.float32, device=device)
 
 
+_I32 = torch.int32
+
+
 def _attend(op, q, cache, block_table, seq_lens, q_start, tile_req, tile_q0, scale, out, softcap, window, causal, tmp):
     if out is None and q.is_cuda:
         out = torch.empty((q.shape[0], q.shape[1]), dtype=q.dtype, device=q.device)
-    validate(op, q=q, cache=cache, block_table=block_table, seq_lens=seq_lens, q_start=q_start, tile_req=tile_req, tile_q0=tile_q0,
-             out=out, scale=scale, softcap=softcap, tmp=tmp)
+    # What the rules of ops.validate say, in a fraction of their time (a decode step calls this in every layer); they name what is
+    # wrong, and judge what is rare.
+    try:
+        (rows, cols), (nb, H, cells, width), (reqs, pages), (n,) = q.shape, cache.shape, block_table.shape, seq_lens.shape
+        dev, D = q.get_device(), width // 18
+        ok = (dev >= 0 and dev == cache.get_device() == out.get_device() == block_table.get_device() == seq_lens.get_device()
+              and q.dtype is BF16 and out.dtype is BF16 and cache.dtype is torch.uint8 and block_table.dtype is _I32
+              and seq_lens.dtype is _I32 and D in (64, 128, 256) and width == 18 * D and cells > 0 and pages > 0 and cols > 0
+              and cols % (D * H) == 0 and out.shape == q.shape and cache.is_contiguous() and seq_lens.is_contiguous()
+              and q.stride(1) == 1 and out.stride(1) == 1 and block_table.stride(1) == 1 and scale > 0 and softcap >= 0
+              and (q.data_ptr() | out.data_ptr() | cache.data_ptr() | 2 * q.stride(0) | 2 * out.stride(0)) % 16 == 0
+              and q.data_ptr() != out.data_ptr()
+              and (tmp is None or (tmp.dtype is torch.float32 and tmp.get_device() == dev and tmp.is_contiguous()
+                                   and tmp.data_ptr() % 16 == 0 and tmp.numel() >= scratch_floats(q.device, D, q_start is not None))))
+        if q_start is None:
+            ok = ok and reqs >= rows and n >= rows
+        else:
+            ok = ok and (q_start.dtype is tile_req.dtype is tile_q0.dtype is _I32 and q_start.dim() == tile_req.dim() == tile_q0.dim() == 1
+                         and dev == q_start.get_device() == tile_req.get_device() == tile_q0.get_device() and q_start.numel() > 0
+                         and q_start.is_contiguous() and tile_req.is_contiguous() and tile_q0.is_contiguous()
+                         and tile_q0.numel() >= tile_req.numel())
+    except (TypeError, ValueError, AttributeError):
+        ok = False
+    if not ok:
+        validate(op, q=q, cache=cache, block_table=block_table, seq_lens=seq_lens, q_start=q_start, tile_req=tile_req,
+                 tile_q0=tile_q0, out=out, scale=scale, softcap=softcap, tmp=tmp)
+        (rows, cols), (nb, H, cells, width), (reqs, pages), (n,) = q.shape, cache.shape, block_table.shape, seq_lens.shape
+        D = width // 18
     _declare()
-    a = AttnArgs()
-    a.num_blocks, a.Hkv, a.block_size, D = shape_of(cache)
-    a.Hq, a.D = q.shape[1] // D, D
-    a.q, a.ldq, a.out, a.ldo, a.cache = q.data_ptr(), q.stride(0), out.data_ptr(), out.stride(0), cache.data_ptr()
-    a.block_table, a.ldt, a.max_blocks = block_table.data_ptr(), block_table.stride(0), block_table.shape[1]
-    a.seq_lens, a.total_q = seq_lens.data_ptr(), q.shape[0]
-    if q_start is None:
-        a.num_reqs = q.shape[0]
-    else:
-        a.q_start, a.num_reqs = q_start.data_ptr(), min(q_start.numel() - 1, block_table.shape[0], seq_lens.numel())
-        a.tile_req, a.tile_q0, a.num_tiles = tile_req.data_ptr(), tile_q0.data_ptr(), tile_req.numel()
-    a.window, a.causal, a.scale, a.softcap = window, causal, scale, softcap
     if tmp is None:
         tmp = scratch(q.device, D, q_start is not None)
-    a.parts = tmp.data_ptr()
-    _launch(q.device, lambda s: lib().b200_fp4_attn(ctypes.byref(a), s), op)
+    a = AttnArgs()
+    a.num_blocks, a.Hkv, a.block_size, a.Hq, a.D = nb, H, cells * CELL, cols // D, D
+    a.q, a.out, a.cache, a.parts = q.data_ptr(), out.data_ptr(), cache.data_ptr(), tmp.data_ptr()
+    if rows > 1:                   # (the stride of a single row says nothing)
+        a.ldq, a.ldo = q.stride(0), out.stride(0)
+    a.block_table, a.ldt, a.max_blocks = block_table.data_ptr(), block_table.stride(0), pages
+    a.seq_lens, a.total_q, a.num_reqs = seq_lens.data_ptr(), rows, rows
+    if q_start is not None:
+        a.q_start, a.num_reqs = q_start.data_ptr(), min(q_start.numel() - 1, reqs, n)
+        a.tile_req, a.tile_q0, a.num_tiles = tile_req.data_ptr(), tile_q0.data_ptr(), tile_req.numel()
+    a.window, a.causal, a.scale, a.softcap = window, causal, scale, softcap
+    _launch(q, _attn, a, op)
     return out
 
 
