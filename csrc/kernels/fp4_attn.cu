@@ -13,12 +13,15 @@
 // Work is shared out evenly whatever the lengths (fp4_work.cuh). The warps of a CTA take the cells of a piece in turn, fetched ahead by bulk copies
 // into a ring of their own. An item that lies in one stretch is finished there; of one that was cut the parts (m, l, O) go to scratch, and a second
 // kernel joins them.
+#include <type_traits>
+
 #include "api.h"
 #include "fp4_work.cuh"
 
 namespace b200 {
 
-static constexpr int kRowWarps = 8, kRowStages = 4;
+static constexpr int kRowWarps = 8, kRowStages = 2;
+static constexpr int kNoKey = 0x7fffff00;                // first key of a cell that is not there: behind every row
 
 __device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
@@ -39,12 +42,15 @@ __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t b
                : "memory");
 }
 
+// What is left of a wait whose first look found nothing.
+__device__ __noinline__ bool fp4_wait(uint64_t* bar, uint32_t parity, int* status) { return mbar_wait(bar, parity, status); }
+
 template <int D, int NT>
 struct Fp4RowsShape {
   static constexpr int kRows = 8 * NT, kMT = D / 16;
   static constexpr int kMergeTiles = kMT * NT <= 8 ? kMT : 8 / NT;                   // m-tiles of the merge buffer (32 KB)
   static constexpr int kMergeRow = kMergeTiles * 16 + 8;                             // floats of a row in it
-  static constexpr int kRingBytes = kRowWarps * kRowStages * Fp4Cell<D>::kBytes;
+  static constexpr int kRingBytes = kRowWarps * kRowStages * 2 * Fp4Cell<D>::kBytes;
   static constexpr int kMergeBytes = kRowWarps * kRows * kMergeRow * 4;
   static constexpr int kFixed = kRingBytes + kMergeBytes + kRowWarps * kRows * 8 + kRowWarps * kRowStages * 8;
 };
@@ -62,7 +68,7 @@ __global__ void __launch_bounds__(kRowWarps * 32, NT == 1 && D <= 128 ? 2 : 1) f
   uint64_t* bars = reinterpret_cast<uint64_t*>(sums + kRowWarps * kRows);
   uint32_t* line = reinterpret_cast<uint32_t*>(bars + kRowWarps * kRowStages);
   const int warp = warp_index(), lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  uint8_t* ring = smem + warp * kRowStages * Cell::kBytes;
+  uint8_t* ring = smem + warp * kRowStages * 2 * Cell::kBytes;
   uint64_t* full = bars + warp * kRowStages;
   if (lane < kRowStages) mbar_init(&full[lane], 1);
   mbar_fence_init();
@@ -70,46 +76,63 @@ __global__ void __launch_bounds__(kRowWarps * 32, NT == 1 && D <= 128 ? 2 : 1) f
   pdl_launch_dependents();
   fp4_line<Seq>(p, line);
   const uint32_t total = line[p.num_reqs], ctas = fp4_ctas(total, gridDim.x, kRowWarps);
-  if (blockIdx.x >= ctas) return;
-  const uint32_t from = fp4_begin<Seq>(p, line, total, blockIdx.x, ctas), to = fp4_begin<Seq>(p, line, total, blockIdx.x + 1, ctas);
+  const bool mine = blockIdx.x < ctas;
+  const uint32_t from = mine ? fp4_begin<Seq>(p, line, total, blockIdx.x, ctas) : 0, to = mine ? fp4_begin<Seq>(p, line, total, blockIdx.x + 1, ctas) : 0;
+  if (threadIdx.x == 0) fp4_say_cut<Seq, D>(p, line, total, ctas, from, to, parts);
+  if (from >= to) return;
 
-  // ---- fetching ahead: the warp's cells in their order, kRowStages of them in flight
+  // ---- fetching ahead: the warp's pairs of cells in their order, one on its way while another is worked on. Two neighbouring lanes have the
+  // addresses of one of the next 16 pairs.
   Fp4Piece<Seq> f;
   f.at(p, line, from, to);
-  int fc = f.c0 + warp, fj = 32, page = 0;      // next cell; page ids of the next 32 cells, a lane each
-  uint32_t bad = 0, phase = 0, flying = 0;      // of each stage: nothing was fetched (no such page); parity of its barrier; not waited for yet
+  int fc = f.c0 + warp, fj = 0, fn = 0;         // the next lot's first pair; next of this lot's, how many it has
+  const uint8_t* src = nullptr;
+  uint32_t have = 0;                            // cells of the lot that there are (behind the keys there is none, nor on a page outside the cache)
+  uint32_t held_cells = 0, phase = 0, flying = 0;       // of each stage: cells that it has (2 bits); parity of its barrier; not waited for yet
   const auto fetch = [&](int st) {
-    while (f.more() && fc >= f.c1) {
-      f.next(p, line);
-      fc = f.c0 + warp;
-      fj = 32;
-    }
-    if (!f.more()) return;
-    if (fj == 32) {
-      const int c = fc + lane * kRowWarps, pg = (f.e.begin + c) / p.cells_per_page;
-      page = c < f.c1 && pg < p.max_blocks && f.e.len > 0 ? p.block_table[f.b * p.ldt + pg] : -1;
+    if (fj == fn) {
+      while (f.more() && fc >= f.c1) {
+        f.next(p, line);
+        fc = f.c0 + warp;
+      }
+      if (!f.more()) return;
+      const int pair = fc + (lane >> 1) * kRowWarps, c = 2 * (f.e.begin + pair) + (lane & 1), pg = c / p.cells_per_page, h = f.item / f.e.tiles;
+      const int id = pair < f.c1 && c * kCellTokens < f.e.len ? p.block_table[f.b * p.ldt + pg] : -1;
+      src = id >= 0 && id < p.num_blocks
+                ? p.cache + (((long long)id * p.Hkv + h) * p.cells_per_page + (c - pg * p.cells_per_page)) * Cell::kBytes : nullptr;
+      have = __ballot_sync(0xffffffffu, src != nullptr);
       fj = 0;
+      fn = min(16, (f.c1 - fc + kRowWarps - 1) / kRowWarps);
+      fc += fn * kRowWarps;
     }
-    const int id = __shfl_sync(0xffffffffu, page, fj);
-    const bool there = id >= 0 && id < p.num_blocks;
-    bad = there ? bad & ~(1u << st) : bad | 1u << st;
-    flying |= there ? 1u << st : 0;
-    if (there && lane == 0) {
-      const int h = f.item / f.e.tiles, cell = (f.e.begin + fc) % p.cells_per_page;
-      mbar_expect_tx(&full[st], Cell::kBytes);
-      bulk_load(ring + st * Cell::kBytes, p.cache + (((long long)id * p.Hkv + h) * p.cells_per_page + cell) * Cell::kBytes, Cell::kBytes, &full[st]);
+    const uint32_t two = have & 3u;
+    have >>= 2;
+    held_cells = (held_cells & ~(3u << 2 * st)) | two << 2 * st;
+    if (two) {
+      flying |= 1u << st;
+      if ((lane >> 1) == fj) {
+        if (!(lane & 1)) mbar_expect_tx(&full[st], two == 3u ? 2 * Cell::kBytes : Cell::kBytes);
+        if (src) bulk_load(ring + (st * 2 + (lane & 1)) * Cell::kBytes, src, Cell::kBytes, &full[st]);
+      }
+      __syncwarp();
     }
-    __syncwarp();
-    fc += kRowWarps;
     ++fj;
   };
 #pragma unroll
   for (int st = 0; st < kRowStages; ++st) fetch(st);
   int st = 0;
   bool ok = true;
+  const float cap_in = p.softcap2 > 0.f ? 2.8853900817779268f / p.softcap2 : 0.f;
 
-  Fp4Piece<Seq> w;
-  for (w.at(p, line, from, to); w.more(); w.next(p, line)) {
+  __shared__ Fp4Piece<Seq> held[kRowWarps];      // each warp's piece, out of the registers of its loop over cells
+  Fp4Piece<Seq>& w = held[warp];
+  {
+    Fp4Piece<Seq> x;
+    x.at(p, line, from, to);
+    if (lane == 0) w = x;
+    __syncwarp();
+  }
+  while (w.more()) {
     const Seq& s = w.e;
     const int h = w.item / s.tiles, r0 = (w.item - h * s.tiles) * kRows, nrows = min(kRows, s.rows - r0), first = s.first;
     // ---- the tile's queries: B operand, lane (g, t) has dims [t D / 4, + D / 4) of row g
@@ -158,153 +181,187 @@ __global__ void __launch_bounds__(kRowWarps * 32, NT == 1 && D <= 128 ? 2 : 1) f
     const int least_hi = p.causal ? first + tok0 : s.len - 1, most_hi = p.causal ? first + tok1 : s.len - 1;
     const int most_lo = fp4_lowest(p, first + tok1), least_lo = fp4_lowest(p, first + tok0);
 
-    float o[NT][kMT][4], m[NT][2], l[NT][2];
+    // off: what is added to a score in log2 units, kUp less its row's reference
+    float o[NT][kMT][4], off[NT][2], l[NT][2];
+    const int k0 = 4 * (g >> 1) + (g & 1);                                       // the lane's key of a cell, and two on
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
       for (int i = 0; i < kMT; ++i)
 #pragma unroll
         for (int e = 0; e < 4; ++e) o[nt][i][e] = 0.f;
-      m[nt][0] = m[nt][1] = -INFINITY;
+      off[nt][0] = off[nt][1] = INFINITY;
       l[nt][0] = l[nt][1] = 0.f;
     }
-    for (int c = w.c0 + warp; c < w.c1; c += kRowWarps) {
-      const int key0 = (s.begin + c) * kCellTokens;
-      const bool there = !(bad >> st & 1);
-      if (there) {
-        if (ok) ok = __all_sync(0xffffffffu, mbar_wait(&full[st], phase >> st & 1, p.status));
+    const int c1 = w.c1, begin = s.begin, len = s.len;
+    for (int c = w.c0 + warp; c < c1; c += kRowWarps) {
+      const uint32_t two = held_cells >> 2 * st & 3u;
+      const int key = (begin + c) * kPairKeys;
+      if (two) {
+        if (ok && !mbar_try_wait(&full[st], phase >> st & 1)) ok = fp4_wait(&full[st], phase >> st & 1, p.status);
+        if (ok) ok = __all_sync(0xffffffffu, ok);
         if (ok) flying &= ~(1u << st);
         phase ^= 1u << st;
       }
-      if (there && ok && key0 <= most_hi && key0 + kCellTokens > least_lo) {
-        const uint8_t* cell = ring + st * Cell::kBytes;
+      if (two && ok && key <= most_hi && key + kPairKeys > least_lo) {
+        const uint8_t* cells[2] = {ring + st * 2 * Cell::kBytes, ring + (st * 2 + 1) * Cell::kBytes};
         // S^T: rows g and g + 8 of the tile are keys 4 (g / 2) + g % 2 and two on
-        const int k0 = 4 * (g >> 1) + (g & 1);
-        uint32_t kw[2][kKW], ks[2][kKW / 2];
+        float sc[2][NT][4];
 #pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          const uint8_t* row = cell + (k0 + 2 * r) * Cell::kRow + t * (D / 8);
-          const uint8_t* sc = cell + Cell::kKeyScales + (k0 + 2 * r) * Cell::kScales + t * (D / 64);
-          if constexpr (D == 64) {
-            const uint2 x = *reinterpret_cast<const uint2*>(row);
-            kw[r][0] = x.x; kw[r][1] = x.y;
-            ks[r][0] = scales_f16x2(*sc, 0, 0);
-          } else {
+        for (int u = 0; u < 2; ++u) {
+          uint32_t kw[2][kKW], ks[2][kKW / 2];
 #pragma unroll
-            for (int i = 0; i < kKW / 4; ++i) {
-              const uint4 x = *reinterpret_cast<const uint4*>(row + i * 16);
-              kw[r][4 * i] = x.x; kw[r][4 * i + 1] = x.y; kw[r][4 * i + 2] = x.z; kw[r][4 * i + 3] = x.w;
-              const uint32_t two = *reinterpret_cast<const uint16_t*>(sc + i * 2);
-              ks[r][2 * i] = scales_f16x2(two, 0, 0);
-              ks[r][2 * i + 1] = scales_f16x2(two, 1, 1);
-            }
-          }
-        }
-        float sc[NT][4];
+          for (int r = 0; r < 2; ++r) {
+            const uint8_t* row = cells[u] + (k0 + 2 * r) * Cell::kRow + t * (D / 8);
+            const uint8_t* sb = cells[u] + Cell::kKeyScales + (k0 + 2 * r) * Cell::kScales + t * (D / 64);
+            if constexpr (D == 64) {
+              const uint2 x = *reinterpret_cast<const uint2*>(row);
+              kw[r][0] = x.x; kw[r][1] = x.y;
+              ks[r][0] = scales_f16x2(*sb, 0, 0);
+            } else {
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) sc[nt][0] = sc[nt][1] = sc[nt][2] = sc[nt][3] = 0.f;
-#pragma unroll
-        for (int i = 0; i < kKW; ++i) {
-          uint32_t x[4], y[4];
-          cvt_e2m1x8(kw[0][i], x);
-          cvt_e2m1x8(kw[1][i], y);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            x[e] = mul_f16x2(x[e], ks[0][i >> 1]);
-            y[e] = mul_f16x2(y[e], ks[1][i >> 1]);
-          }
-          const uint32_t a0[4] = {x[0], y[0], x[1], y[1]}, a1[4] = {x[2], y[2], x[3], y[3]};
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt) {
-            mma_f16(sc[nt], a0, bq[nt][2 * i][0], bq[nt][2 * i][1]);
-            mma_f16(sc[nt], a1, bq[nt][2 * i + 1][0], bq[nt][2 * i + 1][1]);
-          }
-        }
-        const bool edge = key0 + kCellTokens - 1 > least_hi || key0 < most_lo;
-        uint32_t bp[NT][2];
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-          float over = -INFINITY;
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            float x = sc[nt][e] * mul[nt][e & 1];
-            if (p.softcap2 > 0.f) x = p.softcap2 * tanhf(x / p.softcap2);
-            if (edge) {
-              const int key = key0 + k0 + (e & 2);
-              if (key > hi[nt][e & 1] || key < lo[nt][e & 1]) x = -INFINITY;
-            }
-            sc[nt][e] = x;
-            over = fmaxf(over, x - m[nt][e & 1]);
-          }
-          // the reference is raised when a score passes it by 8 (p stays below 2^8), and at the first visible key
-          if (__any_sync(0xffffffffu, over > 8.f)) {
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              float x = fmaxf(sc[nt][e], sc[nt][e + 2]);
-#pragma unroll
-              for (int d = 4; d < 32; d <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, d));
-              x = fmaxf(x, m[nt][e]);
-              const float alpha = m[nt][e] == -INFINITY ? 0.f : ex2_of(m[nt][e] - x);
-              m[nt][e] = x;
-              l[nt][e] *= alpha;
-#pragma unroll
-              for (int i = 0; i < kMT; ++i) {
-                o[nt][i][e] *= alpha;
-                o[nt][i][e + 2] *= alpha;
+              for (int i = 0; i < kKW / 4; ++i) {
+                const uint4 x = *reinterpret_cast<const uint4*>(row + i * 16);
+                kw[r][4 * i] = x.x; kw[r][4 * i + 1] = x.y; kw[r][4 * i + 2] = x.z; kw[r][4 * i + 3] = x.w;
+                const uint32_t two = *reinterpret_cast<const uint16_t*>(sb + i * 2);
+                ks[r][2 * i] = scales_f16x2(two, 0, 0);
+                ks[r][2 * i + 1] = scales_f16x2(two, 1, 1);
               }
             }
           }
-          float pr[4];
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            pr[e] = ex2_of(sc[nt][e] - (m[nt][e & 1] == -INFINITY ? 0.f : m[nt][e & 1] - kUp));
-            l[nt][e & 1] += pr[e];
+          for (int nt = 0; nt < NT; ++nt) sc[u][nt][0] = sc[u][nt][1] = sc[u][nt][2] = sc[u][nt][3] = 0.f;
+#pragma unroll
+          for (int i = 0; i < kKW; ++i) {
+            uint32_t x[4], y[4];
+            cvt_e2m1x8(kw[0][i], x);
+            cvt_e2m1x8(kw[1][i], y);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              x[e] = mul_f16x2(x[e], ks[0][i >> 1]);
+              y[e] = mul_f16x2(y[e], ks[1][i >> 1]);
+            }
+            const uint32_t a0[4] = {x[0], y[0], x[1], y[1]}, a1[4] = {x[2], y[2], x[3], y[3]};
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+              mma_f16(sc[u][nt], a0, bq[nt][2 * i][0], bq[nt][2 * i][1]);
+              mma_f16(sc[u][nt], a1, bq[nt][2 * i + 1][0], bq[nt][2 * i + 1][1]);
+            }
           }
-          bp[nt][0] = transposed(pack_f16x2(pr[0], pr[1]));
-          bp[nt][1] = transposed(pack_f16x2(pr[2], pr[3]));
+        }
+        const bool edge = two != 3u || key + kPairKeys - 1 > least_hi || key < most_lo;
+        const int key0[2] = {two & 1 ? key : kNoKey, two & 2 ? key + kCellTokens : kNoKey};
+        uint32_t bp[2][NT][2];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          if (p.softcap2 > 0.f) {                      // (scores in log2 units from here on)
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) sc[u][nt][e] = fp4_capped(sc[u][nt][e], mul[nt][e & 1] * cap_in, p.softcap2);
+          }
+          const float m0 = p.softcap2 > 0.f ? 1.f : mul[nt][0], m1 = p.softcap2 > 0.f ? 1.f : mul[nt][1];
+          // exponents; the reference is raised when one passes it by 8 (p stays below 2^8 2^kUp), and at the first visible key (off is infinite)
+          float x[2][4], over = -INFINITY;
+          const auto exponents = [&] {
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) x[u][e] = fmaf(sc[u][nt][e], e & 1 ? m1 : m0, off[nt][e & 1]);
+            if (edge) {
+#pragma unroll
+              for (int u = 0; u < 2; ++u)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                  const int at = key0[u] + k0 + (e & 2);
+                  if (at > hi[nt][e & 1] || at < lo[nt][e & 1]) x[u][e] = -INFINITY;
+                }
+            }
+          };
+          exponents();
+#pragma unroll
+          for (int u = 0; u < 2; ++u) over = fmaxf(over, fmaxf(fmaxf(x[u][0], x[u][1]), fmaxf(x[u][2], x[u][3])));
+          if (__any_sync(0xffffffffu, over > 8.f + kUp)) {
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              float top = -INFINITY;
+#pragma unroll
+              for (int u = 0; u < 2; ++u)
+#pragma unroll
+                for (int i = e; i < 4; i += 2)
+                  if (x[u][i] != -INFINITY) top = fmaxf(top, sc[u][nt][i] * (e ? m1 : m0));
+#pragma unroll
+              for (int d = 4; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+              const float now = kUp - top;                                       // (+infinity where nothing is visible yet)
+              if (now < off[nt][e]) {
+                const float alpha = off[nt][e] == INFINITY ? 0.f : ex2_of(now - off[nt][e]);
+                off[nt][e] = now;
+                l[nt][e] *= alpha;
+#pragma unroll
+                for (int i = 0; i < kMT; ++i) {
+                  o[nt][i][e] *= alpha;
+                  o[nt][i][e + 2] *= alpha;
+                }
+              }
+            }
+            exponents();
+          }
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              x[u][e] = ex2_of(x[u][e]);
+              l[nt][e & 1] += x[u][e];
+            }
+            bp[u][nt][0] = transposed(pack_f16x2(x[u][0], x[u][1]));
+            bp[u][nt][1] = transposed(pack_f16x2(x[u][2], x[u][3]));
+          }
         }
         // O^T: lane (g, t) has keys 4t..4t+3 and dims [g D / 8, + D / 8); the m-tile i is its dims 2i (row g) and 2i + 1 (row g + 8)
-        uint32_t vw[4][kVW];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const uint8_t* at = cell + Cell::kValues + (((4 * t + j) * Cell::kRow + g * (D / 16)) ^ (32 * t));
-          if constexpr (D == 64) {
-            vw[j][0] = *reinterpret_cast<const uint32_t*>(at);
-          } else if constexpr (D == 128) {
-            const uint2 x = *reinterpret_cast<const uint2*>(at);
-            vw[j][0] = x.x; vw[j][1] = x.y;
-          } else {
-            const uint4 x = *reinterpret_cast<const uint4*>(at);
-            vw[j][0] = x.x; vw[j][1] = x.y; vw[j][2] = x.z; vw[j][3] = x.w;
+        for (int u = 0; u < 2; ++u) {
+          uint32_t vw[4][kVW];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const uint8_t* at = cells[u] + Cell::kValues + (((4 * t + j) * Cell::kRow + g * (D / 16)) ^ (32 * t));
+            if constexpr (D == 64) {
+              vw[j][0] = *reinterpret_cast<const uint32_t*>(at);
+            } else if constexpr (D == 128) {
+              const uint2 x = *reinterpret_cast<const uint2*>(at);
+              vw[j][0] = x.x; vw[j][1] = x.y;
+            } else {
+              const uint4 x = *reinterpret_cast<const uint4*>(at);
+              vw[j][0] = x.x; vw[j][1] = x.y; vw[j][2] = x.z; vw[j][3] = x.w;
+            }
           }
-        }
 #pragma unroll
-        for (int i = 0; i < kVW; ++i) {
-          const int group = (g * (D / 8) + 8 * i) / 16;
-          uint32_t scales = *reinterpret_cast<const uint32_t*>(cell + Cell::kValueScales + group * kCellTokens + 4 * t);
-          if (edge) {              // what lies behind the sequence or before every window may be anything: NaN times 0 too
-            const int key = key0 + 4 * t;
+          for (int i = 0; i < kVW; ++i) {
+            const int group = (g * (D / 8) + 8 * i) / 16;
+            uint32_t scales = *reinterpret_cast<const uint32_t*>(cells[u] + Cell::kValueScales + group * kCellTokens + 4 * t);
+            if (edge) {              // what lies behind the sequence or before every window may be anything: NaN times 0 too
+              const int at4 = key0[u] + 4 * t;
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-              if (key + j >= s.len || key + j < least_lo) scales &= ~(0xffu << (8 * j));
-          }
-          const uint32_t s01 = scales_f16x2(scales, 0, 1), s23 = scales_f16x2(scales, 2, 3);
-          uint32_t e01[4], d01[4], e23[4], d23[4];             // even dims, odd dims of key pairs
-          cvt_e2m1x8(low_nibbles_else(vw[0][i], vw[1][i] << 4), e01);
-          cvt_e2m1x8(low_nibbles_else(vw[0][i] >> 4, vw[1][i]), d01);
-          cvt_e2m1x8(low_nibbles_else(vw[2][i], vw[3][i] << 4), e23);
-          cvt_e2m1x8(low_nibbles_else(vw[2][i] >> 4, vw[3][i]), d23);
+              for (int j = 0; j < 4; ++j)
+                if (at4 + j >= len || at4 + j < least_lo) scales &= ~(0xffu << (8 * j));
+            }
+            const uint32_t s01 = scales_f16x2(scales, 0, 1), s23 = scales_f16x2(scales, 2, 3);
+            uint32_t e01[4], d01[4], e23[4], d23[4];             // even dims, odd dims of key pairs
+            cvt_e2m1x8(low_nibbles_else(vw[0][i], vw[1][i] << 4), e01);
+            cvt_e2m1x8(low_nibbles_else(vw[0][i] >> 4, vw[1][i]), d01);
+            cvt_e2m1x8(low_nibbles_else(vw[2][i], vw[3][i] << 4), e23);
+            cvt_e2m1x8(low_nibbles_else(vw[2][i] >> 4, vw[3][i]), d23);
 #pragma unroll
-          for (int y = 0; y < 4; ++y) {
-            const uint32_t a[4] = {mul_f16x2(e01[y], s01), mul_f16x2(d01[y], s01), mul_f16x2(e23[y], s23), mul_f16x2(d23[y], s23)};
+            for (int y = 0; y < 4; ++y) {
+              const uint32_t a[4] = {mul_f16x2(e01[y], s01), mul_f16x2(d01[y], s01), mul_f16x2(e23[y], s23), mul_f16x2(d23[y], s23)};
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) mma_f16(o[nt][4 * i + y], a, bp[nt][0], bp[nt][1]);
+              for (int nt = 0; nt < NT; ++nt) mma_f16(o[nt][4 * i + y], a, bp[u][nt][0], bp[u][nt][1]);
+            }
           }
         }
       }
       __syncwarp();
       if (ok) fetch(st);
-      if (++st == kRowStages) st = 0;
+      st ^= 1;
     }
     // ---- the warps' parts of the piece together
 #pragma unroll
@@ -315,7 +372,7 @@ __global__ void __launch_bounds__(kRowWarps * 32, NT == 1 && D <= 128 ? 2 : 1) f
 #pragma unroll
         for (int d = 4; d < 32; d <<= 1) x += __shfl_xor_sync(0xffffffffu, x, d);
         if (g == 0) {
-          top[warp * kRows + nt * 8 + 2 * t + e] = m[nt][e];
+          top[warp * kRows + nt * 8 + 2 * t + e] = kUp - off[nt][e];
           sums[warp * kRows + nt * 8 + 2 * t + e] = x;
         }
       }
@@ -328,7 +385,7 @@ __global__ void __launch_bounds__(kRowWarps * 32, NT == 1 && D <= 128 ? 2 : 1) f
         float x = -INFINITY;
 #pragma unroll
         for (int i = 0; i < kRowWarps; ++i) x = fmaxf(x, top[i * kRows + nt * 8 + 2 * t + e]);
-        scale[nt][e] = m[nt][e] == -INFINITY ? 0.f : ex2_of(m[nt][e] - x);
+        scale[nt][e] = off[nt][e] == INFINITY ? 0.f : ex2_of(kUp - off[nt][e] - x);
       }
     const bool whole = w.whole();
     float* part = parts + fp4_part<Seq, D>(blockIdx.x, w.part());
@@ -372,25 +429,29 @@ __global__ void __launch_bounds__(kRowWarps * 32, NT == 1 && D <= 128 ? 2 : 1) f
         }
       }
     }
-    __syncthreads();             // (top, sums and the buffer are written again)
+    Fp4Piece<Seq> x = w;
+    x.next(p, line);
+    __syncthreads();             // (top, sums and the buffer are written again, and the piece)
+    if (lane == 0) w = x;
+    __syncwarp();
   }
   // a wait ran out: what is still on its way to the ring gets the same time again before the CTA gives its memory up
   for (int i = 0; i < kRowStages && !ok; ++i)
     if (flying >> i & 1) mbar_wait(&full[i], phase >> i & 1, p.status);
 }
 
-// Parts of the row kernel's items, each by a block of its own, then those of the tile kernel's, each by kTileShares.
-static constexpr int kTileShares = 8;
+// Parts of the row kernel's items, each by kRowShares blocks, then those of the tile kernel's, each by kTileShares.
+static constexpr int kRowShares = 2;
+static constexpr int kTileShares = 32;
 template <int D, int ROWS>
-__global__ void __launch_bounds__(256) fp4_join_kernel(Fp4Attn p, const float* row_parts, int row_grid, const float* tile_parts, int tile_grid) {
-  extern __shared__ uint32_t line[];
+__global__ void __launch_bounds__(kJoinThreads) fp4_join_kernel(Fp4Attn p, float* row_parts, int row_grid, float* tile_parts, int tile_grid) {
   pdl_wait();
   pdl_launch_dependents();
-  if ((int)blockIdx.x < row_grid) {
-    fp4_join<Fp4Seq<ROWS>, D>(p, row_parts, line, blockIdx.x, row_grid, kRowWarps, 0, 1);
+  if ((int)blockIdx.x < row_grid * kRowShares) {
+    fp4_join<Fp4Seq<ROWS>, D>(p, row_parts, row_grid, blockIdx.x / kRowShares, blockIdx.x % kRowShares, kRowShares);
   } else if constexpr (D <= 128) {
-    const int i = blockIdx.x - row_grid;
-    fp4_join<Fp4Tile, D>(p, tile_parts, line, i / kTileShares, tile_grid, kTileLeast, i % kTileShares, kTileShares);
+    const int i = blockIdx.x - row_grid * kRowShares;
+    fp4_join<Fp4Tile, D>(p, tile_parts, tile_grid, i / kTileShares, i % kTileShares, kTileShares);
   }
 }
 
@@ -401,7 +462,7 @@ static int launch_attn(const Fp4Attn& p, bool rows, bool tiles, float* parts, cu
   using Shape = Fp4RowsShape<D, NT>;
   using Seq = Fp4Seq<Shape::kRows>;
   const int row_grid = rows ? b200_num_sms() * (NT == 1 && D <= 128 ? 2 : 1) : 0, tile_grid = tiles ? fp4_tile_grid() : 0;
-  float* tile_parts = parts + (size_t)row_grid * 2 * Seq::kRows * (D + 2);
+  float* tile_parts = parts + fp4_scratch<Seq, D>(row_grid);
   if (rows) {
     static PerDeviceOnce once;
     if (once.first())
@@ -412,9 +473,8 @@ static int launch_attn(const Fp4Attn& p, bool rows, bool tiles, float* parts, cu
   }
   if (tiles)
     if (const int rc = launch_fp4_tiles(p, D, tile_parts, stream)) return rc;
-  const size_t line = (size_t)((rows ? p.num_reqs : 0) > (tiles ? p.num_tiles : 0) ? p.num_reqs : tiles ? p.num_tiles : 0) * 4 + 4;
-  return launch_pdl(fp4_join_kernel<D, Shape::kRows>, dim3(row_grid + tile_grid * kTileShares), dim3(256), line, stream, p, (const float*)parts, row_grid,
-                    (const float*)tile_parts, tile_grid) == cudaSuccess ? 0 : -2;
+  return launch_pdl(fp4_join_kernel<D, Shape::kRows>, dim3(row_grid * kRowShares + tile_grid * kTileShares), dim3(kJoinThreads), 0, stream, p, parts, row_grid,
+                    tile_parts, tile_grid) == cudaSuccess ? 0 : -2;
 }
 
 }  // namespace b200
@@ -423,8 +483,14 @@ using namespace b200;
 
 // Floats of scratch that b200_fp4_attn needs (B200Fp4Attn.parts).
 extern "C" long long b200_fp4_attn_scratch(int D, int prefill) {
-  const long long sms = b200_num_sms();
-  return (sms * 2 * 16 * 2 + (prefill && D <= 128 ? (long long)fp4_tile_grid() * 2 * Fp4Tile::kRows : 0)) * (D + 2);
+  const auto floats = [&](auto d) {
+    constexpr int kD = decltype(d)::value;
+    const uint32_t sms = b200_num_sms();
+    const size_t one = fp4_scratch<Fp4Seq<8>, kD>(2 * sms), two = fp4_scratch<Fp4Seq<16>, kD>(sms);
+    return (long long)((one > two ? one : two) + (prefill && kD <= 128 ? fp4_scratch<Fp4Tile, kD>(fp4_tile_grid()) : 0));
+  };
+  return D == 64 ? floats(std::integral_constant<int, 64>()) : D == 128 ? floats(std::integral_constant<int, 128>())
+                                                                        : floats(std::integral_constant<int, 256>());
 }
 
 extern "C" int b200_fp4_attn(const B200Fp4Attn* a, cudaStream_t stream) {

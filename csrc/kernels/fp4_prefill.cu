@@ -102,6 +102,7 @@ __global__ void __launch_bounds__(512, 1) fp4_tiles_kernel(Fp4Attn p, float* par
   const bool mine = blockIdx.x < ctas;
   const uint32_t from = mine ? fp4_begin<Fp4Tile>(p, line, total, blockIdx.x, ctas) : 0;
   const uint32_t to = mine ? fp4_begin<Fp4Tile>(p, line, total, blockIdx.x + 1, ctas) : 0;
+  if (threadIdx.x == 0) fp4_say_cut<Fp4Tile, D>(p, line, total, ctas, from, to, parts);
   Fp4Piece<Fp4Tile>& w = held[warp];
   const auto begin = [&] {
     Fp4Piece<Fp4Tile> x;
@@ -286,18 +287,18 @@ __global__ void __launch_bounds__(512, 1) fp4_tiles_kernel(Fp4Attn p, float* par
       const Fp4TilePiece x(p, w);
       const int rr = x.r0 + t * 128 + r, token = rr / p.G, head = x.h * p.G + rr - token * p.G;
       const uint4* src = reinterpret_cast<const uint4*>(p.q + (long long)(w.e.token0 + token) * p.ldq + (long long)head * D);
-      const bool row = x.n > 0 && t * 128 + r < x.rows;
+      const bool row = w.more() && x.n > 0 && t * 128 + r < x.rows;      // (set in any case: what it held before is not kept)
 #pragma unroll
       for (int i = 0; i < D / 8; ++i) raw[i] = row ? src[i] : make_uint4(0, 0, 0, 0);
     };
     begin();
-    if (w.more()) query(w);
+    query(w);
     while (w.more() && ok) {
       const Fp4TilePiece x(p, w);
       if (t >= x.halves) {
         tiles += x.n;
         next();
-        if (w.more()) query(w);
+        query(w);
         continue;
       }
       const int n = x.n, k0 = x.k0;
@@ -349,12 +350,12 @@ __global__ void __launch_bounds__(512, 1) fp4_tiles_kernel(Fp4Attn p, float* par
         for (int c = 0; c < kTileKeys / 32; ++c) tmem_ld_32x32b_x32(s_addr + c * 32, s + c * 32);
         tmem_ld_wait();
         const int kbase = k0 + j * kTileKeys;
-        if (p.softcap2 > 0.f) {                                  // (scores in units of the cap from here on)
-          const float in = sc / p.softcap2;
+        if (p.softcap2 > 0.f) {                                  // (scores in log2 units from here on)
+          const float in = sc * (2.8853900817779268f / p.softcap2);
 #pragma unroll
-          for (int i = 0; i < kTileKeys; ++i) s[i] = __float_as_uint(tanhf(__uint_as_float(s[i]) * in));
+          for (int i = 0; i < kTileKeys; ++i) s[i] = __float_as_uint(fp4_capped(__uint_as_float(s[i]), in, p.softcap2));
         }
-        const float to_log2 = p.softcap2 > 0.f ? p.softcap2 : sc;
+        const float to_log2 = p.softcap2 > 0.f ? 1.f : sc;
         if (kbase + kTileKeys - 1 > hi || kbase < lo) {
 #pragma unroll
           for (int i = 0; i < kTileKeys; ++i)
@@ -430,7 +431,7 @@ __global__ void __launch_bounds__(512, 1) fp4_tiles_kernel(Fp4Attn p, float* par
       const Fp4Piece<Fp4Tile> now = w;
       const Fp4TilePiece y(p, now);
       next();
-      if (w.more()) query(w);
+      query(w);
       if (n > 0) {
         ok = __all_sync(0xffffffffu, mbar_wait(&bars.pv_done[t], pieces & 1, p.status));
         if (!ok) break;

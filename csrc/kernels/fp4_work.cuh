@@ -1,5 +1,5 @@
 // How attention over the 4-bit cache is shared out, for both of its kernels. An entry (a sequence, or a tile of 128 query tokens) has items (kv head,
-// row tile) that all read the same number of key cells. The cells of all items of all entries stand in one line, each CTA takes an equal stretch of
+// row tile) that all read the same number of cells (here: 32 or 128 neighbouring keys). The cells of all items of all entries stand in one line, each CTA takes an equal stretch of
 // it, and the parts of items that the ends of stretches cut are joined afterwards. What an item costs besides its cells (queries, output) stands in
 // the line as kStart cells in front of them: without, the CTAs that get the short items of a causal prompt's beginning finish last.
 #pragma once
@@ -52,6 +52,13 @@ __device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
 // the smallest ones keep their bits.
 static constexpr float kUp = 7.f;
 
+// cap tanh(x / cap) in log2 units: tanh(y) = 1 - 2 / (1 + e^(2 y)). Off by some 2^-22 of the cap, whatever y is; infinities and NaN go through.
+__device__ __forceinline__ float fp4_capped(float x, float to_y2, float cap2) {        // to_y2: x -> 2 y log2(e)
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.f + ex2_of(x * to_y2)));
+  return fmaf(-2.f * cap2, r, cap2);
+}
+
 // lowest position that the query at `pos` sees
 __device__ __forceinline__ int fp4_lowest(const Fp4Attn& p, int pos) {
   return p.window > 0 ? pos - p.window + 1 : p.window < 0 && pos >= 0 ? pos / -p.window * -p.window : 0;
@@ -67,10 +74,11 @@ struct Fp4Span {
 };
 
 // An entry's token0 is the query row of its first row, first that one's position, rows = tokens x G.
+static constexpr int kPairKeys = 2 * kCellTokens;
 template <int ROWS>
-struct Fp4Seq {                // cells of 16 keys, row tiles of ROWS
+struct Fp4Seq {                // pairs of cells, 32 keys; row tiles of ROWS
   static constexpr int kRows = ROWS, kStart = 0, kSnap = 0;
-  int req, len, token0, rows, first, begin, cells, tiles;       // begin: first cell of the sequence that any row sees
+  int req, len, token0, rows, first, begin, cells, tiles;       // begin: first pair of the sequence that any row sees
   static __device__ __forceinline__ int count(const Fp4Attn& p) { return p.num_reqs; }
   __device__ __forceinline__ Fp4Seq() {}
   __device__ __forceinline__ Fp4Seq(const Fp4Attn& p, int b) {
@@ -81,8 +89,8 @@ struct Fp4Seq {                // cells of 16 keys, row tiles of ROWS
     rows = s.q_len * p.G;
     if (rows > p.few) rows = 0;
     first = len - s.q_len;
-    begin = max(0, fp4_lowest(p, first)) / kCellTokens;
-    cells = kStart + max(1, (len + kCellTokens - 1) / kCellTokens - begin);          // (no keys: one cell that counts as masked)
+    begin = max(0, fp4_lowest(p, first)) / kPairKeys;
+    cells = kStart + max(1, (len + kPairKeys - 1) / kPairKeys - begin);          // (no keys: one that counts as masked)
     tiles = (rows + ROWS - 1) / ROWS;
   }
 };
@@ -197,47 +205,106 @@ struct Fp4Piece {
   __device__ __forceinline__ int part() const { return c0 == 0; }
 };
 
-// Scratch of a part: O [rows][D], then (m, l) of each row; in CTA order, two a CTA.
+// Scratch of a part: O [rows][D], then (m, l) of each row; in CTA order, two a CTA. Behind the parts a CTA says what of its last item is to be joined.
 template <class Entry, int D>
-__device__ __forceinline__ size_t fp4_part(uint32_t cta, int part) { return ((size_t)cta * 2 + part) * (Entry::kRows * (D + 2)); }
-
-// Joins the parts of cut items. Block i looks at the line where stretch i + 1 begins; the first cut of an item is the one that joins it: part 1 of the
-// CTA that begins it, part 0 of those behind. `share` of `shares` blocks takes every shares-th 4 dims.
+__host__ __device__ constexpr size_t fp4_part(uint32_t cta, int part) { return ((size_t)cta * 2 + part) * (Entry::kRows * (D + 2)); }
 template <class Entry, int D>
-__device__ __forceinline__ void fp4_join(const Fp4Attn& p, const float* parts, uint32_t* line, uint32_t i, uint32_t grid, int least, int share,
-                                         int shares) {
-  constexpr int kRows = Entry::kRows;
-  fp4_line<Entry>(p, line);
-  const int entries = Entry::count(p);
-  const uint32_t total = line[entries], ctas = fp4_ctas(total, grid, least);
-  if (i + 1 >= ctas) return;
-  const uint32_t u = fp4_begin<Entry>(p, line, total, i + 1, ctas);
-  if (u >= total) return;
-  const int b = fp4_find(line, entries, u);
-  const Entry e(p, b);
-  const uint32_t item = (u - line[b]) / (uint32_t)e.cells, begin = line[b] + item * e.cells;
-  if (begin == u || fp4_begin<Entry>(p, line, total, i, ctas) > begin) return;
-  const uint32_t last = (uint32_t)(((uint64_t)(begin + e.cells) * ctas - 1) / total);         // the CTA that has the item's last cell
-  const int h = item / e.tiles, r0 = (int)(item - h * e.tiles) * kRows, nrows = min(kRows, e.rows - r0);
-  for (int x = threadIdx.x + share * blockDim.x; x < nrows * (D / 4); x += shares * blockDim.x) {
-    const int r = x / (D / 4), d = x % (D / 4) * 4;
-    float mx = -INFINITY;
-    for (uint32_t c = i; c <= last; ++c) mx = fmaxf(mx, parts[fp4_part<Entry, D>(c, c == i) + kRows * D + 2 * r]);
-    float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-    float sum = 0.f;
-#pragma unroll 4
-    for (uint32_t c = i; c <= last; ++c) {
-      const float* part = parts + fp4_part<Entry, D>(c, c == i);
-      const float2 ml = *reinterpret_cast<const float2*>(part + kRows * D + 2 * r);
-      const float4 v = *reinterpret_cast<const float4*>(part + r * D + d);
-      const float f = ml.x == -INFINITY ? 0.f : ex2_of(ml.x - mx);
-      sum += ml.y * f;
-      a.x += v.x * f; a.y += v.y * f; a.z += v.z * f; a.w += v.w * f;
+__host__ __device__ constexpr size_t fp4_scratch(uint32_t grid) { return fp4_part<Entry, D>(grid, 0) + (size_t)grid * 8; }
+struct alignas(16) Fp4Cut {    // of an item that this CTA begins and CTAs up to `last` go on with; rows 0: none
+  int rows, last, token0, head0, row0, pad[3];
+};
+template <class Entry, int D>
+__device__ __forceinline__ Fp4Cut* fp4_cut(float* parts, uint32_t grid, uint32_t cta) {
+  return reinterpret_cast<Fp4Cut*>(parts + fp4_part<Entry, D>(grid, 0)) + cta;
+}
+// The last piece of a CTA's stretch, by one thread; a CTA without work: more() is false.
+template <class Entry, int D>
+__device__ __forceinline__ void fp4_say_cut(const Fp4Attn& p, const uint32_t* line, uint32_t total, uint32_t ctas, uint32_t from, uint32_t to,
+                                            float* parts) {
+  Fp4Cut c = {};
+  if (from < to) {
+    Fp4Piece<Entry> w;
+    w.at(p, line, to - 1, to);                                  // the stretch's last cell
+    const uint32_t begin = line[w.b] + (uint32_t)w.item * w.e.cells;
+    if (w.c1 < w.e.cells && begin >= from) {                    // its item goes on, and begins here
+      const int h = w.item / w.e.tiles;
+      c.row0 = (w.item - h * w.e.tiles) * Entry::kRows;
+      c.rows = min(Entry::kRows, w.e.rows - c.row0);
+      c.last = (int)(((uint64_t)(begin + w.e.cells) * ctas - 1) / total);       // the CTA that has the item's last cell
+      c.token0 = w.e.token0;
+      c.head0 = h * p.G;
     }
-    const float inv = sum == 0.f ? 0.f : 1.f / sum;
-    const int token = (r0 + r) / p.G, head = r0 + r - token * p.G;
-    *reinterpret_cast<uint2*>(p.out + (long long)(e.token0 + token) * p.ldo + (long long)(h * p.G + head) * D + d) =
-        make_uint2(pack_bf16x2(a.x * inv, a.y * inv), pack_bf16x2(a.z * inv, a.w * inv));
+  }
+  *fp4_cut<Entry, D>(parts, gridDim.x, blockIdx.x) = c;
+}
+
+// Joins the parts of the item that CTA i of the kernel before began: part 1 of that CTA, part 0 of those behind. A thread has 4 dims of a row; of more
+// than four parts four threads take every fourth each. Eight parts are on their way at a time. `share` of `shares` blocks takes every shares-th lot.
+static constexpr int kJoinThreads = 256;
+struct Fp4Sum {
+  float4 o;
+  float m, l;
+  __device__ __forceinline__ void add(const float4* v, const float2* ml, int n) {
+    float mx = m;
+    for (int k = 0; k < n; ++k) mx = fmaxf(mx, ml[k].x);
+    const float f0 = m == -INFINITY ? 0.f : ex2_of(m - mx);
+    m = mx;
+    l *= f0;
+    o.x *= f0; o.y *= f0; o.z *= f0; o.w *= f0;
+    for (int k = 0; k < n; ++k) {
+      const float f = ml[k].x == -INFINITY ? 0.f : ex2_of(ml[k].x - mx);
+      l += ml[k].y * f;
+      o.x += v[k].x * f; o.y += v[k].y * f; o.z += v[k].z * f; o.w += v[k].w * f;
+    }
+  }
+};
+template <class Entry, int D>
+__device__ __forceinline__ void fp4_join(const Fp4Attn& p, float* parts, uint32_t grid, int i, int share, int shares) {
+  constexpr int kRows = Entry::kRows;
+  __shared__ float4 sum_o[kJoinThreads];
+  __shared__ float2 sum_ml[kJoinThreads];
+  const Fp4Cut cut = *fp4_cut<Entry, D>(parts, grid, i);
+  const int turns = cut.last - i >= 4 ? 4 : 1, lot = kJoinThreads / turns;
+  const int lane = threadIdx.x & (lot - 1), turn = threadIdx.x / lot;
+  for (int x0 = share * lot; x0 < cut.rows * (D / 4); x0 += shares * lot) {
+    const int x = x0 + lane, r = x / (D / 4), d = x % (D / 4) * 4;
+    Fp4Sum sum = {make_float4(0.f, 0.f, 0.f, 0.f), -INFINITY, 0.f};
+    if (r < cut.rows) {
+      for (int c0 = i + turn; c0 <= cut.last; c0 += 8 * turns) {
+        float2 ml[8];
+        float4 v[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          const int c = c0 + k * turns;
+          const float* part = parts + fp4_part<Entry, D>(c, c == i);
+          ml[k] = c <= cut.last ? *reinterpret_cast<const float2*>(part + kRows * D + 2 * r) : make_float2(-INFINITY, 0.f);
+          v[k] = c <= cut.last ? *reinterpret_cast<const float4*>(part + r * D + d) : make_float4(0.f, 0.f, 0.f, 0.f);
+        }
+        sum.add(v, ml, 8);
+      }
+    }
+    if (turns > 1) {
+      sum_o[threadIdx.x] = sum.o;
+      sum_ml[threadIdx.x] = make_float2(sum.m, sum.l);
+      __syncthreads();
+      if (turn == 0) {
+        float4 v[3];
+        float2 ml[3];
+#pragma unroll
+        for (int k = 0; k < 3; ++k) {
+          v[k] = sum_o[(k + 1) * lot + lane];
+          ml[k] = sum_ml[(k + 1) * lot + lane];
+        }
+        sum.add(v, ml, 3);
+      }
+      __syncthreads();
+    }
+    if (turn == 0 && r < cut.rows) {
+      const float inv = sum.l == 0.f ? 0.f : 1.f / sum.l;
+      const int token = (cut.row0 + r) / p.G, head = cut.head0 + cut.row0 + r - token * p.G;
+      *reinterpret_cast<uint2*>(p.out + (long long)(cut.token0 + token) * p.ldo + (long long)head * D + d) =
+          make_uint2(pack_bf16x2(sum.o.x * inv, sum.o.y * inv), pack_bf16x2(sum.o.z * inv, sum.o.w * inv));
+    }
   }
 }
 
