@@ -20,52 +20,71 @@
 
 namespace b200 {
 
-static constexpr int kRowWarps = 8, kRowStages = 2;
+static constexpr int kRowStages = 2;
 static constexpr int kNoKey = 0x7fffff00;                // first key of a cell that is not there: behind every row
 
 __device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_f16_first(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
+      : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
 }
 __device__ __forceinline__ uint32_t transposed(uint32_t a) {
   uint32_t d;
-  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
   return d;
+}
+__device__ __forceinline__ uint32_t low_half2(uint32_t v) {          // (an operand of a multiplication picks the half)
+  const __half2 h = __low2half2(*reinterpret_cast<const __half2*>(&v));
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ uint32_t high_half2(uint32_t v) {
+  const __half2 h = __high2half2(*reinterpret_cast<const __half2*>(&v));
+  return *reinterpret_cast<const uint32_t*>(&h);
 }
 __device__ __forceinline__ uint32_t low_nibbles_else(uint32_t a, uint32_t b) {     // nibble 0, 2, .. of a, the others of b
   return (a & 0x0f0f0f0fu) | (b & 0xf0f0f0f0u);
 }
-__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
-  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_u32(dst)), "l"(src),
-               "r"(bytes), "r"(smem_u32(bar))
-               : "memory");
+// One lane announces `all` bytes (all != 0) and each lane with a source fetches `bytes` of them, without branches.
+__device__ __forceinline__ void bulk_pair(uint32_t dst, const uint8_t* src, uint32_t bytes, uint32_t bar, uint32_t all) {
+  asm volatile(
+      "{\n\t.reg .pred a, s;\n\t"
+      "setp.ne.u32 a, %4, 0;\n\t"
+      "setp.ne.u64 s, %1, 0;\n\t"
+      "@a mbarrier.arrive.expect_tx.shared::cta.b64 _, [%3], %4;\n\t"
+      "@s cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];\n\t}\n" ::"r"(dst),
+      "l"(src), "r"(bytes), "r"(bar), "r"(all)
+      : "memory");
 }
 
-// What is left of a wait whose first look found nothing.
-__device__ __noinline__ bool fp4_wait(uint64_t* bar, uint32_t parity, int* status) { return mbar_wait(bar, parity, status); }
+// What is left of a warp's wait whose first look found nothing.
+__device__ __noinline__ bool fp4_wait(uint64_t* bar, uint32_t parity, int* status) { return mbar_wait_warp(bar, parity, status); }
 
 template <int D, int NT>
 struct Fp4RowsShape {
+  static constexpr int kWarps = 8;
   static constexpr int kRows = 8 * NT, kMT = D / 16;
   static constexpr int kMergeTiles = kMT * NT <= 8 ? kMT : 8 / NT;                   // m-tiles of the merge buffer (32 KB)
   static constexpr int kMergeRow = kMergeTiles * 16 + 8;                             // floats of a row in it
-  static constexpr int kRingBytes = kRowWarps * kRowStages * 2 * Fp4Cell<D>::kBytes;
-  static constexpr int kMergeBytes = kRowWarps * kRows * kMergeRow * 4;
-  static constexpr int kFixed = kRingBytes + kMergeBytes + kRowWarps * kRows * 8 + kRowWarps * kRowStages * 8;
+  static constexpr int kRingBytes = kWarps * kRowStages * 2 * Fp4Cell<D>::kBytes;
+  static constexpr int kMergeBytes = kWarps * kRows * kMergeRow * 4;
+  static constexpr int kFixed = kRingBytes + kMergeBytes + kWarps * kRows * 8 + kWarps * kRowStages * 8;
 };
 
 template <int D, int NT>
-__global__ void __launch_bounds__(kRowWarps * 32, NT == 1 && D <= 128 ? 2 : 1) fp4_rows_kernel(Fp4Attn p, float* parts) {
+__global__ void __launch_bounds__(Fp4RowsShape<D, NT>::kWarps * 32, NT == 1 && D <= 128 ? 2 : 1) fp4_rows_kernel(Fp4Attn p, float* parts) {
   using Cell = Fp4Cell<D>;
   using Shape = Fp4RowsShape<D, NT>;
   using Seq = Fp4Seq<Shape::kRows>;
-  constexpr int kRows = Shape::kRows, kMT = Shape::kMT, kKW = D / 32, kVW = D / 64;   // m-tiles, words of a lane's keys and values
+  constexpr int kRowWarps = Shape::kWarps, kThreads = kRowWarps * 32, kRows = Shape::kRows, kMT = Shape::kMT, kKW = D / 32, kVW = D / 64;   // m-tiles, words of a lane's keys and values
   extern __shared__ __align__(128) uint8_t smem[];
   float* merge = reinterpret_cast<float*>(smem + Shape::kRingBytes);
-  float* top = reinterpret_cast<float*>(smem + Shape::kRingBytes + Shape::kMergeBytes);      // [warps][rows] m, then l
-  float* sums = top + kRowWarps * kRows;
-  uint64_t* bars = reinterpret_cast<uint64_t*>(sums + kRowWarps * kRows);
+  float2* top = reinterpret_cast<float2*>(smem + Shape::kRingBytes + Shape::kMergeBytes);    // [warps][rows] m, l
+  uint64_t* bars = reinterpret_cast<uint64_t*>(top + kRowWarps * kRows);
   uint32_t* line = reinterpret_cast<uint32_t*>(bars + kRowWarps * kRowStages);
   const int warp = warp_index(), lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   uint8_t* ring = smem + warp * kRowStages * 2 * Cell::kBytes;
@@ -85,24 +104,25 @@ __global__ void __launch_bounds__(kRowWarps * 32, NT == 1 && D <= 128 ? 2 : 1) f
   // addresses of one of the next 16 pairs.
   Fp4Piece<Seq> f;
   f.at(p, line, from, to);
-  int fc = f.c0 + warp, fj = 0, fn = 0;         // the next lot's first pair; next of this lot's, how many it has
+  int fc = f.from() + warp, fj = 0, fn = 0;         // the next lot's first pair; next of this lot's, how many it has
   const uint8_t* src = nullptr;
   uint32_t have = 0;                            // cells of the lot that there are (behind the keys there is none, nor on a page outside the cache)
   uint32_t held_cells = 0, phase = 0, flying = 0;       // of each stage: cells that it has (2 bits); parity of its barrier; not waited for yet
+  const uint32_t ring_at = smem_u32(ring) + (lane & 1) * Cell::kBytes, full_at = smem_u32(full);
   const auto fetch = [&](int st) {
     if (fj == fn) {
-      while (f.more() && fc >= f.c1) {
+      while (f.more() && fc >= f.to()) {
         f.next(p, line);
-        fc = f.c0 + warp;
+        fc = f.from() + warp;
       }
       if (!f.more()) return;
       const int pair = fc + (lane >> 1) * kRowWarps, c = 2 * (f.e.begin + pair) + (lane & 1), pg = c / p.cells_per_page, h = f.item / f.e.tiles;
-      const int id = pair < f.c1 && c * kCellTokens < f.e.len ? p.block_table[f.b * p.ldt + pg] : -1;
+      const int id = pair < f.to() && c * kCellTokens < f.e.len ? p.block_table[f.b * p.ldt + pg] : -1;
       src = id >= 0 && id < p.num_blocks
                 ? p.cache + (((long long)id * p.Hkv + h) * p.cells_per_page + (c - pg * p.cells_per_page)) * Cell::kBytes : nullptr;
       have = __ballot_sync(0xffffffffu, src != nullptr);
       fj = 0;
-      fn = min(16, (f.c1 - fc + kRowWarps - 1) / kRowWarps);
+      fn = min(16, (f.to() - fc + kRowWarps - 1) / kRowWarps);
       fc += fn * kRowWarps;
     }
     const uint32_t two = have & 3u;
@@ -110,10 +130,9 @@ __global__ void __launch_bounds__(kRowWarps * 32, NT == 1 && D <= 128 ? 2 : 1) f
     held_cells = (held_cells & ~(3u << 2 * st)) | two << 2 * st;
     if (two) {
       flying |= 1u << st;
-      if ((lane >> 1) == fj) {
-        if (!(lane & 1)) mbar_expect_tx(&full[st], two == 3u ? 2 * Cell::kBytes : Cell::kBytes);
-        if (src) bulk_load(ring + (st * 2 + (lane & 1)) * Cell::kBytes, src, Cell::kBytes, &full[st]);
-      }
+      const bool mine = (lane >> 1) == fj;
+      bulk_pair(ring_at + st * (2 * Cell::kBytes), mine ? src : nullptr, Cell::kBytes, full_at + st * 8,
+                lane == 2 * fj ? (two == 3u ? 2 * Cell::kBytes : Cell::kBytes) : 0);
       __syncwarp();
     }
     ++fj;
@@ -132,24 +151,34 @@ __global__ void __launch_bounds__(kRowWarps * 32, NT == 1 && D <= 128 ? 2 : 1) f
     if (lane == 0) w = x;
     __syncwarp();
   }
+  // queries: lane (g, t) has dims [t D / 4, + D / 4) of row g
+  uint4 raw[NT][D / 32];
+  const auto query = [&](const Fp4Piece<Seq>& x) {
+    const int h = x.more() ? x.item / x.e.tiles : 0, r0 = x.more() ? (x.item - h * x.e.tiles) * kRows : 0;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      const int r = r0 + nt * 8 + g, token = r / p.G, head = h * p.G + r - token * p.G;
+      const __nv_bfloat16* from = p.q + (long long)(x.e.token0 + token) * p.ldq + (long long)head * D + t * (D / 4);
+      const bool row = x.more() && r < x.e.rows;
+#pragma unroll
+      for (int i = 0; i < D / 32; ++i) raw[nt][i] = row ? *reinterpret_cast<const uint4*>(from + i * 8) : make_uint4(0, 0, 0, 0);
+    }
+  };
+  query(w);
+  bool first_piece = true;
   while (w.more()) {
     const Seq& s = w.e;
     const int h = w.item / s.tiles, r0 = (w.item - h * s.tiles) * kRows, nrows = min(kRows, s.rows - r0), first = s.first;
-    // ---- the tile's queries: B operand, lane (g, t) has dims [t D / 4, + D / 4) of row g
+    // ---- the tile's queries: B operand
     uint32_t bq[NT][D / 16][2];
     float mul[NT][2];                                                            // of the lane's rows 2t, 2t + 1: scores to log2 units
     int hi[NT][2], lo[NT][2];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-      const int r = r0 + nt * 8 + g, token = r / p.G, head = r - token * p.G;
-      const bool row = nt * 8 + g < nrows;
-      const __nv_bfloat16* src = p.q + (long long)(s.token0 + token) * p.ldq + (long long)(h * p.G + head) * D + t * (D / 4);
       float big = 0.f;
-      uint4 raw[D / 32];
 #pragma unroll
       for (int i = 0; i < D / 32; ++i) {
-        raw[i] = row ? *reinterpret_cast<const uint4*>(src + i * 8) : make_uint4(0, 0, 0, 0);
-        const uint32_t v[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+        const uint32_t v[4] = {raw[nt][i].x, raw[nt][i].y, raw[nt][i].z, raw[nt][i].w};
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const float2 x = unpack_bf16x2(v[e]);
@@ -162,7 +191,7 @@ __global__ void __launch_bounds__(kRowWarps * 32, NT == 1 && D <= 128 ? 2 : 1) f
       const float down = __uint_as_float((uint32_t)(127 - e2) << 23), up = __uint_as_float((uint32_t)(127 + e2) << 23);
 #pragma unroll
       for (int i = 0; i < D / 32; ++i) {
-        const uint32_t v[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+        const uint32_t v[4] = {raw[nt][i].x, raw[nt][i].y, raw[nt][i].z, raw[nt][i].w};
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const float2 x = unpack_bf16x2(v[e]);
@@ -193,13 +222,12 @@ __global__ void __launch_bounds__(kRowWarps * 32, NT == 1 && D <= 128 ? 2 : 1) f
       off[nt][0] = off[nt][1] = INFINITY;
       l[nt][0] = l[nt][1] = 0.f;
     }
-    const int c1 = w.c1, begin = s.begin, len = s.len;
-    for (int c = w.c0 + warp; c < c1; c += kRowWarps) {
+    const int c1 = w.to(), begin = s.begin, len = s.len;
+    for (int c = w.from() + warp; c < c1; c += kRowWarps) {
       const uint32_t two = held_cells >> 2 * st & 3u;
       const int key = (begin + c) * kPairKeys;
       if (two) {
-        if (ok && !mbar_try_wait(&full[st], phase >> st & 1)) ok = fp4_wait(&full[st], phase >> st & 1, p.status);
-        if (ok) ok = __all_sync(0xffffffffu, ok);
+        if (ok && !__all_sync(0xffffffffu, mbar_try_wait(&full[st], phase >> st & 1))) ok = fp4_wait(&full[st], phase >> st & 1, p.status);
         if (ok) flying &= ~(1u << st);
         phase ^= 1u << st;
       }
@@ -217,25 +245,23 @@ __global__ void __launch_bounds__(kRowWarps * 32, NT == 1 && D <= 128 ? 2 : 1) f
             if constexpr (D == 64) {
               const uint2 x = *reinterpret_cast<const uint2*>(row);
               kw[r][0] = x.x; kw[r][1] = x.y;
-              ks[r][0] = scales_f16x2(*sb, 0, 0);
+              ks[r][0] = *sb * 0x800080u;
             } else {
 #pragma unroll
               for (int i = 0; i < kKW / 4; ++i) {
                 const uint4 x = *reinterpret_cast<const uint4*>(row + i * 16);
                 kw[r][4 * i] = x.x; kw[r][4 * i + 1] = x.y; kw[r][4 * i + 2] = x.z; kw[r][4 * i + 3] = x.w;
-                const uint32_t two = *reinterpret_cast<const uint16_t*>(sb + i * 2);
-                ks[r][2 * i] = scales_f16x2(two, 0, 0);
-                ks[r][2 * i + 1] = scales_f16x2(two, 1, 1);
+                const uint32_t pair = scales_f16x2(*reinterpret_cast<const uint16_t*>(sb + i * 2), 0, 1);
+                ks[r][2 * i] = low_half2(pair);
+                ks[r][2 * i + 1] = high_half2(pair);
               }
             }
           }
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt) sc[u][nt][0] = sc[u][nt][1] = sc[u][nt][2] = sc[u][nt][3] = 0.f;
-#pragma unroll
           for (int i = 0; i < kKW; ++i) {
             uint32_t x[4], y[4];
-            cvt_e2m1x8(kw[0][i], x);
-            cvt_e2m1x8(kw[1][i], y);
+            e2m1x8_f16(kw[0][i], x);
+            e2m1x8_f16(kw[1][i], y);
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
               x[e] = mul_f16x2(x[e], ks[0][i >> 1]);
@@ -244,13 +270,22 @@ __global__ void __launch_bounds__(kRowWarps * 32, NT == 1 && D <= 128 ? 2 : 1) f
             const uint32_t a0[4] = {x[0], y[0], x[1], y[1]}, a1[4] = {x[2], y[2], x[3], y[3]};
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
-              mma_f16(sc[u][nt], a0, bq[nt][2 * i][0], bq[nt][2 * i][1]);
+              if (i == 0) mma_f16_first(sc[u][nt], a0, bq[nt][0][0], bq[nt][0][1]);
+              else mma_f16(sc[u][nt], a0, bq[nt][2 * i][0], bq[nt][2 * i][1]);
               mma_f16(sc[u][nt], a1, bq[nt][2 * i + 1][0], bq[nt][2 * i + 1][1]);
             }
           }
         }
         const bool edge = two != 3u || key + kPairKeys - 1 > least_hi || key < most_lo;
         const int key0[2] = {two & 1 ? key : kNoKey, two & 2 ? key + kCellTokens : kNoKey};
+        uint32_t keep[2] = {0xffffffffu, 0xffffffffu};     // of the scales of the lane's four values
+        if (edge) {                  // what lies behind the sequence or before every window may be anything: NaN times 0 too
+#pragma unroll
+          for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              if (key0[u] + 4 * t + j >= len || key0[u] + 4 * t + j < least_lo) keep[u] &= ~(0xffu << (8 * j));
+        }
         uint32_t bp[2][NT][2];
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
@@ -337,19 +372,13 @@ __global__ void __launch_bounds__(kRowWarps * 32, NT == 1 && D <= 128 ? 2 : 1) f
 #pragma unroll
           for (int i = 0; i < kVW; ++i) {
             const int group = (g * (D / 8) + 8 * i) / 16;
-            uint32_t scales = *reinterpret_cast<const uint32_t*>(cells[u] + Cell::kValueScales + group * kCellTokens + 4 * t);
-            if (edge) {              // what lies behind the sequence or before every window may be anything: NaN times 0 too
-              const int at4 = key0[u] + 4 * t;
-#pragma unroll
-              for (int j = 0; j < 4; ++j)
-                if (at4 + j >= len || at4 + j < least_lo) scales &= ~(0xffu << (8 * j));
-            }
+            const uint32_t scales = *reinterpret_cast<const uint32_t*>(cells[u] + Cell::kValueScales + group * kCellTokens + 4 * t) & keep[u];
             const uint32_t s01 = scales_f16x2(scales, 0, 1), s23 = scales_f16x2(scales, 2, 3);
             uint32_t e01[4], d01[4], e23[4], d23[4];             // even dims, odd dims of key pairs
-            cvt_e2m1x8(low_nibbles_else(vw[0][i], vw[1][i] << 4), e01);
-            cvt_e2m1x8(low_nibbles_else(vw[0][i] >> 4, vw[1][i]), d01);
-            cvt_e2m1x8(low_nibbles_else(vw[2][i], vw[3][i] << 4), e23);
-            cvt_e2m1x8(low_nibbles_else(vw[2][i] >> 4, vw[3][i]), d23);
+            e2m1x8_f16(low_nibbles_else(vw[0][i], vw[1][i] << 4), e01);
+            e2m1x8_f16(low_nibbles_else(vw[0][i] >> 4, vw[1][i]), d01);
+            e2m1x8_f16(low_nibbles_else(vw[2][i], vw[3][i] << 4), e23);
+            e2m1x8_f16(low_nibbles_else(vw[2][i] >> 4, vw[3][i]), d23);
 #pragma unroll
             for (int y = 0; y < 4; ++y) {
               const uint32_t a[4] = {mul_f16x2(e01[y], s01), mul_f16x2(d01[y], s01), mul_f16x2(e23[y], s23), mul_f16x2(d23[y], s23)};
@@ -363,78 +392,74 @@ __global__ void __launch_bounds__(kRowWarps * 32, NT == 1 && D <= 128 ? 2 : 1) f
       if (ok) fetch(st);
       st ^= 1;
     }
-    // ---- the warps' parts of the piece together
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        float x = l[nt][e];
-#pragma unroll
-        for (int d = 4; d < 32; d <<= 1) x += __shfl_xor_sync(0xffffffffu, x, d);
-        if (g == 0) {
-          top[warp * kRows + nt * 8 + 2 * t + e] = kUp - off[nt][e];
-          sums[warp * kRows + nt * 8 + 2 * t + e] = x;
-        }
-      }
-    __syncthreads();
-    float scale[NT][2];
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        float x = -INFINITY;
-#pragma unroll
-        for (int i = 0; i < kRowWarps; ++i) x = fmaxf(x, top[i * kRows + nt * 8 + 2 * t + e]);
-        scale[nt][e] = off[nt][e] == INFINITY ? 0.f : ex2_of(kUp - off[nt][e] - x);
-      }
+    // ---- the warps' parts of the piece together; the next piece's queries are on their way meanwhile
     const bool whole = w.whole();
     float* part = parts + fp4_part<Seq, D>(blockIdx.x, w.part());
+    const int token0 = s.token0;
+    {
+      Fp4Piece<Seq> x = w;
+      x.next(p, line);
+      query(x);
+      __syncwarp();
+      if (lane == 0) w = x;
+      __syncwarp();
+    }
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int e = 0; e < 2; ++e)
+#pragma unroll
+        for (int d = 4; d < 32; d <<= 1) l[nt][e] += __shfl_xor_sync(0xffffffffu, l[nt][e], d);
     constexpr int kMC = Shape::kMergeTiles, kMR = Shape::kMergeRow;
 #pragma unroll
     for (int i0 = 0; i0 < kMT; i0 += kMC) {
-      if (i0) __syncthreads();
+      // all have read what was there before (they say so, and go on): barrier 1
+      if (!first_piece || i0) asm volatile("bar.sync 1, %0;" ::"n"(2 * kThreads) : "memory");
+      if (i0 == 0 && g == 0) {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) top[warp * kRows + nt * 8 + 2 * t + e] = make_float2(kUp - off[nt][e], l[nt][e]);
+      }
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int i = 0; i < kMC; ++i)
+        for (int e = 0; e < 2; ++e)
+          if (nt * 8 + 2 * t + e < nrows) {
 #pragma unroll
-          for (int e = 0; e < 2; ++e)
-            *reinterpret_cast<float2*>(merge + (warp * kRows + nt * 8 + 2 * t + e) * kMR + (i * 8 + g) * 2) =
-                make_float2(o[nt][i0 + i][e] * scale[nt][e], o[nt][i0 + i][e + 2] * scale[nt][e]);
+            for (int i = 0; i < kMC; ++i)
+              *reinterpret_cast<float2*>(merge + (warp * kRows + nt * 8 + 2 * t + e) * kMR + (i * 8 + g) * 2) =
+                  make_float2(o[nt][i0 + i][e], o[nt][i0 + i][e + 2]);
+          }
       __syncthreads();
-      for (int x = threadIdx.x; x < nrows * kMC * 8; x += kRowWarps * 32) {
+      for (int x = threadIdx.x; x < nrows * kMC * 8; x += kThreads) {
         const int i = x % kMC, gg = x / kMC % 8, r = x / (kMC * 8), d = gg * (D / 8) + 2 * (i0 + i);
         float a = 0.f, b = 0.f, mx = -INFINITY, sum = 0.f;
 #pragma unroll
-        for (int y = 0; y < kRowWarps; ++y) {
-          const float2 v = *reinterpret_cast<const float2*>(merge + (y * kRows + r) * kMR + (i * 8 + gg) * 2);
-          a += v.x;
-          b += v.y;
-          mx = fmaxf(mx, top[y * kRows + r]);
-        }
+        for (int y = 0; y < kRowWarps; ++y) mx = fmaxf(mx, top[y * kRows + r].x);
 #pragma unroll
-        for (int y = 0; y < kRowWarps; ++y)
-          sum += top[y * kRows + r] == -INFINITY ? 0.f : sums[y * kRows + r] * ex2_of(top[y * kRows + r] - mx);
+        for (int y = 0; y < kRowWarps; ++y) {
+          const float2 ml = top[y * kRows + r], v = *reinterpret_cast<const float2*>(merge + (y * kRows + r) * kMR + (i * 8 + gg) * 2);
+          const float f = ml.x == -INFINITY ? 0.f : ex2_of(ml.x - mx);
+          a = fmaf(v.x, f, a);
+          b = fmaf(v.y, f, b);
+          sum = fmaf(ml.y, f, sum);
+        }
         if (whole) {
           const int token = (r0 + r) / p.G, head = r0 + r - token * p.G;
           const float inv = sum == 0.f ? 0.f : 1.f / sum;
-          *reinterpret_cast<uint32_t*>(p.out + (long long)(s.token0 + token) * p.ldo + (long long)(h * p.G + head) * D + d) =
+          *reinterpret_cast<uint32_t*>(p.out + (long long)(token0 + token) * p.ldo + (long long)(h * p.G + head) * D + d) =
               pack_bf16x2(a * inv, b * inv);
         } else {
           *reinterpret_cast<float2*>(part + r * D + d) = make_float2(a, b);
-          if (d == 0) {
-            part[kRows * D + 2 * r] = mx;
-            part[kRows * D + 2 * r + 1] = sum;
-          }
+          if (d == 0) *reinterpret_cast<float2*>(part + kRows * D + 2 * r) = make_float2(mx, sum);
         }
       }
+      asm volatile("bar.arrive 1, %0;" ::"n"(2 * kThreads) : "memory");
     }
-    Fp4Piece<Seq> x = w;
-    x.next(p, line);
-    __syncthreads();             // (top, sums and the buffer are written again, and the piece)
-    if (lane == 0) w = x;
-    __syncwarp();
+    first_piece = false;
   }
+  if (!first_piece) asm volatile("bar.sync 1, %0;" ::"n"(2 * kThreads) : "memory");      // (nobody leaves while others' arrivals are pending)
   // a wait ran out: what is still on its way to the ring gets the same time again before the CTA gives its memory up
   for (int i = 0; i < kRowStages && !ok; ++i)
     if (flying >> i & 1) mbar_wait(&full[i], phase >> i & 1, p.status);
@@ -467,7 +492,7 @@ static int launch_attn(const Fp4Attn& p, bool rows, bool tiles, float* parts, cu
     static PerDeviceOnce once;
     if (once.first())
       cudaFuncSetAttribute(fp4_rows_kernel<D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape::kFixed + (kMostReqs + 1) * 4);
-    if (launch_pdl(fp4_rows_kernel<D, NT>, dim3(row_grid), dim3(kRowWarps * 32), Shape::kFixed + (size_t)(p.num_reqs + 1) * 4, stream, p, parts) !=
+    if (launch_pdl(fp4_rows_kernel<D, NT>, dim3(row_grid), dim3(Shape::kWarps * 32), Shape::kFixed + (size_t)(p.num_reqs + 1) * 4, stream, p, parts) !=
         cudaSuccess)
       return -2;
   }

@@ -264,7 +264,7 @@ __global__ void __launch_bounds__(512, 1) fp4_tiles_kernel(Fp4Attn p, float* par
             const int g = 2 * k + (e >> 1), piece = 4 * k + e;                   // scale, 16 bytes of the row
             const uint32_t sc = scales_f16x2(s[g / 4], g % 4, g % 4);
             uint32_t v[4];
-            cvt_e2m1x8(word[e], v);
+            e2m1x8_f16(word[e], v);
             *reinterpret_cast<uint4*>(row + (piece / 8) * Shape::kPlane + (((piece % 8) ^ (r & 7)) << 4)) =
                 make_uint4(mul_f16x2(v[0], sc), mul_f16x2(v[1], sc), mul_f16x2(v[2], sc), mul_f16x2(v[3], sc));
           }

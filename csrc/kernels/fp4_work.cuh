@@ -1,7 +1,8 @@
 // How attention over the 4-bit cache is shared out, for both of its kernels. An entry (a sequence, or a tile of 128 query tokens) has items (kv head,
 // row tile) that all read the same number of cells (here: 32 or 128 neighbouring keys). The cells of all items of all entries stand in one line, each CTA takes an equal stretch of
 // it, and the parts of items that the ends of stretches cut are joined afterwards. What an item costs besides its cells (queries, output) stands in
-// the line as kStart cells in front of them: without, the CTAs that get the short items of a causal prompt's beginning finish last.
+// the line as kStart cells in front of them: without, the CTAs that get the short items (of a causal prompt's beginning, of short sequences) finish
+// last.
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -41,6 +42,17 @@ __device__ __forceinline__ uint32_t mul_f16x2(uint32_t a, uint32_t b) {
   asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
   return d;
 }
+// cvt_e2m1x8 that the compiler may move.
+__device__ __forceinline__ void e2m1x8_f16(uint32_t w, uint32_t (&h)[4]) {
+  asm("{\n\t.reg .b8 b0, b1, b2, b3;\n\t"
+      "mov.b32 {b0, b1, b2, b3}, %4;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %0, b0;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %1, b1;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %2, b2;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %3, b3;\n\t}\n"
+      : "=r"(h[0]), "=r"(h[1]), "=r"(h[2]), "=r"(h[3])
+      : "r"(w));
+}
 // Scale bytes lo and hi (selectors of __byte_perm) of w -> f16x2.
 __device__ __forceinline__ uint32_t scales_f16x2(uint32_t w, int lo, int hi) { return __byte_perm(w, 0, 0x4040 | lo | hi << 8) << 7; }
 __device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
@@ -77,7 +89,7 @@ struct Fp4Span {
 static constexpr int kPairKeys = 2 * kCellTokens;
 template <int ROWS>
 struct Fp4Seq {                // pairs of cells, 32 keys; row tiles of ROWS
-  static constexpr int kRows = ROWS, kStart = 0, kSnap = 0;
+  static constexpr int kRows = ROWS, kStart = 8, kSnap = 8;
   int req, len, token0, rows, first, begin, cells, tiles;       // begin: first pair of the sequence that any row sees
   static __device__ __forceinline__ int count(const Fp4Attn& p) { return p.num_reqs; }
   __device__ __forceinline__ Fp4Seq() {}
@@ -161,7 +173,7 @@ __device__ __forceinline__ uint32_t fp4_ctas(uint32_t total, uint32_t grid, int 
 template <class Entry>
 __device__ __forceinline__ uint32_t fp4_begin(const Fp4Attn& p, const uint32_t* line, uint32_t total, uint32_t i, uint32_t ctas) {
   const uint32_t u = (uint32_t)((uint64_t)total * i / ctas);
-  if (Entry::kSnap == 0 || u == 0 || u >= total) return u;
+  if (u == 0 || u >= total) return u;
   const int b = fp4_find(line, Entry::count(p), u);
   const uint32_t n = Entry(p, b).cells, off = (u - line[b]) % n;
   return n <= Entry::kSnap + Entry::kStart ? u - off + (2 * off >= n ? n : 0) : off <= Entry::kStart ? u - off : u;
