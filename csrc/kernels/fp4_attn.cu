@@ -24,18 +24,18 @@ static constexpr int kRowStages = 2;
 static constexpr int kNoKey = 0x7fffff00;                // first key of a cell that is not there: behind every row
 
 __device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 __device__ __forceinline__ void mma_f16_first(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
       : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
 }
 __device__ __forceinline__ uint32_t transposed(uint32_t a) {
   uint32_t d;
-  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
   return d;
 }
 __device__ __forceinline__ uint32_t low_half2(uint32_t v) {          // (an operand of a multiplication picks the half)
@@ -49,18 +49,17 @@ __device__ __forceinline__ uint32_t high_half2(uint32_t v) {
 __device__ __forceinline__ uint32_t low_nibbles_else(uint32_t a, uint32_t b) {     // nibble 0, 2, .. of a, the others of b
   return (a & 0x0f0f0f0fu) | (b & 0xf0f0f0f0u);
 }
-// One lane announces `all` bytes (all != 0) and each lane with a source fetches `bytes` of them, without branches.
-__device__ __forceinline__ void bulk_pair(uint32_t dst, const uint8_t* src, uint32_t bytes, uint32_t bar, uint32_t all) {
+// The lane that `says` announces `all` bytes and each lane with a source fetches `bytes` of them, without branches.
+__device__ __forceinline__ void bulk_pair(uint32_t dst, const uint8_t* src, uint32_t bytes, uint32_t bar, bool says, uint32_t all) {
   asm volatile(
       "{\n\t.reg .pred a, s;\n\t"
       "setp.ne.u32 a, %4, 0;\n\t"
       "setp.ne.u64 s, %1, 0;\n\t"
-      "@a mbarrier.arrive.expect_tx.shared::cta.b64 _, [%3], %4;\n\t"
+      "@a mbarrier.arrive.expect_tx.shared::cta.b64 _, [%3], %5;\n\t"
       "@s cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];\n\t}\n" ::"r"(dst),
-      "l"(src), "r"(bytes), "r"(bar), "r"(all)
+      "l"(src), "r"(bytes), "r"(bar), "r"((uint32_t)says), "r"(all)
       : "memory");
 }
-
 // What is left of a warp's wait whose first look found nothing.
 __device__ __noinline__ bool fp4_wait(uint64_t* bar, uint32_t parity, int* status) { return mbar_wait_warp(bar, parity, status); }
 
@@ -107,7 +106,8 @@ __global__ void __launch_bounds__(Fp4RowsShape<D, NT>::kWarps * 32, NT == 1 && D
   int fc = f.from() + warp, fj = 0, fn = 0;         // the next lot's first pair; next of this lot's, how many it has
   const uint8_t* src = nullptr;
   uint32_t have = 0;                            // cells of the lot that there are (behind the keys there is none, nor on a page outside the cache)
-  uint32_t held_cells = 0, phase = 0, flying = 0;       // of each stage: cells that it has (2 bits); parity of its barrier; not waited for yet
+  uint32_t cells_at[2] = {0, 0};                // cells (bit 0, bit 1) of the pair that is worked on next, and of the one behind it
+  int issued = 0;                               // pairs that were fetched and not waited for
   const uint32_t ring_at = smem_u32(ring) + (lane & 1) * Cell::kBytes, full_at = smem_u32(full);
   const auto fetch = [&](int st) {
     if (fj == fn) {
@@ -125,21 +125,21 @@ __global__ void __launch_bounds__(Fp4RowsShape<D, NT>::kWarps * 32, NT == 1 && D
       fn = min(16, (f.to() - fc + kRowWarps - 1) / kRowWarps);
       fc += fn * kRowWarps;
     }
-    const uint32_t two = have & 3u;
+    const uint32_t two = have & 3u;               // (none: the barrier's phase ends at once)
     have >>= 2;
-    held_cells = (held_cells & ~(3u << 2 * st)) | two << 2 * st;
-    if (two) {
-      flying |= 1u << st;
-      const bool mine = (lane >> 1) == fj;
-      bulk_pair(ring_at + st * (2 * Cell::kBytes), mine ? src : nullptr, Cell::kBytes, full_at + st * 8,
-                lane == 2 * fj ? (two == 3u ? 2 * Cell::kBytes : Cell::kBytes) : 0);
-      __syncwarp();
-    }
+    cells_at[1] = two;
+    const bool mine = (lane >> 1) == fj;
+    bulk_pair(ring_at + st * (2 * Cell::kBytes), mine ? src : nullptr, Cell::kBytes, full_at + st * 8, lane == 2 * fj,
+              __popc(two) * Cell::kBytes);
+    __syncwarp();
+    ++issued;
     ++fj;
   };
-#pragma unroll
-  for (int st = 0; st < kRowStages; ++st) fetch(st);
+  fetch(0);
+  cells_at[0] = cells_at[1];
+  fetch(1);
   int st = 0;
+  uint32_t parity = 0;
   bool ok = true;
   const float cap_in = p.softcap2 > 0.f ? 2.8853900817779268f / p.softcap2 : 0.f;
 
@@ -207,7 +207,7 @@ __global__ void __launch_bounds__(Fp4RowsShape<D, NT>::kWarps * 32, NT == 1 && D
       }
     }
     const int tok0 = r0 / p.G, tok1 = (r0 + nrows - 1) / p.G;                    // the tile's tokens
-    const int least_hi = p.causal ? first + tok0 : s.len - 1, most_hi = p.causal ? first + tok1 : s.len - 1;
+    const int least_hi = p.causal ? first + tok0 : s.len - 1;
     const int most_lo = fp4_lowest(p, first + tok1), least_lo = fp4_lowest(p, first + tok0);
 
     // off: what is added to a score in log2 units, kUp less its row's reference
@@ -223,16 +223,17 @@ __global__ void __launch_bounds__(Fp4RowsShape<D, NT>::kWarps * 32, NT == 1 && D
       l[nt][0] = l[nt][1] = 0.f;
     }
     const int c1 = w.to(), begin = s.begin, len = s.len;
-    for (int c = w.from() + warp; c < c1; c += kRowWarps) {
-      const uint32_t two = held_cells >> 2 * st & 3u;
-      const int key = (begin + c) * kPairKeys;
-      if (two) {
-        if (ok && !__all_sync(0xffffffffu, mbar_try_wait(&full[st], phase >> st & 1))) ok = fp4_wait(&full[st], phase >> st & 1, p.status);
-        if (ok) flying &= ~(1u << st);
-        phase ^= 1u << st;
+    const int inner0 = (max(most_lo, 0) + kPairKeys - 1) / kPairKeys, inner1 = (least_hi + 1) / kPairKeys;   // pairs that every row sees all of
+    for (int c = w.from() + warp; c < c1 && ok; c += kRowWarps) {
+      if (!__all_sync(0xffffffffu, mbar_try_wait(&full[st], parity)) && !fp4_wait(&full[st], parity, p.status)) {
+        ok = false;
+        break;
       }
-      if (two && ok && key <= most_hi && key + kPairKeys > least_lo) {
-        const uint8_t* cells[2] = {ring + st * 2 * Cell::kBytes, ring + (st * 2 + 1) * Cell::kBytes};
+      --issued;
+      {
+        const uint32_t two = cells_at[0];
+        const int pair = begin + c, key = pair * kPairKeys;
+        const uint8_t* cells[2] = {ring + st * (2 * Cell::kBytes), ring + st * (2 * Cell::kBytes) + Cell::kBytes};
         // S^T: rows g and g + 8 of the tile are keys 4 (g / 2) + g % 2 and two on
         float sc[2][NT][4];
 #pragma unroll
@@ -276,7 +277,7 @@ __global__ void __launch_bounds__(Fp4RowsShape<D, NT>::kWarps * 32, NT == 1 && D
             }
           }
         }
-        const bool edge = two != 3u || key + kPairKeys - 1 > least_hi || key < most_lo;
+        const bool edge = two != 3u || pair < inner0 || pair >= inner1;
         const int key0[2] = {two & 1 ? key : kNoKey, two & 2 ? key + kCellTokens : kNoKey};
         uint32_t keep[2] = {0xffffffffu, 0xffffffffu};     // of the scales of the lane's four values
         if (edge) {                  // what lies behind the sequence or before every window may be anything: NaN times 0 too
@@ -389,8 +390,10 @@ __global__ void __launch_bounds__(Fp4RowsShape<D, NT>::kWarps * 32, NT == 1 && D
         }
       }
       __syncwarp();
-      if (ok) fetch(st);
+      cells_at[0] = cells_at[1];
+      fetch(st);
       st ^= 1;
+      parity ^= st ^ 1;
     }
     // ---- the warps' parts of the piece together; the next piece's queries are on their way meanwhile
     const bool whole = w.whole();
@@ -461,8 +464,8 @@ __global__ void __launch_bounds__(Fp4RowsShape<D, NT>::kWarps * 32, NT == 1 && D
   }
   if (!first_piece) asm volatile("bar.sync 1, %0;" ::"n"(2 * kThreads) : "memory");      // (nobody leaves while others' arrivals are pending)
   // a wait ran out: what is still on its way to the ring gets the same time again before the CTA gives its memory up
-  for (int i = 0; i < kRowStages && !ok; ++i)
-    if (flying >> i & 1) mbar_wait(&full[i], phase >> i & 1, p.status);
+  if (!ok)
+    for (int i = 0; i < issued; ++i, st ^= 1, parity ^= st ^ 1) mbar_wait(&full[st], parity, p.status);
 }
 
 // Parts of the row kernel's items, each by kRowShares blocks, then those of the tile kernel's, each by kTileShares.
