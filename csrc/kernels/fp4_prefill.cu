@@ -282,14 +282,24 @@ __global__ void __launch_bounds__(512, 1) fp4_tiles_kernel(Fp4Attn p, float* par
     const uint32_t s_addr = tmem + t * 128 + lane_off, o_addr = tmem + 256 + t * 128 + lane_off;
     uint32_t pieces = 0, count = 0, tiles = 0;
     bool ok = true;
-    uint4 raw[D / 8];
-    const auto query = [&](const Fp4Piece<Fp4Tile>& w) {         // the row's query of a piece, on its way
+    // Queries come and outputs go in whole lines: a warp's 32 rows, kTurnRows of them at a time, a lane 16 bytes. (A lane a row takes a line a lane:
+    // the loads and stores of 256 rows were 8000 cycles a piece so.)
+    constexpr int kRowLanes = D / 8, kTurnRows = 32 / kRowLanes;
+    const int piece16 = lane % kRowLanes, turn_row = lane / kRowLanes, row0 = t * 128 + quarter * 32;
+    uint8_t* own = sQ + t * Shape::kSlot + quarter * 32 * 128;   // the warp's rows of Q (in each plane); the outputs pass through there too
+    uint4 raw[kRowLanes];
+    const auto query = [&](const Fp4Piece<Fp4Tile>& w) {         // the rows' queries of a piece, on their way
       const Fp4TilePiece x(p, w);
-      const int rr = x.r0 + t * 128 + r, token = rr / p.G, head = x.h * p.G + rr - token * p.G;
-      const uint4* src = reinterpret_cast<const uint4*>(p.q + (long long)(w.e.token0 + token) * p.ldq + (long long)head * D);
-      const bool row = w.more() && x.n > 0 && t * 128 + r < x.rows;      // (set in any case: what it held before is not kept)
+      const int rr = x.r0 + row0 + turn_row;
+      int token = rr / p.G, head = rr - token * p.G;
+      const __nv_bfloat16* q = p.q + (long long)w.e.token0 * p.ldq + (long long)x.h * p.G * D + piece16 * 8;
+      const bool some = w.more() && x.n > 0;                     // (set in any case: what it held before is not kept)
 #pragma unroll
-      for (int i = 0; i < D / 8; ++i) raw[i] = row ? src[i] : make_uint4(0, 0, 0, 0);
+      for (int i = 0; i < kRowLanes; ++i) {
+        raw[i] = some && row0 + turn_row + i * kTurnRows < x.rows ? *reinterpret_cast<const uint4*>(q + token * p.ldq + head * D)
+                                                                  : make_uint4(0, 0, 0, 0);
+        for (head += kTurnRows; head >= p.G; head -= p.G) ++token;
+      }
     };
     begin();
     query(w);
@@ -310,31 +320,31 @@ __global__ void __launch_bounds__(512, 1) fp4_tiles_kernel(Fp4Attn p, float* par
         lo = fp4_lowest(p, pos);
       }
       if (n > 0) {
-        // ---- the row's query (every product of the piece before is done: its last scores have been read)
-        float big = 0.f;
+        // ---- the rows' queries (every product of the piece before is done: its last scores have been read)
 #pragma unroll
-        for (int i = 0; i < D / 8; ++i) {
+        for (int i = 0; i < kRowLanes; ++i) {
+          const int at = i * kTurnRows + turn_row;
           const uint32_t v[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+          float big = 0.f;
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             const float2 f = unpack_bf16x2(v[e]);
             big = fmaxf(big, fmaxf(fabsf(f.x), fabsf(f.y)));
           }
-        }
-        const int e2 = min(max((int)(__float_as_uint(big) >> 23) - 127, -100), 100);
-        const float down = __uint_as_float((uint32_t)(127 - e2) << 23);
-        sc *= __uint_as_float((uint32_t)(127 + e2) << 23);
-        uint8_t* dst = sQ + t * Shape::kSlot + r * 128;
 #pragma unroll
-        for (int i = 0; i < D / 8; ++i) {
-          const uint32_t v[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+          for (int o = kRowLanes / 2; o > 0; o >>= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, o));
+          const int e2 = min(max((int)(__float_as_uint(big) >> 23) - 127, -100), 100);
+          const float down = __uint_as_float((uint32_t)(127 - e2) << 23), up = __uint_as_float((uint32_t)(127 + e2) << 23);
+          const float lane_up = __shfl_sync(0xffffffffu, up, lane % kTurnRows * kRowLanes);      // of the lane's own row, if it is among these
+          if (lane / kTurnRows == i) sc = p.scale_log2 * lane_up;
           uint32_t f16[4];
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             const float2 f = unpack_bf16x2(v[e]);
             f16[e] = pack_f16x2(f.x * down, f.y * down);
           }
-          *reinterpret_cast<uint4*>(dst + (i / 8) * Shape::kPlane + (((i % 8) ^ (r & 7)) << 4)) = make_uint4(f16[0], f16[1], f16[2], f16[3]);
+          *reinterpret_cast<uint4*>(own + (piece16 / 8) * Shape::kPlane + at * 128 + (((piece16 % 8) ^ (at & 7)) << 4)) =
+              make_uint4(f16[0], f16[1], f16[2], f16[3]);
         }
         fence_proxy_async_smem();
         tc_fence_before_sync();
@@ -438,36 +448,61 @@ __global__ void __launch_bounds__(512, 1) fp4_tiles_kernel(Fp4Attn p, float* par
         ++pieces;
         tc_fence_after_sync();
       }
-      const bool row = t * 128 + r < y.rows, whole = now.whole();
-      const int rr = y.r0 + min(t * 128 + r, y.rows - 1), token = rr / p.G, head = y.h * p.G + rr - token * p.G;
-      const float inv = l == 0.f ? 0.f : 1.f / l;
-      float* part = parts + fp4_part<Fp4Tile, D>(blockIdx.x, now.part());
-      __nv_bfloat16* dst = p.out + (long long)(now.e.token0 + token) * p.ldo + (long long)head * D;
+      const bool row = t * 128 + r < y.rows;
+      if (now.whole()) {
+        const float inv = l == 0.f ? 0.f : 1.f / l;
+        constexpr int kPart = 4096 / (2 * D);                    // rows of the warp's part of a plane
+        const auto at = [&](int row, int piece) { return own + row / kPart * Shape::kPlane + row % kPart * (2 * D) + ((piece ^ (row & 7)) << 4); };
+#pragma unroll 1
+        for (int c = 0; c < D / 32; ++c) {
+          uint32_t o[32];
+          if (n > 0) {
+            tmem_ld_32x32b_x32(o_addr + c * 32, o);   // (whole warp)
+            tmem_ld_wait();
+          } else {
 #pragma unroll
-      for (int c = 0; c < D / 32; ++c) {
-        uint32_t o[32];
-        if (n > 0) {
-          tmem_ld_32x32b_x32(o_addr + c * 32, o);   // (whole warp)
-          tmem_ld_wait();
-        } else {
+            for (int i = 0; i < 32; ++i) o[i] = 0;
+          }
 #pragma unroll
-          for (int i = 0; i < 32; ++i) o[i] = 0;
-        }
-        if (row && whole) {
-#pragma unroll
-          for (int i = 0; i < 32; i += 8) {
+          for (int i = 0; i < 4; ++i) {
             uint32_t v[4];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) v[e] = pack_bf16x2(__uint_as_float(o[i + 2 * e]) * inv, __uint_as_float(o[i + 2 * e + 1]) * inv);
-            *reinterpret_cast<uint4*>(dst + c * 32 + i) = make_uint4(v[0], v[1], v[2], v[3]);
+            for (int e = 0; e < 4; ++e)
+              v[e] = pack_bf16x2(__uint_as_float(o[8 * i + 2 * e]) * inv, __uint_as_float(o[8 * i + 2 * e + 1]) * inv);
+            *reinterpret_cast<uint4*>(at(lane, c * 4 + i)) = make_uint4(v[0], v[1], v[2], v[3]);
           }
-        } else if (row) {
-#pragma unroll
-          for (int i = 0; i < 32; i += 4)
-            *reinterpret_cast<uint4*>(part + (t * 128 + r) * D + c * 32 + i) = make_uint4(o[i], o[i + 1], o[i + 2], o[i + 3]);
         }
+        __syncwarp();
+        const int rr = y.r0 + row0 + turn_row;
+        int token = rr / p.G, head = rr - token * p.G;
+        __nv_bfloat16* out = p.out + (long long)now.e.token0 * p.ldo + (long long)y.h * p.G * D + piece16 * 8;
+#pragma unroll 1
+        for (int i = 0; i < kRowLanes; ++i) {
+          if (row0 + turn_row + i * kTurnRows < y.rows)
+            *reinterpret_cast<uint4*>(out + token * p.ldo + head * D) = *reinterpret_cast<const uint4*>(at(turn_row + i * kTurnRows, piece16));
+          for (head += kTurnRows; head >= p.G; head -= p.G) ++token;
+        }
+        __syncwarp();
+      } else {
+        float* part = parts + fp4_part<Fp4Tile, D>(blockIdx.x, now.part());
+#pragma unroll 1
+        for (int c = 0; c < D / 32; ++c) {
+          uint32_t o[32];
+          if (n > 0) {
+            tmem_ld_32x32b_x32(o_addr + c * 32, o);   // (whole warp)
+            tmem_ld_wait();
+          } else {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) o[i] = 0;
+          }
+          if (row) {
+#pragma unroll
+            for (int i = 0; i < 32; i += 4)
+              *reinterpret_cast<uint4*>(part + fp4_part_at<Fp4Tile, D>(t * 128 + r, c * 32 + i)) = make_uint4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+          }
+        }
+        if (row) *reinterpret_cast<float2*>(part + Fp4Tile::kRows * D + 2 * (t * 128 + r)) = make_float2(m, l);
       }
-      if (row && !whole) *reinterpret_cast<float2*>(part + Fp4Tile::kRows * D + 2 * (t * 128 + r)) = make_float2(m, l);
     }
   }
   tc_fence_before_sync();

@@ -217,9 +217,12 @@ struct Fp4Piece {
   __device__ __forceinline__ int part() const { return c0 == 0; }
 };
 
-// Scratch of a part: O [rows][D], then (m, l) of each row; in CTA order, two a CTA. Behind the parts a CTA says what of its last item is to be joined.
+// Scratch of a part: O in pieces of 4 dims (fp4_part_at), then (m, l) of each row; in CTA order, two a CTA. Behind the parts a CTA says what of its last item is to be joined.
 template <class Entry, int D>
 __host__ __device__ constexpr size_t fp4_part(uint32_t cta, int part) { return ((size_t)cta * 2 + part) * (Entry::kRows * (D + 2)); }
+// (The row kernel writes a row's dims side by side, the tile kernel a lane a row.)
+template <class Entry, int D>
+__host__ __device__ constexpr int fp4_part_at(int row, int d) { return Entry::kRows > 16 ? (d / 4 * Entry::kRows + row) * 4 + d % 4 : row * D + d; }
 template <class Entry, int D>
 __host__ __device__ constexpr size_t fp4_scratch(uint32_t grid) { return fp4_part<Entry, D>(grid, 0) + (size_t)grid * 8; }
 struct alignas(16) Fp4Cut {    // of an item that this CTA begins and CTAs up to `last` go on with; rows 0: none
@@ -278,8 +281,9 @@ __device__ __forceinline__ void fp4_join(const Fp4Attn& p, float* parts, uint32_
   const Fp4Cut cut = *fp4_cut<Entry, D>(parts, grid, i);
   const int turns = cut.last - i >= 4 ? 4 : 1, lot = kJoinThreads / turns;
   const int lane = threadIdx.x & (lot - 1), turn = threadIdx.x / lot;
-  for (int x0 = share * lot; x0 < cut.rows * (D / 4); x0 += shares * lot) {
-    const int x = x0 + lane, r = x / (D / 4), d = x % (D / 4) * 4;
+  constexpr bool kByRow = kRows <= 16;
+  for (int x0 = share * lot; x0 < (kByRow ? cut.rows : cut.rows > 0 ? kRows : 0) * (D / 4); x0 += shares * lot) {
+    const int x = x0 + lane, r = kByRow ? x / (D / 4) : x % kRows, d = (kByRow ? x % (D / 4) : x / kRows) * 4;
     Fp4Sum sum = {make_float4(0.f, 0.f, 0.f, 0.f), -INFINITY, 0.f};
     if (r < cut.rows) {
       for (int c0 = i + turn; c0 <= cut.last; c0 += 8 * turns) {
@@ -290,7 +294,7 @@ __device__ __forceinline__ void fp4_join(const Fp4Attn& p, float* parts, uint32_
           const int c = c0 + k * turns;
           const float* part = parts + fp4_part<Entry, D>(c, c == i);
           ml[k] = c <= cut.last ? *reinterpret_cast<const float2*>(part + kRows * D + 2 * r) : make_float2(-INFINITY, 0.f);
-          v[k] = c <= cut.last ? *reinterpret_cast<const float4*>(part + r * D + d) : make_float4(0.f, 0.f, 0.f, 0.f);
+          v[k] = c <= cut.last ? *reinterpret_cast<const float4*>(part + fp4_part_at<Entry, D>(r, d)) : make_float4(0.f, 0.f, 0.f, 0.f);
         }
         sum.add(v, ml, 8);
       }
