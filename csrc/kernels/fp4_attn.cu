@@ -116,7 +116,7 @@ __global__ void __launch_bounds__(Fp4RowsShape<D, NT>::kWarps * 32, NT == 1 && D
         fc = f.from() + warp;
       }
       if (!f.more()) return;
-      const int pair = fc + (lane >> 1) * kRowWarps, c = 2 * (f.e.begin + pair) + (lane & 1), pg = c / p.cells_per_page, h = f.item / f.e.tiles;
+      const int pair = fc + (lane >> 1) * kRowWarps, c = 2 * (f.e.begin + pair) + (lane & 1), pg = p.by_page_cells.of(c), h = fp4_head(f.item, f.e.tiles);
       const int id = pair < f.to() && c * kCellTokens < f.e.len ? p.block_table[f.b * p.ldt + pg] : -1;
       src = id >= 0 && id < p.num_blocks
                 ? p.cache + (((long long)id * p.Hkv + h) * p.cells_per_page + (c - pg * p.cells_per_page)) * Cell::kBytes : nullptr;
@@ -154,10 +154,10 @@ __global__ void __launch_bounds__(Fp4RowsShape<D, NT>::kWarps * 32, NT == 1 && D
   // queries: lane (g, t) has dims [t D / 4, + D / 4) of row g
   uint4 raw[NT][D / 32];
   const auto query = [&](const Fp4Piece<Seq>& x) {
-    const int h = x.more() ? x.item / x.e.tiles : 0, r0 = x.more() ? (x.item - h * x.e.tiles) * kRows : 0;
+    const int h = x.more() ? fp4_head(x.item, x.e.tiles) : 0, r0 = x.more() ? (x.item - h * x.e.tiles) * kRows : 0;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-      const int r = r0 + nt * 8 + g, token = r / p.G, head = h * p.G + r - token * p.G;
+      const int r = r0 + nt * 8 + g, token = p.by_group.of(r), head = h * p.G + r - token * p.G;
       const __nv_bfloat16* from = p.q + (long long)(x.e.token0 + token) * p.ldq + (long long)head * D + t * (D / 4);
       const bool row = x.more() && r < x.e.rows;
 #pragma unroll
@@ -168,7 +168,7 @@ __global__ void __launch_bounds__(Fp4RowsShape<D, NT>::kWarps * 32, NT == 1 && D
   bool first_piece = true;
   while (w.more()) {
     const Seq& s = w.e;
-    const int h = w.item / s.tiles, r0 = (w.item - h * s.tiles) * kRows, nrows = min(kRows, s.rows - r0), first = s.first;
+    const int h = fp4_head(w.item, s.tiles), r0 = (w.item - h * s.tiles) * kRows, nrows = min(kRows, s.rows - r0), first = s.first;
     // ---- the tile's queries: B operand
     uint32_t bq[NT][D / 16][2];
     float mul[NT][2];                                                            // of the lane's rows 2t, 2t + 1: scores to log2 units
@@ -201,12 +201,12 @@ __global__ void __launch_bounds__(Fp4RowsShape<D, NT>::kWarps * 32, NT == 1 && D
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         mul[nt][e] = __shfl_sync(0xffffffffu, up, (2 * t + e) * 4) * p.scale_log2;
-        const int rr = min(nt * 8 + 2 * t + e, nrows - 1) + r0, pos = first + rr / p.G;
+        const int rr = min(nt * 8 + 2 * t + e, nrows - 1) + r0, pos = first + p.by_group.of(rr);
         hi[nt][e] = p.causal ? pos : s.len - 1;
         lo[nt][e] = fp4_lowest(p, pos);
       }
     }
-    const int tok0 = r0 / p.G, tok1 = (r0 + nrows - 1) / p.G;                    // the tile's tokens
+    const int tok0 = p.by_group.of(r0), tok1 = p.by_group.of(r0 + nrows - 1);                    // the tile's tokens
     const int least_hi = p.causal ? first + tok0 : s.len - 1;
     const int most_lo = fp4_lowest(p, first + tok1), least_lo = fp4_lowest(p, first + tok0);
 
@@ -449,7 +449,7 @@ __global__ void __launch_bounds__(Fp4RowsShape<D, NT>::kWarps * 32, NT == 1 && D
           sum = fmaf(ml.y, f, sum);
         }
         if (whole) {
-          const int token = (r0 + r) / p.G, head = r0 + r - token * p.G;
+          const int token = p.by_group.of(r0 + r), head = r0 + r - token * p.G;
           const float inv = sum == 0.f ? 0.f : 1.f / sum;
           *reinterpret_cast<uint32_t*>(p.out + (long long)(token0 + token) * p.ldo + (long long)(h * p.G + head) * D + d) =
               pack_bf16x2(a * inv, b * inv);
@@ -534,6 +534,8 @@ extern "C" int b200_fp4_attn(const B200Fp4Attn* a, cudaStream_t stream) {
   // cells of the whole line in 31 bits, whatever the lengths
   if ((double)a->max_blocks * (a->block_size / kCellTokens) * a->Hkv * ((double)a->total_q * G / 8 + a->num_reqs) > 2147483647.0) return -4;
   if ((double)a->max_blocks * a->block_size > 2147483647.0) return -4;
+  if ((double)a->total_q * G * G >= 4294967296.0 || (double)a->max_blocks * (a->block_size / kCellTokens) * (a->block_size / kCellTokens) >= 4294967296.0)
+    return -4;       // (Fp4Div)
   Fp4Attn p;
   p.q = (const __nv_bfloat16*)a->q; p.ldq = a->ldq;
   p.out = (__nv_bfloat16*)a->out; p.ldo = a->ldo;
@@ -544,6 +546,9 @@ extern "C" int b200_fp4_attn(const B200Fp4Attn* a, cudaStream_t stream) {
   p.num_reqs = a->num_reqs; p.total_q = a->total_q; p.num_tiles = a->q_start ? a->num_tiles : 0;
   p.Hkv = a->Hkv; p.G = G; p.cells_per_page = a->block_size / kCellTokens;
   p.window = a->window; p.causal = a->causal;
+  const auto by = [](int d) { return Fp4Div{d == 1 ? 0u : (uint32_t)(((1ull << 32) + d - 1) / d)}; };
+  p.by_group = by(G);
+  p.by_page_cells = by(p.cells_per_page);
   p.scale_log2 = a->scale * 1.4426950408889634f;
   p.softcap2 = a->softcap * 1.4426950408889634f;
   p.status = device_status_word();

@@ -48,12 +48,12 @@ struct Fp4TilePiece {
   int h, r0, rows, halves, k0, n, first;       // k0: first key of the piece's first tile, n: tiles
   __device__ __forceinline__ Fp4TilePiece(const Fp4Attn& p, const Fp4Piece<Fp4Tile>& w) {
     const Fp4Tile& e = w.e;
-    h = w.item / e.tiles;
+    h = fp4_head(w.item, e.tiles);
     r0 = (w.item - h * e.tiles) * Fp4Tile::kRows;
     rows = min(Fp4Tile::kRows, e.rows - r0);
     halves = rows > 128 ? 2 : 1;
     first = e.first;
-    const int low = max(0, fp4_lowest(p, first + r0 / p.G)), high = min(p.causal ? first + (r0 + rows - 1) / p.G : e.len - 1, e.len - 1);
+    const int low = max(0, fp4_lowest(p, first + p.by_group.of(r0))), high = min(p.causal ? first + p.by_group.of(r0 + rows - 1) : e.len - 1, e.len - 1);
     const int t0 = max(e.begin + w.from(), low / kTileKeys), t1 = min(e.begin + w.to(), high < 0 ? 0 : high / kTileKeys + 1);
     k0 = t0 * kTileKeys;
     n = max(0, t1 - t0);
@@ -200,13 +200,13 @@ __global__ void __launch_bounds__(512, 1) fp4_tiles_kernel(Fp4Attn p, float* par
       const Fp4TilePiece x(p, w);
       if (x.n == 0) continue;
       const int32_t* table = p.block_table + w.e.req * p.ldt;
-      const int low = max(0, fp4_lowest(p, x.first + x.r0 / p.G));
+      const int low = max(0, fp4_lowest(p, x.first + p.by_group.of(x.r0)));
       const auto page_of = [&](int j) {                          // -1: none; -2: not a key that any row sees
         const int pos = x.k0 + j * kTileKeys + r;
-        return pos >= low && pos < w.e.len ? max(-1, table[pos / (p.cells_per_page * kCellTokens)]) : -2;
+        return pos >= low && pos < w.e.len ? max(-1, table[p.by_page_cells.of(pos / kCellTokens)]) : -2;
       };
       const auto cell_of = [&](int j, int page) -> const uint8_t* {
-        const int cell = (x.k0 + j * kTileKeys + r) / kCellTokens % p.cells_per_page;
+        const int c = (x.k0 + j * kTileKeys + r) / kCellTokens, cell = c - p.by_page_cells.of(c) * p.cells_per_page;
         return page >= 0 && page < p.num_blocks ? p.cache + ((long long)page * p.Hkv + x.h) * head_bytes + (long long)cell * Cell::kBytes : nullptr;
       };
       uint4 code[D / 32];
@@ -287,11 +287,15 @@ __global__ void __launch_bounds__(512, 1) fp4_tiles_kernel(Fp4Attn p, float* par
     constexpr int kRowLanes = D / 8, kTurnRows = 32 / kRowLanes;
     const int piece16 = lane % kRowLanes, turn_row = lane / kRowLanes, row0 = t * 128 + quarter * 32;
     uint8_t* own = sQ + t * Shape::kSlot + quarter * 32 * 128;   // the warp's rows of Q (in each plane); the outputs pass through there too
+    constexpr int kPart = 4096 / (2 * D);                        // rows of D bf16 in the warp's part of a plane
+    const auto own_at = [&](int row, int piece) {
+      return own + row / kPart * Shape::kPlane + row % kPart * (2 * D) + ((piece ^ (row & 7)) << 4);
+    };
     uint4 raw[kRowLanes];
     const auto query = [&](const Fp4Piece<Fp4Tile>& w) {         // the rows' queries of a piece, on their way
       const Fp4TilePiece x(p, w);
       const int rr = x.r0 + row0 + turn_row;
-      int token = rr / p.G, head = rr - token * p.G;
+      int token = p.by_group.of(rr), head = rr - token * p.G;
       const __nv_bfloat16* q = p.q + (long long)w.e.token0 * p.ldq + (long long)x.h * p.G * D + piece16 * 8;
       const bool some = w.more() && x.n > 0;                     // (set in any case: what it held before is not kept)
 #pragma unroll
@@ -315,35 +319,40 @@ __global__ void __launch_bounds__(512, 1) fp4_tiles_kernel(Fp4Attn p, float* par
       int hi, lo;
       float sc = p.scale_log2, m = -INFINITY, l = 0.f;
       {
-        const int token = (x.r0 + min(t * 128 + r, x.rows - 1)) / p.G, pos = x.first + token;
+        const int token = p.by_group.of(x.r0 + min(t * 128 + r, x.rows - 1)), pos = x.first + token;
         hi = min(p.causal ? pos : w.e.len - 1, w.e.len - 1);
         lo = fp4_lowest(p, pos);
       }
       if (n > 0) {
-        // ---- the rows' queries (every product of the piece before is done: its last scores have been read)
+        // ---- the rows' queries (every product of the piece before is done: its last scores have been read), turned to a lane a row on the way
+#pragma unroll
+        for (int i = 0; i < kRowLanes; ++i) *reinterpret_cast<uint4*>(own_at(i * kTurnRows + turn_row, piece16)) = raw[i];
+        __syncwarp();
+#pragma unroll
+        for (int i = 0; i < kRowLanes; ++i) raw[i] = *reinterpret_cast<const uint4*>(own_at(lane, i));
+        __syncwarp();
+        __nv_bfloat162 most = __float2bfloat162_rn(0.f);
 #pragma unroll
         for (int i = 0; i < kRowLanes; ++i) {
-          const int at = i * kTurnRows + turn_row;
           const uint32_t v[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
-          float big = 0.f;
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float2 f = unpack_bf16x2(v[e]);
-            big = fmaxf(big, fmaxf(fabsf(f.x), fabsf(f.y)));
-          }
+          for (int e = 0; e < 4; ++e) most = __hmax2(most, __habs2(*reinterpret_cast<const __nv_bfloat162*>(&v[e])));
+        }
+        const float big = fmaxf(__low2float(most), __high2float(most));
+        const int e2 = min(max((int)(__float_as_uint(big) >> 23) - 127, -100), 100);
+        const __nv_bfloat162 down = __float2bfloat162_rn(__uint_as_float((uint32_t)(127 - e2) << 23));       // (exact)
+        sc = p.scale_log2 * __uint_as_float((uint32_t)(127 + e2) << 23);
 #pragma unroll
-          for (int o = kRowLanes / 2; o > 0; o >>= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, o));
-          const int e2 = min(max((int)(__float_as_uint(big) >> 23) - 127, -100), 100);
-          const float down = __uint_as_float((uint32_t)(127 - e2) << 23), up = __uint_as_float((uint32_t)(127 + e2) << 23);
-          const float lane_up = __shfl_sync(0xffffffffu, up, lane % kTurnRows * kRowLanes);      // of the lane's own row, if it is among these
-          if (lane / kTurnRows == i) sc = p.scale_log2 * lane_up;
+        for (int i = 0; i < kRowLanes; ++i) {
+          const uint32_t v[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
           uint32_t f16[4];
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            const float2 f = unpack_bf16x2(v[e]);
-            f16[e] = pack_f16x2(f.x * down, f.y * down);
+            const __nv_bfloat162 y = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&v[e]), down);
+            const float2 f = __bfloat1622float2(y);
+            f16[e] = pack_f16x2(f.x, f.y);
           }
-          *reinterpret_cast<uint4*>(own + (piece16 / 8) * Shape::kPlane + at * 128 + (((piece16 % 8) ^ (at & 7)) << 4)) =
+          *reinterpret_cast<uint4*>(own + (i / 8) * Shape::kPlane + lane * 128 + (((i % 8) ^ (lane & 7)) << 4)) =
               make_uint4(f16[0], f16[1], f16[2], f16[3]);
         }
         fence_proxy_async_smem();
@@ -451,9 +460,7 @@ __global__ void __launch_bounds__(512, 1) fp4_tiles_kernel(Fp4Attn p, float* par
       const bool row = t * 128 + r < y.rows;
       if (now.whole()) {
         const float inv = l == 0.f ? 0.f : 1.f / l;
-        constexpr int kPart = 4096 / (2 * D);                    // rows of the warp's part of a plane
-        const auto at = [&](int row, int piece) { return own + row / kPart * Shape::kPlane + row % kPart * (2 * D) + ((piece ^ (row & 7)) << 4); };
-#pragma unroll 1
+#pragma unroll
         for (int c = 0; c < D / 32; ++c) {
           uint32_t o[32];
           if (n > 0) {
@@ -469,23 +476,23 @@ __global__ void __launch_bounds__(512, 1) fp4_tiles_kernel(Fp4Attn p, float* par
 #pragma unroll
             for (int e = 0; e < 4; ++e)
               v[e] = pack_bf16x2(__uint_as_float(o[8 * i + 2 * e]) * inv, __uint_as_float(o[8 * i + 2 * e + 1]) * inv);
-            *reinterpret_cast<uint4*>(at(lane, c * 4 + i)) = make_uint4(v[0], v[1], v[2], v[3]);
+            *reinterpret_cast<uint4*>(own_at(lane, c * 4 + i)) = make_uint4(v[0], v[1], v[2], v[3]);
           }
         }
         __syncwarp();
         const int rr = y.r0 + row0 + turn_row;
-        int token = rr / p.G, head = rr - token * p.G;
+        int token = p.by_group.of(rr), head = rr - token * p.G;
         __nv_bfloat16* out = p.out + (long long)now.e.token0 * p.ldo + (long long)y.h * p.G * D + piece16 * 8;
-#pragma unroll 1
+#pragma unroll 8
         for (int i = 0; i < kRowLanes; ++i) {
           if (row0 + turn_row + i * kTurnRows < y.rows)
-            *reinterpret_cast<uint4*>(out + token * p.ldo + head * D) = *reinterpret_cast<const uint4*>(at(turn_row + i * kTurnRows, piece16));
+            *reinterpret_cast<uint4*>(out + token * p.ldo + head * D) = *reinterpret_cast<const uint4*>(own_at(turn_row + i * kTurnRows, piece16));
           for (head += kTurnRows; head >= p.G; head -= p.G) ++token;
         }
         __syncwarp();
       } else {
         float* part = parts + fp4_part<Fp4Tile, D>(blockIdx.x, now.part());
-#pragma unroll 1
+#pragma unroll
         for (int c = 0; c < D / 32; ++c) {
           uint32_t o[32];
           if (n > 0) {

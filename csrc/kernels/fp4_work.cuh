@@ -12,6 +12,14 @@
 
 namespace b200 {
 
+// Division by a number that the host knows: n / d for n d < 2^32 (mul = 2^32 / d rounded up, 0 for d = 1).
+struct Fp4Div {
+  uint32_t mul;
+#ifdef __CUDACC__
+  __device__ __forceinline__ int of(int n) const { return mul ? (int)__umulhi((uint32_t)n, mul) : n; }
+#endif
+};
+
 struct Fp4Attn {
   const __nv_bfloat16* q;
   long long ldq;
@@ -28,9 +36,12 @@ struct Fp4Attn {
   int num_reqs, total_q, num_tiles;
   int Hkv, G, cells_per_page, window, causal;
   int few;                     // sequences of at most so many rows (query tokens x G) are the row kernel's, the others the tile kernel's
+  Fp4Div by_group, by_page_cells;
   float scale_log2, softcap2;
   int* status;
 };
+// h = item / tiles; one division, and none for a single tile
+__device__ __forceinline__ int fp4_head(int item, int tiles) { return tiles == 1 ? item : item / tiles; }
 
 __device__ __forceinline__ float ex2_of(float x) {
   float y;
@@ -242,7 +253,7 @@ __device__ __forceinline__ void fp4_say_cut(const Fp4Attn& p, const uint32_t* li
     w.at(p, line, to - 1, to);                                  // the stretch's last cell
     const uint32_t begin = line[w.b] + (uint32_t)w.item * w.e.cells;
     if (w.c1 < w.e.cells && begin >= from) {                    // its item goes on, and begins here
-      const int h = w.item / w.e.tiles;
+      const int h = fp4_head(w.item, w.e.tiles);
       c.row0 = (w.item - h * w.e.tiles) * Entry::kRows;
       c.rows = min(Entry::kRows, w.e.rows - c.row0);
       c.last = (int)(((uint64_t)(begin + w.e.cells) * ctas - 1) / total);       // the CTA that has the item's last cell
@@ -317,7 +328,7 @@ __device__ __forceinline__ void fp4_join(const Fp4Attn& p, float* parts, uint32_
     }
     if (turn == 0 && r < cut.rows) {
       const float inv = sum.l == 0.f ? 0.f : 1.f / sum.l;
-      const int token = (cut.row0 + r) / p.G, head = cut.head0 + cut.row0 + r - token * p.G;
+      const int token = p.by_group.of(cut.row0 + r), head = cut.head0 + cut.row0 + r - token * p.G;
       *reinterpret_cast<uint2*>(p.out + (long long)(cut.token0 + token) * p.ldo + (long long)head * D + d) =
           make_uint2(pack_bf16x2(sum.o.x * inv, sum.o.y * inv), pack_bf16x2(sum.o.z * inv, sum.o.w * inv));
     }
