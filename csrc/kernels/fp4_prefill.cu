@@ -46,6 +46,7 @@ struct alignas(8) Fp4TileBars {
 // What a piece has for its two halves: `rows` of the tile's 256 exist, key tiles [c0, c1) of the item are seen by any of them.
 struct Fp4TilePiece {
   int h, r0, rows, halves, k0, n, first;       // k0: first key of the piece's first tile, n: tiles
+  __device__ __forceinline__ Fp4TilePiece() {}
   __device__ __forceinline__ Fp4TilePiece(const Fp4Attn& p, const Fp4Piece<Fp4Tile>& w) {
     const Fp4Tile& e = w.e;
     h = fp4_head(w.item, e.tiles);
@@ -68,7 +69,8 @@ __global__ void __launch_bounds__(512, 1) fp4_tiles_kernel(Fp4Attn p, float* par
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   __shared__ Fp4TileBars bars;
   __shared__ uint32_t no_page[4][4];                            // key tiles in turn: keys of a warp of expanders that have no page
-  __shared__ Fp4Piece<Fp4Tile> held[16];                        // each warp's piece, out of the registers of its loop over tiles
+  __shared__ Fp4Piece<Fp4Tile> held[16];                        // each warp's piece, out of the registers of its loop over tiles,
+  __shared__ Fp4TilePiece held_tile[16];                        // and what it comes to
   uint8_t* sQ = smem;
   uint8_t* ring = smem + 2 * Shape::kSlot;
   uint32_t* line = reinterpret_cast<uint32_t*>(smem + Shape::kLine);
@@ -104,18 +106,26 @@ __global__ void __launch_bounds__(512, 1) fp4_tiles_kernel(Fp4Attn p, float* par
   const uint32_t to = mine ? fp4_begin<Fp4Tile>(p, line, total, blockIdx.x + 1, ctas) : 0;
   if (threadIdx.x == 0) fp4_say_cut<Fp4Tile, D>(p, line, total, ctas, from, to, parts);
   Fp4Piece<Fp4Tile>& w = held[warp];
-  const auto begin = [&] {
-    Fp4Piece<Fp4Tile> x;
-    x.at(p, line, from, to);
-    if (lane == 0) w = x;
+  Fp4TilePiece& x = held_tile[warp];
+  const auto hold = [&](const Fp4Piece<Fp4Tile>& now) {
+    Fp4TilePiece y;
+    if (now.more()) y = Fp4TilePiece(p, now);
+    __syncwarp();
+    if (lane == 0) {
+      w = now;
+      x = y;
+    }
     __syncwarp();
   };
+  const auto begin = [&] {
+    Fp4Piece<Fp4Tile> now;
+    now.at(p, line, from, to);
+    hold(now);
+  };
   const auto next = [&] {
-    Fp4Piece<Fp4Tile> x = w;
-    x.next(p, line);
-    __syncwarp();
-    if (lane == 0) w = x;
-    __syncwarp();
+    Fp4Piece<Fp4Tile> now = w;
+    now.next(p, line);
+    hold(now);
   };
 
   if (group == 0) {
@@ -126,7 +136,6 @@ __global__ void __launch_bounds__(512, 1) fp4_tiles_kernel(Fp4Attn p, float* par
       uint32_t sq = 0, pieces[2] = {0, 0}, count[2] = {0, 0};    // ring items, pieces and tiles of each half so far
       bool ok = true;
       for (begin(); w.more() && ok; next()) {
-        const Fp4TilePiece x(p, w);
         const int n = x.n, halves = x.halves;
         if (n == 0) continue;
         const auto qk = [&](int t, uint32_t slot, bool last) {      // S(t) = Q(t) K^T
@@ -197,17 +206,17 @@ __global__ void __launch_bounds__(512, 1) fp4_tiles_kernel(Fp4Attn p, float* par
     uint32_t sq = 0, tiles = 0;
     bool ok = true;
     for (begin(); w.more() && ok; next()) {
-      const Fp4TilePiece x(p, w);
-      if (x.n == 0) continue;
+      const int n = x.n, k0 = x.k0, len = w.e.len, h = x.h;
+      if (n == 0) continue;
       const int32_t* table = p.block_table + w.e.req * p.ldt;
       const int low = max(0, fp4_lowest(p, x.first + p.by_group.of(x.r0)));
       const auto page_of = [&](int j) {                          // -1: none; -2: not a key that any row sees
-        const int pos = x.k0 + j * kTileKeys + r;
-        return pos >= low && pos < w.e.len ? max(-1, table[p.by_page_cells.of(pos / kCellTokens)]) : -2;
+        const int pos = k0 + j * kTileKeys + r;
+        return pos >= low && pos < len ? max(-1, table[p.by_page_cells.of(pos / kCellTokens)]) : -2;
       };
       const auto cell_of = [&](int j, int page) -> const uint8_t* {
-        const int c = (x.k0 + j * kTileKeys + r) / kCellTokens, cell = c - p.by_page_cells.of(c) * p.cells_per_page;
-        return page >= 0 && page < p.num_blocks ? p.cache + ((long long)page * p.Hkv + x.h) * head_bytes + (long long)cell * Cell::kBytes : nullptr;
+        const int c = (k0 + j * kTileKeys + r) / kCellTokens, cell = c - p.by_page_cells.of(c) * p.cells_per_page;
+        return page >= 0 && page < p.num_blocks ? p.cache + ((long long)page * p.Hkv + h) * head_bytes + (long long)cell * Cell::kBytes : nullptr;
       };
       uint4 code[D / 32];
       uint32_t scale[D / 64];
@@ -231,7 +240,7 @@ __global__ void __launch_bounds__(512, 1) fp4_tiles_kernel(Fp4Attn p, float* par
       int page = page_of(0);
       const uint8_t* cell = cell_of(0, page);
       load(cell, 0);
-      for (int i = 0; i < 2 * x.n; ++i, ++sq) {
+      for (int i = 0; i < 2 * n; ++i, ++sq) {
         const int j = i >> 1, kv = i & 1;
         const uint32_t slot = sq % kFRing;
         const bool none = page != -2 && cell == nullptr;
@@ -244,8 +253,8 @@ __global__ void __launch_bounds__(512, 1) fp4_tiles_kernel(Fp4Attn p, float* par
         // the next item's loads, and in front of a key tile's the page
         if (kv == 0) {
           load(cell, 1);
-          if (j + 1 < x.n) page = page_of(j + 1);
-        } else if (j + 1 < x.n) {
+          if (j + 1 < n) page = page_of(j + 1);
+        } else if (j + 1 < n) {
           cell = cell_of(j + 1, page);
           load(cell, 0);
         }
@@ -291,28 +300,42 @@ __global__ void __launch_bounds__(512, 1) fp4_tiles_kernel(Fp4Attn p, float* par
     const auto own_at = [&](int row, int piece) {
       return own + row / kPart * Shape::kPlane + row % kPart * (2 * D) + ((piece ^ (row & 7)) << 4);
     };
+    // a value that the compiler takes for new: what follows from it is not kept in registers over the loop of tiles
+    const auto here = [](int v) {
+      asm volatile("" : "+r"(v));
+      return v;
+    };
     uint4 raw[kRowLanes];
-    const auto query = [&](const Fp4Piece<Fp4Tile>& w) {         // the rows' queries of a piece, on their way
-      const Fp4TilePiece x(p, w);
-      const int rr = x.r0 + row0 + turn_row;
-      int token = p.by_group.of(rr), head = rr - token * p.G;
-      const __nv_bfloat16* q = p.q + (long long)w.e.token0 * p.ldq + (long long)x.h * p.G * D + piece16 * 8;
-      const bool some = w.more() && x.n > 0;                     // (set in any case: what it held before is not kept)
+    const auto rows_from = [&](int r0, long long ld, auto&& each) {      // each(i, offset of the lane's piece of turn i's row)
+      const int G = here(p.G), rr = r0 + row0 + here(turn_row), token = p.by_group.of(rr), step_token = p.by_group.of(kTurnRows), step_head = kTurnRows - step_token * G;
+      int head = rr - token * G;
+      long long at = token * ld + head * D + piece16 * 8;
+      const long long step = step_token * ld + step_head * D, wrap = ld - G * D;
 #pragma unroll
       for (int i = 0; i < kRowLanes; ++i) {
-        raw[i] = some && row0 + turn_row + i * kTurnRows < x.rows ? *reinterpret_cast<const uint4*>(q + token * p.ldq + head * D)
-                                                                  : make_uint4(0, 0, 0, 0);
-        for (head += kTurnRows; head >= p.G; head -= p.G) ++token;
+        each(i, at);
+        head += step_head;
+        at += step;
+        if (head >= G) {
+          head -= G;
+          at += wrap;
+        }
       }
     };
+    const auto query = [&] {                                     // the rows' queries of the piece, on their way
+      const int left = w.more() && x.n > 0 ? x.rows - row0 - turn_row : 0;       // (raw is set in any case: what it held before is not kept)
+      const __nv_bfloat16* q = p.q + (long long)w.e.token0 * p.ldq + (long long)x.h * p.G * D;
+      rows_from(x.r0, p.ldq, [&](int i, long long at) {
+        raw[i] = i * kTurnRows < left ? *reinterpret_cast<const uint4*>(q + at) : make_uint4(0, 0, 0, 0);
+      });
+    };
     begin();
-    query(w);
+    query();
     while (w.more() && ok) {
-      const Fp4TilePiece x(p, w);
       if (t >= x.halves) {
         tiles += x.n;
         next();
-        query(w);
+        query();
         continue;
       }
       const int n = x.n, k0 = x.k0;
@@ -325,11 +348,12 @@ __global__ void __launch_bounds__(512, 1) fp4_tiles_kernel(Fp4Attn p, float* par
       }
       if (n > 0) {
         // ---- the rows' queries (every product of the piece before is done: its last scores have been read), turned to a lane a row on the way
+        const int mine = here(lane), turn = here(turn_row);
 #pragma unroll
-        for (int i = 0; i < kRowLanes; ++i) *reinterpret_cast<uint4*>(own_at(i * kTurnRows + turn_row, piece16)) = raw[i];
+        for (int i = 0; i < kRowLanes; ++i) *reinterpret_cast<uint4*>(own_at(i * kTurnRows + turn, piece16)) = raw[i];
         __syncwarp();
 #pragma unroll
-        for (int i = 0; i < kRowLanes; ++i) raw[i] = *reinterpret_cast<const uint4*>(own_at(lane, i));
+        for (int i = 0; i < kRowLanes; ++i) raw[i] = *reinterpret_cast<const uint4*>(own_at(mine, i));
         __syncwarp();
         __nv_bfloat162 most = __float2bfloat162_rn(0.f);
 #pragma unroll
@@ -352,7 +376,7 @@ __global__ void __launch_bounds__(512, 1) fp4_tiles_kernel(Fp4Attn p, float* par
             const float2 f = __bfloat1622float2(y);
             f16[e] = pack_f16x2(f.x, f.y);
           }
-          *reinterpret_cast<uint4*>(own + (i / 8) * Shape::kPlane + lane * 128 + (((i % 8) ^ (lane & 7)) << 4)) =
+          *reinterpret_cast<uint4*>(own + (i / 8) * Shape::kPlane + mine * 128 + (((i % 8) ^ (mine & 7)) << 4)) =
               make_uint4(f16[0], f16[1], f16[2], f16[3]);
         }
         fence_proxy_async_smem();
@@ -447,19 +471,20 @@ __global__ void __launch_bounds__(512, 1) fp4_tiles_kernel(Fp4Attn p, float* par
         if (lane == 0) mbar_arrive(&bars.p_full[t]);
       }
       if (!ok) break;
-      const Fp4Piece<Fp4Tile> now = w;
-      const Fp4TilePiece y(p, now);
+      const int left = x.rows - row0, r0 = x.r0, part_of = w.part();
+      const bool whole = w.whole();
+      const long long out0 = (long long)w.e.token0 * p.ldo + (long long)x.h * p.G * D;
       next();
-      query(w);
+      query();
       if (n > 0) {
         ok = __all_sync(0xffffffffu, mbar_wait(&bars.pv_done[t], pieces & 1, p.status));
         if (!ok) break;
         ++pieces;
         tc_fence_after_sync();
       }
-      const bool row = t * 128 + r < y.rows;
-      if (now.whole()) {
+      if (whole) {
         const float inv = l == 0.f ? 0.f : 1.f / l;
+        const int mine = here(lane), turn = here(turn_row);
 #pragma unroll
         for (int c = 0; c < D / 32; ++c) {
           uint32_t o[32];
@@ -476,22 +501,19 @@ __global__ void __launch_bounds__(512, 1) fp4_tiles_kernel(Fp4Attn p, float* par
 #pragma unroll
             for (int e = 0; e < 4; ++e)
               v[e] = pack_bf16x2(__uint_as_float(o[8 * i + 2 * e]) * inv, __uint_as_float(o[8 * i + 2 * e + 1]) * inv);
-            *reinterpret_cast<uint4*>(own_at(lane, c * 4 + i)) = make_uint4(v[0], v[1], v[2], v[3]);
+            *reinterpret_cast<uint4*>(own_at(mine, c * 4 + i)) = make_uint4(v[0], v[1], v[2], v[3]);
           }
         }
         __syncwarp();
-        const int rr = y.r0 + row0 + turn_row;
-        int token = p.by_group.of(rr), head = rr - token * p.G;
-        __nv_bfloat16* out = p.out + (long long)now.e.token0 * p.ldo + (long long)y.h * p.G * D + piece16 * 8;
-#pragma unroll 8
-        for (int i = 0; i < kRowLanes; ++i) {
-          if (row0 + turn_row + i * kTurnRows < y.rows)
-            *reinterpret_cast<uint4*>(out + token * p.ldo + head * D) = *reinterpret_cast<const uint4*>(own_at(turn_row + i * kTurnRows, piece16));
-          for (head += kTurnRows; head >= p.G; head -= p.G) ++token;
-        }
+        __nv_bfloat16* out = p.out + out0;
+        rows_from(r0, p.ldo, [&](int i, long long at) {
+          const uint4 v = *reinterpret_cast<const uint4*>(own_at(turn + i * kTurnRows, piece16));
+          if (turn + i * kTurnRows < left) *reinterpret_cast<uint4*>(out + at) = v;
+          if (i % 4 == 3) asm volatile("" ::: "memory");         // (few at a time: the next queries hold their registers)
+        });
         __syncwarp();
       } else {
-        float* part = parts + fp4_part<Fp4Tile, D>(blockIdx.x, now.part());
+        float* part = parts + fp4_part<Fp4Tile, D>(blockIdx.x, part_of);
 #pragma unroll
         for (int c = 0; c < D / 32; ++c) {
           uint32_t o[32];
@@ -502,13 +524,13 @@ __global__ void __launch_bounds__(512, 1) fp4_tiles_kernel(Fp4Attn p, float* par
 #pragma unroll
             for (int i = 0; i < 32; ++i) o[i] = 0;
           }
-          if (row) {
+          if (lane < left) {
 #pragma unroll
             for (int i = 0; i < 32; i += 4)
               *reinterpret_cast<uint4*>(part + fp4_part_at<Fp4Tile, D>(t * 128 + r, c * 32 + i)) = make_uint4(o[i], o[i + 1], o[i + 2], o[i + 3]);
           }
         }
-        if (row) *reinterpret_cast<float2*>(part + Fp4Tile::kRows * D + 2 * (t * 128 + r)) = make_float2(m, l);
+        if (lane < left) *reinterpret_cast<float2*>(part + Fp4Tile::kRows * D + 2 * (t * 128 + r)) = make_float2(m, l);
       }
     }
   }
