@@ -468,9 +468,9 @@ __global__ void __launch_bounds__(Fp4RowsShape<D, NT>::kWarps * 32, NT == 1 && D
     for (int i = 0; i < issued; ++i, st ^= 1, parity ^= st ^ 1) mbar_wait(&full[st], parity, p.status);
 }
 
-// Parts of the row kernel's items, each by kRowShares blocks, then those of the tile kernel's, each by kTileShares.
-static constexpr int kRowShares = 2;
-static constexpr int kTileShares = 32;
+// Parts of the row kernel's items, each by kRowShares blocks, then those of the tile kernel's: kTileShares shares each, of which a block takes kTurns
+// one after another, of items that lie far apart. (One block a share was four waves of blocks, most of them with nothing to do.)
+static constexpr int kRowShares = 2, kTileShares = 32, kTurns = 4;
 template <int D, int ROWS>
 __global__ void __launch_bounds__(kJoinThreads) fp4_join_kernel(Fp4Attn p, float* row_parts, int row_grid, float* tile_parts, int tile_grid) {
   pdl_wait();
@@ -478,8 +478,16 @@ __global__ void __launch_bounds__(kJoinThreads) fp4_join_kernel(Fp4Attn p, float
   if ((int)blockIdx.x < row_grid * kRowShares) {
     fp4_join<Fp4Seq<ROWS>, D>(p, row_parts, row_grid, blockIdx.x / kRowShares, blockIdx.x % kRowShares, kRowShares);
   } else if constexpr (D <= 128) {
-    const int i = blockIdx.x - row_grid * kRowShares;
-    fp4_join<Fp4Tile, D>(p, tile_parts, tile_grid, i / kTileShares, i % kTileShares, kTileShares);
+    const int n = tile_grid * (kTileShares / kTurns);
+    uint32_t turns = 0;
+#pragma unroll
+    for (int k = 0; k < kTurns; ++k)
+      if (fp4_cut<Fp4Tile, D>(tile_parts, tile_grid, (blockIdx.x - row_grid * kRowShares + k * n) / kTileShares)->rows > 0) turns |= 1u << k;
+#pragma unroll 1
+    for (; turns; turns &= turns - 1) {
+      const int i = blockIdx.x - row_grid * kRowShares + (__ffs(turns) - 1) * n;
+      fp4_join<Fp4Tile, D>(p, tile_parts, tile_grid, i / kTileShares, i % kTileShares, kTileShares);
+    }
   }
 }
 
@@ -501,7 +509,7 @@ static int launch_attn(const Fp4Attn& p, bool rows, bool tiles, float* parts, cu
   }
   if (tiles)
     if (const int rc = launch_fp4_tiles(p, D, tile_parts, stream)) return rc;
-  return launch_pdl(fp4_join_kernel<D, Shape::kRows>, dim3(row_grid * kRowShares + tile_grid * kTileShares), dim3(kJoinThreads), 0, stream, p, parts, row_grid,
+  return launch_pdl(fp4_join_kernel<D, Shape::kRows>, dim3(row_grid * kRowShares + tile_grid * (kTileShares / kTurns)), dim3(kJoinThreads), 0, stream, p, parts, row_grid,
                     tile_parts, tile_grid) == cudaSuccess ? 0 : -2;
 }
 
@@ -532,7 +540,8 @@ extern "C" int b200_fp4_attn(const B200Fp4Attn* a, cudaStream_t stream) {
   if (a->num_reqs > kMostReqs || a->num_tiles > kMostTiles) return -4;
   const int G = a->Hq / a->Hkv;
   // cells of the whole line in 31 bits, whatever the lengths
-  if ((double)a->max_blocks * (a->block_size / kCellTokens) * a->Hkv * ((double)a->total_q * G / 8 + a->num_reqs) > 2147483647.0) return -4;
+  if (((double)a->max_blocks * (a->block_size / kCellTokens) + Fp4Seq<16>::kStart) * a->Hkv * ((double)a->total_q * G / 8 + a->num_reqs) > 2147483647.0)
+    return -4;
   if ((double)a->max_blocks * a->block_size > 2147483647.0) return -4;
   if ((double)a->total_q * G * G >= 4294967296.0 || (double)a->max_blocks * (a->block_size / kCellTokens) * (a->block_size / kCellTokens) >= 4294967296.0)
     return -4;       // (Fp4Div)
@@ -553,13 +562,13 @@ extern "C" int b200_fp4_attn(const B200Fp4Attn* a, cudaStream_t stream) {
   p.softcap2 = a->softcap * 1.4426950408889634f;
   p.status = device_status_word();
   // Which sequences go to which kernel. Both are launched where the lengths, which only the device knows, may call for both.
-  static constexpr int kFew = 64;
+  static constexpr int kFew = 48;
   const bool tensor = a->D <= 128 && a->q_start && p.num_tiles > 0, long_one = tensor && (long long)a->total_q * G > kFew;
   bool rows = true, tiles = long_one;
   p.few = long_one ? kFew : 0x7fffffff;
   if (long_one && a->num_reqs == 1) { rows = false; p.few = -1; }
   float* parts = (float*)a->parts;
-  const bool two = a->D <= 128 && (a->q_start ? G > 4 || a->total_q > a->num_reqs : G > 8);      // row tiles of 16
+  const bool two = a->D <= 128 && (long long)a->total_q * G > 8ll * a->num_reqs;      // row tiles of 16
   if (a->D == 64) return two ? launch_attn<64, 2>(p, rows, tiles, parts, stream) : launch_attn<64, 1>(p, rows, tiles, parts, stream);
   if (a->D == 128) return two ? launch_attn<128, 2>(p, rows, tiles, parts, stream) : launch_attn<128, 1>(p, rows, tiles, parts, stream);
   return launch_attn<256, 1>(p, rows, tiles, parts, stream);

@@ -160,24 +160,33 @@ __global__ void __launch_bounds__(128) fp4_append_kernel(B200Fp4Append p) {
           other[e] = d < rot ? b[side * D + (d < half ? d + half : d - half)] : 0.f;
         }
       }
-      if (!is_v) {
+      if (p.neox && !(half & 7)) {                              // the lane's dims are all turned, or none is
+        if (!is_v && l * 8 < rot) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) y[e] = x[e] * c[e] + other[e] * s[e];
+        }
+      } else if (!is_v) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) y[e] = l * 8 + e < rot ? x[e] * c[e] + other[e] * s[e] : x[e];
       }
+    }
+    const auto query = [&] {
+      __nv_bfloat16* dst = p.q_out ? (__nv_bfloat16*)p.q_out + (size_t)t * p.ldo + h * D
+                                   : (__nv_bfloat16*)p.q + (size_t)t * p.ldq + (size_t)h * p.q_head_stride;
+      *reinterpret_cast<uint4*>(dst + l * 8) = make_uint4(pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3]), pack_bf16x2(y[4], y[5]),
+                                                          pack_bf16x2(y[6], y[7]));
+    };
+    if (h0 + (i + 1) * kHeads <= p.Hq) {                        // (the warp's heads are all query heads)
+      query();
+      continue;
     }
     uint32_t top = 0;                                           // of |y|, as bits: a NaN is above infinity
 #pragma unroll
     for (int e = 0; e < 8; ++e) top = max(top, __float_as_uint(y[e]) & 0x7fffffffu);
     top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
     if (h >= nheads) continue;
-    if (is_q) {
-      __nv_bfloat16* dst = p.q_out ? (__nv_bfloat16*)p.q_out + (size_t)t * p.ldo + h * D
-                                   : (__nv_bfloat16*)p.q + (size_t)t * p.ldq + (size_t)h * p.q_head_stride;
-      *reinterpret_cast<uint4*>(dst + l * 8) = make_uint4(pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3]), pack_bf16x2(y[4], y[5]),
-                                                          pack_bf16x2(y[6], y[7]));
-      continue;
-    }
-    if (!cell) continue;
+    if (is_q) query();
+    if (is_q || !cell) continue;
     const uint8_t scale = fp4_scale_byte(__fdiv_rn(__uint_as_float(top), 6.f));
     const float sf = fp4_scale_value(scale);
     // Quotients by the scale's reciprocal and one correction by the remainder (fma): values of few bits lie exactly between two codes, and there

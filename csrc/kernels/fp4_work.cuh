@@ -100,7 +100,7 @@ struct Fp4Span {
 static constexpr int kPairKeys = 2 * kCellTokens;
 template <int ROWS>
 struct Fp4Seq {                // pairs of cells, 32 keys; row tiles of ROWS
-  static constexpr int kRows = ROWS, kStart = 8, kSnap = 8;
+  static constexpr int kRows = ROWS, kStart = ROWS > 8 ? 28 : 20, kSnap = 8;
   int req, len, token0, rows, first, begin, cells, tiles;       // begin: first pair of the sequence that any row sees
   static __device__ __forceinline__ int count(const Fp4Attn& p) { return p.num_reqs; }
   __device__ __forceinline__ Fp4Seq() {}
