@@ -500,9 +500,11 @@ static int launch_attn(const Fp4Attn& p, bool rows, bool tiles, float* parts, cu
   const int row_grid = rows ? b200_num_sms() * (NT == 1 && D <= 128 ? 2 : 1) : 0, tile_grid = tiles ? fp4_tile_grid() : 0;
   float* tile_parts = parts + fp4_scratch<Seq, D>(row_grid);
   if (rows) {
-    static PerDeviceOnce once;
-    if (once.first())
-      cudaFuncSetAttribute(fp4_rows_kernel<D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape::kFixed + (kMostReqs + 1) * 4);
+    static Fp4Once once;
+    if (!once.run([] {
+          return cudaFuncSetAttribute(fp4_rows_kernel<D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape::kFixed + (kMostReqs + 1) * 4) == cudaSuccess;
+        }))
+      return -2;
     if (launch_pdl(fp4_rows_kernel<D, NT>, dim3(row_grid), dim3(Shape::kWarps * 32), Shape::kFixed + (size_t)(p.num_reqs + 1) * 4, stream, p, parts) !=
         cudaSuccess)
       return -2;
@@ -542,7 +544,7 @@ extern "C" int b200_fp4_attn(const B200Fp4Attn* a, cudaStream_t stream) {
   // cells of the whole line in 31 bits, whatever the lengths
   if (((double)a->max_blocks * (a->block_size / kCellTokens) + Fp4Seq<16>::kStart) * a->Hkv * ((double)a->total_q * G / 8 + a->num_reqs) > 2147483647.0)
     return -4;
-  if ((double)a->max_blocks * a->block_size > 2147483647.0) return -4;
+  if ((double)a->max_blocks * a->block_size > 2147479552.0) return -4;          // (positions and a tile behind them in 31 bits)
   if ((double)a->total_q * G * G >= 4294967296.0 || (double)a->max_blocks * (a->block_size / kCellTokens) * (a->block_size / kCellTokens) >= 4294967296.0)
     return -4;       // (Fp4Div)
   Fp4Attn p;
@@ -554,7 +556,7 @@ extern "C" int b200_fp4_attn(const B200Fp4Attn* a, cudaStream_t stream) {
   p.tile_req = (const int32_t*)a->tile_req; p.tile_q0 = (const int32_t*)a->tile_q0;
   p.num_reqs = a->num_reqs; p.total_q = a->total_q; p.num_tiles = a->q_start ? a->num_tiles : 0;
   p.Hkv = a->Hkv; p.G = G; p.cells_per_page = a->block_size / kCellTokens;
-  p.window = a->window; p.causal = a->causal;
+  p.window = max(-(1 << 30), min(a->window, 1 << 30)); p.causal = a->causal;
   const auto by = [](int d) { return Fp4Div{d == 1 ? 0u : (uint32_t)(((1ull << 32) + d - 1) / d)}; };
   p.by_group = by(G);
   p.by_page_cells = by(p.cells_per_page);

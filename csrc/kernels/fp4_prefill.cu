@@ -545,17 +545,14 @@ int fp4_tile_grid() { return b200_num_sms(); }
 template <int D>
 static int launch_tiles(const Fp4Attn& p, float* parts, cudaStream_t stream) {
   const size_t smem = 1024 + Fp4TileShape<D>::kLine + (size_t)(p.num_tiles + 1) * 4;
-  static PerDeviceOnce once;
-  static std::atomic<int> regs{0};
-  if (once.first()) {
-    cudaFuncAttributes attr;
-    if (cudaFuncGetAttributes(&attr, fp4_tiles_kernel<D>) != cudaSuccess) return -2;
-    if (cudaFuncSetAttribute(fp4_tiles_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, 1024 + Fp4TileShape<D>::kLine + 8001 * 4) != cudaSuccess)
-      return -2;
-    regs = attr.numRegs;
-  }
-  // a warpgroup waits without limit for registers that the launch did not bring
-  if (4 * regs < kRegsIssue + 2 * kRegsSoftmax + kRegsExpand) return -2;
+  static Fp4Once once;
+  if (!once.run([] {
+        cudaFuncAttributes attr;
+        // (a warpgroup waits without limit for registers that the launch did not bring)
+        return cudaFuncGetAttributes(&attr, fp4_tiles_kernel<D>) == cudaSuccess && 4 * attr.numRegs >= kRegsIssue + 2 * kRegsSoftmax + kRegsExpand &&
+               cudaFuncSetAttribute(fp4_tiles_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, 1024 + Fp4TileShape<D>::kLine + 8001 * 4) == cudaSuccess;
+      }))
+    return -2;
   return launch_pdl(fp4_tiles_kernel<D>, dim3(fp4_tile_grid()), dim3(512), smem, stream, p, parts) == cudaSuccess ? 0 : -2;
 }
 

@@ -7,6 +7,8 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <mutex>
+
 #include "fp4_cache.cuh"
 #include "sm100.cuh"
 
@@ -334,6 +336,23 @@ __device__ __forceinline__ void fp4_join(const Fp4Attn& p, float* parts, uint32_
     }
   }
 }
+
+// What a kernel needs set once a device, before its first launch there; a call that comes meanwhile waits.
+struct Fp4Once {
+  std::mutex lock;
+  unsigned long long done = 0;
+  template <class Set>
+  bool run(Set set) {
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess) return false;
+    const std::lock_guard<std::mutex> held(lock);
+    const unsigned long long bit = dev < 64 ? 1ull << dev : 0;
+    if (done & bit) return true;
+    if (!set()) return false;
+    done |= bit;
+    return true;
+  }
+};
 
 // The tile kernel (fp4_prefill.cu): the grid it runs on, its least cells a CTA, and its launch.
 int fp4_tile_grid();

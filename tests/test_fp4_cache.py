@@ -174,3 +174,32 @@ def test_refusals_without_a_gpu():
     refused("qkv is", C.append, qkv.float(), pos, cs, cache, slots, num_q_heads=6)
     refused("head_dim", C.alloc, 2, 2, 24, 64, "cpu")
     refused("head_dim", C.alloc, 2, 2, 16, 96, "cpu")
+
+
+def test_refusals_of_rows_that_share_memory_and_of_numbers_past_the_limits():
+    cache = C.alloc(2, 2, 16, 64, "cpu")
+    q = torch.zeros((3, 256), dtype=torch.bfloat16)
+    table, lens = torch.zeros((3, 2), dtype=torch.int32), torch.ones(3, dtype=torch.int32)
+    good = dict(block_table=table, seq_lens=lens, scale=1.0, out=torch.zeros_like(q))
+
+    def refused(rule, call, *a, **kw):
+        with pytest.raises(OpArgumentError, match=rule):
+            call(*a, **kw)
+    refused("out is like q", C.decode, q, cache, **{**good, "out": torch.zeros((1, 256), dtype=torch.bfloat16).expand(3, 256)})
+    refused("window in 32 bits", C.decode, q, cache, window=2 ** 31, **good)
+    refused("window in 32 bits", C.decode, q, cache, window=-2 ** 31, **good)
+    refused("softcap finite", C.decode, q, cache, softcap=float("inf"), **good)
+    refused("scale is positive", C.decode, q, cache, **{**good, "scale": float("nan")})
+    many = torch.zeros((8193, 256), dtype=torch.bfloat16)
+    refused("8192 sequences", C.decode, many, cache, block_table=table.new_zeros((8193, 1)), seq_lens=lens.new_zeros(8193), scale=1.0,
+            out=torch.zeros_like(many))
+    ints = torch.zeros(8194, dtype=torch.int32)
+    refused("8000 tiles", C.prefill, q, cache, q_start=ints[:4], tile_req=ints[:8001], tile_q0=ints[:8001], **good)
+    refused("8192 sequences", C.prefill, q, cache, q_start=ints, tile_req=ints[:1], tile_q0=ints[:1], scale=1.0, out=good["out"],
+            block_table=table.new_zeros((8193, 1)), seq_lens=lens.new_zeros(8193))
+    refused("q_start", C.prefill, q, cache, q_start=None, tile_req=ints[:1], tile_q0=ints[:1], **good)
+    qkv, slots = torch.zeros((3, 640), dtype=torch.bfloat16), torch.zeros(3, dtype=torch.int64)
+    refused("apart from one another", C.append, qkv, None, None, cache, slots, num_q_heads=4, q_head_stride=32)
+    refused("apart from one another", C.append, qkv, None, None, cache, slots, num_q_heads=6, offsets=(0, 320, 512))
+    refused("apart from one another", C.append, qkv[:1].expand(3, 640), None, None, cache, slots, num_q_heads=6)
+    refused("q_out", C.append, qkv, None, None, cache, slots, num_q_heads=1, q_out=torch.zeros((1, 64), dtype=torch.bfloat16).expand(3, 64))

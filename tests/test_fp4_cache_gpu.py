@@ -448,3 +448,130 @@ def test_two_streams_at_once():
     torch.cuda.synchronize()
     for i, (_, want, _) in enumerate(work):
         assert all(torch.equal(x, want) for x in got[i])
+
+
+BORDER = [
+    # sequences on both sides of the line between the kernels (48 rows), and of the rule for row tiles of 8 and 16
+    ([400] * 6, [11, 12, 13, 12, 1, 130], 16, 4, 128, 32),
+    ([90, 49, 48, 47], [90, 49, 48, 47], 4, 4, 64, 16),
+    ([700] * 5, [1, 2, 1, 1, 1], 8, 2, 128, 32),
+    ([700] * 5, [3, 2, 1, 4, 2], 8, 2, 128, 32),
+    ([300, 49, 70], [48, 49, 3], 3, 3, 256, 16),
+]
+
+
+@pytest.mark.parametrize("lens,new,Hq,Hkv,D,bs", BORDER)
+def test_both_sides_of_the_choices(lens, new, Hq, Hkv, D, bs):
+    q, cache, table, n = _case(lens, new, Hq, Hkv, D, bs, 0, seed=sum(lens))
+    req, q0 = _tiles(new)
+    out = C.prefill(q.to(DEV), cache.to(DEV), block_table=table.to(DEV), seq_lens=n.to(DEV), q_start=torch.tensor([0] + new).cumsum(0).int().to(DEV),
+                    tile_req=req, tile_q0=q0, scale=0.1)
+    _check(out, q, cache, table, lens, new, Hq, D, bs, 0.1, 0.0, 0)
+    assert _status() == 0
+
+
+@pytest.mark.parametrize("D,Hq,Hkv", [(64, 1, 1), (128, 2, 1), (128, 16, 1), (256, 1, 1)])
+def test_as_many_sequences_as_a_call_takes(D, Hq, Hkv):
+    """8192 sequences of 0 to 3 keys, in pages that neighbours share."""
+    R, bs, gen = 8192, 16, _gen(D + Hq)
+    cache = F.random_cache(9, Hkv, bs, D, gen)
+    page = torch.randint(0, 9, (R, 1), generator=gen, dtype=torch.int32)
+    n = torch.randint(0, 4, (R,), generator=gen, dtype=torch.int32)
+    q = torch.randn((R, Hq * D), generator=gen).to(torch.bfloat16)
+    got = C.decode(q.to(DEV), cache.to(DEV), block_table=page.to(DEV), seq_lens=n.to(DEV), scale=0.1).cpu()
+    for at in range(9):
+        for length in range(4):
+            rows = ((page[:, 0] == at) & (n == length)).nonzero()[:, 0]
+            if length == 0:
+                assert not got[rows].any()
+                continue
+            k, v = C.ref_read(cache, torch.arange(at * bs, at * bs + length))
+            want = F.attention(q[rows].view(len(rows), Hq, D), k, v, 0, 0.1, 0.0, 0, causal=False)
+            F.check_attention(got[rows].view(len(rows), Hq, D), *want)
+    assert _status() == 0
+
+
+@pytest.mark.parametrize("window", [1, 2 ** 31 - 1, -(2 ** 31 - 1)])
+def test_windows_of_one_key_and_past_every_sequence(window):
+    lens, new, Hq, Hkv, D, bs = [300, 1, 65], [300, 1, 2], 4, 2, 128, 16
+    q, cache, table, n = _case(lens, new, Hq, Hkv, D, bs, 1 if window == 1 else 0, seed=9)
+    req, q0 = _tiles(new)
+    args = dict(block_table=table.to(DEV), seq_lens=n.to(DEV), scale=0.1, window=window)
+    out = C.prefill(q.to(DEV), cache.to(DEV), q_start=torch.tensor([0] + new).cumsum(0).int().to(DEV), tile_req=req, tile_q0=q0, **args)
+    _check(out, q, cache, table, lens, new, Hq, D, bs, 0.1, 0.0, 1 if window == 1 else 0)
+    last = torch.tensor(new).cumsum(0) - 1
+    out = C.decode(q[last].to(DEV), cache.to(DEV), **args)
+    _check(out, q[last], cache, table, lens, [1] * 3, Hq, D, bs, 0.1, 0.0, 1 if window == 1 else 0)
+
+
+def test_a_tile_listed_twice_and_pages_that_sequences_share():
+    lens, new, Hq, Hkv, D, bs = [700, 690], [300, 290], 8, 2, 128, 32
+    q, cache, table, n = _case(lens, new, Hq, Hkv, D, bs, 0, seed=31)
+    table[1] = table[0]
+    req, q0 = _tiles(new)
+    req, q0 = torch.cat([req, req[:2]]), torch.cat([q0, q0[:2]])
+    out = C.prefill(q.to(DEV), cache.to(DEV), block_table=table.to(DEV), seq_lens=n.to(DEV), q_start=torch.tensor([0, 300, 590], dtype=torch.int32, device=DEV),
+                    tile_req=req, tile_q0=q0, scale=0.1)
+    _check(out, q, cache, table, lens, new, Hq, D, bs, 0.1, 0.0, 0)
+
+
+def test_two_graphs_that_share_scratch():
+    """Two steps captured over one scratch, replayed one after the other in both orders, with lengths that change."""
+    Hq, Hkv, D, bs, new = 8, 2, 128, 32, [40, 3]
+    one, two = ([900, 700], 2), ([1300, 64], 5)
+    tmp = C.scratch(torch.device(DEV, torch.cuda.current_device()), D)
+    req, q0 = _tiles(new)
+    start = torch.tensor([0, 40, 43], dtype=torch.int32, device=DEV)
+    graphs = []
+    for lens, seed in (one, two):
+        q, cache, table, n = _case(lens, new, Hq, Hkv, D, bs, 0, seed=seed)
+        t = [x.to(DEV) for x in (q, cache, table, n)]
+        out = torch.empty_like(t[0])
+
+        def run(t=t, out=out):
+            C.prefill(t[0], t[1], block_table=t[2], seq_lens=t[3], q_start=start, tile_req=req, tile_q0=q0, scale=0.1, out=out, tmp=tmp)
+        run()
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            run()
+        graphs.append((g, out, (q, cache, table, lens), t))      # (the graph reads what t holds)
+    for order in ((0, 1), (1, 0), (0, 0, 1)):
+        for _, out, _, _ in graphs:
+            out.fill_(5)
+        for i in order:
+            graphs[i][0].replay()
+        torch.cuda.synchronize()
+        for _, out, (q, cache, table, lens), _ in graphs:
+            _check(out, q, cache, table, lens, new, Hq, D, bs, 0.1, 0.0, 0)
+
+
+def test_two_threads_at_once():
+    import threading
+    Hq, Hkv, D, bs = 8, 2, 64, 32
+    work = []
+    for i, (lens, new) in enumerate((([500, 50], [200, 50]), ([40, 2500, 900], [3, 700, 9]))):
+        q, cache, table, n = _case(lens, new, Hq, Hkv, D, bs, 0, seed=40 + i)
+        req, q0 = _tiles(new)
+        work.append(((q.to(DEV), cache.to(DEV)), dict(block_table=table.to(DEV), seq_lens=n.to(DEV), tile_req=req, tile_q0=q0, scale=0.1,
+                                                      q_start=torch.tensor([0] + new).cumsum(0).int().to(DEV)), (q, cache, table, lens, new)))
+    torch.cuda.synchronize()
+    got, errors = [[], []], []
+
+    def thread(i):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(10):
+                    got[i].append(C.prefill(*work[i][0], **work[i][1]))
+        except Exception as e:                                   # (a thread's exception does not end the test by itself)
+            errors.append(e)
+    threads = [threading.Thread(target=thread, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert not errors
+    for i, (_, _, (q, cache, table, lens, new)) in enumerate(work):
+        for out in got[i]:
+            _check(out, q, cache, table, lens, new, Hq, D, bs, 0.1, 0.0, 0)

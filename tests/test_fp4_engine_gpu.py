@@ -89,3 +89,15 @@ def test_chunks_of_a_gpu_cache_travel_as_bf16():
     for a, b in zip(caches, back):
         assert torch.equal(fp4_cache.ref_expand(a)[blocks[:4]], fp4_cache.ref_expand(b)[others])
     store.client.close()
+
+
+def test_a_draft_model_with_a_cache_in_bf16():
+    from vllm_cpp_b200.spec_decode import SpeculativeConfig
+    cfg = _cfg()
+    prompts = _prompts(cfg, (60, 45))
+    plain, _ = _run("cuda", cfg, prompts, kv_cache_dtype="fp4")
+    drafted, llm = _run("cuda", cfg, prompts, kv_cache_dtype="fp4", speculative_config=SpeculativeConfig(
+        method="draft_model", num_speculative_tokens=2, draft_model_config=_cfg()))
+    assert llm.runner.drafter.model.kv_caches[0].dtype == torch.bfloat16
+    assert _agreement(plain, drafted) > 0.9
+    assert ops.read_status() == 0

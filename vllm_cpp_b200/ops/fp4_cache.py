@@ -98,7 +98,7 @@ def append(qkv: torch.Tensor, positions: Optional[torch.Tensor], cos_sin: Option
            q_out: Optional[torch.Tensor] = None, q_head_stride: Optional[int] = None,
            offsets: Optional[tuple[int, int, int]] = None) -> None:
     """Per-head RMSNorm of q and k (weights bf16 ``[D]``, optional) and rotation of merged ``[T, q | k | v]`` rows; q in place or to
-    ``q_out`` ``[T, Hq * D]``, k and v into the cache. ``cos_sin``: fp32 ``[positions, cos | sin]`` (None: no rotation), ``rot_dim``
+    ``q_out`` ``[T, Hq * D]`` (apart from ``qkv``), k and v into the cache. ``cos_sin``: fp32 ``[positions, cos | sin]`` (None: no rotation), ``rot_dim``
     its width, pairs half of it apart (``neox``) or neighbours. ``offsets``: columns where q, k and v begin; ``q_head_stride``:
     columns between q heads. The slots of a call differ; slots outside the cache (-1) write nothing, and a position
     outside the table makes its row NaN. The k and v columns of ``qkv`` stay as they are."""
@@ -114,7 +114,7 @@ def append(qkv: torch.Tensor, positions: Optional[torch.Tensor], cos_sin: Option
               and bs > 0 and cache.dtype is torch.uint8 and cache.is_contiguous() and qkv.dtype is BF16 and qkv.stride(1) == 1
               and slots.dtype is torch.int64 and slots.is_contiguous() and n >= T and hs == D and num_q_heads >= 0
               and offsets == (0, num_q_heads * D, (num_q_heads + H) * D) and cols >= (num_q_heads + 2 * H) * D
-              and (qkv.data_ptr() | cache.data_ptr() | 2 * qkv.stride(0)) % 16 == 0)
+              and (qkv.data_ptr() | cache.data_ptr() | 2 * qkv.stride(0)) % 16 == 0 and (T <= 1 or qkv.stride(0) >= cols))
         if ok and cos_sin is not None:
             rows, width = cos_sin.shape
             ok = (cos_sin.dtype is torch.float32 and cos_sin.is_contiguous() and width == rot and rows > 0 and 0 < rot <= D and rot % 2 == 0
@@ -122,7 +122,8 @@ def append(qkv: torch.Tensor, positions: Optional[torch.Tensor], cos_sin: Option
                   and dev == cos_sin.get_device() == positions.get_device())
         if ok and q_out is not None:
             ok = (q_out.dtype is BF16 and q_out.get_device() == dev and q_out.dim() == 2 and q_out.stride(1) == 1 and q_out.shape[0] >= T
-                  and q_out.shape[1] == num_q_heads * D and (q_out.data_ptr() | 2 * q_out.stride(0)) % 16 == 0)
+                  and q_out.shape[1] == num_q_heads * D and (q_out.data_ptr() | 2 * q_out.stride(0)) % 16 == 0
+                  and (T <= 1 or q_out.stride(0) >= q_out.shape[1]))
         for w in (q_norm, k_norm):
             if ok and w is not None:
                 ok = w.dtype is BF16 and w.get_device() == dev and w.numel() == D and w.is_contiguous() and w.data_ptr() % 16 == 0
@@ -204,6 +205,7 @@ def scratch(device: torch.device, head_dim: int, prefill: bool = True) -> torch.
 
 
 _I32 = torch.int32
+_MOST = 2 ** 31
 
 
 def _attend(op, q, cache, block_table, seq_lens, q_start, tile_req, tile_q0, scale, out, softcap, window, causal, tmp):
@@ -218,23 +220,24 @@ def _attend(op, q, cache, block_table, seq_lens, q_start, tile_req, tile_q0, sca
               and q.dtype is BF16 and out.dtype is BF16 and cache.dtype is torch.uint8 and block_table.dtype is _I32
               and seq_lens.dtype is _I32 and D in (64, 128, 256) and width == 18 * D and cells > 0 and pages > 0 and cols > 0
               and cols % (D * H) == 0 and out.shape == q.shape and cache.is_contiguous() and seq_lens.is_contiguous()
-              and q.stride(1) == 1 and out.stride(1) == 1 and block_table.stride(1) == 1 and scale > 0 and softcap >= 0
+              and q.stride(1) == 1 and out.stride(1) == 1 and block_table.stride(1) == 1 and scale > 0 and 0 <= softcap < math.inf
+              and -_MOST < window < _MOST
               and (q.data_ptr() | out.data_ptr() | cache.data_ptr() | 2 * q.stride(0) | 2 * out.stride(0)) % 16 == 0
-              and q.data_ptr() != out.data_ptr()
+              and q.data_ptr() != out.data_ptr() and (rows <= 1 or out.stride(0) >= cols)
               and (tmp is None or (tmp.dtype is torch.float32 and tmp.get_device() == dev and tmp.is_contiguous()
                                    and tmp.data_ptr() % 16 == 0 and tmp.numel() >= scratch_floats(q.device, D, q_start is not None))))
-        if q_start is None:
-            ok = ok and reqs >= rows and n >= rows
+        if op == "fp4_decode":
+            ok = ok and reqs >= rows and n >= rows and rows <= 8192
         else:
             ok = ok and (q_start.dtype is tile_req.dtype is tile_q0.dtype is _I32 and q_start.dim() == tile_req.dim() == tile_q0.dim() == 1
-                         and dev == q_start.get_device() == tile_req.get_device() == tile_q0.get_device() and q_start.numel() > 0
+                         and dev == q_start.get_device() == tile_req.get_device() == tile_q0.get_device() and 8193 >= q_start.numel() > 0
                          and q_start.is_contiguous() and tile_req.is_contiguous() and tile_q0.is_contiguous()
-                         and tile_q0.numel() >= tile_req.numel())
+                         and tile_q0.numel() >= tile_req.numel() <= 8000)
     except (TypeError, ValueError, AttributeError):
         ok = False
     if not ok:
         validate(op, q=q, cache=cache, block_table=block_table, seq_lens=seq_lens, q_start=q_start, tile_req=tile_req,
-                 tile_q0=tile_q0, out=out, scale=scale, softcap=softcap, tmp=tmp)
+                 tile_q0=tile_q0, out=out, scale=scale, softcap=softcap, window=window, tmp=tmp)
         (rows, cols), (nb, H, cells, width), (reqs, pages), (n,) = q.shape, cache.shape, block_table.shape, seq_lens.shape
         D = width // 18
     _declare()
@@ -260,7 +263,7 @@ def decode(q: torch.Tensor, cache: torch.Tensor, *, block_table: torch.Tensor, s
            tmp: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Attention of one query row a sequence, ``q`` ``[B, Hq * D]``, at its last position. ``seq_lens`` int32 ``[B]`` counts the row's own
     key; 0: zeros come out. ``window`` as in :func:`vllm_cpp_b200.ops.attn_decode`; entries of ``block_table`` outside the cache count as
-    masked keys. ``tmp``: :func:`scratch`, allocated if not given."""
+    masked keys. ``out`` shares no memory with ``q``. ``tmp``: :func:`scratch`, allocated if not given. At most 8192 sequences."""
     return _attend("fp4_decode", q, cache, block_table, seq_lens, None, None, None, scale, out, softcap, window, True, tmp)
 
 
@@ -269,7 +272,7 @@ def prefill(q: torch.Tensor, cache: torch.Tensor, *, block_table: torch.Tensor, 
             window: int = 0, causal: bool = True, tmp: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Attention of the query rows ``q_start[r]..q_start[r + 1]`` of each sequence, the last of its ``seq_lens[r]`` positions.
     ``tile_req`` / ``tile_q0`` list their 128-row tiles, as in :func:`vllm_cpp_b200.ops.attn_prefill`. Rows outside every
-    sequence stay as they are."""
+    sequence stay as they are. At most 8192 sequences and 8000 tiles."""
     return _attend("fp4_prefill", q, cache, block_table, seq_lens, q_start, tile_req, tile_q0, scale, out, softcap, window, causal, tmp)
 
 

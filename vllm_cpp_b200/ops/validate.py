@@ -9,6 +9,8 @@ shape / dtype / layout errors in front of every backend).
 """
 from __future__ import annotations
 
+import math
+
 import torch
 
 
@@ -114,16 +116,31 @@ def _bf16_rows(t) -> bool:
     return t.dim() == 2 and t.dtype == BF16 and (t.shape[0] <= 1 or _rows16(t)) and (t.shape[1] <= 1 or t.stride(1) == 1) and t.data_ptr() % 16 == 0
 
 
+def _apart(t) -> bool:
+    """Rows that a kernel may write: none begins inside another."""
+    return t.shape[0] <= 1 or t.stride(0) >= t.shape[1]
+
+
+def _apart_from_keys(H, D, num_q_heads, stride, offsets) -> bool:
+    """Query heads that a kernel may write in place lie apart from one another and from the keys and values."""
+    heads = [(offsets[0] + i * stride, offsets[0] + i * stride + D) for i in range(num_q_heads)]
+    return (num_q_heads <= 1 or stride >= D) and not any(a < o + H * D and o < b for a, b in heads for o in offsets[1:])
+
+
 _FP4_CACHE = ("cache is uint8 [blocks, kv heads, block_size / 16, 18 head_dim], contiguous, head_dim 64, 128 or 256", _fp4_cache)
 _FP4_ATTN = [
     _FP4_CACHE,
     ("q is [rows, Hq * head_dim] bf16 with rows on 16-byte boundaries, Hq a multiple of the kv heads", lambda q, cache, **_: _bf16_rows(q)
      and q.shape[1] > 0 and q.shape[1] % (cache.shape[3] // 18 * cache.shape[1]) == 0),
-    ("out is like q and apart from it", lambda q, out, **_: _bf16_rows(out) and out.shape == q.shape and (
-        q.numel() == 0 or out.data_ptr() != q.data_ptr())),
+    ("out is like q and apart from it, its rows apart from one another", lambda q, out, **_: _bf16_rows(out) and out.shape == q.shape and _apart(out)
+     and (q.numel() == 0 or out.data_ptr() != q.data_ptr())),
     ("block_table is int32 [sequences, pages], rows contiguous", lambda block_table, **_: block_table.dtype == torch.int32
      and block_table.dim() == 2 and block_table.shape[1] > 0 and (block_table.shape[1] == 1 or block_table.stride(1) == 1)),
-    ("scale is positive and softcap is not negative", lambda scale, softcap, **_: scale > 0 and softcap >= 0),
+    ("scale is positive, softcap finite and not negative, window in 32 bits", lambda scale, softcap, window=0, **_: scale > 0
+     and 0 <= softcap < math.inf and -2 ** 31 < window < 2 ** 31),
+    ("there are at most 8192 sequences and 8000 tiles", lambda q, block_table, seq_lens, tile_req=None, q_start=None, **_: (
+        q.shape[0] if q_start is None else min(block_table.shape[0], seq_lens.numel(), q_start.numel() - 1)) <= 8192 and (
+            tile_req is None or tile_req.numel() <= 8000)),
     ("tmp is fp32 and large enough", lambda cache, q_start=None, tmp=None, **_: tmp is None or (
         tmp.dtype == torch.float32 and tmp.is_contiguous() and tmp.data_ptr() % 16 == 0
         and tmp.numel() >= _fp4_scratch(cache, q_start is not None))),
@@ -145,6 +162,9 @@ RULES.update({
          num_q_heads >= 0 and all(o >= 0 and o % 8 == 0 for o in (*offsets, q_head_stride)) and max(
              offsets[0] + (num_q_heads - 1) * q_head_stride + cache.shape[3] // 18 if num_q_heads else 0,
              max(offsets[1:]) + cache.shape[1] * (cache.shape[3] // 18)) <= qkv.shape[1]),
+        ("query heads turned in place lie apart from one another, from the keys and from the values", lambda qkv, cache, num_q_heads, q_head_stride,
+         offsets, q_out, **_: q_out is not None or (
+             _apart(qkv) and _apart_from_keys(cache.shape[1], cache.shape[3] // 18, num_q_heads, q_head_stride, offsets))),
         ("slots is int64 [T]", lambda qkv, slots, **_: _ids(slots, torch.int64, qkv.shape[0])),
         ("cos_sin is fp32 [positions, rot_dim] with positions int64 [T], rot_dim even and at most head_dim",
          lambda qkv, cache, cos_sin, positions, rot_dim, **_: cos_sin is None or (
@@ -155,7 +175,7 @@ RULES.update({
             w is None or (w.dtype == BF16 and w.is_contiguous() and w.numel() == cache.shape[3] // 18 and w.data_ptr() % 16 == 0)
             for w in (q_norm, k_norm))),
         ("q_out is [T, Hq * head_dim] bf16 with rows on 16-byte boundaries", lambda qkv, cache, num_q_heads, q_out, **_: q_out is None or (
-            _bf16_rows(q_out) and q_out.shape[0] >= qkv.shape[0] and q_out.shape[1] == num_q_heads * (cache.shape[3] // 18))),
+            _bf16_rows(q_out) and _apart(q_out) and q_out.shape[0] >= qkv.shape[0] and q_out.shape[1] == num_q_heads * (cache.shape[3] // 18))),
         ("all tensors are on one GPU", lambda qkv, cache, slots, positions, cos_sin, q_norm, k_norm, q_out, **_:
          _on_gpu(qkv, cache, slots, positions, cos_sin, q_norm, k_norm, q_out)),
     ],
@@ -178,10 +198,10 @@ RULES.update({
         ("block_table and seq_lens (int32) have a row for each of q", lambda q, block_table, seq_lens, **_:
          block_table.shape[0] >= q.shape[0] and _ids(seq_lens, torch.int32, q.shape[0])),
     ],
-    "fp4_prefill": _FP4_ATTN + [
-        ("q_start, seq_lens, tile_req and tile_q0 are int32", lambda seq_lens, q_start, tile_req, tile_q0, **_: _ids(q_start, torch.int32, 1)
+    "fp4_prefill": [
+        ("q_start, seq_lens, tile_req and tile_q0 are int32", lambda seq_lens, q_start, tile_req, tile_q0, **_: q_start is not None and _ids(q_start, torch.int32, 1)
          and _ids(seq_lens, torch.int32, 0) and _ids(tile_req, torch.int32, 0) and _ids(tile_q0, torch.int32, tile_req.numel())),
-    ],
+    ] + _FP4_ATTN,
 })
 
 
