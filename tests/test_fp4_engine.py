@@ -130,3 +130,21 @@ def test_chunks_travel_as_bf16_and_come_back_as_the_same_codes():
         for x, y in zip(blocks[:4], others):
             assert torch.equal(fp4_cache.ref_expand(a)[x], fp4_cache.ref_expand(b)[y])
     store.client.close()
+
+
+def test_a_model_class_that_says_nothing_of_its_cache(monkeypatch):
+    from vllm_cpp_b200.models import registry
+    from vllm_cpp_b200.models.dense import DenseModel
+
+    class Quiet:
+        """What an engine asks of a model, from one that it is made of; no KV_CACHE_DTYPES."""
+        DTYPES = ("bfloat16",)
+
+        def __new__(cls, *a, **kw):
+            return DenseModel(*a, **kw)
+    monkeypatch.setattr(registry, "resolve", lambda architectures: ("Quiet", Quiet))
+    cfg = _cfg()
+    llm = LLM(EngineArgs(model_config=cfg, device="cpu", max_model_len=64, num_blocks=8))
+    assert llm.model.kv_caches[0].dtype == torch.bfloat16
+    with pytest.raises(ValueError, match="holds its KV cache in auto, not in fp4"):
+        LLM(EngineArgs(model_config=cfg, device="cpu", kv_cache_dtype="fp4", max_model_len=64, num_blocks=8))

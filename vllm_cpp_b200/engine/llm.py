@@ -80,8 +80,9 @@ class LLM:
             if args.dtype not in cls.DTYPES:
                 raise ValueError(f"{cfg.architecture} runs in {', '.join(cls.DTYPES)}, not in {args.dtype}")
             cfg.dtype = args.dtype
-        if args.kv_cache_dtype not in cls.KV_CACHE_DTYPES:
-            raise ValueError(f"{cfg.architecture} holds its KV cache in {', '.join(cls.KV_CACHE_DTYPES)}, not in {args.kv_cache_dtype}")
+        held = getattr(cls, "KV_CACHE_DTYPES", ("auto",))          # (a registered class may say nothing)
+        if args.kv_cache_dtype not in held:
+            raise ValueError(f"{cfg.architecture} holds its KV cache in {', '.join(held)}, not in {args.kv_cache_dtype}")
         if args.max_score_rows and par.tensor_parallel_size > 1:
             raise ValueError("scored positions need the whole vocabulary on one rank")
         self.model = cls(cfg, device=device, parallel=par, comm=self.comm, max_position=max_len)
