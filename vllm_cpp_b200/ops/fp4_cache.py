@@ -109,12 +109,12 @@ def append(qkv: torch.Tensor, positions: Optional[torch.Tensor], cos_sin: Option
     rot = (D if cos_sin is None else cos_sin.shape[1]) if rot_dim is None else rot_dim
     # (the rules of ops.validate for the plain call of a model's layer, in a fraction of their time)
     try:
-        (T, cols), dev, (n,) = qkv.shape, qkv.get_device(), slots.shape
+        (T, cols), (ld, one), dev, (n,), at = qkv.shape, qkv.stride(), qkv.get_device(), slots.shape, qkv.data_ptr()
         ok = (dev >= 0 and dev == cache.get_device() == slots.get_device() and D in (64, 128, 256) and cache.shape[3] == 18 * D
-              and bs > 0 and cache.dtype is torch.uint8 and cache.is_contiguous() and qkv.dtype is BF16 and qkv.stride(1) == 1
+              and bs > 0 and cache.dtype is torch.uint8 and cache.is_contiguous() and qkv.dtype is BF16 and one == 1
               and slots.dtype is torch.int64 and slots.is_contiguous() and n >= T and hs == D and num_q_heads >= 0
               and offsets == (0, num_q_heads * D, (num_q_heads + H) * D) and cols >= (num_q_heads + 2 * H) * D
-              and (qkv.data_ptr() | cache.data_ptr() | 2 * qkv.stride(0)) % 16 == 0 and (T <= 1 or qkv.stride(0) >= cols))
+              and (at | cache.data_ptr() | 2 * ld) % 16 == 0 and (T <= 1 or ld >= cols))
         if ok and cos_sin is not None:
             rows, width = cos_sin.shape
             ok = (cos_sin.dtype is torch.float32 and cos_sin.is_contiguous() and width == rot and rows > 0 and 0 < rot <= D and rot % 2 == 0
@@ -132,13 +132,12 @@ def append(qkv: torch.Tensor, positions: Optional[torch.Tensor], cos_sin: Option
     if not ok:
         validate("fp4_append", qkv=qkv, cache=cache, slots=slots, positions=positions, cos_sin=cos_sin, q_norm=q_norm, k_norm=k_norm,
                  q_out=q_out, num_q_heads=num_q_heads, rot_dim=rot, q_head_stride=hs, offsets=offsets)
-        T = qkv.shape[0]
+        T, ld, at = qkv.shape[0], qkv.stride(0), qkv.data_ptr()
     _declare()
     a = AppendArgs()
-    at = qkv.data_ptr()
     a.q, a.k, a.v = at + 2 * offsets[0], at + 2 * offsets[1], at + 2 * offsets[2]
     if T > 1:                      # (the stride of a single row says nothing)
-        a.ldq = a.ldk = a.ldv = qkv.stride(0)
+        a.ldq = a.ldk = a.ldv = ld
     if q_out is not None:
         a.q_out, a.ldo = q_out.data_ptr(), q_out.stride(0) if T > 1 else 0
     if cos_sin is not None:
@@ -177,9 +176,10 @@ def read(cache: torch.Tensor, slots: torch.Tensor, k: Optional[torch.Tensor] = N
     a = ReadArgs()
     a.num_blocks, a.Hkv, a.block_size, a.D = nb, H, bs, D
     n = a.n = slots.numel()
-    if k is None or v is None:
-        both = torch.empty((2, n, H, D), dtype=BF16, device=cache.device)
-        k, v = both[0] if k is None else k, both[1] if v is None else v
+    if k is None:
+        k = cache.new_empty((n, H, D), dtype=BF16)
+    if v is None:
+        v = torch.empty_like(k)
     a.cache, a.slots, a.k, a.v = cache.data_ptr(), slots.data_ptr(), k.data_ptr(), v.data_ptr()
     _launch(cache, _read, a, "fp4_read")
     return k, v
@@ -209,23 +209,25 @@ _MOST = 2 ** 31
 
 
 def _attend(op, q, cache, block_table, seq_lens, q_start, tile_req, tile_q0, scale, out, softcap, window, causal, tmp):
-    if out is None and q.is_cuda:
-        out = torch.empty((q.shape[0], q.shape[1]), dtype=q.dtype, device=q.device)
     # What the rules of ops.validate say, in a fraction of their time (a decode step calls this in every layer); they name what is
     # wrong, and judge what is rare.
+    given = out is not None
     try:
         (rows, cols), (nb, H, cells, width), (reqs, pages), (n,) = q.shape, cache.shape, block_table.shape, seq_lens.shape
-        dev, D = q.get_device(), width // 18
-        ok = (dev >= 0 and dev == cache.get_device() == out.get_device() == block_table.get_device() == seq_lens.get_device()
-              and q.dtype is BF16 and out.dtype is BF16 and cache.dtype is torch.uint8 and block_table.dtype is _I32
-              and seq_lens.dtype is _I32 and D in (64, 128, 256) and width == 18 * D and cells > 0 and pages > 0 and cols > 0
-              and cols % (D * H) == 0 and out.shape == q.shape and cache.is_contiguous() and seq_lens.is_contiguous()
-              and q.stride(1) == 1 and out.stride(1) == 1 and block_table.stride(1) == 1 and scale > 0 and 0 <= softcap < math.inf
-              and -_MOST < window < _MOST
-              and (q.data_ptr() | out.data_ptr() | cache.data_ptr() | 2 * q.stride(0) | 2 * out.stride(0)) % 16 == 0
-              and q.data_ptr() != out.data_ptr() and (rows <= 1 or out.stride(0) >= cols)
-              and (tmp is None or (tmp.dtype is torch.float32 and tmp.get_device() == dev and tmp.is_contiguous()
-                                   and tmp.data_ptr() % 16 == 0 and tmp.numel() >= scratch_floats(q.device, D, q_start is not None))))
+        (ldq, q1), (ldt, t1) = q.stride(), block_table.stride()
+        dev, D, qp, cp = q.get_device(), width // 18, q.data_ptr(), cache.data_ptr()
+        ok = (dev >= 0 and dev == cache.get_device() == block_table.get_device() == seq_lens.get_device()
+              and q.dtype is BF16 and cache.dtype is torch.uint8 and block_table.dtype is _I32
+              and seq_lens.dtype is _I32 and (D == 128 or D == 64 or D == 256) and width == 18 * D and cells > 0 and pages > 0 and cols > 0
+              and cols % (D * H) == 0 and cache.is_contiguous() and seq_lens.is_contiguous() and q1 == t1 == 1 and scale > 0
+              and 0 <= softcap < math.inf and -_MOST < window < _MOST and (qp | cp | 2 * ldq) % 16 == 0)
+        if ok and given:
+            (orows, ocols), (ldo, o1), op_ = out.shape, out.stride(), out.data_ptr()
+            ok = (orows == rows and ocols == cols and out.dtype is BF16 and out.get_device() == dev and o1 == 1
+                  and (op_ | 2 * ldo) % 16 == 0 and op_ != qp and (rows <= 1 or ldo >= cols))
+        if ok and tmp is not None:
+            ok = (tmp.dtype is torch.float32 and tmp.get_device() == dev and tmp.is_contiguous()
+                  and tmp.data_ptr() % 16 == 0 and tmp.numel() >= scratch_floats(q.device, D, op == "fp4_prefill"))
         if op == "fp4_decode":
             ok = ok and reqs >= rows and n >= rows and rows <= 8192
         else:
@@ -235,22 +237,25 @@ def _attend(op, q, cache, block_table, seq_lens, q_start, tile_req, tile_q0, sca
                          and tile_q0.numel() >= tile_req.numel() <= 8000)
     except (TypeError, ValueError, AttributeError):
         ok = False
+    if not given:
+        out = q.new_empty(q.shape)
+        op_, ldo = out.data_ptr(), out.stride(0) if out.dim() == 2 else 0
     if not ok:
         validate(op, q=q, cache=cache, block_table=block_table, seq_lens=seq_lens, q_start=q_start, tile_req=tile_req,
                  tile_q0=tile_q0, out=out, scale=scale, softcap=softcap, window=window, tmp=tmp)
         (rows, cols), (nb, H, cells, width), (reqs, pages), (n,) = q.shape, cache.shape, block_table.shape, seq_lens.shape
-        D = width // 18
+        D, qp, cp, op_, ldq, ldo, ldt = width // 18, q.data_ptr(), cache.data_ptr(), out.data_ptr(), q.stride(0), out.stride(0), block_table.stride(0)
     _declare()
     if tmp is None:
-        tmp = scratch(q.device, D, q_start is not None)
+        tmp = q.new_empty(scratch_floats(q.device, D, op == "fp4_prefill"), dtype=torch.float32)
     a = AttnArgs()
     a.num_blocks, a.Hkv, a.block_size, a.Hq, a.D = nb, H, cells * CELL, cols // D, D
-    a.q, a.out, a.cache, a.parts = q.data_ptr(), out.data_ptr(), cache.data_ptr(), tmp.data_ptr()
+    a.q, a.out, a.cache, a.parts = qp, op_, cp, tmp.data_ptr()
     if rows > 1:                   # (the stride of a single row says nothing)
-        a.ldq, a.ldo = q.stride(0), out.stride(0)
-    a.block_table, a.ldt, a.max_blocks = block_table.data_ptr(), block_table.stride(0), pages
+        a.ldq, a.ldo = ldq, ldo
+    a.block_table, a.ldt, a.max_blocks = block_table.data_ptr(), ldt, pages
     a.seq_lens, a.total_q, a.num_reqs = seq_lens.data_ptr(), rows, rows
-    if q_start is not None:
+    if op == "fp4_prefill":
         a.q_start, a.num_reqs = q_start.data_ptr(), min(q_start.numel() - 1, reqs, n)
         a.tile_req, a.tile_q0, a.num_tiles = tile_req.data_ptr(), tile_q0.data_ptr(), tile_req.numel()
     a.window, a.causal, a.scale, a.softcap = window, causal, scale, softcap
