@@ -94,15 +94,24 @@ __global__ void __launch_bounds__(Fp4RowsShape<D, NT>::kWarps * 32, NT == 1 && D
   pdl_launch_dependents();
   fp4_line<Seq>(p, line);
   const uint32_t total = line[p.num_reqs], ctas = fp4_ctas(total, gridDim.x, kRowWarps);
-  const bool mine = blockIdx.x < ctas;
-  const uint32_t from = mine ? fp4_begin<Seq>(p, line, total, blockIdx.x, ctas) : 0, to = mine ? fp4_begin<Seq>(p, line, total, blockIdx.x + 1, ctas) : 0;
-  if (threadIdx.x == 0) fp4_say_cut<Seq, D>(p, line, total, ctas, from, to, parts);
-  if (from >= to) return;
+  const uint2 stretch = fp4_stretch<Seq>(p, line, total, ctas);
+  const uint32_t from = stretch.x, to = stretch.y;
+  const auto say_cut = [&] {                     // (the last warp, whose pairs run out first)
+    if (threadIdx.x == kThreads - 1) fp4_say_cut<Seq, D>(p, line, total, ctas, from, to, parts);
+  };
+  if (from >= to) {
+    say_cut();
+    return;
+  }
 
   // ---- fetching ahead: the warp's pairs of cells in their order, one on its way while another is worked on. Two neighbouring lanes have the
   // addresses of one of the next 16 pairs.
   Fp4Piece<Seq> f;
   f.at(p, line, from, to);
+  __shared__ Fp4Piece<Seq> held[kRowWarps];      // each warp's piece, out of the registers of its loop over cells
+  Fp4Piece<Seq>& w = held[warp];
+  if (lane == 0) w = f;
+  __syncwarp();
   int fc = f.from() + warp, fj = 0, fn = 0;         // the next lot's first pair; next of this lot's, how many it has
   const uint8_t* src = nullptr;
   uint32_t have = 0;                            // cells of the lot that there are (behind the keys there is none, nor on a page outside the cache)
@@ -138,19 +147,12 @@ __global__ void __launch_bounds__(Fp4RowsShape<D, NT>::kWarps * 32, NT == 1 && D
   fetch(0);
   cells_at[0] = cells_at[1];
   fetch(1);
+  say_cut();
   int st = 0;
   uint32_t parity = 0;
   bool ok = true;
   const float cap_in = p.softcap2 > 0.f ? 2.8853900817779268f / p.softcap2 : 0.f;
 
-  __shared__ Fp4Piece<Seq> held[kRowWarps];      // each warp's piece, out of the registers of its loop over cells
-  Fp4Piece<Seq>& w = held[warp];
-  {
-    Fp4Piece<Seq> x;
-    x.at(p, line, from, to);
-    if (lane == 0) w = x;
-    __syncwarp();
-  }
   // queries: lane (g, t) has dims [t D / 4, + D / 4) of row g
   uint4 raw[NT][D / 32];
   const auto query = [&](const Fp4Piece<Seq>& x) {

@@ -101,10 +101,9 @@ __global__ void __launch_bounds__(512, 1) fp4_tiles_kernel(Fp4Attn p, float* par
   pdl_launch_dependents();
   fp4_line<Fp4Tile>(p, line);
   const uint32_t total = line[p.num_tiles], ctas = fp4_ctas(total, gridDim.x, kTileLeast);
-  const bool mine = blockIdx.x < ctas;
-  const uint32_t from = mine ? fp4_begin<Fp4Tile>(p, line, total, blockIdx.x, ctas) : 0;
-  const uint32_t to = mine ? fp4_begin<Fp4Tile>(p, line, total, blockIdx.x + 1, ctas) : 0;
-  if (threadIdx.x == 0) fp4_say_cut<Fp4Tile, D>(p, line, total, ctas, from, to, parts);
+  const uint2 stretch = fp4_stretch<Fp4Tile>(p, line, total, ctas);
+  const uint32_t from = stretch.x, to = stretch.y;
+  if (threadIdx.x == 32) fp4_say_cut<Fp4Tile, D>(p, line, total, ctas, from, to, parts);        // (of a warp without a part to play)
   Fp4Piece<Fp4Tile>& w = held[warp];
   Fp4TilePiece& x = held_tile[warp];
   const auto hold = [&](const Fp4Piece<Fp4Tile>& now) {

@@ -185,11 +185,18 @@ __device__ __forceinline__ int fp4_find(const uint32_t* line, int n, uint32_t u)
 __device__ __forceinline__ uint32_t fp4_ctas(uint32_t total, uint32_t grid, int least) { return max(1u, min(grid, total / least)); }
 template <class Entry>
 __device__ __forceinline__ uint32_t fp4_begin(const Fp4Attn& p, const uint32_t* line, uint32_t total, uint32_t i, uint32_t ctas) {
-  const uint32_t u = (uint32_t)((uint64_t)total * i / ctas);
+  const uint32_t each = total / ctas, u = each * i + (total - each * ctas) * i / ctas;      // total i / ctas, in 32 bits
   if (u == 0 || u >= total) return u;
   const int b = fp4_find(line, Entry::count(p), u);
   const uint32_t n = Entry(p, b).cells, off = (u - line[b]) % n;
   return n <= Entry::kSnap + Entry::kStart ? u - off + (2 * off >= n ? n : 0) : off <= Entry::kStart ? u - off : u;
+}
+
+// The CTA's stretch: its two ends by two lanes at once. By whole warps.
+template <class Entry>
+__device__ __forceinline__ uint2 fp4_stretch(const Fp4Attn& p, const uint32_t* line, uint32_t total, uint32_t ctas) {
+  const uint32_t at = blockIdx.x < ctas ? fp4_begin<Entry>(p, line, total, blockIdx.x + (threadIdx.x & 1), ctas) : 0;
+  return make_uint2(__shfl_sync(0xffffffffu, at, 0), __shfl_sync(0xffffffffu, at, 1));
 }
 
 // A piece of an item: cells [c0, c1) of the e.cells that it has, kStart among them.
