@@ -38,31 +38,30 @@ __device__ __forceinline__ void unpack_bf16x8(const uint4& v, float (&x)[8]) {
   }
 }
 
-// A lane has 8 dims (16 bytes) of a head, so a head is D / 8 lanes and a group of 16 dims two neighbours. A warp takes PASSES times
-// the heads that its lanes hold, all of one token, whose position, slot, cos and sin are fetched once behind the heads' loads.
-template <int D, int PASSES>
-__global__ void __launch_bounds__(128) fp4_append_kernel(B200Fp4Append p) {
+// A lane has 8 dims (16 bytes) of a head, so a head is D / 8 lanes and a group of 16 dims two neighbours. A warp takes `passes` times
+// the heads that its lanes hold, all of one token, whose position, slot, cos and sin are fetched once behind the first heads' loads.
+// Query heads have a loop of their own: two thirds of the work, and half as many instructions as keys and values take.
+template <int D, bool MANY>
+__global__ void __launch_bounds__(128, MANY ? 8 : 9) fp4_append_kernel(B200Fp4Append p, int parts, int passes) {
   using Cell = Fp4Cell<D>;
   constexpr int kLanes = D / 8, kHeads = 32 / kLanes;
   __shared__ float exchange[4][256];
   pdl_wait();
   pdl_launch_dependents();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, l = lane % kLanes, side = lane / kLanes;
-  const int nheads = p.Hq + 2 * p.Hkv, v0 = p.Hq + p.Hkv, parts = (nheads + kHeads * PASSES - 1) / (kHeads * PASSES);
+  const int nheads = p.Hq + 2 * p.Hkv, v0 = p.Hq + p.Hkv;
   const uint32_t gw = blockIdx.x * 4 + warp;                     // (T * parts < 2^31)
-  const int t = (int)(gw / (uint32_t)parts), h0 = (int)(gw - (uint32_t)t * parts) * (kHeads * PASSES);
+  const int t = (int)(gw / (uint32_t)parts), h0 = (int)(gw - (uint32_t)t * parts) * (kHeads * passes), h1 = min(nheads, h0 + kHeads * passes);
   if (t >= p.T) return;
-  const __nv_bfloat16* qrow = (const __nv_bfloat16*)p.q + (size_t)t * p.ldq;
-  const __nv_bfloat16* krow = (const __nv_bfloat16*)p.k + (size_t)t * p.ldk;
-  const __nv_bfloat16* vrow = (const __nv_bfloat16*)p.v + (size_t)t * p.ldv;
-  uint4 raw[PASSES];
-#pragma unroll
-  for (int i = 0; i < PASSES; ++i) {
-    const int h = h0 + i * kHeads + side;
-    if (h < nheads)
-      raw[i] = *reinterpret_cast<const uint4*>((h < p.Hq ? qrow + (size_t)h * p.q_head_stride : h < v0 ? krow + (h - p.Hq) * D
-                                                                                                  : vrow + (h - v0) * D) + l * 8);
-  }
+  const __nv_bfloat16* qrow = (const __nv_bfloat16*)p.q + (size_t)t * p.ldq + l * 8;
+  const __nv_bfloat16* krow = (const __nv_bfloat16*)p.k + (size_t)t * p.ldk + l * 8;
+  const __nv_bfloat16* vrow = (const __nv_bfloat16*)p.v + (size_t)t * p.ldv + l * 8;
+  const auto load = [&](int first) {                            // of the lane's head behind `first`
+    const int h = first + side;
+    return h >= h1 ? make_uint4(0, 0, 0, 0)
+                   : *reinterpret_cast<const uint4*>(h < p.Hq ? qrow + (size_t)h * p.q_head_stride : h < v0 ? krow + (h - p.Hq) * D : vrow + (h - v0) * D);
+  };
+  uint4 ahead[2] = {load(h0), MANY ? load(h0 + kHeads) : make_uint4(0, 0, 0, 0)};       // two passes on their way
   const int rot = p.cos_sin ? p.rot : 0, half = rot >> 1;
   float c[8], s[8];                                             // y = x c + partner s
 #pragma unroll
@@ -103,7 +102,7 @@ __global__ void __launch_bounds__(128) fp4_append_kernel(B200Fp4Append p) {
   }
   uint8_t* cell = nullptr;                                      // the token's cell of kv head 0
   int token = 0;
-  if (h0 + kHeads * PASSES > p.Hq) {
+  if (h1 > p.Hq) {
     const int64_t slot = ((const int64_t*)p.slots)[t];
     if (slot >= 0 && slot < p.num_blocks * p.block_size) {
       const int64_t blk = (slot >> 31) == 0 ? (int64_t)((uint32_t)slot / (uint32_t)p.block_size) : slot / p.block_size;
@@ -114,12 +113,11 @@ __global__ void __launch_bounds__(128) fp4_append_kernel(B200Fp4Append p) {
   }
   const size_t head_bytes = (size_t)(p.block_size / kCellTokens) * Cell::kBytes;
   const float g = p.gemma ? 1.f : 0.f;
-#pragma unroll
-  for (int i = 0; i < PASSES; ++i) {
-    const int h = h0 + i * kHeads + side;
-    if (h0 + i * kHeads >= nheads) break;                       // (the warp stays together: shuffles)
+  // norm and rotation of a pass's heads; the warp stays together (shuffles)
+  const auto turned = [&](int first, const uint4& raw, float (&y)[8]) {
+    const int h = first + side;
     float x[8];
-    unpack_bf16x8(raw[i], x);
+    unpack_bf16x8(raw, x);
     const bool is_q = h < p.Hq, is_v = h >= v0;
     if (p.q_norm || p.k_norm) {
       float ss = 0.f;
@@ -136,10 +134,9 @@ __global__ void __launch_bounds__(128) fp4_append_kernel(B200Fp4Append p) {
         for (int e = 0; e < 8; ++e) x[e] = x[e] * inv * (wf[e] + g);
       }
     }
-    float y[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) y[e] = x[e];
-    if (rot && h0 + i * kHeads < v0) {                          // (the same for the warp: a q or k head among its heads)
+    if (rot && first < v0) {                          // (the same for the warp: a q or k head among its heads)
       float other[8];
       if (!p.neox) {
 #pragma unroll
@@ -170,22 +167,46 @@ __global__ void __launch_bounds__(128) fp4_append_kernel(B200Fp4Append p) {
         for (int e = 0; e < 8; ++e) y[e] = l * 8 + e < rot ? x[e] * c[e] + other[e] * s[e] : x[e];
       }
     }
-    const auto query = [&] {
-      __nv_bfloat16* dst = p.q_out ? (__nv_bfloat16*)p.q_out + (size_t)t * p.ldo + h * D
-                                   : (__nv_bfloat16*)p.q + (size_t)t * p.ldq + (size_t)h * p.q_head_stride;
-      *reinterpret_cast<uint4*>(dst + l * 8) = make_uint4(pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3]), pack_bf16x2(y[4], y[5]),
-                                                          pack_bf16x2(y[6], y[7]));
-    };
-    if (h0 + (i + 1) * kHeads <= p.Hq) {                        // (the warp's heads are all query heads)
-      query();
-      continue;
+  };
+  const auto query = [&](int h, const float (&y)[8]) {
+    __nv_bfloat16* dst = p.q_out ? (__nv_bfloat16*)p.q_out + (size_t)t * p.ldo + h * D
+                                 : (__nv_bfloat16*)p.q + (size_t)t * p.ldq + (size_t)h * p.q_head_stride;
+    *reinterpret_cast<uint4*>(dst + l * 8) = make_uint4(pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3]), pack_bf16x2(y[4], y[5]),
+                                                        pack_bf16x2(y[6], y[7]));
+  };
+  const auto next = [&](int first) {
+    const uint4 raw = ahead[0];
+    if constexpr (MANY) {
+      ahead[0] = ahead[1];
+      ahead[1] = load(first + 2 * kHeads);
+    }
+    return raw;
+  };
+  int first = h0;
+  if constexpr (MANY) {
+#pragma unroll 1
+    for (; first + kHeads <= min(p.Hq, h1); first += kHeads) {  // passes of query heads only
+      float y[8];
+      turned(first, next(first), y);
+      query(first + side, y);
+    }
+  }
+#pragma unroll 1
+  for (; first < h1; first += kHeads) {
+    const int h = first + side;
+    float y[8];
+    turned(first, next(first), y);
+    if (!MANY && first + kHeads <= p.Hq) {
+      query(h, y);
+      return;
     }
     uint32_t top = 0;                                           // of |y|, as bits: a NaN is above infinity
 #pragma unroll
     for (int e = 0; e < 8; ++e) top = max(top, __float_as_uint(y[e]) & 0x7fffffffu);
     top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
-    if (h >= nheads) continue;
-    if (is_q) query();
+    if (h >= h1) continue;
+    const bool is_q = h < p.Hq, is_v = h >= v0;
+    if (is_q) query(h, y);
     if (is_q || !cell) continue;
     const uint8_t scale = fp4_scale_byte(__fdiv_rn(__uint_as_float(top), 6.f));
     const float sf = fp4_scale_value(scale);
@@ -256,13 +277,17 @@ template <int D>
 static int launch_append(const B200Fp4Append& p, cudaStream_t stream) {
   constexpr int kHeads = 32 / (D / 8);
   const int nheads = p.Hq + 2 * p.Hkv;
+  const int groups = (nheads + kHeads - 1) / kHeads;
   const auto go = [&](auto kernel, int passes) {
-    const long long warps = (long long)p.T * ((nheads + kHeads * passes - 1) / (kHeads * passes));
+    const int parts = (groups + passes - 1) / passes;
+    const long long warps = (long long)p.T * parts;
     if (warps >= (1ll << 31)) return -4;
-    return launch_pdl(kernel, dim3((unsigned)((warps + 3) / 4)), dim3(128), 0, stream, p) == cudaSuccess ? 0 : -2;
+    return launch_pdl(kernel, dim3((unsigned)((warps + 3) / 4)), dim3(128), 0, stream, p, parts, passes) == cudaSuccess ? 0 : -2;
   };
-  // many tokens: a warp takes four times the heads of a token, so that position, slot, cos and sin are fetched once for them
-  return (long long)p.T * nheads > 4096 * kHeads ? go(fp4_append_kernel<D, 4>, 4) : go(fp4_append_kernel<D, 1>, 1);
+  // Passes that leave some 8192 warps: more of them than one are worth their own kernel, which fetches two heads ahead and keeps to 64 registers
+  // (8192 tokens of 32 + 8 + 8 heads of 128 dims: 48.5 us, one pass a warp 81; 1024 tokens 9.3 and 10.8; 256 tokens are one pass, 4.7).
+  const long long each = ((long long)p.T * groups + 8191) / 8192;
+  return each > 1 ? go(fp4_append_kernel<D, true>, (int)min(each, (long long)groups)) : go(fp4_append_kernel<D, false>, 1);
 }
 
 }  // namespace b200
