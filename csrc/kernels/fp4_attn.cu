@@ -3,7 +3,7 @@
 //
 //   o[r] = sum_j p[r, j] v_j / sum_j p[r, j],   p[r, j] = 2^(scale log2(e) q_r . k_j - m),   m a running reference of the maximum
 //
-// The rows of a sequence that share a kv head (query tokens x heads of the group) are cut into tiles of 8 or 16. A warp takes cells of 16 keys:
+// The rows of a sequence that share a kv head (query tokens x heads of the group) are cut into tiles of 8 or 16. A warp takes pairs of cells, 32 keys:
 //   S^T [16 keys x rows] = K Q^T     A = keys, straight from the cell: codes to f16 (cvt.rn.f16x2.e2m1x2), times their scale, exact
 //   O^T [dims x rows]   += V^T P^T   A = values of four keys a lane; codes of two keys are merged before the conversion, so that a pair of
 //                                    f16 holds two keys of one dim and one multiplication applies both scales; B = P^T, transposed in
@@ -13,6 +13,12 @@
 // Work is shared out evenly whatever the lengths (fp4_work.cuh). The warps of a CTA take the cells of a piece in turn, fetched ahead by bulk copies
 // into a ring of their own. An item that lies in one stretch is finished there; of one that was cut the parts (m, l, O) go to scratch, and a second
 // kernel joins them.
+//
+// mma.sync and not tcgen05: with 8 rows a product of 32 keys is 64 K multiplications a warp, and what takes the time is the 8192 codes in front of
+// it, which would pass through shared or tensor memory once more. 256 sequences of 200 to 3800 keys, 32 heads over 8 of 128 dims: 136 us for 596 MB,
+// 4.4 TB/s. Bound by instructions: some 290 warp instructions a cell (64 conversions, 64 products by scales, 16 matrix products, 16 that merge the
+// codes of two keys), issued in 0.64 of the cycles; memory is at 0.52, the tensor pipe at 0.22. One sequence of 1000 keys takes 9 us: 5.8 us until
+// the first cell is there (line, table, cell: three loads one behind the other), two of work, and the join.
 #include <type_traits>
 
 #include "api.h"
@@ -565,14 +571,19 @@ extern "C" int b200_fp4_attn(const B200Fp4Attn* a, cudaStream_t stream) {
   p.scale_log2 = a->scale * 1.4426950408889634f;
   p.softcap2 = a->softcap * 1.4426950408889634f;
   p.status = device_status_word();
-  // Which sequences go to which kernel. Both are launched where the lengths, which only the device knows, may call for both.
+  // Which sequences go to which kernel. Both are launched where the lengths, which only the device knows, may call for both. 24 sequences of 32 heads
+  // over 8 of 128 dims, in the row kernel / the tile kernel: 32 rows (8 tokens) behind 4000 keys 94 / 135 us, behind none 28 / 32; 64 rows 167 / 136
+  // and 45 / 32; 48 rows lie between.
   static constexpr int kFew = 48;
   const bool tensor = a->D <= 128 && a->q_start && p.num_tiles > 0, long_one = tensor && (long long)a->total_q * G > kFew;
   bool rows = true, tiles = long_one;
   p.few = long_one ? kFew : 0x7fffffff;
   if (long_one && a->num_reqs == 1) { rows = false; p.few = -1; }
   float* parts = (float*)a->parts;
-  const bool two = a->D <= 128 && (long long)a->total_q * G > 8ll * a->num_reqs;      // row tiles of 16
+  // Row tiles of 16 where the sequences have more than 8 rows on average. 48 sequences of 2000 keys, 8 kv heads of 128 dims, in tiles of 8 / of 16: 8 rows
+  // 47 / 61 us, 16 rows 71 / 64, 24 rows 95 / 104, 32 rows 120 / 107. (A tile of 16 costs as much as two of 8 do, but for the products by scales and the
+  // fetches; one CTA an SM instead of two. At 256 dims its accumulators do not fit.)
+  const bool two = a->D <= 128 && (long long)a->total_q * G > 8ll * a->num_reqs;
   if (a->D == 64) return two ? launch_attn<64, 2>(p, rows, tiles, parts, stream) : launch_attn<64, 1>(p, rows, tiles, parts, stream);
   if (a->D == 128) return two ? launch_attn<128, 2>(p, rows, tiles, parts, stream) : launch_attn<128, 1>(p, rows, tiles, parts, stream);
   return launch_attn<256, 1>(p, rows, tiles, parts, stream);

@@ -5,8 +5,14 @@
 //          Sums, rotation and quotients are fp32, and keys are not rounded to bf16 on the way to their codes. Values past 6 * 10240
 //          (infinities too) saturate, a NaN makes its group NaN.
 // read:    code * s for the given slots, exact in bf16.
+//
+// Both are passes over memory. At 8192 tokens of 32 + 8 + 8 heads of 128 dims an append takes 48.5 us for 177 MB (3.65 TB/s), a read back 12.3 us for
+// 43 MB (3.5 TB/s): instructions bound them (an append issues in 0.64 of the cycles, half of it rotation and quotients), not the 27 and 7 us of the
+// bytes. A token or a few take 2.4 us, the latency of position -> angles and slot -> cell.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
+
+#include <type_traits>
 
 #include "api.h"
 #include "fp4_cache.cuh"
@@ -237,39 +243,54 @@ __global__ void __launch_bounds__(128, MANY ? 8 : 9) fp4_append_kernel(B200Fp4Ap
   }
 }
 
-// A lane turns 8 codes into 16 bytes of bf16. A block has one token, or as many as its threads have room for.
-template <int D>
+// A lane turns 8 codes into 16 bytes of bf16, of N lots of `tokens` tokens (one, or as many as a block's threads have room for): the same place
+// in each, whose loads are all on their way at once.
+template <int D, int N>
 __global__ void __launch_bounds__(256) fp4_read_kernel(B200Fp4Read p, int tokens) {
   using Cell = Fp4Cell<D>;
   pdl_wait();
   pdl_launch_dependents();
   const int per = 2 * p.Hkv * (D / 8);                          // lanes of a token
-  const int local = tokens > 1 ? threadIdx.x / per : 0, first = threadIdx.x - local * per;
-  const long long t = (long long)blockIdx.x * tokens + local;
-  if (local >= tokens || t >= p.n) return;
-  const int64_t slot = ((const int64_t*)p.slots)[t];
-  const bool there = slot >= 0 && slot < p.num_blocks * p.block_size;
-  const int64_t blk = !there ? 0 : (slot >> 31) == 0 ? (int64_t)((uint32_t)slot / (uint32_t)p.block_size) : slot / p.block_size;
-  const int off = there ? (int)(slot - blk * p.block_size) : 0, token = off % kCellTokens, cells = p.block_size / kCellTokens;
-  const uint8_t* cell0 = (const uint8_t*)p.cache + (blk * p.Hkv * cells + off / kCellTokens) * Cell::kBytes;
+  const int local = tokens > 1 ? threadIdx.x / per : 0, first = threadIdx.x - local * per, cells = p.block_size / kCellTokens;
+  const long long t0 = (long long)blockIdx.x * tokens * N + local;
+  if (local >= tokens) return;
+  const uint8_t* cell0[N];                                      // the token's cell of kv head 0; null: none
+  int token[N];
+#pragma unroll
+  for (int j = 0; j < N; ++j) {
+    const long long t = t0 + j * tokens;
+    const int64_t slot = t < p.n ? ((const int64_t*)p.slots)[t] : -1;
+    const int64_t blk = (slot >> 31) == 0 ? (int64_t)((uint32_t)slot / (uint32_t)p.block_size) : slot / p.block_size;
+    const int off = (int)(slot - blk * p.block_size);
+    token[j] = off % kCellTokens;
+    cell0[j] = slot >= 0 && slot < p.num_blocks * p.block_size
+                   ? (const uint8_t*)p.cache + (blk * p.Hkv * cells + off / kCellTokens) * Cell::kBytes : nullptr;
+  }
   for (int i = first; i < per; i += 256) {
     const int l = i % (D / 8), h2 = i / (D / 8), kv = h2 >= p.Hkv, h = h2 - kv * p.Hkv;
-    uint32_t o[4] = {0, 0, 0, 0};
-    if (there) {
-      const uint8_t* cell = cell0 + (size_t)h * cells * Cell::kBytes;
-      const uint32_t codes = *reinterpret_cast<const uint32_t*>(cell + (kv ? Cell::value_at(token, l * 4) : token * Cell::kRow + l * 4));
-      const float s = fp4_scale_value(cell[kv ? Cell::kValueScales + (l >> 1) * kCellTokens + token
-                                              : Cell::kKeyScales + token * Cell::kScales + (l >> 1)]);
-      uint32_t f16[4];
-      cvt_e2m1x8(codes, f16);
+    uint32_t codes[N];
+    uint8_t scale[N];
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      const uint8_t* cell = cell0[j] + (size_t)h * cells * Cell::kBytes;
+      codes[j] = cell0[j] ? *reinterpret_cast<const uint32_t*>(cell + (kv ? Cell::value_at(token[j], l * 4) : token[j] * Cell::kRow + l * 4)) : 0;
+      scale[j] = cell0[j] ? cell[kv ? Cell::kValueScales + (l >> 1) * kCellTokens + token[j]
+                                    : Cell::kKeyScales + token[j] * Cell::kScales + (l >> 1)] : 0;
+    }
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      const float s = fp4_scale_value(scale[j]);
+      uint32_t f16[4], o[4];
+      cvt_e2m1x8(codes[j], f16);
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const float2 f = __half22float2(*reinterpret_cast<__half2*>(&f16[e]));
         o[e] = pack_bf16x2(f.x * s, f.y * s);
       }
+      const long long t = t0 + j * tokens;
+      if (t < p.n)
+        *reinterpret_cast<uint4*>((__nv_bfloat16*)(kv ? p.v : p.k) + (t * p.Hkv + h) * D + l * 8) = make_uint4(o[0], o[1], o[2], o[3]);
     }
-    __nv_bfloat16* dst = (__nv_bfloat16*)(kv ? p.v : p.k) + (t * p.Hkv + h) * D + l * 8;
-    *reinterpret_cast<uint4*>(dst) = make_uint4(o[0], o[1], o[2], o[3]);
   }
 }
 
@@ -315,10 +336,16 @@ extern "C" int b200_fp4_read(const B200Fp4Read* a, cudaStream_t stream) {
       !a->cache || !a->k || !a->v)
     return -1;
   const int per = 2 * a->Hkv * (a->D / 8), tokens = per < 256 ? 256 / per : 1;
-  const long long blocks = (a->n + tokens - 1) / tokens;
-  if (blocks >= (1ll << 31)) return -4;
-  const auto go = [&](auto kernel) {
+  const auto go = [&](auto kernel, long long lot) {
+    const long long blocks = (a->n + lot - 1) / lot;
+    if (blocks >= (1ll << 31)) return -4;
     return launch_pdl(kernel, dim3((unsigned)blocks), dim3(256), 0, stream, *a, tokens) == cudaSuccess ? 0 : -2;
   };
-  return a->D == 64 ? go(fp4_read_kernel<64>) : a->D == 128 ? go(fp4_read_kernel<128>) : go(fp4_read_kernel<256>);
+  // two lots a block where that leaves blocks enough for every SM (8192 tokens of 8 heads of 128 dims: 12.3 us, one lot 14.8, four 12.5)
+  const bool many = a->n >= 2ll * tokens * 8 * b200_num_sms();
+  const auto by = [&](auto d) {
+    constexpr int kD = decltype(d)::value;
+    return many ? go(fp4_read_kernel<kD, 2>, 2ll * tokens) : go(fp4_read_kernel<kD, 1>, tokens);
+  };
+  return a->D == 64 ? by(std::integral_constant<int, 64>()) : a->D == 128 ? by(std::integral_constant<int, 128>()) : by(std::integral_constant<int, 256>());
 }

@@ -14,6 +14,11 @@
 // Tensor memory (512 columns): S0 | S1 | O0 | O1; P(t) is the first 64 columns of S(t).
 // Warps (512 threads): 0 issues MMAs and holds tensor memory; 4..7 and 8..11 softmax and output of half 0 and 1, a thread a row; 12..15 expand, a
 // thread a key. Registers move from the first and the last warpgroup to the two of the softmax.
+//
+// 1999 tokens behind 30000, 32 heads over 8 of 128 dims: 915 us, 1.11 PFLOP/s; a causal prompt of 8192 577 us, 0.95 PFLOP/s (0.66 and 0.57 of
+// what a large product reaches). What bounds it: exponentials, 16 a cycle, take as long as the products of a tile, and neither hides all of the other; the
+// masks of the diagonal, the queries and the outputs of a causal prompt's short items come on top. A piece costs some 3500 cycles for queries and output, what
+// short prompts pay: 13 of 3 to 211 tokens take 35 us.
 #include "api.h"
 #include "fp4_work.cuh"
 

@@ -575,3 +575,30 @@ def test_two_threads_at_once():
     for i, (_, _, (q, cache, table, lens, new)) in enumerate(work):
         for out in got[i]:
             _check(out, q, cache, table, lens, new, Hq, D, bs, 0.1, 0.0, 0)
+
+
+APPEND_MANY = [
+    # several passes a warp; heads that do not fill the last one, and passes with query and key heads
+    (2050, 7, 3, 64, 20, True, True, False, 16),
+    (5000, 7, 3, 64, 64, True, False, False, 32),
+    (1400, 5, 3, 128, 96, False, True, True, 48),
+    (700, 12, 2, 256, 256, True, True, False, 64),
+    (9000, 0, 1, 128, 128, True, False, False, 16),
+]
+
+
+@pytest.mark.parametrize("T,Hq,Hkv,D,rot,neox,normed,gemma,bs", APPEND_MANY)
+def test_append_of_many_tokens(T, Hq, Hkv, D, rot, neox, normed, gemma, bs):
+    for in_place in (False, True):
+        test_append(T, Hq, Hkv, D, rot, neox, normed, gemma, bs, in_place)
+
+
+@pytest.mark.parametrize("n,H,D", [(20001, 1, 64), (9000, 3, 128), (6001, 5, 256)])
+def test_read_of_many_tokens(n, H, D):
+    """Slots in any order, some twice, some outside."""
+    bs, nb, gen = 16, 40, _gen(n)
+    cache = F.random_cache(nb, H, bs, D, gen)
+    slots = torch.randint(-3, nb * bs + 3, (n,), generator=gen)
+    k, v = C.read(cache.to(DEV), slots.to(DEV))
+    rk, rv = C.ref_read(cache, slots)
+    assert torch.equal(k.cpu(), rk) and torch.equal(v.cpu(), rv)

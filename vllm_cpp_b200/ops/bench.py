@@ -232,6 +232,32 @@ def small_case(name: str):
         qabs = torch.randn(B, H, 576, device=dev, dtype=torch.bfloat16)
         out = torch.empty(B, H, 512, device=dev, dtype=torch.bfloat16)
         fn = lambda: MLA.mla_decode(qabs, cache, bt, sl, out, 576 ** -0.5, mbs)
+    elif name in ("fp4_decode_small", "fp4_prefill_small", "fp4_append_small"):
+        # the KV cache held in 4 bits, 32 query heads over 8 of 128 dims, 32-token pages
+        from . import fp4_cache as F4
+        H, Hk, Dh, page = 32, 8, 128, 32
+        B, ctx, new = (96, 4096, 1) if name == "fp4_decode_small" else (1, 4096, 4096)
+        nb = ctx // page
+        cache = F4.alloc(B * nb, Hk, page, Dh, dev)
+        x = torch.randn(ctx, (H + 2 * Hk) * Dh, device=dev, dtype=torch.bfloat16)
+        q_out = torch.empty(ctx, H * Dh, device=dev, dtype=torch.bfloat16)
+        slots = (torch.randperm(B * nb, device=dev)[:, None] * page + torch.arange(page, device=dev)).view(B, ctx)
+        table = ref.rope_table(ref.rope_inv_freq(Dh, 1e4), ctx).to(dev)
+        positions = torch.arange(ctx, device=dev)
+        append = lambda b=0: F4.append(x, positions, table, cache, slots[b], num_q_heads=H, q_out=q_out)
+        for b in range(B):
+            append(b)
+        bt = (slots[:, ::page] // page).int().contiguous()
+        sl = torch.full((B,), ctx, dtype=torch.int32, device=dev)
+        q = torch.randn(B * new, H * Dh, device=dev, dtype=torch.bfloat16)
+        if name == "fp4_append_small":
+            fn = append
+        elif new == 1:
+            fn = lambda: F4.decode(q, cache, block_table=bt, seq_lens=sl, scale=Dh ** -0.5)
+        else:
+            req, q0 = (torch.tensor(t, dtype=torch.int32, device=dev) for t in ref.build_prefill_tiles([new]))
+            qs = torch.tensor([0, new], dtype=torch.int32, device=dev)
+            fn = lambda: F4.prefill(q, cache, block_table=bt, seq_lens=sl, q_start=qs, tile_req=req, tile_q0=q0, scale=Dh ** -0.5)
     else:
         raise SystemExit(f"unknown case {name}")
     ms = _time(fn, iters=3, warmup=1)
@@ -248,7 +274,8 @@ def main():
                          "prefill_small | decode_small | gdn_scan_small | "
                          "gdn_decode_small | moe_small | moe_few_small | moe_many_small | gemm_streamk_small | gemm_shared_small | gemm_gated_small | "
                          "gemm_fp8_small | gemm_w4a16_small | gemm_nvfp4_small | gemm_nvfp4_prefill_small | "
-                         "decode_d256_small | mla_decode_small | bias_prefill_small | bias_decode_small | delta_small")
+                         "decode_d256_small | mla_decode_small | bias_prefill_small | bias_decode_small | delta_small | "
+                         "fp4_append_small | fp4_decode_small | fp4_prefill_small")
     args = ap.parse_args()
     if args.case:
         return small_case(args.case)

@@ -138,7 +138,7 @@ def append(qkv: torch.Tensor, positions: Optional[torch.Tensor], cos_sin: Option
     a.q, a.k, a.v = at + 2 * offsets[0], at + 2 * offsets[1], at + 2 * offsets[2]
     if T > 1:                      # (the stride of a single row says nothing)
         a.ldq = a.ldk = a.ldv = ld
-    if q_out is not None:
+    if q_out is not None and num_q_heads:
         a.q_out, a.ldo = q_out.data_ptr(), q_out.stride(0) if T > 1 else 0
     if cos_sin is not None:
         a.positions, a.cos_sin, a.table_rows, a.rot = positions.data_ptr(), cos_sin.data_ptr(), cos_sin.shape[0], rot

@@ -175,7 +175,7 @@ RULES.update({
             w is None or (w.dtype == BF16 and w.is_contiguous() and w.numel() == cache.shape[3] // 18 and w.data_ptr() % 16 == 0)
             for w in (q_norm, k_norm))),
         ("q_out is [T, Hq * head_dim] bf16 with rows on 16-byte boundaries", lambda qkv, cache, num_q_heads, q_out, **_: q_out is None or (
-            _bf16_rows(q_out) and _apart(q_out) and q_out.shape[0] >= qkv.shape[0] and q_out.shape[1] == num_q_heads * (cache.shape[3] // 18))),
+            q_out.dtype == BF16 and q_out.dim() == 2 and (q_out.numel() == 0 or _bf16_rows(q_out) and _apart(q_out)) and q_out.shape[0] >= qkv.shape[0] and q_out.shape[1] == num_q_heads * (cache.shape[3] // 18))),
         ("all tensors are on one GPU", lambda qkv, cache, slots, positions, cos_sin, q_norm, k_norm, q_out, **_:
          _on_gpu(qkv, cache, slots, positions, cos_sin, q_norm, k_norm, q_out)),
     ],
