@@ -17,7 +17,7 @@
 // mma.sync and not tcgen05: with 8 rows a product of 32 keys is 64 K multiplications a warp, and what takes the time is the 8192 codes in front of
 // it, which would pass through shared or tensor memory once more. 256 sequences of 200 to 3800 keys, 32 heads over 8 of 128 dims: 136 us for 596 MB,
 // 4.4 TB/s. Bound by instructions: some 290 warp instructions a cell (64 conversions, 64 products by scales, 16 matrix products, 16 that merge the
-// codes of two keys), issued in 0.64 of the cycles; memory is at 0.52, the tensor pipe at 0.22. One sequence of 1000 keys takes 9 us: 5.8 us until
+// codes of two keys), issued in 0.64 of the cycles; memory is at 0.52, the tensor pipe at 0.22. One sequence of 1000 keys takes 9 us: 3.8 us until
 // the first cell is there (line, table, cell: three loads one behind the other), two of work, and the join.
 #include <type_traits>
 

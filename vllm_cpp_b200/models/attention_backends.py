@@ -47,6 +47,8 @@ REGISTRY: list[AttentionBackend] = [
     AttentionBackend("any-size-bias-prefill", "prefill", "bias", 1, "b200_bias_attn_prefill", lambda **_: True),
     AttentionBackend("mma-fp4-decode", "decode", "fp4", 0, "b200_fp4_attn",
                      lambda head_dim, block_size, **_: head_dim in (64, 128, 256) and block_size % 16 == 0),
+    AttentionBackend("tcgen05-fp4-prefill", "prefill", "fp4", 0, "b200_fp4_attn",
+                     lambda head_dim, block_size, **_: head_dim in (64, 128) and block_size % 16 == 0),
     AttentionBackend("mma-fp4-prefill", "prefill", "fp4", 1, "b200_fp4_attn",
                      lambda head_dim, block_size, **_: head_dim in (64, 128, 256) and block_size % 16 == 0),
     AttentionBackend("mla-absorbed-decode", "decode", "mla", 0, "b200_mla_decode",
