@@ -602,3 +602,15 @@ def test_read_of_many_tokens(n, H, D):
     k, v = C.read(cache.to(DEV), slots.to(DEV))
     rk, rv = C.ref_read(cache, slots)
     assert torch.equal(k.cpu(), rk) and torch.equal(v.cpu(), rv)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+def test_as_many_tiles_as_a_call_takes(D):
+    """8000 tiles: those of two prompts, over and over."""
+    lens, new, Hq, Hkv, bs = [200, 150], [200, 150], 2, 1, 16
+    q, cache, table, n = _case(lens, new, Hq, Hkv, D, bs, 0, seed=D)
+    req, q0 = _tiles(new)
+    out = C.prefill(q.to(DEV), cache.to(DEV), block_table=table.to(DEV), seq_lens=n.to(DEV), q_start=torch.tensor([0, 200, 350], dtype=torch.int32, device=DEV),
+                    tile_req=req.repeat(2000), tile_q0=q0.repeat(2000), scale=0.1)
+    _check(out, q, cache, table, lens, new, Hq, D, bs, 0.1, 0.0, 0)
+    assert _status() == 0

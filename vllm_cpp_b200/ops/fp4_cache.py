@@ -210,7 +210,7 @@ _MOST = 2 ** 31
 
 def _attend(op, q, cache, block_table, seq_lens, q_start, tile_req, tile_q0, scale, out, softcap, window, causal, tmp):
     # What the rules of ops.validate say, in a fraction of their time (a decode step calls this in every layer); they name what is
-    # wrong, and judge what is rare.
+    # wrong, and decide what is rare.
     given = out is not None
     try:
         (rows, cols), (nb, H, cells, width), (reqs, pages), (n,) = q.shape, cache.shape, block_table.shape, seq_lens.shape
