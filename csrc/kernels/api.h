@@ -266,6 +266,7 @@ typedef struct B200Fp4Attn {
   int max_blocks, num_reqs, total_q, num_tiles;
   int Hq, Hkv, D, block_size;
   int window, causal;
+  int most_q;                  // query rows of the longest sequence, 0: not known; only chooses between kernels
   float scale, softcap;
 } B200Fp4Attn;
 

@@ -575,7 +575,7 @@ extern "C" int b200_fp4_attn(const B200Fp4Attn* a, cudaStream_t stream) {
   // over 8 of 128 dims, in the row kernel / the tile kernel: 32 rows (8 tokens) behind 4000 keys 94 / 135 us, behind none 28 / 32; 64 rows 167 / 136
   // and 45 / 32; 48 rows lie between.
   static constexpr int kFew = 48;
-  const bool tensor = a->D <= 128 && a->q_start && p.num_tiles > 0, long_one = tensor && (long long)a->total_q * G > kFew;
+  const bool tensor = a->D <= 128 && a->q_start && p.num_tiles > 0, long_one = tensor && (long long)(a->most_q > 0 ? min(a->most_q, a->total_q) : a->total_q) * G > kFew;
   bool rows = true, tiles = long_one;
   p.few = long_one ? kFew : 0x7fffffff;
   if (long_one && a->num_reqs == 1) { rows = false; p.few = -1; }

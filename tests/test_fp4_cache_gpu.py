@@ -614,3 +614,15 @@ def test_as_many_tiles_as_a_call_takes(D):
                     tile_req=req.repeat(2000), tile_q0=q0.repeat(2000), scale=0.1)
     _check(out, q, cache, table, lens, new, Hq, D, bs, 0.1, 0.0, 0)
     assert _status() == 0
+
+
+@pytest.mark.parametrize("said", [3, 12, 13, 200, 10 ** 6])
+def test_the_longest_sequence_only_chooses_between_kernels(said):
+    """Whatever is said of it, also what is not so."""
+    lens, new, Hq, Hkv, D, bs = [900, 300, 12, 77], [12, 13, 2, 40], 16, 4, 128, 32
+    q, cache, table, n = _case(lens, new, Hq, Hkv, D, bs, 0, seed=77)
+    req, q0 = _tiles(new)
+    out = C.prefill(q.to(DEV), cache.to(DEV), block_table=table.to(DEV), seq_lens=n.to(DEV), q_start=torch.tensor([0] + new).cumsum(0).int().to(DEV),
+                    tile_req=req, tile_q0=q0, scale=0.1, max_query_len=said)
+    _check(out, q, cache, table, lens, new, Hq, D, bs, 0.1, 0.0, 0)
+    assert _status() == 0

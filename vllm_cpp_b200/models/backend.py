@@ -654,7 +654,7 @@ class GpuBackend(FusedLinearMixin):
                 P = ctx.num_prefills
                 fp4_cache.prefill(q[nd:], kv_cache, block_table=bt[nd: nd + P], seq_lens=ctx.seq_lens[nd: nd + P],
                                   q_start=ctx.prefill_q_start[: P + 1], tile_req=ctx.tile_req[:ctx.num_tiles],
-                                  tile_q0=ctx.tile_q0[:ctx.num_tiles], out=out[nd:], **common)
+                                  tile_q0=ctx.tile_q0[:ctx.num_tiles], out=out[nd:], max_query_len=ctx.max_query_len, **common)
             return out
         if nd > 0:
             self.ops.attn_decode(q[:nd], kv_cache, block_table=bt[:nd], seq_lens=ctx.seq_lens[:nd],

@@ -41,7 +41,7 @@ class AttnArgs(ctypes.Structure):
     _fields_ = [("q", _P), ("out", _P), ("ldq", _L), ("ldo", _L), ("ldt", _L), ("cache", _P), ("num_blocks", _L),
                 ("block_table", _P), ("seq_lens", _P), ("q_start", _P), ("tile_req", _P), ("tile_q0", _P), ("parts", _P),
                 ("max_blocks", _I), ("num_reqs", _I), ("total_q", _I), ("num_tiles", _I), ("Hq", _I), ("Hkv", _I), ("D", _I),
-                ("block_size", _I), ("window", _I), ("causal", _I), ("scale", _F), ("softcap", _F)]
+                ("block_size", _I), ("window", _I), ("causal", _I), ("most_q", _I), ("scale", _F), ("softcap", _F)]
 
 
 class ReadArgs(ctypes.Structure):
@@ -208,7 +208,7 @@ _I32 = torch.int32
 _MOST = 2 ** 31
 
 
-def _attend(op, q, cache, block_table, seq_lens, q_start, tile_req, tile_q0, scale, out, softcap, window, causal, tmp):
+def _attend(op, q, cache, block_table, seq_lens, q_start, tile_req, tile_q0, scale, out, softcap, window, causal, tmp, most_q=0):
     # What the rules of ops.validate say, in a fraction of their time (a decode step calls this in every layer); they name what is
     # wrong, and decide what is rare.
     given = out is not None
@@ -258,6 +258,7 @@ def _attend(op, q, cache, block_table, seq_lens, q_start, tile_req, tile_q0, sca
     if op == "fp4_prefill":
         a.q_start, a.num_reqs = q_start.data_ptr(), min(q_start.numel() - 1, reqs, n)
         a.tile_req, a.tile_q0, a.num_tiles = tile_req.data_ptr(), tile_q0.data_ptr(), tile_req.numel()
+        a.most_q = max(0, min(most_q, rows))
     a.window, a.causal, a.scale, a.softcap = window, causal, scale, softcap
     _launch(q, _attn, a, op)
     return out
@@ -274,11 +275,12 @@ def decode(q: torch.Tensor, cache: torch.Tensor, *, block_table: torch.Tensor, s
 
 def prefill(q: torch.Tensor, cache: torch.Tensor, *, block_table: torch.Tensor, seq_lens: torch.Tensor, q_start: torch.Tensor,
             tile_req: torch.Tensor, tile_q0: torch.Tensor, scale: float, out: Optional[torch.Tensor] = None, softcap: float = 0.0,
-            window: int = 0, causal: bool = True, tmp: Optional[torch.Tensor] = None) -> torch.Tensor:
+            window: int = 0, causal: bool = True, tmp: Optional[torch.Tensor] = None, max_query_len: int = 0) -> torch.Tensor:
     """Attention of the query rows ``q_start[r]..q_start[r + 1]`` of each sequence, the last of its ``seq_lens[r]`` positions.
     ``tile_req`` / ``tile_q0`` list their 128-row tiles, as in :func:`vllm_cpp_b200.ops.attn_prefill`. Rows outside every
-    sequence stay as they are. At most 8192 sequences and 8000 tiles."""
-    return _attend("fp4_prefill", q, cache, block_table, seq_lens, q_start, tile_req, tile_q0, scale, out, softcap, window, causal, tmp)
+    sequence stay as they are. ``max_query_len``, the rows of the longest sequence, only chooses between kernels (0: not known, which costs
+    a step of few rows a sequence one launch more). At most 8192 sequences and 8000 tiles."""
+    return _attend("fp4_prefill", q, cache, block_table, seq_lens, q_start, tile_req, tile_q0, scale, out, softcap, window, causal, tmp, max_query_len)
 
 
 # ------------------------------------------------------------------------------ restatements
