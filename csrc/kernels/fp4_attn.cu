@@ -131,7 +131,7 @@ __global__ void __launch_bounds__(Fp4RowsShape<D, NT>::kWarps * 32, NT == 1 && D
         fc = f.from() + warp;
       }
       if (!f.more()) return;
-      const int pair = fc + (lane >> 1) * kRowWarps, c = 2 * (f.e.begin + pair) + (lane & 1), pg = p.by_page_cells.of(c), h = fp4_head(f.item, f.e.tiles);
+      const int pair = fc + (lane >> 1) * kRowWarps, c = 2 * (f.e.begin + pair) + (lane & 1), pg = p.by_page_cells.of(c), h = fp4_head(p, f.item, f.e.tiles);
       const int id = pair < f.to() && c * kCellTokens < f.e.len ? p.block_table[f.b * p.ldt + pg] : -1;
       src = id >= 0 && id < p.num_blocks
                 ? p.cache + (((long long)id * p.Hkv + h) * p.cells_per_page + (c - pg * p.cells_per_page)) * Cell::kBytes : nullptr;
@@ -162,7 +162,7 @@ __global__ void __launch_bounds__(Fp4RowsShape<D, NT>::kWarps * 32, NT == 1 && D
   // queries: lane (g, t) has dims [t D / 4, + D / 4) of row g
   uint4 raw[NT][D / 32];
   const auto query = [&](const Fp4Piece<Seq>& x) {
-    const int h = x.more() ? fp4_head(x.item, x.e.tiles) : 0, r0 = x.more() ? (x.item - h * x.e.tiles) * kRows : 0;
+    const int h = x.more() ? fp4_head(p, x.item, x.e.tiles) : 0, r0 = x.more() ? (x.item - h * x.e.tiles) * kRows : 0;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       const int r = r0 + nt * 8 + g, token = p.by_group.of(r), head = h * p.G + r - token * p.G;
@@ -176,7 +176,7 @@ __global__ void __launch_bounds__(Fp4RowsShape<D, NT>::kWarps * 32, NT == 1 && D
   bool first_piece = true;
   while (w.more()) {
     const Seq& s = w.e;
-    const int h = fp4_head(w.item, s.tiles), r0 = (w.item - h * s.tiles) * kRows, nrows = min(kRows, s.rows - r0), first = s.first;
+    const int h = fp4_head(p, w.item, s.tiles), r0 = (w.item - h * s.tiles) * kRows, nrows = min(kRows, s.rows - r0), first = s.first;
     // ---- the tile's queries: B operand
     uint32_t bq[NT][D / 16][2];
     float mul[NT][2];                                                            // of the lane's rows 2t, 2t + 1: scores to log2 units
@@ -551,6 +551,9 @@ extern "C" int b200_fp4_attn(const B200Fp4Attn* a, cudaStream_t stream) {
   const int G = a->Hq / a->Hkv;
   // cells of the whole line in 31 bits, whatever the lengths
   if (((double)a->max_blocks * (a->block_size / kCellTokens) + Fp4Seq<16>::kStart) * a->Hkv * ((double)a->total_q * G / 8 + a->num_reqs) > 2147483647.0)
+    return -4;
+  if (a->q_start && ((double)a->max_blocks * a->block_size / kTileKeys + Fp4Tile::kStart + 1) * a->Hkv * a->num_tiles *
+                            ((a->total_q < kTileTokens ? a->total_q : kTileTokens) * G / Fp4Tile::kRows + 1) > 2147483647.0)
     return -4;
   if ((double)a->max_blocks * a->block_size > 2147479552.0) return -4;          // (positions and a tile behind them in 31 bits)
   if ((double)a->total_q * G * G >= 4294967296.0 || (double)a->max_blocks * (a->block_size / kCellTokens) * (a->block_size / kCellTokens) >= 4294967296.0)

@@ -54,7 +54,7 @@ struct Fp4TilePiece {
   __device__ __forceinline__ Fp4TilePiece() {}
   __device__ __forceinline__ Fp4TilePiece(const Fp4Attn& p, const Fp4Piece<Fp4Tile>& w) {
     const Fp4Tile& e = w.e;
-    h = fp4_head(w.item, e.tiles);
+    h = fp4_head(p, w.item, e.tiles);
     r0 = (w.item - h * e.tiles) * Fp4Tile::kRows;
     rows = min(Fp4Tile::kRows, e.rows - r0);
     halves = rows > 128 ? 2 : 1;

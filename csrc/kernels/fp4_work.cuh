@@ -42,8 +42,11 @@ struct Fp4Attn {
   float scale_log2, softcap2;
   int* status;
 };
-// h = item / tiles; one division, and none for a single tile
-__device__ __forceinline__ int fp4_head(int item, int tiles) { return tiles == 1 ? item : item / tiles; }
+// h = item / tiles; one division, and none for a single tile. Never past the heads, whatever the sequences' bounds are (overlapping ones could make
+// the line longer than 32 bits count): rows then lie behind the last, and are neither read nor written.
+__device__ __forceinline__ int fp4_head(const Fp4Attn& p, int item, int tiles) {
+  return (int)min((uint32_t)(tiles == 1 ? item : item / tiles), (uint32_t)p.Hkv - 1u);
+}
 
 __device__ __forceinline__ float ex2_of(float x) {
   float y;
@@ -264,10 +267,10 @@ __device__ __forceinline__ void fp4_say_cut(const Fp4Attn& p, const uint32_t* li
     w.at(p, line, to - 1, to);                                  // the stretch's last cell
     const uint32_t begin = line[w.b] + (uint32_t)w.item * w.e.cells;
     if (w.c1 < w.e.cells && begin >= from) {                    // its item goes on, and begins here
-      const int h = fp4_head(w.item, w.e.tiles);
+      const int h = fp4_head(p, w.item, w.e.tiles);
       c.row0 = (w.item - h * w.e.tiles) * Entry::kRows;
       c.rows = min(Entry::kRows, w.e.rows - c.row0);
-      c.last = (int)(((uint64_t)(begin + w.e.cells) * ctas - 1) / total);       // the CTA that has the item's last cell
+      c.last = (int)min(((uint64_t)(begin + w.e.cells) * ctas - 1) / total, (uint64_t)ctas - 1);       // the CTA that has the item's last cell
       c.token0 = w.e.token0;
       c.head0 = h * p.G;
     }

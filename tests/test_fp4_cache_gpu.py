@@ -626,3 +626,31 @@ def test_the_longest_sequence_only_chooses_between_kernels(said):
                     tile_req=req, tile_q0=q0, scale=0.1, max_query_len=said)
     _check(out, q, cache, table, lens, new, Hq, D, bs, 0.1, 0.0, 0)
     assert _status() == 0
+
+
+def test_refusals_of_lines_past_31_bits():
+    """What the lengths allow at most, whatever they are: the kernels count cells in 31 bits."""
+    from vllm_cpp_b200.ops._lib import KernelError
+    cache = C.alloc(1, 1, 2048, 64, DEV)
+    q = torch.zeros((128, 4 * 64), dtype=torch.bfloat16, device=DEV)
+    lens, start = torch.full((1,), 128, dtype=torch.int32, device=DEV), torch.tensor([0, 128], dtype=torch.int32, device=DEV)
+    ids = torch.zeros(8000, dtype=torch.int32, device=DEV)
+    for pages, tiles, ok in ((1 << 14, 8000, False), (1 << 14, 1, True), (1 << 20, 1, False)):
+        args = dict(block_table=torch.zeros((1, pages), dtype=torch.int32, device=DEV), seq_lens=lens, q_start=start, tile_req=ids[:tiles],
+                    tile_q0=ids[:tiles], scale=0.1)
+        if ok:
+            assert not C.prefill(q, cache, **args).any()
+        else:
+            with pytest.raises(KernelError, match="-4"):
+                C.prefill(q, cache, **args)
+
+
+def test_sequences_that_share_query_rows():
+    """Bounds that go back: the second sequence has no rows, the third those of the first, over keys of its own or the same."""
+    lens, Hq, Hkv, D, bs = [100, 5, 100], 8, 2, 128, 16
+    q, cache, table, n = _case(lens, [70, 0, 0], Hq, Hkv, D, bs, 0, seed=6)
+    table[2] = table[0]
+    req, q0 = _tiles([70, 0, 70])
+    out = C.prefill(q.to(DEV), cache.to(DEV), block_table=table.to(DEV), seq_lens=n.to(DEV), q_start=torch.tensor([0, 70, 0, 70], dtype=torch.int32, device=DEV),
+                    tile_req=req, tile_q0=q0, scale=0.1)
+    _check(out, q, cache, table, [100], [70], Hq, D, bs, 0.1, 0.0, 0)
