@@ -98,8 +98,7 @@ __global__ void __launch_bounds__(Fp4RowsShape<D, NT>::kWarps * 32, NT == 1 && D
   mbar_fence_init();
   pdl_wait();
   pdl_launch_dependents();
-  fp4_line<Seq>(p, line);
-  const uint32_t total = line[p.num_reqs], ctas = fp4_ctas(total, gridDim.x, kRowWarps);
+  const uint32_t total = fp4_line<Seq>(p, line), ctas = fp4_ctas(total, gridDim.x, kRowWarps);
   const uint2 stretch = fp4_stretch<Seq>(p, line, total, ctas);
   const uint32_t from = stretch.x, to = stretch.y;
   const auto say_cut = [&] {                     // (the last warp, whose pairs run out first)
@@ -131,7 +130,7 @@ __global__ void __launch_bounds__(Fp4RowsShape<D, NT>::kWarps * 32, NT == 1 && D
         fc = f.from() + warp;
       }
       if (!f.more()) return;
-      const int pair = fc + (lane >> 1) * kRowWarps, c = 2 * (f.e.begin + pair) + (lane & 1), pg = p.by_page_cells.of(c), h = fp4_head(p, f.item, f.e.tiles);
+      const int pair = fc + (lane >> 1) * kRowWarps, c = 2 * (f.e.begin + pair) + (lane & 1), pg = p.by_page_cells.of(c), h = fp4_head(f.item, f.e.tiles);
       const int id = pair < f.to() && c * kCellTokens < f.e.len ? p.block_table[f.b * p.ldt + pg] : -1;
       src = id >= 0 && id < p.num_blocks
                 ? p.cache + (((long long)id * p.Hkv + h) * p.cells_per_page + (c - pg * p.cells_per_page)) * Cell::kBytes : nullptr;
@@ -162,7 +161,7 @@ __global__ void __launch_bounds__(Fp4RowsShape<D, NT>::kWarps * 32, NT == 1 && D
   // queries: lane (g, t) has dims [t D / 4, + D / 4) of row g
   uint4 raw[NT][D / 32];
   const auto query = [&](const Fp4Piece<Seq>& x) {
-    const int h = x.more() ? fp4_head(p, x.item, x.e.tiles) : 0, r0 = x.more() ? (x.item - h * x.e.tiles) * kRows : 0;
+    const int h = x.more() ? fp4_head(x.item, x.e.tiles) : 0, r0 = x.more() ? (x.item - h * x.e.tiles) * kRows : 0;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       const int r = r0 + nt * 8 + g, token = p.by_group.of(r), head = h * p.G + r - token * p.G;
@@ -176,7 +175,7 @@ __global__ void __launch_bounds__(Fp4RowsShape<D, NT>::kWarps * 32, NT == 1 && D
   bool first_piece = true;
   while (w.more()) {
     const Seq& s = w.e;
-    const int h = fp4_head(p, w.item, s.tiles), r0 = (w.item - h * s.tiles) * kRows, nrows = min(kRows, s.rows - r0), first = s.first;
+    const int h = fp4_head(w.item, s.tiles), r0 = (w.item - h * s.tiles) * kRows, nrows = min(kRows, s.rows - r0), first = s.first;
     // ---- the tile's queries: B operand
     uint32_t bq[NT][D / 16][2];
     float mul[NT][2];                                                            // of the lane's rows 2t, 2t + 1: scores to log2 units

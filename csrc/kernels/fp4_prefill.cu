@@ -54,7 +54,7 @@ struct Fp4TilePiece {
   __device__ __forceinline__ Fp4TilePiece() {}
   __device__ __forceinline__ Fp4TilePiece(const Fp4Attn& p, const Fp4Piece<Fp4Tile>& w) {
     const Fp4Tile& e = w.e;
-    h = fp4_head(p, w.item, e.tiles);
+    h = fp4_head(w.item, e.tiles);
     r0 = (w.item - h * e.tiles) * Fp4Tile::kRows;
     rows = min(Fp4Tile::kRows, e.rows - r0);
     halves = rows > 128 ? 2 : 1;
@@ -104,8 +104,7 @@ __global__ void __launch_bounds__(512, 1) fp4_tiles_kernel(Fp4Attn p, float* par
   const uint32_t tmem = bars.tmem_base;
   pdl_wait();
   pdl_launch_dependents();
-  fp4_line<Fp4Tile>(p, line);
-  const uint32_t total = line[p.num_tiles], ctas = fp4_ctas(total, gridDim.x, kTileLeast);
+  const uint32_t total = fp4_line<Fp4Tile>(p, line), ctas = fp4_ctas(total, gridDim.x, kTileLeast);
   const uint2 stretch = fp4_stretch<Fp4Tile>(p, line, total, ctas);
   const uint32_t from = stretch.x, to = stretch.y;
   if (threadIdx.x == 32) fp4_say_cut<Fp4Tile, D>(p, line, total, ctas, from, to, parts);        // (of a warp without a part to play)

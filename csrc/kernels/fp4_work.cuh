@@ -42,11 +42,8 @@ struct Fp4Attn {
   float scale_log2, softcap2;
   int* status;
 };
-// h = item / tiles; one division, and none for a single tile. Never past the heads, whatever the sequences' bounds are (overlapping ones could make
-// the line longer than 32 bits count): rows then lie behind the last, and are neither read nor written.
-__device__ __forceinline__ int fp4_head(const Fp4Attn& p, int item, int tiles) {
-  return (int)min((uint32_t)(tiles == 1 ? item : item / tiles), (uint32_t)p.Hkv - 1u);
-}
+// h = item / tiles; one division, and none for a single tile
+__device__ __forceinline__ int fp4_head(int item, int tiles) { return tiles == 1 ? item : item / tiles; }
 
 __device__ __forceinline__ float ex2_of(float x) {
   float y;
@@ -146,35 +143,47 @@ struct Fp4Tile {               // tiles of 128 keys, row tiles of 256
   }
 };
 
-// line[i] = cells in the line in front of entry i (count + 1 values). All threads of the block take part.
+// line[i] = cells in the line in front of entry i (count + 1 values); gives the line's length. All threads of the block take part. Sequences whose bounds
+// overlap could make it longer than 31 bits count: then it is empty, and the call does nothing.
 template <class Entry>
-__device__ void fp4_line(const Fp4Attn& p, uint32_t* line) {
+__device__ uint32_t fp4_line(const Fp4Attn& p, uint32_t* line) {
   __shared__ uint32_t warp_sum[32];
   const int n = Entry::count(p), per = (n + blockDim.x - 1) / blockDim.x, b0 = min((int)threadIdx.x * per, n), b1 = min(b0 + per, n);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
   uint32_t sum = 0;
+  bool past = false;                                           // a sum has passed 32 bits
   for (int b = b0; b < b1; ++b) {
     const Entry e(p, b);
     const uint32_t c = (uint32_t)e.cells * (uint32_t)(e.tiles * p.Hkv);
     line[b + 1] = c;
     sum += c;
+    past |= sum < c;
   }
   uint32_t x = sum;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
     const uint32_t y = __shfl_up_sync(0xffffffffu, x, o);
-    if (lane >= o) x += y;
+    if (lane >= o) {
+      x += y;
+      past |= x < y;
+    }
   }
   if (lane == 31) warp_sum[warp] = x;
   __syncthreads();
   uint32_t before = x - sum;
-  for (int w = 0; w < warps; ++w) before += w < warp ? warp_sum[w] : 0;
+  for (int w = 0; w < warps; ++w) {
+    const uint32_t y = w < warp ? warp_sum[w] : 0;
+    before += y;
+    past |= before < y;
+  }
   for (int b = b0; b < b1; ++b) {
-    before += line[b + 1];
+    const uint32_t y = line[b + 1];
+    before += y;
+    past |= before < y || before >> 31;
     line[b + 1] = before;
   }
   if (threadIdx.x == 0) line[0] = 0;
-  __syncthreads();
+  return __syncthreads_or(past) ? 0 : line[n];
 }
 __device__ __forceinline__ int fp4_find(const uint32_t* line, int n, uint32_t u) {   // the entry that cell u is of
   int lo = 0, hi = n - 1;
@@ -267,7 +276,7 @@ __device__ __forceinline__ void fp4_say_cut(const Fp4Attn& p, const uint32_t* li
     w.at(p, line, to - 1, to);                                  // the stretch's last cell
     const uint32_t begin = line[w.b] + (uint32_t)w.item * w.e.cells;
     if (w.c1 < w.e.cells && begin >= from) {                    // its item goes on, and begins here
-      const int h = fp4_head(p, w.item, w.e.tiles);
+      const int h = fp4_head(w.item, w.e.tiles);
       c.row0 = (w.item - h * w.e.tiles) * Entry::kRows;
       c.rows = min(Entry::kRows, w.e.rows - c.row0);
       c.last = (int)min(((uint64_t)(begin + w.e.cells) * ctas - 1) / total, (uint64_t)ctas - 1);       // the CTA that has the item's last cell

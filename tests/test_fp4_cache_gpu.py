@@ -654,3 +654,17 @@ def test_sequences_that_share_query_rows():
     out = C.prefill(q.to(DEV), cache.to(DEV), block_table=table.to(DEV), seq_lens=n.to(DEV), q_start=torch.tensor([0, 70, 0, 70], dtype=torch.int32, device=DEV),
                     tile_req=req, tile_q0=q0, scale=0.1)
     _check(out, q, cache, table, [100], [70], Hq, D, bs, 0.1, 0.0, 0)
+
+
+def test_bounds_that_overlap_until_the_line_is_too_long():
+    """4096 sequences that each claim all query rows: more cells than 31 bits count. The call does nothing."""
+    R, H, D, bs, keys = 8192, 16, 256, 2048, 32768
+    cache = C.alloc(1, H, bs, D, DEV)
+    q = torch.ones((16, 16 * H * D), dtype=torch.bfloat16, device=DEV)
+    start = (torch.arange(R + 1, dtype=torch.int32, device=DEV) % 2) * 16
+    ids = torch.zeros(1, dtype=torch.int32, device=DEV)
+    out = torch.full_like(q, 7.0)
+    C.prefill(q, cache, block_table=torch.zeros((R, keys // bs), dtype=torch.int32, device=DEV), q_start=start, tile_req=ids, tile_q0=ids,
+              seq_lens=torch.full((R,), keys, dtype=torch.int32, device=DEV), scale=0.1, out=out)
+    assert bool((out == 7.0).all())
+    assert _status() == 0
