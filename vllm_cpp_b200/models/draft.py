@@ -63,11 +63,14 @@ class DraftModel:
         extra.pop("inputs_embeds", None)
         return extra
 
-    def fill(self, ctx) -> None:
-        """The draft model over the target's step: writes its KV cache; one logits row, unused."""
+    def fill(self, ctx, decode_splits: int = 1, decode_tmp=None) -> None:
+        """The draft model over the target's step: writes its KV cache; one logits row, unused. ``decode_splits`` and
+        ``decode_tmp``: how this model's decode attention is split, and its scratch (the target's are of other shapes)."""
         self.rows[:1].zero_()
-        ctx2 = dataclasses.replace(ctx, logits_indices=self.rows[:1], num_logits=1,
-                                   decode_only_full_logits=False, extra=self._own_extra(ctx))
+        extra = self._own_extra(ctx)
+        extra["decode_tmp"] = decode_tmp
+        ctx2 = dataclasses.replace(ctx, logits_indices=self.rows[:1], num_logits=1, decode_splits=decode_splits,
+                                   decode_only_full_logits=False, extra=extra)
         self.model.forward(ctx2)
 
     def decode(self, ctx) -> torch.Tensor:

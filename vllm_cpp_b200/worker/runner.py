@@ -144,9 +144,7 @@ class ModelRunner(E.ModelRunnerBase):
             from ..ops import _lib
             self._status_dev = _lib.status_word(self.device)
             self._status_host = torch.zeros(1, dtype=torch.int32, pin_memory=True)
-            Hq, Hkv, D = model.hq, model.hkv, model.D
-            self._decode_tmp: dict[int, tuple] = {}
-            self._Hq, self._Hkv, self._D = Hq, Hkv, D
+            self._decode_tmp: dict[tuple, tuple] = {}
 
     # ------------------------------------------------------------------ helpers
     def _make_views(self, buf: torch.Tensor) -> dict:
@@ -206,20 +204,21 @@ class ModelRunner(E.ModelRunnerBase):
             return False        # draft verification reads the sampled ids on the host every step
         return self.is_cuda
 
-    def _decode_splits(self, batch: int) -> tuple[int, tuple | None]:
+    def _decode_splits(self, batch: int, model=None) -> tuple[int, tuple | None]:
+        """(splits, scratch) of a decode batch of ``model`` (None: the target): a draft model's heads, and the type
+        its cache is held in, are its own."""
         if not self.is_cuda:
             return 1, None
-        key = batch
-        if key not in self._decode_tmp and hasattr(self.model, "decode_workspace"):
-            self._decode_tmp[key] = self.model.decode_workspace(batch, self.max_model_len, self.block_size)
+        m = self.model if model is None else model
+        key = (batch, m is not self.model)
+        if key not in self._decode_tmp and hasattr(m, "decode_workspace"):
+            self._decode_tmp[key] = m.decode_workspace(batch, self.max_model_len, self.block_size)
         if key not in self._decode_tmp:
-            s = self.ops.attn_decode_splits(batch, self._Hkv, self._Hq // self._Hkv, self._D,
-                                            self.max_model_len, self.block_size)
+            s = self.ops.attn_decode_splits(batch, m.hkv, m.hq // m.hkv, m.D, self.max_model_len, self.block_size)
             tmp = None
             if s > 1:
-                tmp = (torch.empty((batch, self._Hq, s, self._D), dtype=torch.float32,
-                                   device=self.device),
-                       torch.empty((batch, self._Hq, s), dtype=torch.float32, device=self.device))
+                tmp = (torch.empty((batch, m.hq, s, m.D), dtype=torch.float32, device=self.device),
+                       torch.empty((batch, m.hq, s), dtype=torch.float32, device=self.device))
             self._decode_tmp[key] = (s, tmp)
         return self._decode_tmp[key]
 
@@ -766,7 +765,7 @@ class ModelRunner(E.ModelRunnerBase):
         m.d_pos[:n].copy_(pos)
         m.d_slots[:n].copy_(blk * bs + pos % bs)
         m.d_seq[:n].copy_((pos + 1).to(torch.int32))
-        splits, tmp = self._decode_splits(n) if self.is_cuda else (1, None)
+        splits, tmp = self._decode_splits(n, m.model if m is self.drafter else None)
         ctx = StepContext(
             num_tokens=n, num_reqs=n, num_decodes=n, num_prefills=0, num_prefill_tokens=0, num_tiles=0,
             num_logits=n, input_ids=m.next_ids, positions=m.d_pos, slot_mapping=[m.d_slots],
@@ -792,7 +791,8 @@ class ModelRunner(E.ModelRunnerBase):
         decode-only passes from the token each request just got. ``toks`` as in _propose_mtp."""
         d, hv = self.drafter, self.host_views
         R = info.num_reqs
-        d.fill(self._last_ctx)
+        nd = self._last_ctx.num_decodes
+        d.fill(self._last_ctx, *(self._decode_splits(nd, d.model) if nd > 0 else (1, None)))
         qs = hv["query_start"][: R + 1].tolist()
         reqs, rids, first, pos_last = [], [], [], []
         for r in range(R):
