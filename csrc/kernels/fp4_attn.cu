@@ -80,7 +80,8 @@ struct Fp4RowsShape {
   static constexpr int kFixed = kRingBytes + kMergeBytes + kWarps * kRows * 8 + kWarps * kRowStages * 8;
 };
 
-template <int D, int NT>
+// SEVERAL: a sequence may have several query tokens, so that rows of a tile differ in what they see.
+template <int D, int NT, bool SEVERAL>
 __global__ void __launch_bounds__(Fp4RowsShape<D, NT>::kWarps * 32, NT == 1 && D <= 128 ? 2 : 1) fp4_rows_kernel(Fp4Attn p, float* parts) {
   using Cell = Fp4Cell<D>;
   using Shape = Fp4RowsShape<D, NT>;
@@ -229,7 +230,7 @@ __global__ void __launch_bounds__(Fp4RowsShape<D, NT>::kWarps * 32, NT == 1 && D
       off[nt][0] = off[nt][1] = INFINITY;
       l[nt][0] = l[nt][1] = 0.f;
     }
-    const int c1 = w.to(), begin = s.begin, len = s.len;
+    const int c1 = w.to(), begin = s.begin, end = SEVERAL && p.causal ? first + tok1 + 1 : s.len;     // end: behind the last key that any row sees
     const int inner0 = (max(most_lo, 0) + kPairKeys - 1) / kPairKeys, inner1 = (least_hi + 1) / kPairKeys;   // pairs that every row sees all of
     for (int c = w.from() + warp; c < c1 && ok; c += kRowWarps) {
       if (!__all_sync(0xffffffffu, mbar_try_wait(&full[st], parity)) && !fp4_wait(&full[st], parity, p.status)) {
@@ -287,12 +288,12 @@ __global__ void __launch_bounds__(Fp4RowsShape<D, NT>::kWarps * 32, NT == 1 && D
         const bool edge = two != 3u || pair < inner0 || pair >= inner1;
         const int key0[2] = {two & 1 ? key : kNoKey, two & 2 ? key + kCellTokens : kNoKey};
         uint32_t keep[2] = {0xffffffffu, 0xffffffffu};     // of the scales of the lane's four values
-        if (edge) {                  // what lies behind the sequence or before every window may be anything: NaN times 0 too
+        if (edge) {                  // what no row sees may be anything: NaN times 0 too
 #pragma unroll
           for (int u = 0; u < 2; ++u)
 #pragma unroll
             for (int j = 0; j < 4; ++j)
-              if (key0[u] + 4 * t + j >= len || key0[u] + 4 * t + j < least_lo) keep[u] &= ~(0xffu << (8 * j));
+              if (key0[u] + 4 * t + j >= end || key0[u] + 4 * t + j < least_lo) keep[u] &= ~(0xffu << (8 * j));
         }
         uint32_t bp[2][NT][2];
 #pragma unroll
@@ -358,6 +359,57 @@ __global__ void __launch_bounds__(Fp4RowsShape<D, NT>::kWarps * 32, NT == 1 && D
             }
             bp[u][nt][0] = transposed(pack_f16x2(x[u][0], x[u][1]));
             bp[u][nt][1] = transposed(pack_f16x2(x[u][2], x[u][3]));
+          }
+        }
+        // Where rows differ in what they see, a NaN among the values is not left to the product: 0 times it would reach the rows that do not see it.
+        // A product of its own says which rows do, their outputs become NaN, and its scale in the ring zero. (48 sequences of 2 to 6 drafts: 77 us
+        // without, 79 with it. A call of decode has no such rows, and a kernel without this: 256 sequences 143 us, 147 with it.)
+        if (SEVERAL && edge && tok0 != tok1) {
+          constexpr int kWords = D > 128 ? D / 128 : 1;      // groups of a lane's dims
+          const auto word_at = [&](int u, int w) {
+            return reinterpret_cast<uint32_t*>(ring + (2 * st + u) * Cell::kBytes + Cell::kValueScales + (g * (D / 8) / 16 + w) * kCellTokens + 4 * t);
+          };
+          uint32_t odd = 0;
+#pragma unroll
+          for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int w = 0; w < kWords; ++w) odd |= nan_scales(*word_at(u, w) & keep[u]);
+          if (__any_sync(0xffffffffu, odd != 0)) {
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+              uint32_t sees[NT][2];
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt) {
+                float f[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                  const int at = key0[u] + k0 + (e & 2);
+                  f[e] = at <= hi[nt][e & 1] && at >= lo[nt][e & 1] ? 1.f : 0.f;
+                }
+                sees[nt][0] = transposed(pack_f16x2(f[0], f[1]));
+                sees[nt][1] = transposed(pack_f16x2(f[2], f[3]));
+              }
+#pragma unroll
+              for (int w = 0; w < kWords; ++w) {
+                const uint32_t scales = *word_at(u, w), bad = nan_scales(scales & keep[u]) >> 7;          // 1 a byte
+                const uint32_t n01 = __byte_perm(bad, 0, 0x4140) * 0x3c00u, n23 = __byte_perm(bad, 0, 0x4342) * 0x3c00u;
+                const uint32_t a[4] = {n01, n01, n23, n23};
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
+                  float n[4];
+                  mma_f16_first(n, a, sees[nt][0], sees[nt][1]);
+#pragma unroll
+                  for (int i = w * (kMT / kWords); i < (w + 1) * (kMT / kWords); ++i)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                      if (n[e & 1] > 0.f) o[nt][i][e] = __int_as_float(0x7fffffff);
+                }
+                __syncwarp();
+                *word_at(u, w) = scales & ~(bad * 255u);
+              }
+            }
+            fence_proxy_async_smem();                        // (the next copies into the ring follow)
+            __syncwarp();
           }
         }
         // O^T: lane (g, t) has keys 4t..4t+3 and dims [g D / 8, + D / 8); the m-tile i is its dims 2i (row g) and 2i + 1 (row g + 8)
@@ -500,22 +552,26 @@ __global__ void __launch_bounds__(kJoinThreads) fp4_join_kernel(Fp4Attn p, float
 
 static constexpr int kMostReqs = 8192, kMostTiles = 8000;         // (the line of a step is in shared memory)
 
+template <int D, int NT, bool SEVERAL>
+static int launch_rows(const Fp4Attn& p, int grid, float* parts, cudaStream_t stream) {
+  using Shape = Fp4RowsShape<D, NT>;
+  static Fp4Once once;
+  if (!once.run([] {
+        return cudaFuncSetAttribute(fp4_rows_kernel<D, NT, SEVERAL>, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape::kFixed + (kMostReqs + 1) * 4) == cudaSuccess;
+      }))
+    return -2;
+  return launch_pdl(fp4_rows_kernel<D, NT, SEVERAL>, dim3(grid), dim3(Shape::kWarps * 32), Shape::kFixed + (size_t)(p.num_reqs + 1) * 4, stream, p, parts) ==
+                 cudaSuccess ? 0 : -2;
+}
+
 template <int D, int NT>
 static int launch_attn(const Fp4Attn& p, bool rows, bool tiles, float* parts, cudaStream_t stream) {
   using Shape = Fp4RowsShape<D, NT>;
   using Seq = Fp4Seq<Shape::kRows>;
   const int row_grid = rows ? b200_num_sms() * (NT == 1 && D <= 128 ? 2 : 1) : 0, tile_grid = tiles ? fp4_tile_grid() : 0;
   float* tile_parts = parts + fp4_scratch<Seq, D>(row_grid);
-  if (rows) {
-    static Fp4Once once;
-    if (!once.run([] {
-          return cudaFuncSetAttribute(fp4_rows_kernel<D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape::kFixed + (kMostReqs + 1) * 4) == cudaSuccess;
-        }))
-      return -2;
-    if (launch_pdl(fp4_rows_kernel<D, NT>, dim3(row_grid), dim3(Shape::kWarps * 32), Shape::kFixed + (size_t)(p.num_reqs + 1) * 4, stream, p, parts) !=
-        cudaSuccess)
-      return -2;
-  }
+  if (rows)
+    if (const int rc = p.q_start ? launch_rows<D, NT, true>(p, row_grid, parts, stream) : launch_rows<D, NT, false>(p, row_grid, parts, stream)) return rc;
   if (tiles)
     if (const int rc = launch_fp4_tiles(p, D, tile_parts, stream)) return rc;
   return launch_pdl(fp4_join_kernel<D, Shape::kRows>, dim3(row_grid * kRowShares + tile_grid * (kTileShares / kTurns)), dim3(kJoinThreads), 0, stream, p, parts, row_grid,

@@ -73,7 +73,10 @@ __global__ void __launch_bounds__(512, 1) fp4_tiles_kernel(Fp4Attn p, float* par
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   __shared__ Fp4TileBars bars;
-  __shared__ uint32_t no_page[4][4];                            // key tiles in turn: keys of a warp of expanders that have no page
+  __shared__ uint32_t no_page[4][4];                            // key tiles in turn: keys of a warp of expanders that have no page,
+  __shared__ uint32_t odd_keys[4][4];                           // those, and the ones with a NaN among their values;
+  __shared__ uint8_t nan_groups[4][kTileKeys];                  // of such a key: the groups (16 dims) that are NaN
+  __shared__ uint8_t row_nan[Fp4Tile::kRows];                   // the groups of which a row has seen a NaN
   __shared__ Fp4Piece<Fp4Tile> held[16];                        // each warp's piece, out of the registers of its loop over tiles,
   __shared__ Fp4TilePiece held_tile[16];                        // and what it comes to
   uint8_t* sQ = smem;
@@ -222,22 +225,24 @@ __global__ void __launch_bounds__(512, 1) fp4_tiles_kernel(Fp4Attn p, float* par
         return page >= 0 && page < p.num_blocks ? p.cache + ((long long)page * p.Hkv + h) * head_bytes + (long long)cell * Cell::kBytes : nullptr;
       };
       uint4 code[D / 32];
-      uint32_t scale[D / 64];
+      uint32_t scale[D / 64], value_scale[D / 64];              // (those of a key's values come with the key)
       const auto load = [&](const uint8_t* cell, int kv) {
 #pragma unroll
         for (int i = 0; i < D / 32; ++i) code[i] = make_uint4(0, 0, 0, 0);
 #pragma unroll
-        for (int i = 0; i < D / 64; ++i) scale[i] = 0;
+        for (int i = 0; i < D / 64; ++i) {
+          scale[i] = kv ? value_scale[i] : 0;
+          if (!kv) value_scale[i] = 0;
+        }
         if (!cell) return;
 #pragma unroll
         for (int i = 0; i < D / 32; ++i)
           code[i] = *reinterpret_cast<const uint4*>(cell + (kv ? Cell::value_at(token, i * 16) : token * Cell::kRow + i * 16));
-        if (kv) {
-#pragma unroll
-          for (int i = 0; i < D / 16; ++i) scale[i / 4] |= (uint32_t)cell[Cell::kValueScales + i * kCellTokens + token] << (i % 4 * 8);
-        } else {
+        if (!kv) {
 #pragma unroll
           for (int i = 0; i < D / 64; ++i) scale[i] = reinterpret_cast<const uint32_t*>(cell + Cell::kKeyScales + token * Cell::kScales)[i];
+#pragma unroll
+          for (int i = 0; i < D / 16; ++i) value_scale[i / 4] |= (uint32_t)cell[Cell::kValueScales + i * kCellTokens + token] << (i % 4 * 8);
         }
       };
       int page = page_of(0);
@@ -252,7 +257,12 @@ __global__ void __launch_bounds__(512, 1) fp4_tiles_kernel(Fp4Attn p, float* par
 #pragma unroll
         for (int k = 0; k < D / 32; ++k) c[k] = code[k];
 #pragma unroll
-        for (int k = 0; k < D / 64; ++k) s[k] = scale[k];
+        for (int k = 0; k < D / 64; ++k) {
+          s[k] = scale[k];
+          // A NaN among values does not go to the product, where 0 times it would reach the rows that do not see its key: their softmax marks the rows
+          // that do.
+          if (kv) s[k] &= ~((nan_scales(s[k]) >> 7) * 255u);
+        }
         // the next item's loads, and in front of a key tile's the page
         if (kv == 0) {
           load(cell, 1);
@@ -262,11 +272,6 @@ __global__ void __launch_bounds__(512, 1) fp4_tiles_kernel(Fp4Attn p, float* par
           load(cell, 0);
         }
         if (!(ok = __all_sync(0xffffffffu, mbar_wait(&bars.kv_empty[slot], ((sq / kFRing) & 1) ^ 1, p.status)))) break;
-        if (kv == 0) {
-          const uint32_t mask = __ballot_sync(0xffffffffu, none);
-          if (lane == 0) no_page[tiles % 4][warp & 3] = mask;
-          ++tiles;
-        }
         uint8_t* row = ring + slot * Shape::kSlot + r * 128;
 #pragma unroll
         for (int k = 0; k < D / 32; ++k) {
@@ -280,6 +285,18 @@ __global__ void __launch_bounds__(512, 1) fp4_tiles_kernel(Fp4Attn p, float* par
             *reinterpret_cast<uint4*>(row + (piece / 8) * Shape::kPlane + (((piece % 8) ^ (r & 7)) << 4)) =
                 make_uint4(mul_f16x2(v[0], sc), mul_f16x2(v[1], sc), mul_f16x2(v[2], sc), mul_f16x2(v[3], sc));
           }
+        }
+        if (kv == 0) {                                           // (`scale` has the values' by now)
+          uint32_t nan = 0;
+#pragma unroll
+          for (int k = 0; k < D / 64; ++k) nan |= ((nan_scales(scale[k]) >> 7) * 0x10204080u >> 28) << (4 * k);
+          const uint32_t mask = __ballot_sync(0xffffffffu, none), odd = mask | __ballot_sync(0xffffffffu, nan != 0);
+          if (lane == 0) {
+            no_page[tiles % 4][warp & 3] = mask;
+            odd_keys[tiles % 4][warp & 3] = odd;
+          }
+          if (odd) nan_groups[tiles % 4][r] = nan;
+          ++tiles;
         }
         fence_proxy_async_smem();
         __syncwarp();
@@ -349,6 +366,7 @@ __global__ void __launch_bounds__(512, 1) fp4_tiles_kernel(Fp4Attn p, float* par
         hi = min(p.causal ? pos : w.e.len - 1, w.e.len - 1);
         lo = fp4_lowest(p, pos);
       }
+      *const_cast<volatile uint8_t*>(row_nan + t * 128 + r) = 0;
       if (n > 0) {
         // ---- the rows' queries (every product of the piece before is done: its last scores have been read), turned to a lane a row on the way
         const int mine = here(lane), turn = here(turn_row);
@@ -407,12 +425,22 @@ __global__ void __launch_bounds__(512, 1) fp4_tiles_kernel(Fp4Attn p, float* par
           for (int i = 0; i < kTileKeys; ++i)
             if (kbase + i > hi || kbase + i < lo) s[i] = 0xff800000u;       // -inf
         }
-        const volatile uint32_t* gone = no_page[tiles % 4];
-        const uint32_t g0 = gone[0], g1 = gone[1], g2 = gone[2], g3 = gone[3];
-        if (g0 | g1 | g2 | g3) {
+        const volatile uint32_t* odd = odd_keys[tiles % 4];
+        if (odd[0] | odd[1] | odd[2] | odd[3]) {
+          const volatile uint32_t* gone = no_page[tiles % 4];
+          const uint32_t g0 = gone[0], g1 = gone[1], g2 = gone[2], g3 = gone[3];
 #pragma unroll
           for (int i = 0; i < kTileKeys; ++i)
             if ((i < 32 ? g0 : i < 64 ? g1 : i < 96 ? g2 : g3) >> (i & 31) & 1) s[i] = 0xff800000u;
+          uint32_t seen = 0;                                     // groups that are NaN, of the keys that the row sees (0 for those without a page)
+#pragma unroll 1
+          for (int k = 0; k < 4; ++k)
+            for (uint32_t left = odd[k]; left; left &= left - 1) {
+              const int i = k * 32 + __ffs(left) - 1;
+              if (kbase + i <= hi && kbase + i >= lo) seen |= nan_groups[tiles % 4][i];
+            }
+          volatile uint8_t* mine = row_nan + t * 128 + r;
+          *mine = *mine | seen;
         }
         float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
@@ -485,6 +513,14 @@ __global__ void __launch_bounds__(512, 1) fp4_tiles_kernel(Fp4Attn p, float* par
         ++pieces;
         tc_fence_after_sync();
       }
+      const uint32_t nan = *const_cast<const volatile uint8_t*>(row_nan + t * 128 + r);
+      const auto mark = [&](uint32_t (&o)[32], int c) {          // of 32 dims
+        if (__any_sync(0xffffffffu, nan != 0)) {
+#pragma unroll
+          for (int i = 0; i < 32; ++i)
+            if (nan >> (2 * c + i / 16) & 1) o[i] = 0x7fffffffu;
+        }
+      };
       if (whole) {
         const float inv = l == 0.f ? 0.f : 1.f / l;
         const int mine = here(lane), turn = here(turn_row);
@@ -498,6 +534,7 @@ __global__ void __launch_bounds__(512, 1) fp4_tiles_kernel(Fp4Attn p, float* par
 #pragma unroll
             for (int i = 0; i < 32; ++i) o[i] = 0;
           }
+          mark(o, c);
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             uint32_t v[4];
@@ -527,6 +564,7 @@ __global__ void __launch_bounds__(512, 1) fp4_tiles_kernel(Fp4Attn p, float* par
 #pragma unroll
             for (int i = 0; i < 32; ++i) o[i] = 0;
           }
+          mark(o, c);
           if (lane < left) {
 #pragma unroll
             for (int i = 0; i < 32; i += 4)

@@ -68,6 +68,8 @@ __device__ __forceinline__ void e2m1x8_f16(uint32_t w, uint32_t (&h)[4]) {
 }
 // Scale bytes lo and hi (selectors of __byte_perm) of w -> f16x2.
 __device__ __forceinline__ uint32_t scales_f16x2(uint32_t w, int lo, int hi) { return __byte_perm(w, 0, 0x4040 | lo | hi << 8) << 7; }
+// Of four scale bytes the ones that are NaN (or infinite): 0x80 each.
+__device__ __forceinline__ uint32_t nan_scales(uint32_t w) { return ((w & 0x78787878u) + 0x08080808u) & w & 0x80808080u; }
 __device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
   const __half2 h = __floats2half2_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&h);
@@ -85,9 +87,10 @@ __device__ __forceinline__ float fp4_capped(float x, float to_y2, float cap2) { 
 }
 
 // lowest position that the query at `pos` sees
-__device__ __forceinline__ int fp4_lowest(const Fp4Attn& p, int pos) {
-  return p.window > 0 ? pos - p.window + 1 : p.window < 0 && pos >= 0 ? pos / -p.window * -p.window : 0;
+__device__ __forceinline__ int fp4_lowest(int window, int pos) {
+  return window > 0 ? pos - window + 1 : window < 0 && pos >= 0 ? pos / -window * -window : 0;
 }
+__device__ __forceinline__ int fp4_lowest(const Fp4Attn& p, int pos) { return fp4_lowest(p.window, pos); }
 // Rows of query tokens [q_begin, + q_len) of a sequence with len keys.
 struct Fp4Span {
   int len, q_begin, q_len;
