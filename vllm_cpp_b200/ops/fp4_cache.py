@@ -98,7 +98,7 @@ def append(qkv: torch.Tensor, positions: Optional[torch.Tensor], cos_sin: Option
            q_out: Optional[torch.Tensor] = None, q_head_stride: Optional[int] = None,
            offsets: Optional[tuple[int, int, int]] = None) -> None:
     """Per-head RMSNorm of q and k (weights bf16 ``[D]``, optional) and rotation of merged ``[T, q | k | v]`` rows; q in place or to
-    ``q_out`` ``[T, Hq * D]`` (apart from ``qkv``), k and v into the cache. ``cos_sin``: fp32 ``[positions, cos | sin]`` (None: no rotation), ``rot_dim``
+    ``q_out`` ``[T, Hq * D]`` (apart from the heads of ``qkv``), k and v into the cache. ``cos_sin``: fp32 ``[positions, cos | sin]`` (None: no rotation), ``rot_dim``
     its width, pairs half of it apart (``neox``) or neighbours. ``offsets``: columns where q, k and v begin; ``q_head_stride``:
     columns between q heads. The slots of a call differ; slots outside the cache (-1) write nothing, and a position
     outside the table makes its row NaN. The k and v columns of ``qkv`` stay as they are."""
@@ -123,7 +123,10 @@ def append(qkv: torch.Tensor, positions: Optional[torch.Tensor], cos_sin: Option
         if ok and q_out is not None:
             ok = (q_out.dtype is BF16 and q_out.get_device() == dev and q_out.dim() == 2 and q_out.stride(1) == 1 and q_out.shape[0] >= T
                   and q_out.shape[1] == num_q_heads * D and (q_out.data_ptr() | 2 * q_out.stride(0)) % 16 == 0
-                  and (T <= 1 or q_out.stride(0) >= q_out.shape[1]))
+                  and (T <= 1 or q_out.stride(0) >= q_out.shape[1]) and num_q_heads > 0)
+            if ok:
+                out, ldo = q_out.data_ptr(), q_out.stride(0)
+                ok = out >= at + 2 * ((T - 1) * ld + cols) or at >= out + 2 * ((T - 1) * ldo + q_out.shape[1])
         for w in (q_norm, k_norm):
             if ok and w is not None:
                 ok = w.dtype is BF16 and w.get_device() == dev and w.numel() == D and w.is_contiguous() and w.data_ptr() % 16 == 0
@@ -224,7 +227,8 @@ def _attend(op, q, cache, block_table, seq_lens, q_start, tile_req, tile_q0, sca
         if ok and given:
             (orows, ocols), (ldo, o1), op_ = out.shape, out.stride(), out.data_ptr()
             ok = (orows == rows and ocols == cols and out.dtype is BF16 and out.get_device() == dev and o1 == 1
-                  and (op_ | 2 * ldo) % 16 == 0 and op_ != qp and (rows <= 1 or ldo >= cols))
+                  and (op_ | 2 * ldo) % 16 == 0 and (rows <= 1 or ldo >= cols)
+                  and (op_ >= qp + 2 * ((rows - 1) * ldq + cols) or qp >= op_ + 2 * ((rows - 1) * ldo + cols)))
         if ok and tmp is not None:
             ok = (tmp.dtype is torch.float32 and tmp.get_device() == dev and tmp.is_contiguous()
                   and tmp.data_ptr() % 16 == 0 and tmp.numel() >= scratch_floats(q.device, D, op == "fp4_prefill"))
@@ -269,7 +273,7 @@ def decode(q: torch.Tensor, cache: torch.Tensor, *, block_table: torch.Tensor, s
            tmp: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Attention of one query row a sequence, ``q`` ``[B, Hq * D]``, at its last position. ``seq_lens`` int32 ``[B]`` counts the row's own
     key; 0: zeros come out. ``window`` as in :func:`vllm_cpp_b200.ops.attn_decode`; entries of ``block_table`` outside the cache count as
-    masked keys. ``out`` shares no memory with ``q``. ``tmp``: :func:`scratch`, allocated if not given. At most 8192 sequences."""
+    masked keys. ``out`` shares no memory with the rows of ``q``. ``tmp``: :func:`scratch`, allocated if not given. At most 8192 sequences."""
     return _attend("fp4_decode", q, cache, block_table, seq_lens, None, None, None, scale, out, softcap, window, True, tmp)
 
 

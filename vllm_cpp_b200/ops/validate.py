@@ -127,13 +127,34 @@ def _apart_from_keys(H, D, num_q_heads, stride, offsets) -> bool:
     return (num_q_heads <= 1 or stride >= D) and not any(a < o + H * D and o < b for a, b in heads for o in offsets[1:])
 
 
+def _apart_rows(a, b) -> bool:
+    """No byte of the rows of ``a`` is one of the rows of ``b`` (2-d, columns side by side, any distance between rows)."""
+    if a.numel() == 0 or b.numel() == 0:
+        return True
+    (pa, na, la, wa), (pb, nb, lb, wb) = ((t.data_ptr(), t.shape[0], t.stride(0) * t.element_size() if t.shape[0] > 1 else 0,
+                                           t.shape[1] * t.element_size()) for t in (a, b))
+    if pa + (na - 1) * la + wa <= pb or pb + (nb - 1) * lb + wb <= pa:
+        return True
+    first = pa + la * torch.arange(na)
+    other = pb + lb * torch.arange(nb)
+    # of a's rows as many end at or before a row of b as begin before its end
+    return torch.equal(torch.searchsorted(first, other + wb), torch.searchsorted(first + wa, other, right=True))
+
+
+def _apart_from_heads(q_out, qkv, cache, num_q_heads, stride, offsets) -> bool:
+    """Query rows that go elsewhere lie apart from the heads that are read."""
+    D, T = cache.shape[3] // 18, qkv.shape[0]
+    read = [(offsets[0] + i * stride, D) for i in range(num_q_heads)] + [(o, cache.shape[1] * D) for o in offsets[1:]]
+    return _apart_rows(q_out[:T], qkv) or all(_apart_rows(q_out[:T], qkv[:, at: at + n]) for at, n in read)
+
+
 _FP4_CACHE = ("cache is uint8 [blocks, kv heads, block_size / 16, 18 head_dim], contiguous, head_dim 64, 128 or 256", _fp4_cache)
 _FP4_ATTN = [
     _FP4_CACHE,
     ("q is [rows, Hq * head_dim] bf16 with rows on 16-byte boundaries, Hq a multiple of the kv heads", lambda q, cache, **_: _bf16_rows(q)
      and q.shape[1] > 0 and q.shape[1] % (cache.shape[3] // 18 * cache.shape[1]) == 0),
     ("out is like q and apart from it, its rows apart from one another", lambda q, out, **_: _bf16_rows(out) and out.shape == q.shape and _apart(out)
-     and (q.numel() == 0 or out.data_ptr() != q.data_ptr())),
+     and _apart_rows(q, out)),
     ("block_table is int32 [sequences, pages], rows contiguous", lambda block_table, **_: block_table.dtype == torch.int32
      and block_table.dim() == 2 and block_table.shape[1] > 0 and (block_table.shape[1] == 1 or block_table.stride(1) == 1)),
     ("scale is positive, softcap finite and not negative, window in 32 bits", lambda scale, softcap, window=0, **_: scale > 0
@@ -176,6 +197,8 @@ RULES.update({
             for w in (q_norm, k_norm))),
         ("q_out is [T, Hq * head_dim] bf16 with rows on 16-byte boundaries", lambda qkv, cache, num_q_heads, q_out, **_: q_out is None or (
             q_out.dtype == BF16 and q_out.dim() == 2 and (q_out.numel() == 0 or _bf16_rows(q_out) and _apart(q_out)) and q_out.shape[0] >= qkv.shape[0] and q_out.shape[1] == num_q_heads * (cache.shape[3] // 18))),
+        ("q_out lies apart from what is read of qkv", lambda qkv, cache, num_q_heads, q_head_stride, offsets, q_out, **_: q_out is None
+         or num_q_heads == 0 or _apart_from_heads(q_out, qkv, cache, num_q_heads, q_head_stride, offsets)),
         ("all tensors are on one GPU", lambda qkv, cache, slots, positions, cos_sin, q_norm, k_norm, q_out, **_:
          _on_gpu(qkv, cache, slots, positions, cos_sin, q_norm, k_norm, q_out)),
     ],
@@ -192,6 +215,7 @@ RULES.update({
         ("k and v are bf16 [n, kv heads, head_dim], contiguous", lambda cache, slots, k=None, v=None, **_: all(
             x is None or (x.dtype == BF16 and x.is_contiguous() and x.data_ptr() % 16 == 0
                           and tuple(x.shape) == (slots.numel(), cache.shape[1], cache.shape[3] // 18)) for x in (k, v))),
+        ("k and v lie apart from one another", lambda k=None, v=None, **_: k is None or v is None or _apart_rows(k.flatten(1), v.flatten(1))),
         ("all tensors are on one GPU", lambda cache, slots, k=None, v=None, **_: _on_gpu(cache, slots, k, v)),
     ],
     "fp4_decode": _FP4_ATTN + [
