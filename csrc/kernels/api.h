@@ -250,7 +250,10 @@ typedef struct B200Fp4Read {
 
 // Attention over that cache (fp4_attn.cu). q_start null: one query a sequence (decode), else [num_reqs + 1] and causal from the end of each sequence
 // (causal 0: every query sees every key) and with its 128-token query tiles. window as in b200_attn_decode, scale > 0. parts: b200_fp4_attn_scratch
-// floats, for this call alone until it is done. At most 8192 sequences and 8000 tiles.
+// floats, for this call alone until it is done. At most 8192 sequences and 8000 tiles. What the tables' width allows at most is counted in 31 bits:
+// positions (at most 2^31 - 4096; times block size below 2^40) / 32 times kv heads times row tiles of 8 or 16 (query tokens times group, and a tile more a
+// sequence), and positions / 128 times kv heads times row tiles of 256; query tokens times group^2 is below 2^32. Else -4 (b200_fp4_attn_takes tells, without
+// a GPU). Bounds in q_start ascend. Where they go back so often that their sequences come to more, the call does nothing.
 typedef struct B200Fp4Attn {
   const void* q;
   void* out;
@@ -530,6 +533,7 @@ void b200_outer_workspace(int kind, int D, int* values);
 int b200_outer_chunk(const B200Outer* a, cudaStream_t stream);
 // ---- fp4_attn.cu
 long long b200_fp4_attn_scratch(int D, int prefill);
+int b200_fp4_attn_takes(const B200Fp4Attn* a);
 int b200_fp4_attn(const B200Fp4Attn* a, cudaStream_t stream);
 // ---- fp4_cache.cu
 int b200_fp4_append(const B200Fp4Append* a, cudaStream_t stream);

@@ -594,25 +594,67 @@ extern "C" long long b200_fp4_attn_scratch(int D, int prefill) {
                                                                         : floats(std::integral_constant<int, 256>());
 }
 
+namespace b200 {
+
+// What a call comes to: its kernels, rows of a row tile; rc: refused (-1: no such call, -4: more than is counted in 31 bits).
+struct Fp4Plan {
+  int rc, few, row_tile;
+  bool rows, tiles;
+};
+static Fp4Plan fp4_plan(const B200Fp4Attn& a) {
+  Fp4Plan x = {-1, 0x7fffffff, 8, true, false};
+  if ((a.D != 64 && a.D != 128 && a.D != 256) || a.Hkv <= 0 || a.Hq <= 0 || a.Hq % a.Hkv || a.block_size <= 0 || a.block_size % kCellTokens ||
+      a.max_blocks <= 0 || a.num_reqs <= 0 || a.total_q <= 0)
+    return x;
+  x.rc = -4;
+  if (a.num_reqs > kMostReqs || (a.q_start && a.num_tiles > kMostTiles)) return x;
+  const int G = a.Hq / a.Hkv, cells = a.block_size / kCellTokens;
+  const double keys = (double)a.max_blocks * a.block_size, q_rows = (double)a.total_q * G;
+  if (keys > 2147479552.0) return x;          // (positions and a tile behind them in 31 bits)
+  if (q_rows * G >= 4294967296.0 || (double)a.max_blocks * cells * cells >= 4294967296.0) return x;       // (Fp4Div)
+  // Which sequences go to which kernel. Both are launched where the lengths, which only the device knows, may call for both. 24 sequences of 32 heads
+  // over 8 of 128 dims, in the row kernel / the tile kernel: 32 rows (8 tokens) behind 4000 keys 94 / 135 us, behind none 28 / 32; 64 rows 167 / 136
+  // and 45 / 32; 48 rows lie between.
+  static constexpr int kFew = 48;
+  const double most_rows = (double)(a.most_q > 0 && a.most_q < a.total_q ? a.most_q : a.total_q) * G;
+  x.tiles = a.D <= 128 && a.q_start && a.num_tiles > 0 && most_rows > kFew;
+  x.rows = !x.tiles || a.num_reqs > 1;
+  if (x.tiles) x.few = x.rows ? kFew : -1;
+  // Row tiles of 16 where the sequences have more than 8 rows on average. 48 sequences of 2000 keys, 8 kv heads of 128 dims, in tiles of 8 / of 16: 8 rows
+  // 47 / 61 us, 16 rows 71 / 64, 24 rows 95 / 104, 32 rows 120 / 107. (A tile of 16 costs as much as two of 8 do, but for the products by scales and the
+  // fetches; one CTA an SM instead of two. At 256 dims its accumulators do not fit.)
+  if (a.D <= 128 && q_rows > 8.0 * a.num_reqs) x.row_tile = 16;
+  // The longest line of each kernel in 31 bits, for bounds of sequences that ascend: each sequence has one row tile that is not full. (Bounds that go back
+  // can make it longer: fp4_line. An item's cells times an entry's items stay in 31 bits even then.)
+  const auto up = [](double n, int d) { return (double)(((long long)n + d - 1) / d); };
+  if (x.rows) {
+    const double seqs = a.num_reqs < a.total_q ? a.num_reqs : a.total_q;
+    double items = q_rows / x.row_tile + seqs;
+    if (x.tiles) items = min(items, seqs * up(kFew, x.row_tile));
+    if ((up(keys, kPairKeys) + Fp4Seq<16>::kStart) * a.Hkv * items > 2147483647.0) return x;
+  }
+  if (x.tiles) {
+    const double items = a.num_tiles * up((double)(a.total_q < kTileTokens ? a.total_q : kTileTokens) * G, Fp4Tile::kRows);
+    if ((up(keys, kTileKeys) + Fp4Tile::kStart) * a.Hkv * items > 2147483647.0) return x;
+  }
+  x.rc = 0;
+  return x;
+}
+
+}  // namespace b200
+
+// 0 where b200_fp4_attn takes a step of these sizes (pointers are not looked at, but whether there is a q_start); otherwise what it would return.
+extern "C" int b200_fp4_attn_takes(const B200Fp4Attn* a) { return a->num_reqs <= 0 || a->total_q <= 0 ? 0 : fp4_plan(*a).rc; }
+
 extern "C" int b200_fp4_attn(const B200Fp4Attn* a, cudaStream_t stream) {
   if (a->num_reqs <= 0 || a->total_q <= 0) return 0;
-  if ((a->D != 64 && a->D != 128 && a->D != 256) || a->Hkv <= 0 || a->Hq <= 0 || a->Hq % a->Hkv || a->block_size <= 0 ||
-      a->block_size % kCellTokens || a->num_blocks <= 0 || a->max_blocks <= 0 || !(a->scale > 0.f))
-    return -1;
+  if (a->num_blocks <= 0 || !(a->scale > 0.f)) return -1;
   const uintptr_t bits = (uintptr_t)a->q | (uintptr_t)a->out | (uintptr_t)a->cache | (uintptr_t)a->parts | (uintptr_t)((a->ldq | a->ldo) * 2);
   if ((bits & 15) || !a->q || !a->out || !a->cache || !a->block_table || !a->seq_lens || !a->parts || (a->q_start && (!a->tile_req || !a->tile_q0)))
     return -1;
-  if (a->num_reqs > kMostReqs || a->num_tiles > kMostTiles) return -4;
+  const Fp4Plan x = fp4_plan(*a);
+  if (x.rc) return x.rc;
   const int G = a->Hq / a->Hkv;
-  // cells of the whole line in 31 bits, whatever the lengths
-  if (((double)a->max_blocks * (a->block_size / kCellTokens) + Fp4Seq<16>::kStart) * a->Hkv * ((double)a->total_q * G / 8 + a->num_reqs) > 2147483647.0)
-    return -4;
-  if (a->q_start && ((double)a->max_blocks * a->block_size / kTileKeys + Fp4Tile::kStart + 1) * a->Hkv * a->num_tiles *
-                            ((a->total_q < kTileTokens ? a->total_q : kTileTokens) * G / Fp4Tile::kRows + 1) > 2147483647.0)
-    return -4;
-  if ((double)a->max_blocks * a->block_size > 2147479552.0) return -4;          // (positions and a tile behind them in 31 bits)
-  if ((double)a->total_q * G * G >= 4294967296.0 || (double)a->max_blocks * (a->block_size / kCellTokens) * (a->block_size / kCellTokens) >= 4294967296.0)
-    return -4;       // (Fp4Div)
   Fp4Attn p;
   p.q = (const __nv_bfloat16*)a->q; p.ldq = a->ldq;
   p.out = (__nv_bfloat16*)a->out; p.ldo = a->ldo;
@@ -623,26 +665,16 @@ extern "C" int b200_fp4_attn(const B200Fp4Attn* a, cudaStream_t stream) {
   p.num_reqs = a->num_reqs; p.total_q = a->total_q; p.num_tiles = a->q_start ? a->num_tiles : 0;
   p.Hkv = a->Hkv; p.G = G; p.cells_per_page = a->block_size / kCellTokens;
   p.window = max(-(1 << 30), min(a->window, 1 << 30)); p.causal = a->causal;
+  p.few = x.few;
   const auto by = [](int d) { return Fp4Div{d == 1 ? 0u : (uint32_t)(((1ull << 32) + d - 1) / d)}; };
   p.by_group = by(G);
   p.by_page_cells = by(p.cells_per_page);
   p.scale_log2 = a->scale * 1.4426950408889634f;
   p.softcap2 = a->softcap * 1.4426950408889634f;
   p.status = device_status_word();
-  // Which sequences go to which kernel. Both are launched where the lengths, which only the device knows, may call for both. 24 sequences of 32 heads
-  // over 8 of 128 dims, in the row kernel / the tile kernel: 32 rows (8 tokens) behind 4000 keys 94 / 135 us, behind none 28 / 32; 64 rows 167 / 136
-  // and 45 / 32; 48 rows lie between.
-  static constexpr int kFew = 48;
-  const bool tensor = a->D <= 128 && a->q_start && p.num_tiles > 0, long_one = tensor && (long long)(a->most_q > 0 ? min(a->most_q, a->total_q) : a->total_q) * G > kFew;
-  bool rows = true, tiles = long_one;
-  p.few = long_one ? kFew : 0x7fffffff;
-  if (long_one && a->num_reqs == 1) { rows = false; p.few = -1; }
   float* parts = (float*)a->parts;
-  // Row tiles of 16 where the sequences have more than 8 rows on average. 48 sequences of 2000 keys, 8 kv heads of 128 dims, in tiles of 8 / of 16: 8 rows
-  // 47 / 61 us, 16 rows 71 / 64, 24 rows 95 / 104, 32 rows 120 / 107. (A tile of 16 costs as much as two of 8 do, but for the products by scales and the
-  // fetches; one CTA an SM instead of two. At 256 dims its accumulators do not fit.)
-  const bool two = a->D <= 128 && (long long)a->total_q * G > 8ll * a->num_reqs;
-  if (a->D == 64) return two ? launch_attn<64, 2>(p, rows, tiles, parts, stream) : launch_attn<64, 1>(p, rows, tiles, parts, stream);
-  if (a->D == 128) return two ? launch_attn<128, 2>(p, rows, tiles, parts, stream) : launch_attn<128, 1>(p, rows, tiles, parts, stream);
-  return launch_attn<256, 1>(p, rows, tiles, parts, stream);
+  const bool two = x.row_tile == 16;
+  if (a->D == 64) return two ? launch_attn<64, 2>(p, x.rows, x.tiles, parts, stream) : launch_attn<64, 1>(p, x.rows, x.tiles, parts, stream);
+  if (a->D == 128) return two ? launch_attn<128, 2>(p, x.rows, x.tiles, parts, stream) : launch_attn<128, 1>(p, x.rows, x.tiles, parts, stream);
+  return launch_attn<256, 1>(p, x.rows, x.tiles, parts, stream);
 }

@@ -285,6 +285,16 @@ class DenseModel:
             self.decode_workspace = self._fp4_workspace
         self.kv_cache_dtype = name
 
+    def check_steps(self, max_tokens: int, max_reqs: int, max_tiles: int, max_blocks: int, block_size: int) -> None:
+        """ValueError where the attention over this model's cache could refuse a step of these sizes."""
+        if self.kv_cache_dtype != "fp4":
+            return
+        from ..ops import fp4_cache
+        if not fp4_cache.steps_fit(head_dim=self.D, num_q_heads=self.hq, num_kv_heads=self.hkv, block_size=block_size, max_blocks=max_blocks,
+                                   max_reqs=max_reqs, max_tokens=max_tokens, max_tiles=max_tiles):
+            raise ValueError(f"attention over a 4-bit KV cache does not take every step of {max_reqs} sequences and {max_tokens} tokens with "
+                             f"{max_blocks * block_size} positions a sequence: lower max_num_seqs, max_num_batched_tokens or max_model_len")
+
     def _fp4_workspace(self, batch: int, max_seq_len: int, block_size: int):
         """(splits, scratch) of a decode batch as the runner keeps them: one scratch for all steps, which follow one another."""
         if getattr(self, "_fp4_scratch", None) is None:

@@ -60,6 +60,7 @@ def _declare():
     for name, args in (("b200_fp4_append", AppendArgs), ("b200_fp4_read", ReadArgs), ("b200_fp4_attn", AttnArgs)):
         _lib.declare(name, [ctypes.POINTER(args), _P], _I)
     _lib.declare("b200_fp4_attn_scratch", [_I, _I], _L)
+    _lib.declare("b200_fp4_attn_takes", [ctypes.POINTER(AttnArgs)], _I)
     l = lib()
     _append, _read, _attn = l.b200_fp4_append, l.b200_fp4_read, l.b200_fp4_attn
     _declared = True
@@ -207,6 +208,24 @@ def scratch(device: torch.device, head_dim: int, prefill: bool = True) -> torch.
     return torch.empty(scratch_floats(device, head_dim, prefill), dtype=torch.float32, device=device)
 
 
+def steps_fit(*, head_dim: int, num_q_heads: int, num_kv_heads: int, block_size: int, max_blocks: int, max_reqs: int, max_tokens: int,
+              max_tiles: int) -> bool:
+    """Whether ``decode`` and ``prefill`` take every step of up to so many sequences, query tokens and tiles with tables of ``max_blocks``
+    entries a sequence (no GPU is needed to say)."""
+    _declare()
+
+    def taken(tokens, reqs, tiles=0, most_q=0):
+        a = AttnArgs()
+        a.D, a.Hq, a.Hkv, a.block_size, a.max_blocks = head_dim, num_q_heads, num_kv_heads, block_size, max_blocks
+        a.total_q, a.num_reqs, a.num_tiles, a.most_q, a.q_start = tokens, reqs, tiles, most_q, 1 if tiles else None
+        return lib().b200_fp4_attn_takes(a) == 0
+    # both kernels; one sequence; the row kernel alone, as for sequences of at most 48 rows, with row tiles of 16 and, where they are most, of 8
+    group = max(1, num_q_heads // num_kv_heads)
+    few = min(max_tokens, max_reqs * max(1, 48 // group))
+    return (taken(max_reqs, max_reqs) and taken(max_tokens, max_reqs, max_tiles) and taken(max_tokens, 1, max_tiles)
+            and taken(few, max_reqs, max_tiles, 1) and taken(max(1, min(few, 8 * max_reqs // group)), max_reqs, max_tiles, 1))
+
+
 _I32 = torch.int32
 _MOST = 2 ** 31
 
@@ -283,7 +302,9 @@ def prefill(q: torch.Tensor, cache: torch.Tensor, *, block_table: torch.Tensor, 
     """Attention of the query rows ``q_start[r]..q_start[r + 1]`` of each sequence, the last of its ``seq_lens[r]`` positions.
     ``tile_req`` / ``tile_q0`` list their 128-row tiles, as in :func:`vllm_cpp_b200.ops.attn_prefill`. Rows outside every
     sequence stay as they are. A NaN that the cache holds reaches the queries that see its key, and no others. ``max_query_len``, the rows of the longest sequence, only chooses between kernels (0: not known, which costs
-    a step of few rows a sequence one launch more). At most 8192 sequences and 8000 tiles."""
+    a step of few rows a sequence one launch more). At most 8192 sequences and 8000 tiles; what a table of this width allows is counted in 31
+    bits (:func:`steps_fit`: 32 heads over 8 of 128 dims with tables for four million tokens, of 256 dims for one million, in steps of 8192 tokens and 256
+    sequences are within; a ``KernelError`` says what is not). The bounds of ``q_start`` ascend: where they go back so often that the sequences come to more than that, the call writes nothing."""
     return _attend("fp4_prefill", q, cache, block_table, seq_lens, q_start, tile_req, tile_q0, scale, out, softcap, window, causal, tmp, max_query_len)
 
 

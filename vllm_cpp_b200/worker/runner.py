@@ -95,6 +95,8 @@ class ModelRunner(E.ModelRunnerBase):
         self.max_blocks = (max_model_len + block_size - 1) // block_size + 1
         self.layout = E.StepLayout.make(self.max_tokens, max_num_seqs, self.max_blocks,
                                         self.num_groups, self.max_spec, max_score_rows)
+        if self.is_cuda and hasattr(model, "check_steps"):
+            model.check_steps(self.max_tokens, max_num_seqs, self.layout.max_tiles, self.max_blocks, block_size)
         self.off = self.layout.offsets()
         nbytes = self.layout.total_bytes
         # two pinned staging buffers: with a step in flight its copy may not have run yet when
