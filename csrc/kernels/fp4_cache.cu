@@ -218,7 +218,7 @@ __global__ void __launch_bounds__(128, MANY ? 8 : 9) fp4_append_kernel(B200Fp4Ap
     const float sf = fp4_scale_value(scale);
     // Quotients by the scale's reciprocal and one correction by the remainder (fma): values of few bits lie exactly between two codes, and there
     // a product with the rounded reciprocal alone decides by its own rounding. With the correction a quotient that fp32 holds exactly, as every
-    // border between codes is, comes out exactly. (7168 of these a token of 8 + 8 heads; divisions took twice the kernel's time.)
+    // border between codes is, comes out exactly. (2048 of these a token of 8 + 8 heads of 128 dims; divisions took twice the kernel's time.)
     float inv, r[8];
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(sf));
     if (sf == 0.f) inv = 0.f;

@@ -157,7 +157,7 @@ def append(qkv: torch.Tensor, positions: Optional[torch.Tensor], cos_sin: Option
 
 def write(k: torch.Tensor, v: torch.Tensor, cache: torch.Tensor, slots: torch.Tensor) -> None:
     """Keys and values ``[n, Hkv * D]`` (or ``[n, Hkv, D]``) that are normed and rotated already, into the cache. What :func:`read`
-    gave comes back to the same values, but for groups whose scale was below 2^-14 or that had saturated."""
+    gave comes back to the same values, but for groups whose scale was below 2^-14."""
     k, v = k.flatten(1), v.flatten(1)
     validate("fp4_write", k=k, v=v, cache=cache, slots=slots)
     _declare()

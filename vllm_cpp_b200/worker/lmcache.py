@@ -40,7 +40,7 @@ class LMCacheStore:
                  hash_algo: str = "blake3"):
         """``kv_caches``: one ``[num_blocks, 2, block_size, Hkv, D]`` tensor per attention layer, or one 4-bit cache
         (``ops/fp4_cache.py``): its keys and values travel as the bf16 values they stand for, under a model name of their own,
-        and come back to the same codes."""
+        and come back to the same values, but for groups whose scale was below 2^-14 (``fp4_cache.write``)."""
         host, port = parse_url(url)
         self.client = lm.RemoteClient(host, port)
         if connect:
