@@ -80,8 +80,8 @@ struct Fp4RowsShape {
   static constexpr int kFixed = kRingBytes + kMergeBytes + kWarps * kRows * 8 + kWarps * kRowStages * 8;
 };
 
-// SEVERAL: a sequence may have several query tokens, so that rows of a tile differ in what they see.
-template <int D, int NT, bool SEVERAL>
+// SEVERAL: a sequence may have several query tokens, so that rows of a tile differ in what they see. CAP: scores are capped.
+template <int D, int NT, bool SEVERAL, bool CAP>
 __global__ void __launch_bounds__(Fp4RowsShape<D, NT>::kWarps * 32, NT == 1 && D <= 128 ? 2 : 1) fp4_rows_kernel(Fp4Attn p, float* parts) {
   using Cell = Fp4Cell<D>;
   using Shape = Fp4RowsShape<D, NT>;
@@ -157,7 +157,7 @@ __global__ void __launch_bounds__(Fp4RowsShape<D, NT>::kWarps * 32, NT == 1 && D
   int st = 0;
   uint32_t parity = 0;
   bool ok = true;
-  const float cap_in = p.softcap2 > 0.f ? 2.8853900817779268f / p.softcap2 : 0.f;
+  const float cap_in = CAP ? fp4_cap_in(1.f, p.softcap2) : 0.f;
 
   // queries: lane (g, t) has dims [t D / 4, + D / 4) of row g
   uint4 raw[NT][D / 32];
@@ -298,13 +298,15 @@ __global__ void __launch_bounds__(Fp4RowsShape<D, NT>::kWarps * 32, NT == 1 && D
         uint32_t bp[2][NT][2];
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-          if (p.softcap2 > 0.f) {                      // (scores in log2 units from here on)
+          if constexpr (CAP) {                          // (scores in log2 units from here on)
+            const float in[2] = {fminf(mul[nt][0] * cap_in, 3.0e38f), fminf(mul[nt][1] * cap_in, 3.0e38f)};
 #pragma unroll
             for (int u = 0; u < 2; ++u)
 #pragma unroll
-              for (int e = 0; e < 4; ++e) sc[u][nt][e] = fp4_capped(sc[u][nt][e], mul[nt][e & 1] * cap_in, p.softcap2);
+              for (int e = 0; e < 4; ++e)
+                sc[u][nt][e] = p.softcap2 > kWideCap ? fp4_wide_capped(sc[u][nt][e], in[e & 1], p.softcap2) : fp4_capped(sc[u][nt][e], in[e & 1], p.softcap2);
           }
-          const float m0 = p.softcap2 > 0.f ? 1.f : mul[nt][0], m1 = p.softcap2 > 0.f ? 1.f : mul[nt][1];
+          const float m0 = CAP ? 1.f : mul[nt][0], m1 = CAP ? 1.f : mul[nt][1];
           // exponents; the reference is raised when one passes it by 8 (p stays below 2^8 2^kUp), and at the first visible key (off is infinite)
           float x[2][4], over = -INFINITY;
           const auto exponents = [&] {
@@ -552,15 +554,15 @@ __global__ void __launch_bounds__(kJoinThreads) fp4_join_kernel(Fp4Attn p, float
 
 static constexpr int kMostReqs = 8192, kMostTiles = 8000;         // (the line of a step is in shared memory)
 
-template <int D, int NT, bool SEVERAL>
+template <int D, int NT, bool SEVERAL, bool CAP>
 static int launch_rows(const Fp4Attn& p, int grid, float* parts, cudaStream_t stream) {
   using Shape = Fp4RowsShape<D, NT>;
   static Fp4Once once;
   if (!once.run([] {
-        return cudaFuncSetAttribute(fp4_rows_kernel<D, NT, SEVERAL>, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape::kFixed + (kMostReqs + 1) * 4) == cudaSuccess;
+        return cudaFuncSetAttribute(fp4_rows_kernel<D, NT, SEVERAL, CAP>, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape::kFixed + (kMostReqs + 1) * 4) == cudaSuccess;
       }))
     return -2;
-  return launch_pdl(fp4_rows_kernel<D, NT, SEVERAL>, dim3(grid), dim3(Shape::kWarps * 32), Shape::kFixed + (size_t)(p.num_reqs + 1) * 4, stream, p, parts) ==
+  return launch_pdl(fp4_rows_kernel<D, NT, SEVERAL, CAP>, dim3(grid), dim3(Shape::kWarps * 32), Shape::kFixed + (size_t)(p.num_reqs + 1) * 4, stream, p, parts) ==
                  cudaSuccess ? 0 : -2;
 }
 
@@ -570,8 +572,11 @@ static int launch_attn(const Fp4Attn& p, bool rows, bool tiles, float* parts, cu
   using Seq = Fp4Seq<Shape::kRows>;
   const int row_grid = rows ? b200_num_sms() * (NT == 1 && D <= 128 ? 2 : 1) : 0, tile_grid = tiles ? fp4_tile_grid() : 0;
   float* tile_parts = parts + fp4_scratch<Seq, D>(row_grid);
-  if (rows)
-    if (const int rc = p.q_start ? launch_rows<D, NT, true>(p, row_grid, parts, stream) : launch_rows<D, NT, false>(p, row_grid, parts, stream)) return rc;
+  if (rows) {
+    const auto form = p.q_start ? (p.softcap2 > 0.f ? launch_rows<D, NT, true, true> : launch_rows<D, NT, true, false>)
+                                : (p.softcap2 > 0.f ? launch_rows<D, NT, false, true> : launch_rows<D, NT, false, false>);
+    if (const int rc = form(p, row_grid, parts, stream)) return rc;
+  }
   if (tiles)
     if (const int rc = launch_fp4_tiles(p, D, tile_parts, stream)) return rc;
   return launch_pdl(fp4_join_kernel<D, Shape::kRows>, dim3(row_grid * kRowShares + tile_grid * (kTileShares / kTurns)), dim3(kJoinThreads), 0, stream, p, parts, row_grid,
@@ -670,7 +675,7 @@ extern "C" int b200_fp4_attn(const B200Fp4Attn* a, cudaStream_t stream) {
   p.by_group = by(G);
   p.by_page_cells = by(p.cells_per_page);
   p.scale_log2 = a->scale * 1.4426950408889634f;
-  p.softcap2 = a->softcap * 1.4426950408889634f;
+  p.softcap2 = fminf(a->softcap * 1.4426950408889634f, 3.0e38f);
   p.status = device_status_word();
   float* parts = (float*)a->parts;
   const bool two = x.row_tile == 16;

@@ -66,7 +66,8 @@ struct Fp4TilePiece {
   }
 };
 
-template <int D>
+// CAP: scores are as they are (0), capped, or capped far above them (2, fp4_wide_capped). A kernel each: what a call does not need is not in its loop.
+template <int D, int CAP>
 __global__ void __launch_bounds__(512, 1) fp4_tiles_kernel(Fp4Attn p, float* parts) {
   using Cell = Fp4Cell<D>;
   using Shape = Fp4TileShape<D>;
@@ -415,12 +416,15 @@ __global__ void __launch_bounds__(512, 1) fp4_tiles_kernel(Fp4Attn p, float* par
         for (int c = 0; c < kTileKeys / 32; ++c) tmem_ld_32x32b_x32(s_addr + c * 32, s + c * 32);
         tmem_ld_wait();
         const int kbase = k0 + j * kTileKeys;
-        if (p.softcap2 > 0.f) {                                  // (scores in log2 units from here on)
-          const float in = sc * (2.8853900817779268f / p.softcap2);
+        if constexpr (CAP > 0) {                                 // (scores in log2 units from here on)
+          const float in = fp4_cap_in(sc, p.softcap2);
 #pragma unroll
-          for (int i = 0; i < kTileKeys; ++i) s[i] = __float_as_uint(fp4_capped(__uint_as_float(s[i]), in, p.softcap2));
+          for (int i = 0; i < kTileKeys; ++i) {
+            const float x = __uint_as_float(s[i]);
+            s[i] = __float_as_uint(CAP == 2 ? fp4_wide_capped(x, in, p.softcap2) : fp4_capped(x, in, p.softcap2));
+          }
         }
-        const float to_log2 = p.softcap2 > 0.f ? 1.f : sc;
+        const float to_log2 = CAP > 0 ? 1.f : sc;
         if (kbase + kTileKeys - 1 > hi || kbase < lo) {
 #pragma unroll
           for (int i = 0; i < kTileKeys; ++i)
@@ -584,18 +588,22 @@ __global__ void __launch_bounds__(512, 1) fp4_tiles_kernel(Fp4Attn p, float* par
 
 int fp4_tile_grid() { return b200_num_sms(); }
 
-template <int D>
+template <int D, int CAP>
 static int launch_tiles(const Fp4Attn& p, float* parts, cudaStream_t stream) {
   const size_t smem = 1024 + Fp4TileShape<D>::kLine + (size_t)(p.num_tiles + 1) * 4;
   static Fp4Once once;
   if (!once.run([] {
         cudaFuncAttributes attr;
         // (a warpgroup waits without limit for registers that the launch did not bring)
-        return cudaFuncGetAttributes(&attr, fp4_tiles_kernel<D>) == cudaSuccess && 4 * attr.numRegs >= kRegsIssue + 2 * kRegsSoftmax + kRegsExpand &&
-               cudaFuncSetAttribute(fp4_tiles_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, 1024 + Fp4TileShape<D>::kLine + 8001 * 4) == cudaSuccess;
+        return cudaFuncGetAttributes(&attr, fp4_tiles_kernel<D, CAP>) == cudaSuccess && 4 * attr.numRegs >= kRegsIssue + 2 * kRegsSoftmax + kRegsExpand &&
+               cudaFuncSetAttribute(fp4_tiles_kernel<D, CAP>, cudaFuncAttributeMaxDynamicSharedMemorySize, 1024 + Fp4TileShape<D>::kLine + 8001 * 4) == cudaSuccess;
       }))
     return -2;
-  return launch_pdl(fp4_tiles_kernel<D>, dim3(fp4_tile_grid()), dim3(512), smem, stream, p, parts) == cudaSuccess ? 0 : -2;
+  return launch_pdl(fp4_tiles_kernel<D, CAP>, dim3(fp4_tile_grid()), dim3(512), smem, stream, p, parts) == cudaSuccess ? 0 : -2;
+}
+template <int D>
+static int launch_tiles(const Fp4Attn& p, float* parts, cudaStream_t stream) {
+  return p.softcap2 > kWideCap ? launch_tiles<D, 2>(p, parts, stream) : p.softcap2 > 0.f ? launch_tiles<D, 1>(p, parts, stream) : launch_tiles<D, 0>(p, parts, stream);
 }
 
 int launch_fp4_tiles(const Fp4Attn& p, int D, float* parts, cudaStream_t stream) {

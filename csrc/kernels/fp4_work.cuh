@@ -85,6 +85,14 @@ __device__ __forceinline__ float fp4_capped(float x, float to_y2, float cap2) { 
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.f + ex2_of(x * to_y2)));
   return fmaf(-2.f * cap2, r, cap2);
 }
+// That is too much of a cap far above the scores. Under one past kWideCap |y| < 1 / 16 takes y - y^3 / 3 + 2 y^5 / 15, off by 2^-28 of itself.
+static constexpr float kWideCap = 1500.f;
+__device__ __forceinline__ float fp4_wide_capped(float x, float to_y2, float cap2) {
+  const float y2log2e = x * to_y2, y = y2log2e * 0.34657359f, yy = y * y;
+  return fabsf(y) < 0.0625f ? cap2 * y * fmaf(yy, fmaf(yy, 0.13333333f, -0.33333333f), 1.f) : fp4_capped(x, to_y2, cap2);
+}
+// to_y2 for scores of `to_log2`: finite, as a score of 0 times it is 0 however small the cap is.
+__device__ __forceinline__ float fp4_cap_in(float to_log2, float cap2) { return fminf(to_log2 * fminf(2.8853900817779268f / cap2, 3.0e38f), 3.0e38f); }
 
 // lowest position that the query at `pos` sees
 __device__ __forceinline__ int fp4_lowest(int window, int pos) {

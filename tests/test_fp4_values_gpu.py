@@ -56,3 +56,38 @@ def test_queries_of_zeros(D, scale, m):
     k, v = C.read(cache, slots)
     F.check_attention(out.view(m, Hq, D), *F.attention(q.view(m, Hq, D), k, v, n - m, scale, 0.0, window))
     assert ops.read_status() == 0
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("cap", [1e-45, 1e-30, 1e-9, 1000.0, 1e4, 1e6, 1e9, 1e30])
+@pytest.mark.parametrize("m", [1, 5, 300])
+def test_caps_of_every_size(D, cap, m):
+    """Rows of zeros beside rows of up to 1e30: a score of 0 stays 0 under the smallest cap, and the largest ones leave scores as they are."""
+    Hq, Hkv, bs, n = 4, 2, 16, 500
+    gen = torch.Generator().manual_seed(m)
+    cache = F.random_cache(40, Hkv, bs, D, gen, DEV)
+    table = torch.randperm(40, generator=gen)[: n // bs + 1].int().to(DEV)[None]
+    q = torch.randn((m, Hq, D), generator=gen)
+    q[:, 0] = 0
+    q[:, 1] *= 1e30
+    q[:, 2] *= 0.01
+    q = q.to(torch.bfloat16).to(DEV)
+    args = dict(block_table=table, seq_lens=torch.tensor([n], dtype=torch.int32, device=DEV), scale=D ** -0.5, softcap=cap)
+    if m == 1:
+        out = C.decode(q.view(m, -1), cache, **args)
+    else:
+        req, q0 = (torch.tensor(t, dtype=torch.int32, device=DEV) for t in ref.build_prefill_tiles([m]))
+        out = C.prefill(q.view(m, -1), cache, q_start=torch.tensor([0, m], dtype=torch.int32, device=DEV), tile_req=req, tile_q0=q0, **args)
+    slots = (table[0].long()[:, None] * bs + torch.arange(bs, device=DEV)).flatten()[:n]
+    k, v = C.read(cache, slots)
+    if cap < 1:
+        # scores of at most the cap are equal but for 2^-29
+        want, size = F.attention(torch.zeros_like(q), k, v, n - m, 1.0, 0.0, 0)
+        F.check_attention(out.view(m, Hq, D), want, size)
+    else:
+        # a cap far above every score but those of the second head, which is equal to it for many keys
+        want, size = F.attention(q, k, v, n - m, D ** -0.5, cap, 0)
+        keep = [0, 2, 3]
+        F.check_attention(out.view(m, Hq, D)[:, keep], want[:, keep], size[:, keep])
+        assert not out.isnan().any()
+    assert ops.read_status() == 0
