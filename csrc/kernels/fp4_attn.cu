@@ -195,7 +195,7 @@ __global__ void __launch_bounds__(Fp4RowsShape<D, NT>::kWarps * 32, NT == 1 && D
       }
       big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 1));
       big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 2));
-      const int e2 = min(max((int)(__float_as_uint(big) >> 23) - 127, -100), 100);
+      const int e2 = min(max((int)(__float_as_uint(big) >> 23) - 127, -126), 126);
       const float down = __uint_as_float((uint32_t)(127 - e2) << 23), up = __uint_as_float((uint32_t)(127 + e2) << 23);
 #pragma unroll
       for (int i = 0; i < D / 32; ++i) {
@@ -208,7 +208,7 @@ __global__ void __launch_bounds__(Fp4RowsShape<D, NT>::kWarps * 32, NT == 1 && D
       }
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        mul[nt][e] = __shfl_sync(0xffffffffu, up, (2 * t + e) * 4) * p.scale_log2;
+        mul[nt][e] = fminf(__shfl_sync(0xffffffffu, up, (2 * t + e) * 4) * p.scale_log2, 3.0e38f);
         const int rr = min(nt * 8 + 2 * t + e, nrows - 1) + r0, pos = first + p.by_group.of(rr);
         hi[nt][e] = p.causal ? pos : s.len - 1;
         lo[nt][e] = fp4_lowest(p, pos);

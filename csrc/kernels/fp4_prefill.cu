@@ -385,10 +385,10 @@ __global__ void __launch_bounds__(512, 1) fp4_tiles_kernel(Fp4Attn p, float* par
           for (int e = 0; e < 4; ++e) most = __hmax2(most, __habs2(*reinterpret_cast<const __nv_bfloat162*>(&v[e])));
         }
         const float big = fmaxf(__low2float(most), __high2float(most));
-        const int e2 = min(max((int)(__float_as_uint(big) >> 23) - 127, -100), 100);
+        const int e2 = min(max((int)(__float_as_uint(big) >> 23) - 127, -126), 126);
         const __nv_bfloat162 down = __float2bfloat162_rn(__uint_as_float((uint32_t)(127 - e2) << 23));       // (exact)
         // (never 0, as for queries of zeros and a small scale: a masked score, -infinity, times it would be NaN; so small a factor leaves all scores 0)
-        sc = fmaxf(p.scale_log2 * __uint_as_float((uint32_t)(127 + e2) << 23), 1.2e-38f);
+        sc = fminf(fmaxf(p.scale_log2 * __uint_as_float((uint32_t)(127 + e2) << 23), 1.2e-38f), 3.0e38f);
 #pragma unroll
         for (int i = 0; i < kRowLanes; ++i) {
           const uint32_t v[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};

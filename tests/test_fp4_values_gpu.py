@@ -91,3 +91,25 @@ def test_caps_of_every_size(D, cap, m):
         F.check_attention(out.view(m, Hq, D)[:, keep], want[:, keep], size[:, keep])
         assert not out.isnan().any()
     assert ops.read_status() == 0
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("size", [2.0 ** -122, 2.0 ** -110, 2.0 ** 110, 2.0 ** 122])
+@pytest.mark.parametrize("m", [1, 5, 300])
+def test_queries_at_the_ends_of_their_type(D, size, m):
+    """Queries that an f16 does not hold, with a scale that makes their scores ordinary ones."""
+    Hq, Hkv, bs, n = 4, 2, 16, 500
+    gen = torch.Generator().manual_seed(m)
+    cache = F.random_cache(40, Hkv, bs, D, gen, DEV)
+    table = torch.randperm(40, generator=gen)[: n // bs + 1].int().to(DEV)[None]
+    q = (torch.randn((m, Hq, D), generator=gen) * size).to(torch.bfloat16).to(DEV)
+    args = dict(block_table=table, seq_lens=torch.tensor([n], dtype=torch.int32, device=DEV), scale=0.25 / size)
+    if m == 1:
+        out = C.decode(q.view(m, -1), cache, **args)
+    else:
+        req, q0 = (torch.tensor(t, dtype=torch.int32, device=DEV) for t in ref.build_prefill_tiles([m]))
+        out = C.prefill(q.view(m, -1), cache, q_start=torch.tensor([0, m], dtype=torch.int32, device=DEV), tile_req=req, tile_q0=q0, **args)
+    slots = (table[0].long()[:, None] * bs + torch.arange(bs, device=DEV)).flatten()[:n]
+    k, v = C.read(cache, slots)
+    F.check_attention(out.view(m, Hq, D), *F.attention(q, k, v, n - m, 0.25 / size, 0.0, 0))
+    assert ops.read_status() == 0
