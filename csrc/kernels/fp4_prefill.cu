@@ -226,14 +226,15 @@ __global__ void __launch_bounds__(512, 1) fp4_tiles_kernel(Fp4Attn p, float* par
         return page >= 0 && page < p.num_blocks ? p.cache + ((long long)page * p.Hkv + h) * head_bytes + (long long)cell * Cell::kBytes : nullptr;
       };
       uint4 code[D / 32];
-      uint32_t scale[D / 64], value_scale[D / 64];              // (those of a key's values come with the key)
+      uint32_t scale[D / 64], value_scale[D / 16];              // (a byte each; those of a key's values come with the key)
       const auto load = [&](const uint8_t* cell, int kv) {
 #pragma unroll
         for (int i = 0; i < D / 32; ++i) code[i] = make_uint4(0, 0, 0, 0);
+        if (!kv) {
 #pragma unroll
-        for (int i = 0; i < D / 64; ++i) {
-          scale[i] = kv ? value_scale[i] : 0;
-          if (!kv) value_scale[i] = 0;
+          for (int i = 0; i < D / 64; ++i) scale[i] = 0;
+#pragma unroll
+          for (int i = 0; i < D / 16; ++i) value_scale[i] = 0;
         }
         if (!cell) return;
 #pragma unroll
@@ -243,7 +244,7 @@ __global__ void __launch_bounds__(512, 1) fp4_tiles_kernel(Fp4Attn p, float* par
 #pragma unroll
           for (int i = 0; i < D / 64; ++i) scale[i] = reinterpret_cast<const uint32_t*>(cell + Cell::kKeyScales + token * Cell::kScales)[i];
 #pragma unroll
-          for (int i = 0; i < D / 16; ++i) value_scale[i / 4] |= (uint32_t)cell[Cell::kValueScales + i * kCellTokens + token] << (i % 4 * 8);
+          for (int i = 0; i < D / 16; ++i) value_scale[i] = cell[Cell::kValueScales + i * kCellTokens + token];
         }
       };
       int page = page_of(0);
@@ -287,8 +288,11 @@ __global__ void __launch_bounds__(512, 1) fp4_tiles_kernel(Fp4Attn p, float* par
                 make_uint4(mul_f16x2(v[0], sc), mul_f16x2(v[1], sc), mul_f16x2(v[2], sc), mul_f16x2(v[3], sc));
           }
         }
-        if (kv == 0) {                                           // (`scale` has the values' by now)
+        if (kv == 0) {
           uint32_t nan = 0;
+#pragma unroll
+          for (int k = 0; k < D / 64; ++k)
+            scale[k] = value_scale[4 * k] | value_scale[4 * k + 1] << 8 | value_scale[4 * k + 2] << 16 | value_scale[4 * k + 3] << 24;
 #pragma unroll
           for (int k = 0; k < D / 64; ++k) nan |= ((nan_scales(scale[k]) >> 7) * 0x10204080u >> 28) << (4 * k);
           const uint32_t mask = __ballot_sync(0xffffffffu, none), odd = mask | __ballot_sync(0xffffffffu, nan != 0);
