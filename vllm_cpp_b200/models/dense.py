@@ -278,7 +278,8 @@ class DenseModel:
         if name not in self.KV_CACHE_DTYPES:
             raise ValueError(f"kv_cache_dtype {name!r} is none of {', '.join(self.KV_CACHE_DTYPES)}")
         if name == "fp4":
-            if self.D not in (64, 128, 256) or block_size % 16:
+            from .attention_backends import select
+            if not all(select(phase, "fp4", head_dim=self.D, block_size=block_size) for phase in ("decode", "prefill")):
                 raise ValueError(f"a 4-bit KV cache needs head_dim 64, 128 or 256 and a block_size in multiples of 16, not {self.D} and "
                                  f"{block_size}")
             self.native_layers = False

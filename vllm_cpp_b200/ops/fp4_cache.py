@@ -301,7 +301,7 @@ def prefill(q: torch.Tensor, cache: torch.Tensor, *, block_table: torch.Tensor, 
             window: int = 0, causal: bool = True, tmp: Optional[torch.Tensor] = None, max_query_len: int = 0) -> torch.Tensor:
     """Attention of the query rows ``q_start[r]..q_start[r + 1]`` of each sequence, the last of its ``seq_lens[r]`` positions.
     ``tile_req`` / ``tile_q0`` list their 128-row tiles, as in :func:`vllm_cpp_b200.ops.attn_prefill`. Rows outside every
-    sequence stay as they are. A NaN that the cache holds reaches the queries that see its key, and no others. ``max_query_len``, the rows of the longest sequence, only chooses between kernels (0: not known, which costs
+    sequence stay as they are; sequences are as many as ``q_start``, ``block_table`` and ``seq_lens`` all have. A NaN that the cache holds reaches the queries that see its key, and no others. ``max_query_len``, the rows of the longest sequence, only chooses between kernels (0: not known, which costs
     a step of few rows a sequence one launch more). At most 8192 sequences and 8000 tiles; what a table of this width allows is counted in 31
     bits (:func:`steps_fit`: 32 heads over 8 of 128 dims with tables for four million tokens, of 256 dims for one million, in steps of 8192 tokens and 256
     sequences are within; a ``KernelError`` says what is not). The bounds of ``q_start`` ascend: where they go back so often that the sequences come to more than that, the call writes nothing."""
