@@ -15,10 +15,14 @@
 // kernel joins them.
 //
 // mma.sync and not tcgen05: with 8 rows a product of 32 keys is 64 K multiplications a warp, and what takes the time is the 8192 codes in front of
-// it, which would pass through shared or tensor memory once more. 256 sequences of 200 to 3800 keys, 32 heads over 8 of 128 dims: 136 us for 596 MB,
-// 4.4 TB/s. Bound by instructions: some 290 warp instructions a cell (64 conversions, 64 products by scales, 16 matrix products, 16 that merge the
-// codes of two keys), issued in 0.64 of the cycles; memory is at 0.52, the tensor pipe at 0.22. One sequence of 1000 keys takes 9 us: 3.8 us until
-// the first cell is there (line, table, cell: three loads one behind the other), two of work, and the join.
+// it, which would pass through shared or tensor memory once more. 256 sequences of 200 to 3800 keys, 32 heads over 8 of 128 dims: 137 us for 596 MB,
+// 4.35 TB/s. Some 290 warp instructions a cell (64 conversions, 64 products by scales, 16 matrix products, 16 that merge the codes of two keys). No unit
+// is full (96 sequences of 4096 keys): issue 0.64 of the cycles, memory 0.56, the ALU pipe 0.55, FMA 0.36, tensor 0.26; the four warps of a scheduler
+// wait as often for a pipe that another has taken as for their own last instruction. One sequence of 1000 keys takes 9 us: 3.8 us until the first cell
+// is there (line, table, cell: three loads one behind the other), two of work, and the join.
+//
+// At 256 dims there is no other kernel: a prompt's rows are tiles of 8 here, each of which expands all that it sees. 8000 tokens of 16 heads over 8 took a
+// model of eight layers 76 ms where the bf16 cache takes 27.
 #include <type_traits>
 
 #include "api.h"
@@ -364,8 +368,8 @@ __global__ void __launch_bounds__(Fp4RowsShape<D, NT>::kWarps * 32, NT == 1 && D
           }
         }
         // Where rows differ in what they see, a NaN among the values is not left to the product: 0 times it would reach the rows that do not see it.
-        // A product of its own says which rows do, their outputs become NaN, and its scale in the ring zero. (48 sequences of 2 to 6 drafts: 77 us
-        // without, 79 with it. A call of decode has no such rows, and a kernel without this: 256 sequences 143 us, 147 with it.)
+        // A product of its own says which rows do, their outputs become NaN, and its scale in the ring zero. (48 sequences of 2 to 6 drafts: 76 us
+        // without, 78 with it. A call of decode has no such rows, and kernels without this: 256 sequences 143 us from a flushed L2, 147 with it.)
         if (SEVERAL && edge && tok0 != tok1) {
           constexpr int kWords = D > 128 ? D / 128 : 1;      // groups of a lane's dims
           const auto word_at = [&](int u, int w) {

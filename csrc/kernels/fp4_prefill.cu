@@ -15,10 +15,13 @@
 // Warps (512 threads): 0 issues MMAs and holds tensor memory; 4..7 and 8..11 softmax and output of half 0 and 1, a thread a row; 12..15 expand, a
 // thread a key. Registers move from the first and the last warpgroup to the two of the softmax.
 //
-// 1999 tokens behind 30000, 32 heads over 8 of 128 dims: 915 us, 1.11 PFLOP/s; a causal prompt of 8192 577 us, 0.95 PFLOP/s (0.66 and 0.57 of
-// what a large product reaches). What bounds it: exponentials, 16 a cycle, take as long as the products of a tile, and neither hides all of the other; the
-// masks of the diagonal, the queries and the outputs of a causal prompt's short items come on top. A piece costs some 3500 cycles for queries and output, what
-// short prompts pay: 13 of 3 to 211 tokens take 35 us.
+// 1999 tokens behind 30000, 32 heads over 8 of 128 dims: 852 us, 1.19 PFLOP/s; a causal prompt of 8192 572 us, 0.96 PFLOP/s (0.72 and 0.58 of
+// what a large product reaches). What bounds it: a tile's exponentials, 16 a cycle, and its products take some 2050 cycles each, and mostly one after the
+// other: in a prompt of 4096 either unit is busy in 0.45 of the cycles. The masks of the diagonal, the queries and the outputs of a causal prompt's short
+// items come on top. A piece costs some 3500 cycles for queries and output, what short prompts pay: 13 of 3 to 211 tokens take 35 us.
+//
+// Rows differ in what they see of a tile, so a NaN among values does not reach the product: expanders name the keys that have one and put zero, and the
+// softmax marks its row's groups where it sees such a key (8192 tokens 562 us without, 572 with it).
 #include "api.h"
 #include "fp4_work.cuh"
 

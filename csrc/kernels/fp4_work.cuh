@@ -154,8 +154,9 @@ struct Fp4Tile {               // tiles of 128 keys, row tiles of 256
   }
 };
 
-// line[i] = cells in the line in front of entry i (count + 1 values); gives the line's length. All threads of the block take part. Sequences whose bounds
-// overlap could make it longer than 31 bits count: then it is empty, and the call does nothing.
+// line[i] = cells in the line in front of entry i (count + 1 values); gives the line's length. All threads of the block take part. Bounds of sequences that
+// go back (q_start does not ascend) could make it longer than 31 bits count: then it is empty, and the call does nothing. Those that ascend cannot; the host
+// has seen to that.
 template <class Entry>
 __device__ uint32_t fp4_line(const Fp4Attn& p, uint32_t* line) {
   __shared__ uint32_t warp_sum[32];

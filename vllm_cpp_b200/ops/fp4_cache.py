@@ -8,7 +8,7 @@ key codes ``[16, D / 2]`` (the even dimension in the low nibble), value codes ``
 ``n ^ 2 (token // 4)``, key scales ``[16, D / 16]``, value scales ``[D / 16, 16]``.
 
 head_dim 64, 128 or 256; block_size a multiple of 16; bf16 queries, keys and values in rows on 16-byte boundaries. The ``ref_*``
-functions restate the operators in plain PyTorch (any device).
+functions restate the operators in plain PyTorch (any device; a NaN in a cache aside).
 """
 from __future__ import annotations
 
@@ -300,11 +300,16 @@ def prefill(q: torch.Tensor, cache: torch.Tensor, *, block_table: torch.Tensor, 
             tile_req: torch.Tensor, tile_q0: torch.Tensor, scale: float, out: Optional[torch.Tensor] = None, softcap: float = 0.0,
             window: int = 0, causal: bool = True, tmp: Optional[torch.Tensor] = None, max_query_len: int = 0) -> torch.Tensor:
     """Attention of the query rows ``q_start[r]..q_start[r + 1]`` of each sequence, the last of its ``seq_lens[r]`` positions.
-    ``tile_req`` / ``tile_q0`` list their 128-row tiles, as in :func:`vllm_cpp_b200.ops.attn_prefill`. Rows outside every
-    sequence stay as they are; sequences are as many as ``q_start``, ``block_table`` and ``seq_lens`` all have. A NaN that the cache holds reaches the queries that see its key, and no others. ``max_query_len``, the rows of the longest sequence, only chooses between kernels (0: not known, which costs
-    a step of few rows a sequence one launch more). At most 8192 sequences and 8000 tiles; what a table of this width allows is counted in 31
-    bits (:func:`steps_fit`: 32 heads over 8 of 128 dims with tables for four million tokens, of 256 dims for one million, in steps of 8192 tokens and 256
-    sequences are within; a ``KernelError`` says what is not). The bounds of ``q_start`` ascend: where they go back so often that the sequences come to more than that, the call writes nothing."""
+    ``tile_req`` / ``tile_q0`` list their 128-row tiles, as in :func:`vllm_cpp_b200.ops.attn_prefill`. Sequences are as many as ``q_start``,
+    ``block_table`` and ``seq_lens`` all have; rows outside every sequence stay as they are. A NaN that the cache holds reaches the
+    queries that see its key, and no others. ``max_query_len``, the rows of the longest sequence, only chooses between kernels (0: not
+    known, which costs a step of few rows a sequence one launch more). At head_dim 256 many rows take several times what they take over
+    a bf16 cache.
+
+    At most 8192 sequences and 8000 tiles; what a table of this width allows is counted in 31 bits (:func:`steps_fit`: 32 heads over 8 of
+    128 dims with tables for four million tokens, of 256 dims for one million, in steps of 8192 tokens and 256 sequences are within; a
+    ``KernelError`` says what is not). The bounds of ``q_start`` ascend: where they go back so often that the sequences come to more than
+    that, the call writes nothing."""
     return _attend("fp4_prefill", q, cache, block_table, seq_lens, q_start, tile_req, tile_q0, scale, out, softcap, window, causal, tmp, max_query_len)
 
 
