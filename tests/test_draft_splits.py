@@ -66,3 +66,25 @@ def test_drafters_steps_are_split_by_the_drafters_shape(kv, monkeypatch):
         assert r._decode_splits(2)[0] == 1                     # the target's own
     else:
         assert r._decode_splits(2)[0] == 2
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kv", ["auto", "fp4"])
+def test_drafts_of_a_model_with_more_heads(kv):
+    """On the GPU, with parts enough that scratch of the target's shape would not hold them: the tokens are the target's own."""
+    from vllm_cpp_b200 import ops
+    cfg, draft = synthetic_config("tiny-dense"), synthetic_config("tiny-dense")
+    cfg.head_dim = 64
+    draft.head_dim, draft.num_heads, draft.num_kv_heads = 128, 32, 2
+    g = torch.Generator().manual_seed(4)
+    prompts = [torch.randint(0, cfg.vocab_size, (n,), generator=g).tolist() for n in (900, 450)]
+    tokens, llm = [], None
+    for spec in (None, SpeculativeConfig(method="draft_model", num_speculative_tokens=2, draft_model_config=draft)):
+        llm = LLM(EngineArgs(model_config=cfg, device="cuda", block_size=32, num_blocks=100, max_model_len=1024, max_num_seqs=3, max_num_batched_tokens=512,
+                             kv_cache_dtype=kv, speculative_config=spec))
+        tokens.append([o.outputs[0].token_ids for o in llm.generate(prompts, SamplingParams(temperature=0.0, max_tokens=10, ignore_eos=True))])
+    splits, tmp = llm.runner._decode_splits(2, llm.runner.drafter.model)
+    assert splits > 1 and tuple(tmp[0].shape) == (2, 32, splits, 128)
+    # (steps of several query rows add in another order: a near-tie may fall the other way, and what follows it)
+    assert [t[0] for t in tokens[0]] == [t[0] for t in tokens[1]]
+    assert ops.read_status() == 0
