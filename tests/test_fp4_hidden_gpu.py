@@ -61,7 +61,7 @@ def test_nan_that_a_query_does_not_see(lens, new, Hq, Hkv, D, bs, window, causal
     for (k, v), n, m in zip(held, lens, new):
         got, G = out[at: at + m].view(m, Hq, D), Hq // Hkv
         pos, key = torch.arange(n - m, n, device=DEV)[:, None], torch.arange(n, device=DEV)[None]
-        seen = key <= (pos if causal else n)
+        seen = (key <= (pos if causal else n)).expand(m, n)
         if window > 0:
             seen = seen & (key > pos - window)
         elif window < 0:
