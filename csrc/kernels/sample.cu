@@ -10,39 +10,12 @@
 #include <float.h>
 
 #include "api.h"
+#include "row_cluster.cuh"
 #include "sm100.cuh"
 
 namespace b200 {
 
 static constexpr int kSB = 256;  // threads per block for row kernels
-static constexpr float kEps = 1e-5f;
-
-struct ArgPair { float v; int i; };
-__device__ __forceinline__ ArgPair arg_better(ArgPair a, ArgPair b) {
-  return (b.v > a.v || (b.v == a.v && b.i < a.i)) ? b : a;
-}
-__device__ __forceinline__ ArgPair block_argmax(ArgPair a, ArgPair* sh) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    ArgPair b;
-    b.v = __shfl_xor_sync(0xffffffffu, a.v, o);
-    b.i = __shfl_xor_sync(0xffffffffu, a.i, o);
-    a = arg_better(a, b);
-  }
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, nw = blockDim.x >> 5;
-  if (lane == 0) sh[warp] = a;
-  __syncthreads();
-  ArgPair r = (lane < nw) ? sh[lane] : ArgPair{-FLT_MAX, 0x7fffffff};
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    ArgPair b;
-    b.v = __shfl_xor_sync(0xffffffffu, r.v, o);
-    b.i = __shfl_xor_sync(0xffffffffu, r.i, o);
-    r = arg_better(r, b);
-  }
-  __syncthreads();
-  return r;
-}
 __device__ __forceinline__ float block_reduce_max(float v, float* sh) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
@@ -244,16 +217,6 @@ struct RowSlice {
   const float* v;   // where to read it (shared memory, or x)
   int lo, n;        // first column, columns
 };
-__host__ __device__ __forceinline__ int row_slice_cols(int V, int ctas) { return ((V + ctas - 1) / ctas + 3) & ~3; }
-template <int CTAS>
-__device__ __forceinline__ int row_rank() {
-  if constexpr (CTAS > 1) return (int)cluster_ctarank();
-  return 0;
-}
-template <int CTAS>
-__device__ __forceinline__ void row_sync() {
-  if constexpr (CTAS > 1) cluster_sync_all();
-}
 // Loads this CTA's slice of its row (blockIdx.x / CTAS). Every CTA of the cluster runs when it returns.
 template <int CTAS, int T>
 __device__ __forceinline__ RowSlice load_row_slice(float* row, int V, float* stage) {
@@ -279,30 +242,6 @@ __device__ __forceinline__ RowSlice load_row_slice(float* row, int V, float* sta
     __syncthreads();
   }
   return s;
-}
-// Exchange of W words per CTA: each CTA stores its own into every CTA of the cluster, and after one cluster barrier all
-// threads read them at home. Two buffers in turn, so that one barrier a call is enough.
-template <int CTAS, int W>
-struct RowExchange {
-  float slot[2][CTAS][W];
-};
-template <int CTAS, int W>
-__device__ __forceinline__ void row_gather(RowExchange<CTAS, W>& ex, int turn, const float (&mine)[W], float (&all)[CTAS][W]) {
-  if constexpr (CTAS == 1) {
-#pragma unroll
-    for (int w = 0; w < W; ++w) all[0][w] = mine[w];
-    return;
-  }
-  if (threadIdx.x < CTAS) {
-    const uint32_t to = mapa_u32(smem_u32(&ex.slot[turn & 1][cluster_ctarank()][0]), threadIdx.x);
-#pragma unroll
-    for (int w = 0; w < W; ++w) asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(to + 4 * w), "f"(mine[w]) : "memory");
-  }
-  cluster_sync_all();
-#pragma unroll
-  for (int r = 0; r < CTAS; ++r)
-#pragma unroll
-    for (int w = 0; w < W; ++w) all[r][w] = ex.slot[turn & 1][r][w];
 }
 // Sums of W numbers a thread over the whole row (counts stay exact up to 2^24).
 template <int CTAS, int T, int W>
@@ -531,18 +470,6 @@ __global__ void __cluster_dims__(CTAS, 1, 1) __launch_bounds__(T)
 }
 
 // ---- seeded exponential-race sample: argmax_i p_i / (-log u_i) ----
-__host__ __device__ inline uint64_t splitmix64(uint64_t z) {
-  z += 0x9E3779B97F4A7C15ull;
-  z = (z ^ (z >> 30)) * 0xBF58476D1CE4E5B9ull;
-  z = (z ^ (z >> 27)) * 0x94D049BB133111EBull;
-  return z ^ (z >> 31);
-}
-__device__ __forceinline__ float race_key(float prob, uint64_t seed, uint64_t step, int col) {
-  const uint64_t z = splitmix64(seed ^ splitmix64(step * 0x100000001B3ull + (uint64_t)col));
-  const double u = ((double)(z >> 11) + 0.5) * (1.0 / 9007199254740992.0);
-  const float e = (float)(-log(u));
-  return prob / e;
-}
 // (40 rows of 151936 dense probabilities: 314 us with a block of 256 threads per row, 52 with a cluster.)
 template <int CTAS, int T>
 __global__ void __cluster_dims__(CTAS, 1, 1) __launch_bounds__(T)
