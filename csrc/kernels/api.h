@@ -218,6 +218,60 @@ typedef struct B200BiasAttn {
   float out_scale;             // the outputs are multiplied by this
 } B200BiasAttn;
 
+// Attention of trees of drafted tokens over a paged bf16 cache [num_blocks, 2, block_size, Hkv, D] (tree_attn.cu). Request r has the nodes q_start[r] ..
+// q_start[r + 1] (int32, ascending), whose cells are the last of its seq_lens[r]; the cells before them are its context. A node sees the context and the
+// nodes whose bits are set in its row of mask. window > 0: of the context only what lies less than window before the node's position (int64; from the
+// context's length on, a node number more at most). Rows and cache lie on 16-byte boundaries. parts: b200_tree_attn_scratch floats, for this call alone until it
+// is done. At most 8192 requests, 1024 nodes a request; positions / 128 (64 at D = 256) times kv heads times a request's tiles of 128 rows below 2^31 (-4).
+typedef struct B200TreeAttn {
+  const void* q;               // bf16 [total_q][Hq D]
+  void* out;
+  long long ldq, ldo, ldt;
+  const void* cache;
+  long long num_blocks;
+  const void* block_table;     // int32 [num_reqs][max_blocks], rows ldt apart
+  const void* seq_lens;
+  const void* q_start;
+  const void* mask;            // uint64 [total_q][words]
+  const void* positions;       // int64 [total_q], or null: no window
+  void* parts;
+  int max_blocks, num_reqs, total_q, words;
+  int Hq, Hkv, D, block_size;
+  int window;
+  float scale, softcap;
+} B200TreeAttn;
+
+// Drafted tokens against the target's logits (tree_verify.cu; the rule stands there). A request's nodes are q_start[r] .. q_start[r + 1], node 0 its last
+// token, every other a draft below its parent (parents null: below the node before it). At most 393216 columns (-4), 1024 nodes a request count.
+typedef struct B200TreeVerify {
+  const void* logits;          // fp32 [total][V], rows ldl apart
+  const void* probs;           // fp32 [total][V], rows ldp apart: what a node's children were drawn from; null: drafts that were chosen
+  long long ldl, ldp;
+  const void* tokens;          // int64 [total]
+  const void* parents;         // int32 [total]
+  const void* q_start;         // int32 [num_reqs + 1]
+  const void* uniforms;        // fp32 [total], in [0, 1): of the node that is asked
+  const void* seeds;           // 64 bits [num_reqs], as b200_random_sample takes them
+  const void* steps;
+  const void* temperature;     // fp32 [num_reqs] or null: below 1e-5 the request is greedy
+  void* out;                   // int64 [num_reqs][most]: accepted tokens and the last one, then -1
+  void* path;                  // int32 [num_reqs][most]: the root and the accepted nodes, then -1
+  void* count;                 // int32 [num_reqs]: tokens (0 for a request without nodes)
+  int num_reqs, total, V, most;
+} B200TreeVerify;
+
+// Cells of accepted nodes move behind their context (tree_cells.cu): cell c + path[r][i] to c + i, c = seq_lens[r] less the request's nodes, in each of the
+// caches [num_blocks][2][block_size][cell_bytes]. Entries that are not behind their place stay where they are.
+typedef struct B200TreeCompact {
+  const void* const* caches;   // num_caches pointers, in host memory
+  const void* block_table;     // int32 [num_reqs][max_blocks], rows ldt apart
+  const void* seq_lens;
+  const void* q_start;
+  const void* path;            // int32 [num_reqs][most]
+  long long num_blocks, ldt, cell_bytes;
+  int num_caches, max_blocks, num_reqs, total, most, block_size;
+} B200TreeCompact;
+
 // Keys and values of a step into a paged cache held in 4 bits (fp4_cache.cu): per-head RMSNorm of q and k (weights or null), rotation (cos_sin null:
 // none), q to q_out (null: in place), k and v to the cache. Rows of heads: k and v heads D apart, q heads q_head_stride apart. A slot outside the
 // cache writes nothing, a position outside the table gives NaN. Rows, weights and cache lie on 16-byte boundaries.
@@ -531,6 +585,18 @@ int b200_outer_norm(const B200Outer* a, int reqs, int chunks, cudaStream_t strea
 int b200_outer_fits(const B200Outer* a);
 void b200_outer_workspace(int kind, int D, int* values);
 int b200_outer_chunk(const B200Outer* a, cudaStream_t stream);
+// ---- tree_attn.cu
+int b200_tree_attn_takes(const B200TreeAttn* a);
+long long b200_tree_attn_scratch(int D);
+int b200_tree_attn(const B200TreeAttn* a, cudaStream_t stream);
+// ---- tree_cells.cu
+// Of the nodes q_start[r] .. q_start[r + 1] (int32 [num_reqs + 1]) of each request: bits uint64 [total][words], node j at bit j of a row, set for the row's
+// node and those above it, and positions int64 [total]. parents int32 [total]: a node's within its request, below its own number (else the node is a
+// root). At most 16 words; nodes of a request past the 1024th are left out, and rows of no request stay as they are.
+int b200_tree_mask(const void* parents, const void* q_start, const void* seq_lens, int num_reqs, int total, int words, void* bits, void* positions, cudaStream_t stream);
+int b200_tree_compact(const B200TreeCompact* a, cudaStream_t stream);
+// ---- tree_verify.cu
+int b200_tree_verify(const B200TreeVerify* a, cudaStream_t stream);
 // ---- fp4_attn.cu
 long long b200_fp4_attn_scratch(int D, int prefill);
 int b200_fp4_attn_takes(const B200Fp4Attn* a);

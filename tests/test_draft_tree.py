@@ -1,0 +1,226 @@
+"""Drafted trees without a GPU: the restatements against what they restate, refusals, and the sizes that the attention takes."""
+import ctypes
+import math
+import random
+
+import pytest
+import torch
+
+from draft_tree_cases import attention_case, page_table, starts_of, tree_parents
+from vllm_cpp_b200.ops import _lib, draft_tree, reference
+from vllm_cpp_b200.ops.validate import OpArgumentError
+from vllm_cpp_b200.spec_decode import greedy_rejection_sample
+
+
+def test_the_masks_restatement():
+    parents = torch.tensor([-1, 0, 0, 1, 3, -1, 0], dtype=torch.int32)
+    bits, positions = draft_tree.ref_mask(parents, q_start=starts_of([5, 2]), seq_lens=torch.tensor([25, 2], dtype=torch.int32), max_nodes=65)
+    assert bits.tolist() == [[1, 0], [3, 0], [5, 0], [11, 0], [27, 0], [1, 0], [3, 0]] and positions.tolist() == [20, 21, 21, 22, 23, 0, 1]
+    chain = torch.arange(-1, 129, dtype=torch.int32)
+    bits, _ = draft_tree.ref_mask(chain, q_start=starts_of([130]), seq_lens=torch.tensor([130], dtype=torch.int32), max_nodes=130)
+    assert bits[63].tolist() == [-1, 0, 0] and bits[129].tolist() == [-1, -1, 3]
+
+
+@pytest.mark.parametrize("window,softcap", [(0, 0.0), (40, 0.0), (0, 20.0)])
+def test_the_attentions_restatement_of_a_chain_is_causal_attention(window, softcap):
+    case, scale = attention_case([6, 1, 30], [50, 0, 77], hq=4, hkv=2, d=64, page=16, wide=1)
+    got = draft_tree.ref_attention(scale=scale, window=window, softcap=softcap, **case)
+    want = reference.paged_attention(case["q"].float(), case["kv_cache"], case["block_table"], case["seq_lens"], case["q_start"], 4, 2, 64, 16, scale,
+                                     softcap, window)
+    assert float((got - want).abs().max()) < 1e-4
+
+
+def test_the_attentions_restatement_of_a_path_is_causal_attention_of_that_path():
+    """A node of a tree sees what it would see if its ancestors stood alone behind the context."""
+    case, scale = attention_case([17], [33], hq=2, hkv=1, d=64, page=16, wide=4, seed=4)
+    got = draft_tree.ref_attention(scale=scale, dtype=torch.float64, **case)
+    for node in (16, 9):
+        line = [j for j in range(17) if int(case["mask"][node, 0]) >> j & 1]
+        kv = case["kv_cache"][case["block_table"][0].long()].transpose(1, 2).reshape(-1, 2, 1, 64)
+        cells = torch.cat([kv[:33], kv[[33 + j for j in line]]]).double()
+        s = torch.einsum("hd,kd->hk", case["q"][node].view(2, 64).double(), cells[:, 0, 0]) * scale
+        assert torch.allclose(got[node].view(2, 64), s.softmax(-1) @ cells[:, 1, 0], atol=1e-12)
+
+
+def test_the_greedy_rule_is_the_greedy_rejection():
+    gen = torch.Generator().manual_seed(1)
+    sizes, V = [4, 1, 6, 3], 4
+    logits = torch.randn((sum(sizes), V), generator=gen)
+    tokens = torch.where(torch.rand(sum(sizes), generator=gen) < 0.7, logits.argmax(1).roll(1), torch.randint(0, V, (sum(sizes),), generator=gen))
+    q_start = starts_of(sizes)
+    drafts = torch.cat([tokens[int(a) + 1: int(b)] for a, b in zip(q_start, q_start[1:])])
+    want = greedy_rejection_sample(logits.argmax(1), drafts, starts_of([n - 1 for n in sizes]), 5)
+    got, path, count = draft_tree.ref_verify(logits, tokens, q_start=q_start, uniforms=torch.zeros(14), seeds=torch.zeros(4), steps=torch.zeros(4),
+                                             max_tokens=6, temperature=torch.zeros(4))
+    assert torch.equal(got, want) and count.tolist() == (want >= 0).sum(1).tolist()
+    assert [p[:k] for p, k in zip(path.tolist(), count.tolist())] == [list(range(k)) for k in count.tolist()]
+
+
+@pytest.mark.parametrize("drawn", [True, False])
+def test_the_rule_keeps_the_targets_distribution(drawn):
+    """Summed over what is drafted and integrated over the random numbers (each accepted or not, with its probability) the first
+    token has the target's distribution: two children, all pairs of tokens."""
+    gen = torch.Generator().manual_seed(5)
+    p, q = (torch.softmax(torch.randn(4, generator=gen, dtype=torch.float64), 0) for _ in range(2))
+    total = torch.zeros(4, dtype=torch.float64)
+    for x in range(4):
+        for y in range(4):
+            if not drawn and (x, y) != (2, 0):
+                continue
+            weight, left = (q[x] * q[y], p.clone()) if drawn else (torch.ones(()).double(), p.clone())
+            for t in (x, y):
+                point = q if drawn else torch.eye(4, dtype=torch.float64)[t]
+                a = min(1.0, float(left[t] / point[t]))
+                total[t] += weight * a
+                weight = weight * (1 - a)
+                if weight <= 0:
+                    break
+                left = (left - point).clamp(min=0)
+                left /= left.sum()
+            total += weight * left
+    assert torch.allclose(total, p, atol=1e-12)
+
+
+def test_the_draw_of_the_rule_is_the_samplers():
+    p = torch.softmax(torch.randn(300, generator=torch.Generator().manual_seed(2)) * 2, 0)
+    for seed, step in ((3, 0), (2 ** 63 + 5, 77)):
+        assert int((p.double() / draft_tree.race_numbers(seed, step, 300)).argmax()) == reference.race_sample(p, seed, step)
+
+
+def test_the_compactions_restatement_reads_before_it_writes():
+    table, pages = page_table([12], 4, torch.Generator().manual_seed(1))
+    cache = torch.arange(pages * 2 * 4 * 8).view(pages, 2, 4, 1, 8).to(torch.float32)
+    before = cache.clone()
+    draft_tree.ref_compact(cache, block_table=table, seq_lens=torch.tensor([12]), q_start=starts_of([7]), path=torch.tensor([[0, 2, 3, 6, -1]]))
+    cell = lambda c, at: c[table[0, at // 4], :, at % 4]  # noqa: E731
+    for i, node in ((1, 2), (2, 3), (3, 6)):
+        assert torch.equal(cell(cache, 5 + i), cell(before, 5 + node))
+    assert torch.equal(cell(cache, 5), cell(before, 5)) and torch.equal(cell(cache, 9), cell(before, 9))
+
+
+# ------------------------------------------------------------------------------------------------ refusals
+def attention_args():
+    case, scale = attention_case([5, 3], [10, 4], hq=4, hkv=2, d=64, page=16)
+    return dict(case, scale=scale)
+
+
+@pytest.mark.parametrize("what,change", [
+    ("head_dim", lambda a: a.update(kv_cache=a["kv_cache"][..., :32].contiguous(), q=a["q"][:, :128].contiguous())),
+    ("kv_cache is bf16", lambda a: a.update(kv_cache=a["kv_cache"].float())),
+    ("kv_cache is bf16", lambda a: a.update(kv_cache=a["kv_cache"].transpose(2, 3))),
+    ("q is", lambda a: a.update(q=a["q"].half())),
+    ("q is", lambda a: a.update(q=a["q"][:, :192])),
+    ("q is", lambda a: a.update(q=torch.zeros((8, 260), dtype=torch.bfloat16)[:, 4:])),
+    ("q_start", lambda a: a.update(q_start=a["q_start"].long())),
+    ("seq_lens", lambda a: a.update(seq_lens=a["seq_lens"][:1])),
+    ("block_table", lambda a: a.update(block_table=a["block_table"][:1])),
+    ("block_table", lambda a: a.update(block_table=a["block_table"].long())),
+    ("mask is", lambda a: a.update(mask=a["mask"][:5])),
+    ("mask is", lambda a: a.update(mask=a["mask"].int())),
+    ("scale", lambda a: a.update(scale=0.0)),
+    ("scale", lambda a: a.update(scale=math.inf)),
+    ("softcap", lambda a: a.update(softcap=-1.0)),
+    ("window", lambda a: a.update(window=-128)),
+    ("window", lambda a: a.update(window=16, positions=None)),
+    ("out is", lambda a: a.update(out=a["q"])),
+    ("out is", lambda a: a.update(out=torch.zeros((8, 128), dtype=torch.bfloat16))),
+    ("out is", lambda a: a.update(out=torch.zeros((1, 256), dtype=torch.bfloat16).expand(8, 256))),
+    ("tmp", lambda a: a.update(tmp=torch.zeros(7, dtype=torch.int32))),
+    ("one GPU", lambda a: None),
+])
+def test_attention_refuses(what, change):
+    args = attention_args()
+    change(args)
+    with pytest.raises(OpArgumentError, match=what):
+        draft_tree.attention(**args)
+
+
+def mask_args():
+    return dict(parents=torch.tensor([-1, 0, 1], dtype=torch.int32), q_start=starts_of([3]), seq_lens=torch.tensor([7], dtype=torch.int32))
+
+
+@pytest.mark.parametrize("what,change", [
+    ("parents", lambda a: a.update(parents=a["parents"].long())),
+    ("q_start", lambda a: a.update(q_start=a["q_start"].view(1, 2))),
+    ("seq_lens", lambda a: a.update(seq_lens=a["seq_lens"][:0])),
+    ("max_nodes", lambda a: a.update(max_nodes=0)),
+    ("max_nodes", lambda a: a.update(max_nodes=1025)),
+    ("bits", lambda a: a.update(bits=torch.zeros((3, 2), dtype=torch.int64))),
+    ("positions", lambda a: a.update(positions=torch.zeros(3, dtype=torch.int32))),
+    ("apart", lambda a: a.update(bits=(b := torch.zeros((3, 1), dtype=torch.int64)), positions=b[:, 0])),
+    ("one GPU", lambda a: None),
+])
+def test_mask_refuses(what, change):
+    args = mask_args()
+    change(args)
+    with pytest.raises(OpArgumentError, match=what):
+        draft_tree.mask(**args)
+
+
+def verify_args():
+    return dict(logits=torch.zeros((3, 9)), tokens=torch.zeros(3, dtype=torch.int64), q_start=starts_of([3]), uniforms=torch.zeros(3),
+                seeds=torch.zeros(1, dtype=torch.int64), steps=torch.zeros(1, dtype=torch.int64), max_tokens=3)
+
+
+@pytest.mark.parametrize("what,change", [
+    ("logits", lambda a: a.update(logits=a["logits"].bfloat16())),
+    ("logits", lambda a: a.update(logits=torch.zeros((9, 3)).t())),
+    ("tokens", lambda a: a.update(tokens=a["tokens"].int())),
+    ("uniforms", lambda a: a.update(uniforms=a["uniforms"][:2])),
+    ("q_start", lambda a: a.update(q_start=a["q_start"].long())),
+    ("seeds", lambda a: a.update(seeds=a["seeds"].int())),
+    ("temperature", lambda a: a.update(temperature=torch.zeros(0))),
+    ("parents", lambda a: a.update(parents=torch.zeros(2, dtype=torch.int32))),
+    ("draft_probs", lambda a: a.update(draft_probs=torch.zeros((2, 9)))),
+    ("draft_probs", lambda a: a.update(draft_probs=torch.zeros((3, 9), dtype=torch.float64))),
+    ("max_tokens", lambda a: a.update(max_tokens=0)),
+    ("one GPU", lambda a: None),
+])
+def test_verify_refuses(what, change):
+    args = verify_args()
+    change(args)
+    with pytest.raises(OpArgumentError, match=what):
+        draft_tree.verify(**args)
+
+
+def compact_args():
+    return dict(kv_caches=[torch.zeros((4, 2, 16, 1, 64), dtype=torch.bfloat16) for _ in range(2)], block_table=torch.zeros((1, 3), dtype=torch.int32),
+                seq_lens=torch.tensor([20], dtype=torch.int32), q_start=starts_of([5]), path=torch.zeros((1, 3), dtype=torch.int32))
+
+
+@pytest.mark.parametrize("what,change", [
+    ("there is a cache", lambda a: a.update(kv_caches=[])),
+    ("alike", lambda a: a["kv_caches"].append(torch.zeros((4, 2, 16, 1, 64)))),
+    ("alike", lambda a: a["kv_caches"].append(torch.zeros((4, 2, 16, 2, 64), dtype=torch.bfloat16))),
+    ("16-byte", lambda a: a.update(kv_caches=[torch.zeros((4, 2, 16, 1, 4), dtype=torch.bfloat16)])),
+    ("alike", lambda a: a.update(kv_caches=[torch.zeros((4, 2, 3, 16, 64), dtype=torch.bfloat16).transpose(2, 3)])),
+    ("twice", lambda a: a["kv_caches"].append(a["kv_caches"][0])),
+    ("seq_lens", lambda a: a.update(seq_lens=a["seq_lens"].long())),
+    ("block_table", lambda a: a.update(block_table=a["block_table"].t())),
+    ("path", lambda a: a.update(path=torch.zeros((2, 3), dtype=torch.int32))),
+    ("path", lambda a: a.update(path=a["path"].long())),
+    ("one GPU", lambda a: None),
+])
+def test_compact_refuses(what, change):
+    args = compact_args()
+    change(args)
+    with pytest.raises(OpArgumentError, match=what):
+        draft_tree.compact(**args)
+
+
+def test_sizes_that_the_attention_takes():
+    if not _lib.available():
+        pytest.skip("kernel library not built")
+    draft_tree._declare()
+
+    def takes(**more):
+        a = draft_tree.AttnArgs()
+        for k, v in dict(dict(D=128, Hq=32, Hkv=8, block_size=32, max_blocks=4000, num_blocks=100000, num_reqs=64, total_q=2048, words=1), **more).items():
+            setattr(a, k, v)
+        return _lib.lib().b200_tree_attn_takes(ctypes.byref(a))
+    assert takes() == 0 and takes(words=16, total_q=65536, num_reqs=8192) == 0 and takes(D=256, block_size=64) == 0
+    for wrong in (dict(D=96), dict(Hq=30), dict(Hq=129, Hkv=1), dict(block_size=12), dict(block_size=48), dict(block_size=4), dict(words=0),
+                  dict(D=256, block_size=96), dict(block_size=192)):
+        assert takes(**wrong) == -1, wrong
+    for large in (dict(words=17), dict(num_reqs=8193), dict(num_blocks=2 ** 25), dict(max_blocks=2 ** 26), dict(max_blocks=2 ** 25, words=16, total_q=2048)):
+        assert takes(**large) == -4, large

@@ -25,6 +25,8 @@ def _desc(**t) -> str:
     for k, v in t.items():
         if isinstance(v, torch.Tensor):
             parts.append(f"{k}={tuple(v.shape)} {str(v.dtype).replace('torch.', '')} stride={tuple(v.stride())}")
+        elif isinstance(v, list):
+            parts.append(f"{k}=[{'; '.join(_desc(**{str(i): t}) for i, t in enumerate(v[:4]))}{'; ...' if len(v) > 4 else ''}]")
         elif v is not None:
             parts.append(f"{k}={v}")
     return ", ".join(parts)
@@ -227,6 +229,89 @@ RULES.update({
          and _ids(seq_lens, torch.int32, 0) and _ids(tile_req, torch.int32, 0) and _ids(tile_q0, torch.int32, tile_req.numel())),
     ] + _FP4_ATTN,
 })
+
+
+def _paged_cache(c) -> bool:
+    return c.dim() == 5 and c.shape[1] == 2 and min(c.shape[2:]) > 0 and c.is_contiguous() and c.data_ptr() % 16 == 0
+
+
+def _table(t, reqs) -> bool:
+    return t.dtype == torch.int32 and t.dim() == 2 and t.shape[0] >= reqs and t.shape[1] > 0 and (t.shape[1] == 1 or t.stride(1) == 1)
+
+
+_TREE_REQS = ("q_start is int32 [requests + 1], seq_lens int32 [requests]", lambda q_start, seq_lens, **_: _ids(q_start, torch.int32, 1)
+              and _ids(seq_lens, torch.int32, q_start.numel() - 1))
+RULES.update({
+    "tree_mask": [
+        ("parents is int32 [T]", lambda parents, **_: _ids(parents, torch.int32, 0)),
+        _TREE_REQS,
+        ("max_nodes is 1 to 1024", lambda max_nodes, **_: 0 < max_nodes <= 1024),
+        ("bits is int64 [T, ceil(max_nodes / 64)] and positions int64 [T], contiguous", lambda parents, max_nodes, bits, positions, **_: (
+            bits is None or (bits.dtype == torch.int64 and tuple(bits.shape) == (parents.numel(), (max_nodes + 63) // 64) and bits.is_contiguous()))
+         and (positions is None or (_ids(positions, torch.int64, 0) and positions.numel() == parents.numel()))),
+        ("bits, positions and what is read lie apart", lambda parents, q_start, seq_lens, bits, positions, **_: _all_apart(
+            [t for t in (bits, positions) if t is not None], [parents, q_start, seq_lens])),
+        ("all tensors are on one GPU", lambda parents, q_start, seq_lens, bits, positions, **_: _on_gpu(parents, q_start, seq_lens, bits, positions)),
+    ],
+    "tree_attention": [
+        ("kv_cache is bf16 [blocks, 2, block_size, kv heads, head_dim], contiguous, head_dim 64, 128 or 256", lambda kv_cache, **_:
+         _paged_cache(kv_cache) and kv_cache.dtype == BF16 and kv_cache.shape[4] in (64, 128, 256)),
+        ("q is [T, Hq * head_dim] bf16 with rows on 16-byte boundaries, Hq a multiple of the kv heads", lambda q, kv_cache, **_: _bf16_rows(q)
+         and q.shape[1] > 0 and q.shape[1] % (kv_cache.shape[3] * kv_cache.shape[4]) == 0),
+        ("out is like q and apart from it, its rows apart from one another", lambda q, out, **_: _bf16_rows(out) and out.shape == q.shape
+         and _apart(out) and _apart_rows(q, out)),
+        _TREE_REQS,
+        ("block_table is int32 [requests, pages], rows contiguous", lambda block_table, q_start, **_: _table(block_table, q_start.numel() - 1)),
+        ("mask is int64 [T, words], contiguous", lambda q, mask, **_: mask.dtype == torch.int64 and mask.dim() == 2 and mask.shape[0] >= q.shape[0]
+         and mask.shape[1] > 0 and mask.is_contiguous()),
+        ("scale is positive and finite, softcap finite and not negative", lambda scale, softcap, **_: 0 < scale < math.inf and 0 <= softcap < math.inf),
+        ("window is not negative and below 2^31, and has positions int64 [T]", lambda q, window, positions, **_: 0 <= window < 2 ** 31
+         and (window == 0 or (positions is not None and _ids(positions, torch.int64, q.shape[0])))),
+        ("tmp is fp32 and large enough", lambda kv_cache, tmp, **_: tmp is None or (tmp.dtype == torch.float32 and tmp.is_contiguous()
+         and tmp.data_ptr() % 16 == 0 and tmp.numel() >= _tree_scratch(kv_cache))),
+        ("all tensors are on one GPU", lambda q, kv_cache, block_table, seq_lens, q_start, mask, out, tmp, positions, window, **_: _on_gpu(
+            q, kv_cache, block_table, seq_lens, q_start, mask, out, tmp, positions if window else None)),
+    ],
+    "tree_verify": [
+        ("logits is fp32 [T, V], rows contiguous", lambda logits, **_: logits.dim() == 2 and logits.dtype == torch.float32 and logits.shape[1] > 0
+         and (logits.shape[1] == 1 or logits.stride(1) == 1)),
+        ("tokens is int64 [T], uniforms fp32 [T]", lambda logits, tokens, uniforms, **_: _ids(tokens, torch.int64, logits.shape[0])
+         and _ids(uniforms, torch.float32, logits.shape[0])),
+        ("q_start is int32 [requests + 1]", lambda q_start, **_: _ids(q_start, torch.int32, 1)),
+        ("seeds and steps are int64 [requests], temperature fp32 [requests]", lambda q_start, seeds, steps, temperature, **_: all(
+            _ids(t, torch.int64, q_start.numel() - 1) for t in (seeds, steps)) and (
+                temperature is None or _ids(temperature, torch.float32, q_start.numel() - 1))),
+        ("parents is int32 [T]", lambda logits, parents, **_: parents is None or _ids(parents, torch.int32, logits.shape[0])),
+        ("draft_probs is fp32 [T, V], rows contiguous", lambda logits, draft_probs, **_: draft_probs is None or (
+            draft_probs.shape == logits.shape and draft_probs.dtype == torch.float32 and (logits.shape[1] == 1 or draft_probs.stride(1) == 1))),
+        ("max_tokens is at least 1", lambda max_tokens, **_: max_tokens >= 1),
+        ("all tensors are on one GPU", lambda logits, tokens, q_start, uniforms, seeds, steps, parents, draft_probs, temperature, **_: _on_gpu(
+            logits, tokens, q_start, uniforms, seeds, steps, parents, draft_probs, temperature)),
+    ],
+    "tree_compact": [
+        ("there is a cache", lambda caches, **_: len(caches) > 0),
+        ("caches are [blocks, 2, block_size, kv heads, head_dim], contiguous and alike, cells of 16-byte pieces", lambda caches, **_: all(
+            _paged_cache(c) and c.shape == caches[0].shape and c.dtype == caches[0].dtype
+            and c.shape[3] * c.shape[4] * c.element_size() % 16 == 0 for c in caches)),
+        ("no cache is there twice", lambda caches, **_: len({c.data_ptr() for c in caches}) == len(caches)),
+        _TREE_REQS,
+        ("block_table is int32 [requests, pages], rows contiguous", lambda block_table, q_start, **_: _table(block_table, q_start.numel() - 1)),
+        ("path is int32 [requests, steps], contiguous", lambda path, q_start, **_: path.dtype == torch.int32 and path.dim() == 2
+         and path.shape[0] == q_start.numel() - 1 and path.is_contiguous()),
+        ("all tensors are on one GPU", lambda caches, block_table, seq_lens, q_start, path, **_: _on_gpu(*caches, block_table, seq_lens, q_start, path)),
+    ],
+})
+
+
+def _all_apart(written, read) -> bool:
+    """No two of the contiguous tensors share a byte, but for those that are only read."""
+    spans = [(t.data_ptr(), t.data_ptr() + t.numel() * t.element_size()) for t in written + read]
+    return not any(a < d and c < b for i, (a, b) in enumerate(spans[: len(written)]) for c, d in spans[i + 1:])
+
+
+def _tree_scratch(kv_cache) -> int:
+    from .draft_tree import scratch_floats
+    return scratch_floats(kv_cache.device, kv_cache.shape[4])
 
 
 def validate(op: str, **args) -> None:
