@@ -155,12 +155,21 @@ __device__ __forceinline__ float tree_ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-// cap tanh(x / cap) in log2 units: 1 - 2 / (1 + e^(2 y)), off by 2^-22 of the cap; for a cap far above the scores that is too much: tanhf.
+// cap tanh(x / cap) in log2 units, y = x / cap: 1 - 2 / (1 + e^(2 y)) is off by 2^-22 of the cap, which is too much of one far above the scores; small y
+// take y - y^3 / 3 + 2 y^5 / 15, off by 2^-28 of itself below 1 / 16.
 __device__ __forceinline__ float tree_capped(float x, float cap2, float to_2y) {
-  if (cap2 > 1500.f) return cap2 * tanhf(x / cap2);
+  const float t = x * to_2y, y = t * 0.34657359f, yy = y * y;
   float r;
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.f + tree_ex2(x * to_2y)));
-  return fmaf(-2.f * cap2, r, cap2);
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.f + tree_ex2(t)));
+  return fabsf(y) < 0.0625f ? cap2 * y * fmaf(yy, fmaf(yy, 0.13333333f, -0.33333333f), 1.f) : fmaf(-2.f * cap2, r, cap2);
+}
+// The registers of a load from tensor memory may be read after this.
+__device__ __forceinline__ void tmem_ld_wait_for(uint32_t (&r)[32]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]),
+                 "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]), "+r"(r[16]), "+r"(r[17]), "+r"(r[18]),
+                 "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]),
+                 "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31])::"memory");
 }
 __device__ __forceinline__ bool odd_bf16x2(uint32_t w) { return (w & 0x7f80u) == 0x7f80u || (w & 0x7f800000u) == 0x7f800000u; }
 
@@ -444,11 +453,6 @@ __global__ void __launch_bounds__(kTreeThreads, 1)
         // tiles in which the nodes of the request may differ in what they see (need_mask: those of this warp do)
         const bool odd_tile = kbase + kKeys > rq.ctx || (p.window > 0 && kbase < rq.ctx - p.window + rq.n);
         const bool need_mask = kbase + kKeys > rq.ctx || kbase < low_most;
-        uint32_t seen[kKeys / 32];
-        if (need_mask) {
-#pragma unroll
-          for (int q = 0; q < kKeys / 32; ++q) seen[q] = seen_word(kbase + 32 * q);
-        }
         if (odd_tile && (step == 2 || half == 0)) {
           // values that are not finite: out of the tile, and noted
           const uint32_t v = load0 + (w.two ? 2 * j + 1 : j == nt - 1 ? 2 * nt - 1 : 2 * j + 2);
@@ -493,26 +497,46 @@ __global__ void __launch_bounds__(kTreeThreads, 1)
         ++seen_s[t];
         tc_fence_after_sync();
         const uint32_t s_addr = tmem + t * Sh::kSCols + lanes;
-        uint32_t s[kKeys];
+        // Caps and masks go through tensor memory, 32 scores at a time: the registers of the plain path hold a tile's scores and no more.
+        // (Where it is wide the two threads of a row take a half each and wait for one another.)
+        if (p.cap2 > 0.f || (Sh::kWide ? odd_tile : need_mask)) {
+#pragma unroll 1
+          for (int c = Sh::kWide ? half : 0; c < (Sh::kWide ? half + 1 : kWords); ++c) {
+            uint32_t x[32];
+            tmem_ld_32x32b_x32(s_addr + c * 32, x);
+            const uint32_t seen = need_mask ? seen_word(kbase + 32 * c) : 0xffffffffu;
+            tmem_ld_wait();
+            if (p.cap2 > 0.f) {
 #pragma unroll
-        for (int c = 0; c < kKeys / 32; ++c) tmem_ld_32x32b_x32(s_addr + c * 32, s + c * 32);
-        tmem_ld_wait();
-        float sc = p.scale_log2;
-        if (p.cap2 > 0.f) {
+              for (int i = 0; i < 32; ++i) x[i] = __float_as_uint(tree_capped(__uint_as_float(x[i]) * p.scale_log2, p.cap2, cap_in));
+            }
 #pragma unroll
-          for (int i = 0; i < kKeys; ++i) s[i] = __float_as_uint(tree_capped(__uint_as_float(s[i]) * sc, p.cap2, cap_in));
-          sc = 1.f;
+            for (int i = 0; i < 32; ++i)
+              if (!(seen >> i & 1)) x[i] = 0xff800000u;                    // -inf
+            tmem_st_32x32b_x32(s_addr + c * 32, x);
+          }
+          tmem_st_wait();
+          if (Sh::kWide) {
+            tc_fence_before_sync();
+            if (!(ok = meet())) break;
+            tc_fence_after_sync();
+          }
         }
-        if (need_mask) {
-#pragma unroll
-          for (int i = 0; i < kKeys; ++i)
-            if (!(seen[i >> 5] >> (i & 31) & 1)) s[i] = 0xff800000u;       // -inf
-        }
+        const float sc = p.cap2 > 0.f ? 1.f : p.scale_log2;
+        // Two passes over the tile, 32 scores at a time with the next on their way.
+        uint32_t s[2][32];
+        tmem_ld_32x32b_x32(s_addr, s[0]);
         float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-        for (int i = 0; i < kKeys; i += 4)
+        for (int c = 0; c < kWords; ++c) {
+          tmem_ld_wait_for(s[c & 1]);
+          tmem_ld_32x32b_x32(s_addr + (c + 1 < kWords ? c + 1 : Sh::kWide ? half : 0) * 32, s[(c + 1) & 1]);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) mx[e] = fmaxf(mx[e], __uint_as_float(s[i + e]));
+          for (int i = 0; i < 32; i += 4)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) mx[e] = fmaxf(mx[e], __uint_as_float(s[c & 1][i + e]));
+        }
+        tmem_ld_wait_for(s[0]);        // (kWords is even: the second pass begins where the first did)
         // m: reference of the row's maximum, raised lazily (by more than 2^8), so that the accumulator is rescaled rarely; P stays below 256
         const float tile_max = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * sc;
         float alpha = 1.f;
@@ -554,16 +578,17 @@ __global__ void __launch_bounds__(kTreeThreads, 1)
         constexpr int n32 = Sh::kWide ? 1 : kKeys / 32;
 #pragma unroll
         for (int c = 0; c < n32; ++c) {
+          if (c > 0) tmem_ld_wait_for(s[c & 1]);
+          if (c + 1 < n32) tmem_ld_32x32b_x32(s_addr + (c + 1) * 32, s[(c + 1) & 1]);
           uint32_t pk[16];
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
-            const uint32_t x0 = Sh::kWide && half ? s[32 % kKeys + 2 * i] : s[c * 32 + 2 * i];
-            const uint32_t x1 = Sh::kWide && half ? s[32 % kKeys + 2 * i + 1] : s[c * 32 + 2 * i + 1];
             float a, b;
-            unpack_f32x2(fma_f32x2(pack_b32x2(x0, x1), sc2, off2), a, b);
+            unpack_f32x2(fma_f32x2(pack_b32x2(s[c & 1][2 * i], s[c & 1][2 * i + 1]), sc2, off2), a, b);
             pk[i] = pack_bf16x2(tree_ex2(a), tree_ex2(b));
             sum2[i & 1] = add_f32x2(sum2[i & 1], pack_b32x2(pk[i] << 16, pk[i] & 0xffff0000u));
           }
+          // (over scores that both passes have read)
           tmem_st_32x32b_x16((Sh::kWide ? tmem + Sh::kP + t * 32 + half * 16 + lanes : s_addr + c * 16), pk);
         }
         float sum[4];
