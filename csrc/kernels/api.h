@@ -242,7 +242,7 @@ typedef struct B200TreeAttn {
 } B200TreeAttn;
 
 // Drafted tokens against the target's logits (tree_verify.cu; the rule stands there). A request's nodes are q_start[r] .. q_start[r + 1], node 0 its last
-// token, every other a draft below its parent (parents null: below the node before it). At most 393216 columns (-4), 1024 nodes a request count.
+// token, every other a draft below its parent (parents null: below the node before it). At most 778000 columns (-4), 1024 nodes a request count.
 typedef struct B200TreeVerify {
   const void* logits;          // fp32 [total][V], rows ldl apart
   const void* probs;           // fp32 [total][V], rows ldp apart: what a node's children were drawn from; null: drafts that were chosen

@@ -78,6 +78,21 @@ __host__ __device__ inline uint64_t splitmix64(uint64_t z) {
   z = (z ^ (z >> 27)) * 0x94D049BB133111EBull;
   return z ^ (z >> 31);
 }
+// One and the first 23 bits of 1 - u_i, which is more than they say and at most kRaceRest more; at: step times 0x100000001B3 and the column. (The last step of
+// splitmix64 leaves the upper 31 bits as they are.)
+static constexpr float kRaceRest = 1.1920929e-7f;
+__device__ __forceinline__ float race_rest(uint64_t seed, uint64_t at) {
+  uint64_t z = (seed ^ splitmix64(at)) + 0x9E3779B97F4A7C15ull;
+  z = (z ^ (z >> 30)) * 0xBF58476D1CE4E5B9ull;
+  z = (z ^ (z >> 27)) * 0x94D049BB133111EBull;
+  return __uint_as_float((~(uint32_t)(z >> 32) >> 9) | 0x3f800000u);
+}
+// -log u_i in 32 bits, within 2^-20 of itself: by log1p, whose argument is taken from the number's bits, so that a small one keeps its own.
+__device__ __forceinline__ float race_time(uint64_t seed, uint64_t step, int col) {
+  const uint64_t z = splitmix64(seed ^ splitmix64(step * 0x100000001B3ull + (uint64_t)col));
+  const float rest = ((float)(~z >> 11) + 0.5f) * (1.f / 9007199254740992.f), u = ((float)(z >> 11) + 0.5f) * (1.f / 9007199254740992.f);
+  return rest < 0.5f ? -log1pf(-rest) : -logf(u);
+}
 __device__ __forceinline__ float race_key(float prob, uint64_t seed, uint64_t step, int col) {
   const uint64_t z = splitmix64(seed ^ splitmix64(step * 0x100000001B3ull + (uint64_t)col));
   const double u = ((double)(z >> 11) + 0.5) * (1.0 / 9007199254740992.0);

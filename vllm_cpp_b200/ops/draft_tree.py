@@ -189,7 +189,7 @@ def verify(logits: torch.Tensor, tokens: torch.Tensor, *, q_start: torch.Tensor,
 
     -> ``tokens`` int64 ``[requests, max_tokens]``, the accepted ones and one more, then -1; ``path`` int32 of the same shape, the root and the accepted
     nodes, then -1; ``count`` int32 ``[requests]``, tokens of each. The walk ends after ``max_tokens - 1`` accepted drafts. NaN logits count
-    as -inf; where nothing is left to draw from, the likeliest token comes out. At most 393216 columns."""
+    as -inf; where nothing is left to draw from, the likeliest token comes out. At most 778000 columns."""
     try:
         (T, V), (ld, one), dev, (reqs,) = logits.shape, logits.stride(), logits.get_device(), q_start.shape
         ok = (dev >= 0 and logits.dtype is _F32 and (one == 1 or V == 1) and V > 0 and _ids(tokens, _I64, dev, T) and _ids(q_start, _I32, dev, 1)
