@@ -7,19 +7,24 @@
 //
 // Bound: a node's G query heads of a kv head share every key and value, so that rows = n G rows of scores read 4 D bytes a key once: with up to
 // 256 rows a request the cache's bytes are the floor, above it the products and exponentials. Rows are therefore the 128-row operand (a thread
-// owns a row: no sums across threads), keys the other one, and a CTA takes two tiles of rows against each tile of keys. Where a request
-// has only one tile of rows, its two halves (a warpgroup, a score and an output accumulator each) take every second tile of keys
-// instead and are added at the end: the same two chains of products and softmax in flight, with half the bytes' work each.
+// owns a row: no sums across threads), keys the other one, and a CTA takes two tiles of rows against each tile of 64 keys, a warpgroup a tile. Where a request has
+// only one tile of rows the warpgroups take every second tile of keys instead and are added at the end. Either has two score buffers: the products
+// of its next tile run while it works on this one.
 //
 // Work: the key tiles of all items (request, kv head, two tiles of rows) stand in one line, each CTA (one an SM) takes an equal stretch of it, whatever the
-// lengths; an item's start (queries, output) stands in the line as kStart tiles. Parts of items that a stretch's end cuts go to scratch and a short
-// kernel joins them, in a fixed order.
+// lengths; an item's start (queries, output) stands in the line as kTreeStart tiles. Parts of items that a stretch's end cuts go to scratch and a
+// short kernel joins them, in a fixed order.
 //
 // What a node does not see does not reach it: hidden scores become -inf before the softmax, and values are inspected in the tiles where nodes
 // differ in what they see (the product would multiply an infinity or NaN by 0): what is not finite is taken out there and added at
 // the end to the nodes that see it.
 //
-// Warp roles (320 threads): warp 0 TMA, warp 1 MMA + TMEM owner, warps 2..5 / 6..9 softmax and output.
+// head_dim 256 has one accumulator and so one tile of rows: both warpgroups work on each tile of keys, two threads a row, half of its weights and of the
+// accumulator's columns each.
+//
+// Warp roles (384 threads): warps 0..3 / 4..7 softmax and output; warp 8 keys by TMA, and the pieces of the stretch for the others; warp 9 values by TMA; warps
+// 10 / 11 MMA of either warpgroup, warp 10 TMEM owner. (One warp for both kinds of loads bounded the kernel by its instructions, 128 requests 300 us; one issuer
+// for both warpgroups made each wait for the other's turn.)
 #include <limits.h>
 
 #include <algorithm>
@@ -31,9 +36,11 @@
 
 namespace b200 {
 
-static constexpr int kTreeThreads = 320, kTreeReqs = 8192, kTreeNodes = 1024;       // (the last two: at most)
-static constexpr int kTreeStart = 3;          // what an item's start costs, in key tiles
-static constexpr int kTreeLeast = 2;          // tiles of a stretch at the least
+static constexpr int kTreeThreads = 384, kTreeReqs = 8192, kTreeNodes = 1024;       // (the last two: at most)
+static constexpr int kTreeKeys = 64;          // keys of a tile
+static constexpr int kTreeStart = 6;          // what an item's start costs, in key tiles
+static constexpr int kTreeLeast = 3;          // tiles of a stretch at the least
+static constexpr int kTreePieces = 4;         // pieces that the TMA warp is ahead
 
 struct TreeParams {
   const __nv_bfloat16* cache;
@@ -55,44 +62,47 @@ struct TreeParams {
 template <int D>
 struct TreeShape {
   static constexpr bool kWide = D == 256;              // one tile of rows, two threads a row
-  static constexpr int kKeys = kWide ? 64 : 128;
   static constexpr int kParts = D / 64;                // 64-dim pieces of a row
-  static constexpr int kSlot = kKeys * D * 2, kPiece = kKeys * 128;
-  static constexpr int kRing = D == 64 ? 10 : 5;
+  static constexpr int kSlot = kTreeKeys * D * 2, kPiece = kTreeKeys * 128;
+  static constexpr int kKeySlots = D == 64 ? 10 : D == 128 ? 5 : 2, kValueSlots = D == 64 ? 10 : D == 128 ? 5 : 3;
   static constexpr int kQTile = 128 * D * 2, kQTiles = kWide ? 1 : 2;
-  static constexpr int kTiles = kQTiles * kQTile + kRing * kSlot;
+  static constexpr int kTiles = kQTiles * kQTile + (kKeySlots + kValueSlots) * kSlot;
   static constexpr int kRows = 128 * kQTiles;
-  static constexpr long long kPartFloats = (long long)kRows * D + 2 * kRows;
-  // tensor memory: scores of two tiles, accumulators (two; one and the two tiles' P where it is wide)
-  static constexpr int kSCols = kKeys, kO = 2 * kKeys, kP = kWide ? 384 : 0;
+  static constexpr long long kPartFloats = (long long)kRows * D + 2 * kRows;          // [D / 4][kRows][4], then the rows' maxima and sums
+  // Tensor memory. Two buffers of scores for each warpgroup, their P over them; its accumulator. Wide: one set of buffers, P apart (both threads of a
+  // row read all its scores).
+  static constexpr int kO = kWide ? 128 : 256, kP = 384;
   // tiles of a piece in which nodes may differ in what they see: those of 1024 nodes, and where a window ends those of 1024 positions
-  static constexpr int kOdd = 2 * (kTreeNodes / kKeys + 2), kWords = kKeys / 32;
+  static constexpr int kOdd = 2 * (kTreeNodes / kTreeKeys + 2);
 };
 
 struct TreeReq {
   int n, row0, len, ctx, begin, tiles, pairs, items;   // begin: first key tile; tiles: key tiles; pairs: items of a kv head
 };
 template <int D>
-__device__ __forceinline__ TreeReq tree_req(const TreeParams& p, int b) {
+__device__ __forceinline__ TreeReq tree_req(const TreeParams& p, int start, int end, int len) {
   TreeReq r;
-  r.row0 = min(max(p.q_start[b], 0), p.total_q);
-  r.n = max(0, min(p.q_start[b + 1], p.total_q) - r.row0);
-  r.len = min(max(p.seq_lens[b], 0), p.max_len);
+  r.row0 = min(max(start, 0), p.total_q);
+  r.n = max(0, min(end, p.total_q) - r.row0);
+  r.len = min(max(len, 0), p.max_len);
   r.ctx = r.len - r.n;
   const int low = p.window > 0 ? max(0, r.ctx - p.window + 1) : 0;
-  constexpr int K = TreeShape<D>::kKeys;
-  r.begin = min(low, max(r.len - 1, 0)) / K;
-  r.tiles = max(1, (r.len + K - 1) / K - r.begin);     // (no keys: a tile that nobody sees)
+  r.begin = min(low, max(r.len - 1, 0)) / kTreeKeys;
+  r.tiles = max(1, (r.len + kTreeKeys - 1) / kTreeKeys - r.begin);     // (no keys: a tile that nobody sees)
   const int row_tiles = (r.n + p.nodes - 1) / p.nodes;
   r.pairs = (row_tiles + TreeShape<D>::kQTiles - 1) / TreeShape<D>::kQTiles;
   r.items = r.pairs * p.Hkv;
   return r;
 }
+template <int D>
+__device__ __forceinline__ TreeReq tree_req(const TreeParams& p, int b) { return tree_req<D>(p, p.q_start[b], p.q_start[b + 1], p.seq_lens[b]); }
 
-// The pieces of a CTA's stretch, one after the other; every role walks them for itself.
+// A piece of a CTA's stretch: key tiles of an item. nt = 0: no more.
 struct TreePiece {
-  int head, node0, jb, je;             // kv head, first node, key tiles [jb, je) of the item's
-  bool two;                            // a second tile of rows
+  int b, row0, n, len, ctx;
+  int key0, nt;                        // first key, tiles
+  int head, node0;                     // kv head, first node
+  bool two, cut, whole;                // a second tile of rows; the item began before; the piece is all of it
 };
 template <int D>
 struct TreeWalk {
@@ -100,15 +110,27 @@ struct TreeWalk {
   TreeReq r;
   int b, off;                          // request, cells of it that are behind
   long long left;                      // cells of the stretch
+  int end, next_end, next_len;         // where the request's nodes end; of the next request, on their way
   __device__ __forceinline__ TreeWalk(const TreeParams& p_, int b_, int off_, long long left_) : p(p_), b(b_), off(off_), left(left_) {
-    if (left > 0) r = tree_req<D>(p, b);
+    if (left <= 0) return;
+    end = p.q_start[b + 1];
+    ahead();
+    r = tree_req<D>(p, p.q_start[b], end, p.seq_lens[b]);
   }
-  __device__ __forceinline__ bool next(TreePiece& w) {
+  __device__ __forceinline__ void ahead() {
+    const int nb = min(b + 1, p.num_reqs - 1);
+    next_end = p.q_start[nb + 1];
+    next_len = p.seq_lens[nb];
+  }
+  __device__ __forceinline__ bool next(TreePiece& w, int& jb) {
     while (left > 0) {
       const int cells = kTreeStart + r.tiles;
       if (off >= r.items * cells) {
         if (++b >= p.num_reqs) return false;
-        r = tree_req<D>(p, b);
+        const int start = end;
+        end = next_end;
+        r = tree_req<D>(p, start, end, next_len);
+        ahead();
         off = 0;
         continue;
       }
@@ -116,12 +138,16 @@ struct TreeWalk {
       const int take = (int)min((long long)(cells - o), left);
       off += take;
       left -= take;
-      w.jb = max(0, o - kTreeStart);
-      w.je = max(0, o + take - kTreeStart);
-      if (w.je <= w.jb) continue;
+      jb = max(0, o - kTreeStart);
+      w.nt = max(0, o + take - kTreeStart) - jb;
+      if (w.nt <= 0) continue;
+      w.b = b, w.row0 = r.row0, w.n = r.n, w.len = r.len, w.ctx = r.ctx;
+      w.key0 = (r.begin + jb) * kTreeKeys;
       w.head = item / r.pairs;
       w.node0 = (item - w.head * r.pairs) * TreeShape<D>::kQTiles * p.nodes;
       w.two = w.node0 + p.nodes < r.n && TreeShape<D>::kQTiles == 2;
+      w.cut = jb > 0;
+      w.whole = w.nt == r.tiles;
       return true;
     }
     return false;
@@ -130,25 +156,87 @@ struct TreeWalk {
 
 // What the join needs of an item that stretches cut, written by the CTA that has its last part.
 struct TreeCut {
-  int first, last;                     // CTAs; the first's part is its second, the others' their first (first < 0: nothing to join)
+  int first;                           // CTA of the first part, its second one; those up to this CTA have their first (below 0: nothing to join)
   int row0, head, rows;                // output row of the first node, kv head, rows (node-major)
 };
 
 template <int D>
 struct alignas(8) TreeBars {
-  uint64_t q_full, q_empty, kv_full[TreeShape<D>::kRing], kv_empty[TreeShape<D>::kRing];
-  uint64_t s_full[2], p_full[2], o_full, o_free, pv_done, meet;
+  uint64_t q_full, q_empty, k_full[TreeShape<D>::kKeySlots], k_empty[TreeShape<D>::kKeySlots];
+  uint64_t v_full[TreeShape<D>::kValueSlots], v_empty[TreeShape<D>::kValueSlots];
+  uint64_t s_full[2][2], p_full[2][2], pv_done[2], drained[2], o_full, meet;
+  uint64_t piece_full[kTreePieces], piece_empty[kTreePieces];
+  TreePiece piece[kTreePieces];
+  TreeCut cut;
   uint32_t tmem_base;
   int start_req, start_off;
-  long long sums[kTreeThreads / 32];
-  float rows[2][128];                  // what the two threads of a row tell one another
+  union {
+    long long sums[kTreeThreads / 32];
+    float rows[2][128];                // what the two threads of a row tell one another
+  };
   uint32_t odd_any;
   int odd_tile[TreeShape<D>::kOdd];
-  uint32_t odd[TreeShape<D>::kOdd][TreeShape<D>::kWords];     // keys with a value that is not finite
+  uint32_t odd[TreeShape<D>::kOdd][2]; // keys with a value that is not finite
 };
 template <int D>
 constexpr int tree_smem() { return TreeShape<D>::kTiles + 1024 + (int)sizeof(TreeBars<D>); }
 static_assert(tree_smem<64>() <= 227 * 1024 && tree_smem<128>() <= 227 * 1024 && tree_smem<256>() <= 227 * 1024, "shared memory of a CTA");
+
+// A ring's slot and the parity of its use.
+template <int N>
+struct TreeSlot {
+  int at = 0;
+  uint32_t parity = 0;
+  __device__ __forceinline__ void next() {
+    if (++at == N) at = 0, parity ^= 1;
+  }
+  // After a wait that ran out: what was loaded last into each slot arrives before the CTA ends. (A slot without a load has the parity that does not wait.)
+  __device__ __forceinline__ void drain(uint64_t* full, int* status) const {
+    for (int i = 0; i < N; ++i) mbar_wait_warp(full + i, i < at ? parity : parity ^ 1, status);
+  }
+};
+// The rows of the cache's tensor map that hold the tiles of a piece, one tile after the other: a lane holds the first row of each of 32 pages, the next 32 on their way.
+// Pages outside the cache give rows behind it, which read as zeros.
+struct TreePages {
+  const int32_t* table;
+  int bs, kv, per, num_blocks, last;   // per: pages of a tile
+  int base, off, in_page, now, next;
+  __device__ __forceinline__ int rows(int page) const {
+    const int blk = table[min(page, last)];
+    return ((blk < 0 || blk >= num_blocks ? num_blocks : blk) * 2 + kv) * bs;
+  }
+  __device__ __forceinline__ TreePages(const TreeParams& p, const TreePiece& w, int kv_)
+      : table(p.block_table + w.b * p.ldt), bs(p.block_size), kv(kv_), per(max(1, kTreeKeys / p.block_size)), num_blocks((int)p.num_blocks),
+        last(max(0, (w.len - 1) / p.block_size)), base(w.key0 / p.block_size), off(0), in_page(w.key0 - base * p.block_size) {
+    const int lane = threadIdx.x & 31;
+    now = rows(base + lane);
+    next = rows(base + 32 + lane);
+  }
+  // One tile into `dst`; the whole warp calls it.
+  template <int D>
+  __device__ __forceinline__ void load(uint8_t* dst, const CUtensorMap* map, uint64_t* full, int head) {
+    if (off == 32) {                   // (a tile's pages are a power of two: none passes the end)
+      base += 32, off = 0;
+      now = next;
+      next = rows(base + 32 + (threadIdx.x & 31));
+    }
+    for (int x = 0; x < per; ++x) {
+      const int row = __shfl_sync(0xffffffffu, now, off + x) + in_page;
+      if (elect_one()) {
+#pragma unroll
+        for (int d = 0; d < D / 64; ++d) tma_load_3d(dst + d * TreeShape<D>::kPiece, map, full, d * 64, head, row);
+      }
+      __syncwarp();
+      dst += bs * 128;
+    }
+    if (bs <= kTreeKeys) {
+      off += per;
+    } else if ((in_page += kTreeKeys) == bs) {
+      in_page = 0;
+      ++off;
+    }
+  }
+};
 
 __device__ __forceinline__ float tree_ex2(float x) {
   float y;
@@ -163,17 +251,9 @@ __device__ __forceinline__ float tree_capped(float x, float cap2, float to_2y) {
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.f + tree_ex2(t)));
   return fabsf(y) < 0.0625f ? cap2 * y * fmaf(yy, fmaf(yy, 0.13333333f, -0.33333333f), 1.f) : fmaf(-2.f * cap2, r, cap2);
 }
-// The registers of a load from tensor memory may be read after this.
-__device__ __forceinline__ void tmem_ld_wait_for(uint32_t (&r)[32]) {
-  asm volatile("tcgen05.wait::ld.sync.aligned;"
-               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]),
-                 "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]), "+r"(r[16]), "+r"(r[17]), "+r"(r[18]),
-                 "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]),
-                 "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31])::"memory");
-}
 __device__ __forceinline__ bool odd_bf16x2(uint32_t w) { return (w & 0x7f80u) == 0x7f80u || (w & 0x7f800000u) == 0x7f800000u; }
 
-// Bits of the keys kbase + 32 q .. + 31 that a row sees.
+// Bits of the keys key .. key + 31 that a row sees.
 __device__ __forceinline__ uint32_t tree_seen(const uint64_t* mask, int words, int key, int ctx, int len, int low) {
   const int rel = key - ctx;
   uint32_t v = 0xffffffffu;
@@ -192,35 +272,48 @@ template <int D>
 __global__ void __launch_bounds__(kTreeThreads, 1)
     tree_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmKV, TreeParams p) {
   using Sh = TreeShape<D>;
-  constexpr int kRing = Sh::kRing, kKeys = Sh::kKeys, kOdd = Sh::kOdd, kWords = Sh::kWords;
+  constexpr int K = kTreeKeys, kOdd = Sh::kOdd;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* sQ = smem;
-  uint8_t* sKV = sQ + Sh::kQTiles * Sh::kQTile;
+  uint8_t *sK = sQ + Sh::kQTiles * Sh::kQTile, *sV = sK + Sh::kKeySlots * Sh::kSlot;
   TreeBars<D>& bars = *reinterpret_cast<TreeBars<D>*>(smem + Sh::kTiles);
   const int warp = warp_index(), lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     mbar_init(&bars.q_full, 1);
-    mbar_init(&bars.q_empty, 1);
-    for (int i = 0; i < kRing; ++i) {
-      mbar_init(&bars.kv_full[i], 1);
-      mbar_init(&bars.kv_empty[i], 1);
+    // What the issuers share they both take and both give back, tiles of the other warpgroup's too: a wait for one parity of a barrier is good for the
+    // phase after the last one that the waiter has seen, and for no other. (Wide: one issuer gives back twice.)
+    mbar_init(&bars.q_empty, 2);
+    for (int i = 0; i < Sh::kKeySlots; ++i) {
+      mbar_init(&bars.k_full[i], 1);
+      mbar_init(&bars.k_empty[i], 2);
+    }
+    for (int i = 0; i < Sh::kValueSlots; ++i) {
+      mbar_init(&bars.v_full[i], 1);
+      mbar_init(&bars.v_empty[i], 2);
     }
     for (int t = 0; t < 2; ++t) {
-      mbar_init(&bars.s_full[t], 1);
-      mbar_init(&bars.p_full[t], Sh::kWide ? 8 : 4);
+      for (int b = 0; b < 2; ++b) {
+        mbar_init(&bars.s_full[t][b], 1);
+        mbar_init(&bars.p_full[t][b], Sh::kWide ? 8 : 4);
+      }
+      mbar_init(&bars.pv_done[t], 1);
+      mbar_init(&bars.drained[t], 1);
     }
-    mbar_init(&bars.o_full, 1);
-    mbar_init(&bars.o_free, 8);
-    mbar_init(&bars.pv_done, 1);
+    mbar_init(&bars.o_full, 2);
     mbar_init(&bars.meet, 8);
+    for (int i = 0; i < kTreePieces; ++i) {
+      mbar_init(&bars.piece_full[i], 1);
+      mbar_init(&bars.piece_empty[i], 11);
+    }
     mbar_fence_init();
     bars.odd_any = 0;
+    bars.cut.first = -1;
     tma_prefetch_desc(&tmQ);
     tma_prefetch_desc(&tmKV);
   }
-  if (threadIdx.x < kOdd * kWords) bars.odd[threadIdx.x / kWords][threadIdx.x % kWords] = 0;
-  if (warp == 1) {
+  if (threadIdx.x < kOdd * 2) bars.odd[threadIdx.x >> 1][threadIdx.x & 1] = 0;
+  if (warp == 10) {
     tmem_alloc(&bars.tmem_base, 512);
     tmem_relinquish();
   }
@@ -268,18 +361,37 @@ __global__ void __launch_bounds__(kTreeThreads, 1)
     }
   }
   __syncthreads();
-  TreeWalk<D> walk(p, lo < hi ? bars.start_req : 0, lo < hi ? bars.start_off : 0, hi - lo);
-  TreePiece w;
 
-  if (warp == 0) {
-    // ---------------- TMA ----------------
-    const int page_rows = min(p.block_size, kKeys), loads = kKeys / page_rows;       // pages of a tile (at most 16): a lane each
-    uint32_t load = 0, piece = 0;                                                    // of the ring; of the stretch
+  if (warp == 8) {
+    // ---------------- pieces, queries and keys ----------------
+    TreeWalk<D> walk(p, lo < hi ? bars.start_req : 0, lo < hi ? bars.start_off : 0, hi - lo);
+    TreeSlot<Sh::kKeySlots> slot;
+    uint32_t queries = 0;
     bool ok = true;
-    for (; ok && walk.next(w); ++piece) {
-      const TreeReq& r = walk.r;
+    for (uint32_t piece = 0; ok; ++piece) {
+      TreePiece w;
+      int jb = 0;
+      const bool more = walk.next(w, jb);
+      if (!more) w.nt = 0;
+      const int at = piece % kTreePieces;
+      if (piece >= kTreePieces && !(ok = mbar_wait_warp(&bars.piece_empty[at], (piece / kTreePieces - 1) & 1, p.status))) break;
+      if (lane == 0) {
+        bars.piece[at] = w;
+        if (more && w.cut && jb + w.nt == walk.r.tiles) {
+          // the last part of an item that began in the stretch of another CTA: of the one that has the line's cell of its first tile
+          bars.cut.first = (int)((lo - jb) / stretch);
+          bars.cut.row0 = w.row0 + w.node0;
+          bars.cut.head = w.head;
+          bars.cut.rows = min(w.n - w.node0, p.nodes * (w.two ? 2 : 1)) * p.G;
+        }
+        mbar_arrive(&bars.piece_full[at]);
+      }
+      __syncwarp();
+      if (!more) break;
+      TreePages pages(p, w, 0);
       if (piece > 0 && !(ok = mbar_wait_warp(&bars.q_empty, (piece - 1) & 1, p.status))) break;
-      const int row = r.row0 + w.node0, tiles = w.two ? 2 : 1;
+      const int row = w.row0 + w.node0, tiles = w.two ? 2 : 1;
+      ++queries;
       if (lane == 0) mbar_expect_tx(&bars.q_full, tiles * Sh::kParts * p.nodes * p.G * 128);
       __syncwarp();
       if (lane < tiles * Sh::kParts) {
@@ -287,323 +399,289 @@ __global__ void __launch_bounds__(kTreeThreads, 1)
         tma_load_3d(sQ + t * Sh::kQTile + part * 16384, &tmQ, &bars.q_full, part * 64, w.head * p.G, row + t * p.nodes);
       }
       __syncwarp();
-      const int32_t* bt = p.block_table + walk.b * p.ldt;
-      const int last_page = max(0, (r.len - 1) / p.block_size);
-      const int nt = w.je - w.jb, first_key = (r.begin + w.jb) * kKeys;
-      // entries of the table, 32 at a time, the next ones on their way
-      int base = first_key / p.block_size, now = bt[min(base + lane, last_page)], next = bt[min(base + 32 + lane, last_page)];
-      long long k_row = 0, v_row = 0;
-      const auto fetch = [&](int kv, int j) {
-        const int key = first_key + j * kKeys, page = key / p.block_size;
-        if (kv == 0) {
-          if (page >= base + 32) {
-            base += 32;
-            now = next;
-            next = bt[min(base + 32 + lane, last_page)];
-          }
-          v_row = k_row;
-          // (a tile's pages do not pass a multiple of 32 entries from the piece's first: they may begin anywhere in it)
-          const int want = page - base + (p.block_size < kKeys ? lane : 0);
-          const int e0 = __shfl_sync(0xffffffffu, now, want & 31), e1 = __shfl_sync(0xffffffffu, next, want & 31);
-          const int blk = want < 32 ? e0 : e1;
-          k_row = (blk < 0 || blk >= p.num_blocks ? p.num_blocks : (long long)blk) * 2 * p.block_size + key % p.block_size;
-        }
-        const int sl = load % kRing;
-        if (!mbar_wait_warp(&bars.kv_empty[sl], ((load / kRing) & 1) ^ 1, p.status)) return false;
-        if (lane == 0) mbar_expect_tx(&bars.kv_full[sl], Sh::kSlot);
+      for (int j = 0; j < w.nt; ++j, slot.next()) {
+        if (!(ok = mbar_wait_warp(&bars.k_empty[slot.at], slot.parity ^ 1, p.status))) break;
+        if (elect_one()) mbar_expect_tx(&bars.k_full[slot.at], Sh::kSlot);
         __syncwarp();
-        if (lane < loads) {
-          uint8_t* dst = sKV + sl * Sh::kSlot + lane * page_rows * 128;
-          // (of the tile that K is at; V of the tile before it, where K is one ahead)
-          const long long at = kv == 0 ? k_row : (w.two || j == nt - 1 ? k_row : v_row) + p.block_size;
-#pragma unroll
-          for (int d = 0; d < Sh::kParts; ++d) tma_load_3d(dst + d * Sh::kPiece, &tmKV, &bars.kv_full[sl], d * 64, w.head, (int)at);
-        }
-        __syncwarp();
-        ++load;
-        return true;
-      };
-      if (w.two) {
-        for (int j = 0; ok && j < nt; ++j) ok = fetch(0, j) && fetch(1, j);
-      } else {
-        ok = fetch(0, 0);
-        for (int j = 0; ok && j < nt; ++j) {
-          if (j + 1 < nt) ok = fetch(0, j + 1);
-          ok = ok && fetch(1, j);
-        }
+        pages.load<D>(sK + slot.at * Sh::kSlot, &tmKV, &bars.k_full[slot.at], w.head);
       }
     }
-  } else if (warp == 1) {
-    // ---------------- MMA ----------------
-    constexpr uint32_t idesc_qk = umma_idesc_bf16(128, kKeys, 0, 0), idesc_pv = umma_idesc_bf16(128, D, 0, 1);
-    const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0), q_addr = smem_u32(sQ);
-    uint32_t load0 = 0, piece = 0, made[2] = {0, 0};               // tiles of P seen, of either half
+    if (!ok) {
+      slot.drain(bars.k_full, p.status);
+      if (queries) mbar_wait_warp(&bars.q_full, (queries - 1) & 1, p.status);
+    }
+  } else if (warp == 9) {
+    // ---------------- values ----------------
+    TreeSlot<Sh::kValueSlots> slot;
     bool ok = true;
-    const auto full = [&](uint32_t i) { return mbar_wait_warp(&bars.kv_full[i % kRing], (i / kRing) & 1, p.status); };
-    const auto qk = [&](int t, int qt, uint32_t i, bool release, bool last) {
-      const uint32_t k_addr = smem_u32(sKV + (i % kRing) * Sh::kSlot), q = q_addr + qt * Sh::kQTile;
-      if (elect_one()) {
-#pragma unroll
-        for (int kk = 0; kk < D / 16; ++kk)
-          umma_bf16_ss(tm + t * Sh::kSCols, umma_desc_k_sw128(q + (kk / 4) * 16384 + (kk % 4) * 32, 1024),
-                       umma_desc_k_sw128(k_addr + (kk / 4) * Sh::kPiece + (kk % 4) * 32, 1024), idesc_qk, kk != 0);
-        umma_commit(&bars.s_full[t]);
-        if (release) umma_commit(&bars.kv_empty[i % kRing]);
-        if (last) umma_commit(&bars.q_empty);
-      }
+    for (uint32_t piece = 0; ok; ++piece) {
+      const int at = piece % kTreePieces;
+      if (!(ok = mbar_wait_warp(&bars.piece_full[at], (piece / kTreePieces) & 1, p.status))) break;
+      const TreePiece w = bars.piece[at];
       __syncwarp();
-    };
-    const auto pv = [&](int t, uint32_t i, bool add, bool release, bool last) {
-      const uint64_t vd = umma_desc_mn_sw128(smem_u32(sKV + (i % kRing) * Sh::kSlot), Sh::kPiece, 1024);
-      const uint32_t p_at = Sh::kWide ? tm + Sh::kP + t * 32 : tm + t * Sh::kSCols, o_at = Sh::kWide ? tm + Sh::kO : tm + Sh::kO + t * D;
-      if (elect_one()) {
-#pragma unroll
-        for (int kk = 0; kk < kKeys / 16; ++kk) umma_bf16_ts(o_at, p_at + kk * 8, vd + kk * (2048 >> 4), idesc_pv, add || kk != 0);
-        if (release) umma_commit(&bars.kv_empty[i % kRing]);
-        if (Sh::kWide) umma_commit(&bars.pv_done);
-        if (last) umma_commit(&bars.o_full);
+      if (lane == 0) mbar_arrive(&bars.piece_empty[at]);
+      if (w.nt == 0) break;
+      TreePages pages(p, w, 1);
+      for (int j = 0; j < w.nt; ++j, slot.next()) {
+        if (!(ok = mbar_wait_warp(&bars.v_empty[slot.at], slot.parity ^ 1, p.status))) break;
+        if (elect_one()) mbar_expect_tx(&bars.v_full[slot.at], Sh::kSlot);
+        __syncwarp();
+        pages.load<D>(sV + slot.at * Sh::kSlot, &tmKV, &bars.v_full[slot.at], w.head);
       }
+    }
+    if (!ok) slot.drain(bars.v_full, p.status);
+  } else if (warp >= 10) {
+    // ---------------- MMA of warpgroup t ----------------
+    constexpr uint32_t idesc_qk = umma_idesc_bf16(128, K, 0, 0), idesc_pv = umma_idesc_bf16(128, D, 0, 1);
+    // Descriptors of the first operand tiles; the others' lie a constant further (their addresses, in 16 bytes, are the lowest bits).
+    const int t = warp - 10;
+    const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
+    const uint64_t q_desc = umma_desc_k_sw128(smem_u32(sQ), 1024), k_desc = umma_desc_k_sw128(smem_u32(sK), 1024);
+    const uint64_t v_desc = umma_desc_mn_sw128(smem_u32(sV), Sh::kPiece, 1024);
+    TreeSlot<Sh::kKeySlots> ks;
+    TreeSlot<Sh::kValueSlots> vs;
+    uint32_t c_k = 0, c_v = 0;         // tiles of this warpgroup: scores issued, products issued
+    bool ok = true;
+    for (uint32_t piece = 0; ok; ++piece) {
+      const int at = piece % kTreePieces;
+      if (!(ok = mbar_wait_warp(&bars.piece_full[at], (piece / kTreePieces) & 1, p.status))) break;
+      const int nt = __shfl_sync(0xffffffffu, bars.piece[at].nt, 0);
+      const bool two = __shfl_sync(0xffffffffu, (int)bars.piece[at].two, 0) != 0;
       __syncwarp();
-    };
-    for (; ok && walk.next(w); ++piece) {
-      const int nt = w.je - w.jb;
+      if (lane == 0) mbar_arrive(&bars.piece_empty[at]);
+      if (nt == 0) break;
+      if (Sh::kWide && t == 1) continue;                           // (there is one accumulator: the other warp has it all)
+      const bool both = Sh::kWide || two;                          // every tile for every warpgroup
+      const int ahead = both ? 2 : 4, last = both ? nt - 1 : nt - 1 - ((nt - 1 - t) & 1);          // this warpgroup's last tile (below 0: none)
       if (!(ok = mbar_wait_warp(&bars.q_full, piece & 1, p.status))) break;
-      if (w.two) {                     // tile j: K at 2 j, V at 2 j + 1, for both tiles of rows
-        if (!(ok = full(load0))) break;
-        tc_fence_after_sync();
-        qk(0, 0, load0, false, false);
-        qk(1, 1, load0, true, nt == 1);
-        for (int j = 0; ok && j < nt; ++j) {
-          const uint32_t v = load0 + 2 * j + 1;
-          if (!(ok = full(v))) break;
+      if (last < 0) {                  // (for this piece's output, not for one before it that the other issuer is still at)
+        if (lane == 0) mbar_arrive(&bars.q_empty);
+        if (piece > 0 && !(ok = mbar_wait_warp(&bars.o_full, (piece - 1) & 1, p.status))) break;
+        if (lane == 0) mbar_arrive(&bars.o_full);
+      }
+      const uint64_t q = q_desc + (two ? t : 0) * (Sh::kQTile >> 4);
+      const auto qk = [&](int j) {     // scores of tile j
+        if (!mbar_wait_warp(&bars.k_full[ks.at], ks.parity, p.status)) return false;
+        if (both || (j & 1) == t) {
+          tc_fence_after_sync();
+          const uint64_t k = k_desc + ks.at * (Sh::kSlot >> 4);
+          const uint32_t buf = c_k & 1, s_at = tm + (t * 2 + buf) * K;
+          if (elect_one()) {
 #pragma unroll
-          for (int t = 0; t < 2; ++t) {
-            if (!(ok = mbar_wait_warp(&bars.p_full[t], made[t] & 1, p.status))) break;
-            ++made[t];
-            if (j == 0 && t == 0 && piece > 0 && !(ok = mbar_wait_warp(&bars.o_free, (piece - 1) & 1, p.status))) break;
-            tc_fence_after_sync();
-            pv(t, v, j > 0, t == 1, t == 1 && j == nt - 1);
-            if (j + 1 < nt) {
-              if (t == 0) {
-                if (!(ok = full(v + 1))) break;
-                tc_fence_after_sync();
-              }
-              qk(t, t, v + 1, t == 1, t == 1 && j + 2 == nt);
+            for (int kk = 0; kk < D / 16; ++kk)
+              umma_bf16_ss(s_at, q + (((kk / 4) * 16384 + (kk % 4) * 32) >> 4), k + (((kk / 4) * Sh::kPiece + (kk % 4) * 32) >> 4), idesc_qk, kk != 0);
+            umma_commit(&bars.s_full[t][buf]);
+            umma_commit(&bars.k_empty[ks.at]);
+            if (j == last) umma_commit(&bars.q_empty);
+            if (Sh::kWide) {
+              umma_commit(&bars.k_empty[ks.at]);
+              if (j == last) umma_commit(&bars.q_empty);
             }
           }
+          ++c_k;
+        } else if (lane == 0) {
+          mbar_arrive(&bars.k_empty[ks.at]);
         }
-      } else {                         // K0 K1 V0 K2 V1 .. V(nt - 1)
-        const auto k_at = [&](int j) { return load0 + (j == 0 ? 0 : 2 * j - 1); };
-        for (int j = 0; ok && j < min(2, nt); ++j) {
-          if (!(ok = full(k_at(j)))) break;
+        __syncwarp();
+        ks.next();
+        return true;
+      };
+      for (int j = 0; ok && j < min(ahead, nt); ++j) ok = qk(j);
+      for (int j = 0; ok && j < nt; ++j, vs.next()) {
+        if (!(ok = mbar_wait_warp(&bars.v_full[vs.at], vs.parity, p.status))) break;
+        if (both || (j & 1) == t) {
+          const uint32_t buf = c_v & 1;
+          if (!(ok = mbar_wait_warp(&bars.p_full[t][buf], c_v >> 1 & 1, p.status))) break;
+          const bool first = j < (both ? 1 : 2);                   // (the accumulator is free: the weights come from warps that have met at the last output's end)
           tc_fence_after_sync();
-          qk(j, 0, k_at(j), true, j + 1 == nt);
-        }
-        for (int j = 0; ok && j < nt; ++j) {
-          const int t = j & 1;
-          const uint32_t v = load0 + (j == nt - 1 ? 2 * nt - 1 : 2 * j + 2);
-          if (!(ok = full(v))) break;
-          if (!(ok = mbar_wait_warp(&bars.p_full[t], made[t] & 1, p.status))) break;
-          ++made[t];
-          if (j == 0 && piece > 0 && !(ok = mbar_wait_warp(&bars.o_free, (piece - 1) & 1, p.status))) break;
-          tc_fence_after_sync();
-          pv(t, v, Sh::kWide ? j > 0 : j > 1, true, j == nt - 1);
-          if (j + 2 < nt) {
-            if (!(ok = full(k_at(j + 2)))) break;
-            tc_fence_after_sync();
-            qk(t, 0, k_at(j + 2), true, j + 3 == nt);
+          const uint64_t v = v_desc + vs.at * (Sh::kSlot >> 4);
+          const uint32_t p_at = Sh::kWide ? tm + Sh::kP + buf * 32 : tm + (t * 2 + buf) * K, o_at = tm + Sh::kO + t * D;
+          if (elect_one()) {
+#pragma unroll
+            for (int kk = 0; kk < K / 16; ++kk) umma_bf16_ts(o_at, p_at + kk * 8, v + kk * (2048 >> 4), idesc_pv, !first || kk != 0);
+            umma_commit(&bars.v_empty[vs.at]);
+            umma_commit(&bars.pv_done[t]);
+            if (j == last) umma_commit(&bars.o_full);
+            if (Sh::kWide) {
+              umma_commit(&bars.v_empty[vs.at]);
+              if (j == last) umma_commit(&bars.o_full);
+            }
           }
+          ++c_v;
+        } else if (lane == 0) {
+          mbar_arrive(&bars.v_empty[vs.at]);
         }
+        __syncwarp();
+        if (j + ahead < nt) ok = qk(j + ahead);                    // (the tile after this warpgroup's next: the same buffer)
       }
-      load0 += 2 * nt;
+    }
+    if (!ok) {                         // a wait ran out: nothing of this issuer's is under way when the CTA ends
+      if (elect_one()) umma_commit(&bars.drained[t]);
+      __syncwarp();
+      mbar_wait_warp(&bars.drained[t], 0, p.status);
     }
   } else {
     // ---------------- softmax and output: a thread a row (two where it is wide) ----------------
-    const int half = (warp - 2) >> 2, quarter = warp & 3, r = quarter * 32 + lane;
+    const int half = warp >> 2, quarter = warp & 3, r = quarter * 32 + lane, t = Sh::kWide ? 0 : half;
     const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
     const float cap_in = p.cap2 > 0.f ? fminf(2.8853900817779268f / p.cap2, 3.0e38f) : 0.f;
     const int row_node = r / p.G, row_head = r - row_node * p.G;
-    uint32_t load0 = 0, piece = 0, seen_s[2] = {0, 0}, met = 0, pvs = 0;
+    uint32_t tiles0 = 0, piece = 0, made = 0, met = 0;       // tiles of V in the pieces before
     bool ok = true;
-    const auto meet = [&]() {           // both halves
+    const auto meet = [&]() {           // both warpgroups
       __syncwarp();
       if (lane == 0) mbar_arrive(&bars.meet);
       return __all_sync(0xffffffffu, mbar_wait(&bars.meet, met++ & 1, p.status));
     };
-    for (; ok && walk.next(w); ++piece) {
-      const TreeReq rq = walk.r;
-      const int nt = w.je - w.jb;
+    for (;; ++piece) {
+      const int at = piece % kTreePieces;
+      if (!(ok = __all_sync(0xffffffffu, mbar_wait(&bars.piece_full[at], (piece / kTreePieces) & 1, p.status)))) break;
+      const TreePiece w = bars.piece[at];
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bars.piece_empty[at]);
+      if (w.nt == 0) break;
       const int node = w.node0 + (w.two ? half * p.nodes : 0) + row_node;
-      const bool there = row_node < p.nodes && node < rq.n;
-      const uint64_t* bits = p.mask + (size_t)(rq.row0 + (there ? node : 0)) * p.words;
+      const bool there = row_node < p.nodes && node < w.n;
+      const bool idle = !__any_sync(0xffffffffu, there);               // (its rows may hold anything: no other warp reads them)
+      const uint64_t* bits = p.mask + (size_t)(w.row0 + (there ? node : 0)) * p.words;
       int low = 0;
       if (p.window > 0 && there) {     // (a node lies at most n - 1 positions behind the root)
-        const long long depth = p.positions[rq.row0 + node] - rq.ctx;
-        low = min(rq.ctx, rq.ctx + (int)min(max(depth, 0ll), (long long)rq.n - 1) - p.window + 1);
+        const long long depth = p.positions[w.row0 + node] - w.ctx;
+        low = min(w.ctx, w.ctx + (int)min(max(depth, 0ll), (long long)w.n - 1) - p.window + 1);
       }
-      const auto seen_word = [&](int key) { return there ? tree_seen(bits, p.words, key, rq.ctx, rq.len, low) : 0u; };
-      // (the first positions that the nodes of the piece see differ by as much as their positions do)
+      const auto seen_word = [&](int key) { return there ? tree_seen(bits, p.words, key, w.ctx, w.len, low) : 0u; };
       const int low_most = p.window > 0 ? __reduce_max_sync(0xffffffffu, there ? low : INT_MIN) : 0;
       float m = -INFINITY, l = 0.f;
       int odd_n = 0;
-      // tiles of this half
-      const int step = Sh::kWide || w.two ? 1 : 2;
-      for (int j = step == 2 ? half : 0; j < nt; j += step) {
-        const int t = Sh::kWide ? j & 1 : half, kbase = (rq.begin + w.jb + j) * kKeys;
+      const bool both = Sh::kWide || w.two;
+      const int mine = both ? w.nt : (w.nt + 1 - half) / 2;            // tiles of this warpgroup
+      for (int i = 0; i < mine; ++i) {
+        const int j = both ? i : 2 * i + half, kbase = w.key0 + j * K;
+        const uint32_t c = made + i, buf = c & 1;
         // tiles in which the nodes of the request may differ in what they see (need_mask: those of this warp do)
-        const bool odd_tile = kbase + kKeys > rq.ctx || (p.window > 0 && kbase < rq.ctx - p.window + rq.n);
-        const bool need_mask = kbase + kKeys > rq.ctx || kbase < low_most;
-        if (odd_tile && (step == 2 || half == 0)) {
-          // values that are not finite: out of the tile, and noted
-          const uint32_t v = load0 + (w.two ? 2 * j + 1 : j == nt - 1 ? 2 * nt - 1 : 2 * j + 2);
-          ok = __all_sync(0xffffffffu, mbar_wait(&bars.kv_full[v % kRing], (v / kRing) & 1, p.status));
-          if (!ok) break;
-          const int key = Sh::kWide ? r & 63 : r, d0 = Sh::kWide ? (r >> 6) * 2 : 0;
-          uint8_t* row = sKV + (v % kRing) * Sh::kSlot + key * 128;
+        const bool odd_tile = kbase + K > w.ctx || (p.window > 0 && kbase < w.ctx - p.window + w.n);
+        const bool need_mask = kbase + K > w.ctx || kbase < low_most;
+        uint32_t seen[2] = {0xffffffffu, 0xffffffffu};
+        if (need_mask) {
+          seen[0] = seen_word(kbase);
+          seen[1] = seen_word(kbase + 32);
+        }
+        if (!(ok = __all_sync(0xffffffffu, mbar_wait(&bars.s_full[t][buf], c >> 1 & 1, p.status)))) break;
+        if (!idle) {
+          tc_fence_after_sync();
+          const uint32_t s_addr = tmem + (t * 2 + buf) * K + lanes;
+          uint32_t s[64];
+          tmem_ld_32x32b_x32(s_addr, s);
+          tmem_ld_32x32b_x32(s_addr + 32, s + 32);
+          tmem_ld_wait();
+          float sc = p.scale_log2;
+          if (p.cap2 > 0.f) {
+#pragma unroll
+            for (int e = 0; e < 64; ++e) s[e] = __float_as_uint(tree_capped(__uint_as_float(s[e]) * sc, p.cap2, cap_in));
+            sc = 1.f;
+          }
+          if (need_mask) {
+#pragma unroll
+            for (int e = 0; e < 64; ++e)
+              if (!(seen[e >> 5] >> (e & 31) & 1)) s[e] = 0xff800000u;       // -inf
+          }
+          float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+          for (int e = 0; e < 64; e += 4)
+#pragma unroll
+            for (int g = 0; g < 4; ++g) mx[g] = fmaxf(mx[g], __uint_as_float(s[e + g]));
+          // m: reference of the row's maximum, raised lazily (by more than 2^8), so that the accumulator is rescaled rarely; P stays below 256
+          const float tile_max = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * sc;
+          float alpha = 1.f;
+          bool rescale = false;
+          if (tile_max > m + 8.f) {    // also the first finite tile: m == -inf
+            if (m != -INFINITY) {
+              alpha = tree_ex2(m - tile_max);
+              rescale = true;
+            }
+            m = tile_max;
+          }
+          const float m_use = m == -INFINITY ? 0.f : m;
+          if (__any_sync(0xffffffffu, rescale)) {
+            // the product of the tile before may be under way (its successor waits for this tile's weights)
+            if (!(ok = __all_sync(0xffffffffu, mbar_wait(&bars.pv_done[t], (c - 1) & 1, p.status)))) break;
+            tc_fence_after_sync();
+            constexpr int cols = Sh::kWide ? D / 2 : D;
+            const uint32_t o_addr = tmem + Sh::kO + half * cols + lanes;
+#pragma unroll 1
+            for (int x = 0; x < cols / 16; ++x) {
+              uint32_t rr[16];
+              tmem_ld_32x32b_x16(o_addr + x * 16, rr);
+              tmem_ld_wait();
+#pragma unroll
+              for (int e = 0; e < 16; ++e) rr[e] = __float_as_uint(__uint_as_float(rr[e]) * alpha);
+              tmem_st_32x32b_x16(o_addr + x * 16, rr);
+            }
+          }
+          // The sum is that of the rounded values: a row's weights add up to one, and a single key's value comes out as it is.
+          const uint64_t sc2 = pack_f32x2(sc, sc), off2 = pack_f32x2(-m_use, -m_use);
+          uint64_t sum2[2] = {0, 0};
+          constexpr int kMine = Sh::kWide ? 32 : 64;
+          uint32_t pk[kMine / 2];
+#pragma unroll
+          for (int e = 0; e < kMine / 2; ++e) {
+            const uint32_t x0 = Sh::kWide && half ? s[(32 + 2 * e) & 63] : s[2 * e], x1 = Sh::kWide && half ? s[(33 + 2 * e) & 63] : s[2 * e + 1];
+            float a, b;
+            unpack_f32x2(fma_f32x2(pack_b32x2(x0, x1), sc2, off2), a, b);
+            pk[e] = pack_bf16x2(tree_ex2(a), tree_ex2(b));
+            sum2[e & 1] = add_f32x2(sum2[e & 1], pack_b32x2(pk[e] << 16, pk[e] & 0xffff0000u));
+          }
+          if constexpr (Sh::kWide) tmem_st_32x32b_x16(tmem + Sh::kP + buf * 32 + half * 16 + lanes, pk);
+          else tmem_st_32x32b_x32(s_addr, pk);
+          float sum[4];
+          unpack_f32x2(sum2[0], sum[0], sum[1]);
+          unpack_f32x2(sum2[1], sum[2], sum[3]);
+          l = l * alpha + ((sum[0] + sum[1]) + (sum[2] + sum[3]));
+        }
+        if (odd_tile && (!Sh::kWide || half == 0)) {
+          // Values that are not finite: out of the tile, and noted. A thread takes half of a key's dims. (Where both warpgroups take the tile each does all of
+          // it ahead of its own product; they write the same.)
+          const uint32_t v = tiles0 + j;
+          if (!(ok = __all_sync(0xffffffffu, mbar_wait(&bars.v_full[v % Sh::kValueSlots], (v / Sh::kValueSlots) & 1, p.status)))) break;
+          const int key = r & 63;
+          uint8_t* row = sV + (v % Sh::kValueSlots) * Sh::kSlot + key * 128;
           bool odd = false;
 #pragma unroll
-          for (int d = 0; d < (Sh::kWide ? 2 : Sh::kParts); ++d) {
+          for (int x = 0; x < D / 16; ++x) {
+            const int piece16 = (r >> 6) * (D / 16) + x;
+            uint4* at16 = reinterpret_cast<uint4*>(row + (piece16 >> 3) * Sh::kPiece + (((piece16 & 7) ^ (key & 7)) << 4));
+            const uint4 y = *at16;
+            if (odd_bf16x2(y.x) || odd_bf16x2(y.y) || odd_bf16x2(y.z) || odd_bf16x2(y.w)) {
+              uint32_t e[4] = {y.x, y.y, y.z, y.w};
 #pragma unroll
-            for (int c = 0; c < 8; ++c) {
-              uint4* at = reinterpret_cast<uint4*>(row + (d0 + d) * Sh::kPiece + ((c ^ (key & 7)) << 4));
-              const uint4 x = *at;
-              if (odd_bf16x2(x.x) || odd_bf16x2(x.y) || odd_bf16x2(x.z) || odd_bf16x2(x.w)) {
-                uint32_t e[4] = {x.x, x.y, x.z, x.w};
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                  if ((e[i] & 0x7f80u) == 0x7f80u) e[i] &= 0xffff0000u;
-                  if ((e[i] & 0x7f800000u) == 0x7f800000u) e[i] &= 0xffffu;
-                }
-                *at = make_uint4(e[0], e[1], e[2], e[3]);
-                odd = true;
+              for (int g = 0; g < 4; ++g) {
+                if ((e[g] & 0x7f80u) == 0x7f80u) e[g] &= 0xffff0000u;
+                if ((e[g] & 0x7f800000u) == 0x7f800000u) e[g] &= 0xffffu;
               }
+              *at16 = make_uint4(e[0], e[1], e[2], e[3]);
+              odd = true;
             }
           }
           fence_proxy_async_smem();
           const uint32_t who = __ballot_sync(0xffffffffu, odd);
-          if (who) {
-            // (rare: a note in the list that belongs to the half; room for every tile that can be looked at)
-            if (lane == 0) {
-              const int at = (step == 2 ? half * (kOdd / 2) : 0) + odd_n;
-              bars.odd_tile[at] = kbase;
-              atomicOr(&bars.odd[at][Sh::kWide ? quarter & 1 : quarter], who);
-              atomicOr(&bars.odd_any, 1u);
-            }
+          if (who && lane == 0) {      // (rare: a note; room for every tile that can be looked at)
+            const int note = (both ? 0 : half * (kOdd / 2)) + odd_n;
+            bars.odd_tile[note] = kbase;
+            atomicOr(&bars.odd[note][quarter & 1], who);
+            atomicOr(&bars.odd_any, 1u);
           }
           ++odd_n;
         }
-        ok = __all_sync(0xffffffffu, mbar_wait(&bars.s_full[t], seen_s[t] & 1, p.status));
-        if (!ok) break;
-        ++seen_s[t];
-        tc_fence_after_sync();
-        const uint32_t s_addr = tmem + t * Sh::kSCols + lanes;
-        // Caps and masks go through tensor memory, 32 scores at a time: the registers of the plain path hold a tile's scores and no more.
-        // (Where it is wide the two threads of a row take a half each and wait for one another.)
-        if (p.cap2 > 0.f || (Sh::kWide ? odd_tile : need_mask)) {
-#pragma unroll 1
-          for (int c = Sh::kWide ? half : 0; c < (Sh::kWide ? half + 1 : kWords); ++c) {
-            uint32_t x[32];
-            tmem_ld_32x32b_x32(s_addr + c * 32, x);
-            const uint32_t seen = need_mask ? seen_word(kbase + 32 * c) : 0xffffffffu;
-            tmem_ld_wait();
-            if (p.cap2 > 0.f) {
-#pragma unroll
-              for (int i = 0; i < 32; ++i) x[i] = __float_as_uint(tree_capped(__uint_as_float(x[i]) * p.scale_log2, p.cap2, cap_in));
-            }
-#pragma unroll
-            for (int i = 0; i < 32; ++i)
-              if (!(seen >> i & 1)) x[i] = 0xff800000u;                    // -inf
-            tmem_st_32x32b_x32(s_addr + c * 32, x);
-          }
-          tmem_st_wait();
-          if (Sh::kWide) {
-            tc_fence_before_sync();
-            if (!(ok = meet())) break;
-            tc_fence_after_sync();
-          }
-        }
-        const float sc = p.cap2 > 0.f ? 1.f : p.scale_log2;
-        // Two passes over the tile, 32 scores at a time with the next on their way.
-        uint32_t s[2][32];
-        tmem_ld_32x32b_x32(s_addr, s[0]);
-        float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-        for (int c = 0; c < kWords; ++c) {
-          tmem_ld_wait_for(s[c & 1]);
-          tmem_ld_32x32b_x32(s_addr + (c + 1 < kWords ? c + 1 : Sh::kWide ? half : 0) * 32, s[(c + 1) & 1]);
-#pragma unroll
-          for (int i = 0; i < 32; i += 4)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) mx[e] = fmaxf(mx[e], __uint_as_float(s[c & 1][i + e]));
-        }
-        tmem_ld_wait_for(s[0]);        // (kWords is even: the second pass begins where the first did)
-        // m: reference of the row's maximum, raised lazily (by more than 2^8), so that the accumulator is rescaled rarely; P stays below 256
-        const float tile_max = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * sc;
-        float alpha = 1.f;
-        bool rescale = false;
-        if (tile_max > m + 8.f) {      // also the first finite tile: m == -inf
-          if (m != -INFINITY) {
-            alpha = tree_ex2(m - tile_max);
-            rescale = true;
-          }
-          m = tile_max;
-        }
-        const float m_use = m == -INFINITY ? 0.f : m;
-        const int first_of_half = step == 2 ? half : 0;
-        if (Sh::kWide) {               // S(j) is issued ahead of P V(j - 1)
-          if (__any_sync(0xffffffffu, rescale) && j > first_of_half) {
-            ok = __all_sync(0xffffffffu, mbar_wait(&bars.pv_done, (pvs - 1) & 1, p.status));
-            if (!ok) break;
-            tc_fence_after_sync();
-          }
-          ++pvs;
-        }
-        // (not wide: the accumulator is at rest, as S(j) is issued right behind P V of the half's tile before it, by the same lane)
-        if (__any_sync(0xffffffffu, rescale) && j > first_of_half) {
-          constexpr int cols = Sh::kWide ? D / 2 : D;
-          const uint32_t o_addr = tmem + Sh::kO + half * cols + lanes;
-#pragma unroll 1
-          for (int c = 0; c < cols / 16; ++c) {
-            uint32_t rr[16];
-            tmem_ld_32x32b_x16(o_addr + c * 16, rr);
-            tmem_ld_wait();
-#pragma unroll
-            for (int i = 0; i < 16; ++i) rr[i] = __float_as_uint(__uint_as_float(rr[i]) * alpha);
-            tmem_st_32x32b_x16(o_addr + c * 16, rr);
-          }
-        }
-        // The sum is that of the rounded values: a row's weights add up to one, and a single key's value comes out as it is.
-        const uint64_t sc2 = pack_f32x2(sc, sc), off2 = pack_f32x2(-m_use, -m_use);
-        uint64_t sum2[2] = {0, 0};
-        constexpr int n32 = Sh::kWide ? 1 : kKeys / 32;
-#pragma unroll
-        for (int c = 0; c < n32; ++c) {
-          if (c > 0) tmem_ld_wait_for(s[c & 1]);
-          if (c + 1 < n32) tmem_ld_32x32b_x32(s_addr + (c + 1) * 32, s[(c + 1) & 1]);
-          uint32_t pk[16];
-#pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            float a, b;
-            unpack_f32x2(fma_f32x2(pack_b32x2(s[c & 1][2 * i], s[c & 1][2 * i + 1]), sc2, off2), a, b);
-            pk[i] = pack_bf16x2(tree_ex2(a), tree_ex2(b));
-            sum2[i & 1] = add_f32x2(sum2[i & 1], pack_b32x2(pk[i] << 16, pk[i] & 0xffff0000u));
-          }
-          // (over scores that both passes have read)
-          tmem_st_32x32b_x16((Sh::kWide ? tmem + Sh::kP + t * 32 + half * 16 + lanes : s_addr + c * 16), pk);
-        }
-        float sum[4];
-        unpack_f32x2(sum2[0], sum[0], sum[1]);
-        unpack_f32x2(sum2[1], sum[2], sum[3]);
-        l = l * alpha + ((sum[0] + sum[1]) + (sum[2] + sum[3]));
         tmem_st_wait();
         tc_fence_before_sync();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&bars.p_full[t]);
+        if (lane == 0) mbar_arrive(&bars.p_full[t][buf]);
       }
-      load0 += 2 * nt;
       if (!ok) break;
+      tiles0 += w.nt;
+      made += mine;
       // ---- output
-      const bool whole = w.jb == 0 && w.je == rq.tiles, other = step == 2 && nt > 1;       // other: both halves have a share of every row
+      const bool other = !both && w.nt > 1;            // both warpgroups have a share of every row
       if (!w.two && half == 1) {
         bars.rows[0][r] = m;
         bars.rows[1][r] = l;
@@ -623,7 +701,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1)
             a1 = m1 == -INFINITY ? 1.f : tree_ex2(m1 - m);
             l = l * a0 + l1 * a1;
           }
-          if (whole) {
+          if (w.whole) {
             const float inv = l != 0.f ? 1.f / l : 0.f;
             a0 *= inv;
             a1 *= inv;
@@ -634,162 +712,132 @@ __global__ void __launch_bounds__(kTreeThreads, 1)
         if (!(ok = meet())) break;
         a0 = bars.rows[0][r];
         a1 = bars.rows[1][r];
-      } else if (whole) {
+      } else if (w.whole) {
         a0 = l != 0.f ? 1.f / l : 0.f;
       }
       if (!(ok = __all_sync(0xffffffffu, mbar_wait(&bars.o_full, piece & 1, p.status)))) break;
       tc_fence_after_sync();
-      // columns of this thread's: all of its row's, or one half of them
-      constexpr int kHalfCols = D / 2;
-      const int col0 = w.two ? 0 : half * kHalfCols, cols = w.two ? D : kHalfCols;
-      const int part_row = w.two ? half * 128 + r : r;
-      const uint32_t o_addr = tmem + Sh::kO + lanes + (w.two ? half * D : 0);
-      __nv_bfloat16* dst = p.out + (rq.row0 + node) * p.ldo + (w.head * p.G + row_head) * D;
-      float* part = p.parts + (2 * blockIdx.x + (w.jb > 0 ? 0 : 1)) * Sh::kPartFloats;
       const bool odd_any = *(volatile uint32_t*)&bars.odd_any != 0;
+      if (!idle) {
+        // columns of this thread's: all of its row's, or one half of them
+        constexpr int kHalfCols = D / 2;
+        const int col0 = w.two ? 0 : half * kHalfCols, cols = w.two ? D : kHalfCols;
+        const int part_row = w.two ? half * 128 + r : r;
+        const uint32_t o_addr = tmem + Sh::kO + lanes + (w.two ? half * D : 0);
+        __nv_bfloat16* dst = p.out + (w.row0 + node) * p.ldo + (w.head * p.G + row_head) * D;
+        float* part = p.parts + (2 * blockIdx.x + (w.cut ? 0 : 1)) * Sh::kPartFloats;
 #pragma unroll 1
-      for (int c = 0; c < cols; c += 32) {
-        uint32_t rr[32], r1[32];
-        tmem_ld_32x32b_x32(o_addr + col0 + c, rr);
-        if (other) tmem_ld_32x32b_x32(o_addr + D + col0 + c, r1);
-        tmem_ld_wait();
+        for (int x = 0; x < cols; x += 32) {
+          uint32_t rr[32], r1[32];
+          tmem_ld_32x32b_x32(o_addr + col0 + x, rr);
+          if (other) tmem_ld_32x32b_x32(o_addr + D + col0 + x, r1);
+          tmem_ld_wait();
 #pragma unroll
-        for (int i = 0; i < 32; ++i) {
-          const float o = __uint_as_float(rr[i]) * a0;
-          rr[i] = __float_as_uint(other ? fmaf(__uint_as_float(r1[i]), a1, o) : o);
-        }
-        if (odd_any && there) {
-          for (int e = 0; e < kOdd; ++e) {
-            for (int q = 0; q < kWords; ++q) {
-              uint32_t who = bars.odd[e][q];
-              if (who == 0) continue;
-              who &= seen_word(bars.odd_tile[e] + 32 * q);
-              while (who) {
-                const int key = bars.odd_tile[e] + 32 * q + __ffs(who) - 1;
-                who &= who - 1;
-                const int blk = p.block_table[walk.b * p.ldt + key / p.block_size];
-                if (blk < 0 || blk >= p.num_blocks) continue;
-                const __nv_bfloat16* v = p.cache + ((((long long)blk * 2 + 1) * p.block_size + key % p.block_size) * p.Hkv + w.head) * D + col0 + c;
+          for (int e = 0; e < 32; ++e) {
+            const float o = __uint_as_float(rr[e]) * a0;
+            rr[e] = __float_as_uint(other ? fmaf(__uint_as_float(r1[e]), a1, o) : o);
+          }
+          if (odd_any && there) {
+            for (int note = 0; note < kOdd; ++note) {
+              for (int q = 0; q < 2; ++q) {
+                uint32_t who = bars.odd[note][q];
+                if (who == 0) continue;
+                who &= seen_word(bars.odd_tile[note] + 32 * q);
+                while (who) {
+                  const int key = bars.odd_tile[note] + 32 * q + __ffs(who) - 1;
+                  who &= who - 1;
+                  const int blk = p.block_table[w.b * p.ldt + key / p.block_size];
+                  if (blk < 0 || blk >= p.num_blocks) continue;
+                  const __nv_bfloat16* v = p.cache + ((((long long)blk * 2 + 1) * p.block_size + key % p.block_size) * p.Hkv + w.head) * D + col0 + x;
 #pragma unroll
-                for (int i = 0; i < 32; ++i) {
-                  const float x = __bfloat162float(v[i]);
-                  if (!(fabsf(x) <= 3.4028234e38f)) rr[i] = __float_as_uint(__uint_as_float(rr[i]) + x);
+                  for (int e = 0; e < 32; ++e) {
+                    const float y = __bfloat162float(v[e]);
+                    if (!(fabsf(y) <= 3.4028234e38f)) rr[e] = __float_as_uint(__uint_as_float(rr[e]) + y);
+                  }
                 }
               }
             }
           }
-        }
-        if (there) {
-          if (whole) {
+          if (there) {
+            if (w.whole) {
 #pragma unroll
-            for (int i = 0; i < 32; i += 8) {
-              uint4 o;
-              o.x = pack_bf16x2(__uint_as_float(rr[i + 0]), __uint_as_float(rr[i + 1]));
-              o.y = pack_bf16x2(__uint_as_float(rr[i + 2]), __uint_as_float(rr[i + 3]));
-              o.z = pack_bf16x2(__uint_as_float(rr[i + 4]), __uint_as_float(rr[i + 5]));
-              o.w = pack_bf16x2(__uint_as_float(rr[i + 6]), __uint_as_float(rr[i + 7]));
-              *reinterpret_cast<uint4*>(dst + col0 + c + i) = o;
+              for (int e = 0; e < 32; e += 8) {
+                uint4 o;
+                o.x = pack_bf16x2(__uint_as_float(rr[e + 0]), __uint_as_float(rr[e + 1]));
+                o.y = pack_bf16x2(__uint_as_float(rr[e + 2]), __uint_as_float(rr[e + 3]));
+                o.z = pack_bf16x2(__uint_as_float(rr[e + 4]), __uint_as_float(rr[e + 5]));
+                o.w = pack_bf16x2(__uint_as_float(rr[e + 6]), __uint_as_float(rr[e + 7]));
+                *reinterpret_cast<uint4*>(dst + col0 + x + e) = o;
+              }
+            } else {
+#pragma unroll
+              for (int e = 0; e < 32; e += 4)
+                *reinterpret_cast<uint4*>(part + ((size_t)((col0 + x + e) >> 2) * Sh::kRows + part_row) * 4) = make_uint4(rr[e], rr[e + 1], rr[e + 2], rr[e + 3]);
             }
-          } else {
-#pragma unroll
-            for (int i = 0; i < 32; i += 4)
-              *reinterpret_cast<uint4*>(part + (size_t)part_row * D + col0 + c + i) = make_uint4(rr[i], rr[i + 1], rr[i + 2], rr[i + 3]);
           }
         }
-      }
-      if (!whole && there && (w.two || half == 0)) {
-        part[(size_t)Sh::kRows * D + part_row] = m;
-        part[(size_t)Sh::kRows * D + Sh::kRows + part_row] = l;
+        if (!w.whole && there && (w.two || half == 0)) {
+          part[(size_t)Sh::kRows * D + part_row] = m;
+          part[(size_t)Sh::kRows * D + Sh::kRows + part_row] = l;
+        }
       }
       tc_fence_before_sync();
       if (odd_any) {                   // everyone has read the notes: they go
         if (!(ok = meet())) break;
-        const int i = threadIdx.x - 64;
-        if (i < kOdd * kWords) bars.odd[i / kWords][i % kWords] = 0;
-        if (i == 0) bars.odd_any = 0;
+        const int x = threadIdx.x;
+        if (x < kOdd * 2) bars.odd[x >> 1][x & 1] = 0;
+        if (x == 0) bars.odd_any = 0;
       }
-      // (also keeps what the threads of a row told one another, and the notes, from being written before everyone has read them)
+      // (what the threads of a row told one another, the notes and the accumulators are written anew when everyone has read them)
       if (!(ok = meet())) break;
-      if (lane == 0) mbar_arrive(&bars.o_free);
-      if (threadIdx.x == 64) {
-        TreeCut* cut = reinterpret_cast<TreeCut*>(p.parts + 2 * (long long)gridDim.x * Sh::kPartFloats) + blockIdx.x;
-        if (w.jb > 0 && w.je == rq.tiles) {
-          // the line's cell of the item's first tile says which CTA has its first part
-          const long long first = lo - w.jb;
-          cut->row0 = rq.row0 + w.node0;
-          cut->head = w.head;
-          cut->rows = min(rq.n - w.node0, p.nodes * (w.two ? 2 : 1)) * p.G;
-          cut->first = (int)(first / stretch);
-        } else if (piece == 0) {
-          cut->first = -1;
-        }
-      }
-    }
-    if (piece == 0 && threadIdx.x == 64) {
-      TreeCut* cut = reinterpret_cast<TreeCut*>(p.parts + 2 * (long long)gridDim.x * Sh::kPartFloats) + blockIdx.x;
-      cut->first = -1;
     }
   }
   tc_fence_before_sync();
   __syncthreads();
   tc_fence_after_sync();
-  if (warp == 1) tmem_dealloc(tmem, 512);
+  if (warp == 10) tmem_dealloc(tmem, 512);
+  if (threadIdx.x == 0) reinterpret_cast<TreeCut*>(p.parts + 2 * (long long)gridDim.x * Sh::kPartFloats)[blockIdx.x] = bars.cut;
 }
 
-// Parts of items that the ends of stretches cut. Block (b, y): the item whose last part is CTA b's, rows y, y + 8 .. in eights.
+// Parts of items that the ends of stretches cut. Block (b, y): 32 rows of the item whose last part is CTA b's, a lane a row, a warp every eighth four columns.
 template <int D>
 __global__ void __launch_bounds__(256)
     tree_join_kernel(const float* __restrict__ parts, int ctas, __nv_bfloat16* __restrict__ out, long long ldo, int G, int nodes) {
   using Sh = TreeShape<D>;
-  constexpr int kVec = D / 32;
+  constexpr int kQuads = D / 32;
   pdl_wait();
   const TreeCut cut = reinterpret_cast<const TreeCut*>(parts + 2 * (long long)ctas * Sh::kPartFloats)[blockIdx.x];
   if (cut.first < 0) return;
-  const int lane = threadIdx.x & 31, count = (int)blockIdx.x - cut.first + 1;
-  for (int i = blockIdx.y * 8 + (threadIdx.x >> 5); i < cut.rows; i += gridDim.y * 8) {
-    const int node = i / G, head = i - node * G, tile = node / nodes;
-    const int row = tile * 128 + (node - tile * nodes) * G + head;
-    const auto part = [&](int c) { return parts + (2ll * (cut.first + c) + (c == 0)) * Sh::kPartFloats; };
-    float top = -INFINITY;
-    for (int c = lane; c < count; c += 32) top = fmaxf(top, part(c)[(size_t)Sh::kRows * D + row]);
-    top = warp_max_f32(top);
-    float acc[kVec] = {}, total = 0.f;
-    for (int c0 = 0; c0 < count; c0 += 32) {
-      float weight = 0.f;
-      if (c0 + lane < count) {
-        const float* at = part(c0 + lane) + (size_t)Sh::kRows * D + row;
-        const float m = at[0];
-        weight = m == -INFINITY ? 1.f : tree_ex2(m - top);       // (nothing seen: sums of 0, or of NaN that stay)
-        total += at[Sh::kRows] * weight;
-      }
-      const int n = min(32, count - c0);
+  const int warp = threadIdx.x >> 5, row = blockIdx.y * 32 + (threadIdx.x & 31), count = (int)blockIdx.x - cut.first + 1;
+  const int i = (row >> 7) * nodes * G + (row & 127);          // node-major
+  if ((row & 127) >= nodes * G || i >= cut.rows) return;
+  const auto part = [&](int c) { return parts + (2ll * (cut.first + c) + (c == 0)) * Sh::kPartFloats; };
+  float top = -INFINITY;
 #pragma unroll 4
-      for (int c = 0; c < n; ++c) {
-        const float a = __shfl_sync(0xffffffffu, weight, c);
-        const float* o = part(c0 + c) + (size_t)row * D + lane * kVec;
-        if constexpr (kVec == 2) {
-          const float2 v = *reinterpret_cast<const float2*>(o);
-          acc[0] = fmaf(v.x, a, acc[0]);
-          acc[1] = fmaf(v.y, a, acc[1]);
-        } else {
+  for (int c = 0; c < count; ++c) top = fmaxf(top, part(c)[(size_t)Sh::kRows * D + row]);
+  float4 acc[kQuads] = {};
+  float total = 0.f;
+#pragma unroll 2
+  for (int c = 0; c < count; ++c) {
+    const float* at = part(c);
+    const float m = at[(size_t)Sh::kRows * D + row], l = at[(size_t)Sh::kRows * D + Sh::kRows + row];
+    const float a = m == -INFINITY ? 1.f : tree_ex2(m - top);  // (nothing seen: sums of 0, or of NaN that stay)
+    total = fmaf(l, a, total);
 #pragma unroll
-          for (int k = 0; k < kVec; k += 4) {
-            const float4 v = *reinterpret_cast<const float4*>(o + k);
-            acc[k] = fmaf(v.x, a, acc[k]);
-            acc[k + 1] = fmaf(v.y, a, acc[k + 1]);
-            acc[k + 2] = fmaf(v.z, a, acc[k + 2]);
-            acc[k + 3] = fmaf(v.w, a, acc[k + 3]);
-          }
-        }
-      }
+    for (int k = 0; k < kQuads; ++k) {
+      const float4 v = reinterpret_cast<const float4*>(at)[(size_t)(warp + 8 * k) * Sh::kRows + row];
+      acc[k].x = fmaf(v.x, a, acc[k].x);
+      acc[k].y = fmaf(v.y, a, acc[k].y);
+      acc[k].z = fmaf(v.z, a, acc[k].z);
+      acc[k].w = fmaf(v.w, a, acc[k].w);
     }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
-    const float inv = total != 0.f ? 1.f / total : 0.f;
-    uint32_t* dst = reinterpret_cast<uint32_t*>(out + (cut.row0 + node) * ldo + (cut.head * G + head) * D) + lane * (kVec / 2);
-#pragma unroll
-    for (int k = 0; k < kVec / 2; ++k) dst[k] = pack_bf16x2(acc[2 * k] * inv, acc[2 * k + 1] * inv);
   }
+  const float inv = total != 0.f ? 1.f / total : 0.f;
+  const int node = i / G, head = i - node * G;
+  uint2* dst = reinterpret_cast<uint2*>(out + (cut.row0 + node) * ldo + (cut.head * G + head) * D);
+#pragma unroll
+  for (int k = 0; k < kQuads; ++k)
+    dst[warp + 8 * k] = make_uint2(pack_bf16x2(acc[k].x * inv, acc[k].y * inv), pack_bf16x2(acc[k].z * inv, acc[k].w * inv));
 }
 
 template <int D>
@@ -819,7 +867,7 @@ using namespace b200;
 
 // What a call takes, as far as sizes say: 0, or -1 (shape) or -4 (counted in 31 bits: key tiles of all items of a request).
 extern "C" int b200_tree_attn_takes(const B200TreeAttn* a) {
-  const int D = a->D, keys = D == 256 ? 64 : 128;
+  const int D = a->D, keys = kTreeKeys;
   if (D != 64 && D != 128 && D != 256) return -1;
   if (a->Hkv <= 0 || a->Hq <= 0 || a->Hq % a->Hkv || a->Hq / a->Hkv > 128 || a->words <= 0 || a->max_blocks <= 0) return -1;
   const int bs = a->block_size;
@@ -841,7 +889,7 @@ extern "C" int b200_tree_attn(const B200TreeAttn* a, cudaStream_t stream) {
   const int rc = b200_tree_attn_takes(a);
   if (rc) return rc;
   if (a->num_reqs <= 0 || a->total_q <= 0) return 0;
-  const int D = a->D, keys = D == 256 ? 64 : 128, G = a->Hq / a->Hkv, bs = a->block_size;
+  const int D = a->D, keys = kTreeKeys, G = a->Hq / a->Hkv, bs = a->block_size;
   TreeParams p;
   p.cache = (const __nv_bfloat16*)a->cache; p.out = (__nv_bfloat16*)a->out; p.ldo = a->ldo;
   p.block_table = (const int32_t*)a->block_table; p.ldt = a->ldt; p.num_blocks = a->num_blocks; p.max_blocks = a->max_blocks;

@@ -218,9 +218,9 @@ def test_sizes_that_the_attention_takes():
         for k, v in dict(dict(D=128, Hq=32, Hkv=8, block_size=32, max_blocks=4000, num_blocks=100000, num_reqs=64, total_q=2048, words=1), **more).items():
             setattr(a, k, v)
         return _lib.lib().b200_tree_attn_takes(ctypes.byref(a))
-    assert takes() == 0 and takes(words=16, total_q=65536, num_reqs=8192) == 0 and takes(D=256, block_size=64) == 0
+    assert takes() == 0 and takes(block_size=192) == 0 and takes(words=16, total_q=65536, num_reqs=8192) == 0 and takes(D=256, block_size=64) == 0
     for wrong in (dict(D=96), dict(Hq=30), dict(Hq=129, Hkv=1), dict(block_size=12), dict(block_size=48), dict(block_size=4), dict(words=0),
-                  dict(D=256, block_size=96), dict(block_size=192)):
+                  dict(D=256, block_size=96), dict(block_size=72)):
         assert takes(**wrong) == -1, wrong
     for large in (dict(words=17), dict(num_reqs=8193), dict(num_blocks=2 ** 25), dict(max_blocks=2 ** 26), dict(max_blocks=2 ** 25, words=16, total_q=2048)):
         assert takes(**large) == -4, large

@@ -133,8 +133,8 @@ def attention(q: torch.Tensor, kv_cache: torch.Tensor, *, block_table: torch.Ten
     of the context a node sees only what lies less than ``window`` before it; that takes its ``positions`` (from ``c`` to
     ``c + n - 1``; the bits alone say which nodes it sees). What a node does not see does not reach it, infinities and NaN among the values
     included. Entries of ``block_table`` outside the cache count as keys and values of zeros. ``out`` shares no memory with the rows of ``q``. ``tmp``:
-    :func:`scratch`, allocated if not given. head_dim 64, 128 or 256, at most 128 query heads a kv head, pages that divide a tile of 128
-    tokens (64 at head_dim 256) or are whole tiles; at most 8192 requests."""
+    :func:`scratch`, allocated if not given. head_dim 64, 128 or 256, at most 128 query heads a kv head, pages that divide a tile of 64
+    tokens or are whole tiles; at most 8192 requests."""
     given = out is not None
     try:
         (T, cols), (nb, two, bs, H, D), (treqs, pages), (reqs,), (rows, words) = q.shape, kv_cache.shape, block_table.shape, q_start.shape, mask.shape
