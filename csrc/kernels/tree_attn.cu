@@ -550,19 +550,18 @@ __global__ void __launch_bounds__(kTreeThreads, 1)
         low = min(w.ctx, w.ctx + (int)min(max(depth, 0ll), (long long)w.n - 1) - p.window + 1);
       }
       const auto seen_word = [&](int key) { return there ? tree_seen(bits, p.words, key, w.ctx, w.len, low) : 0u; };
-      const int low_most = p.window > 0 ? __reduce_max_sync(0xffffffffu, there ? low : INT_MIN) : 0;
+      // tiles in which the nodes of the request may differ in what they see: up to where a window begins for all of them, and from the context's end on
+      const int odd_to = p.window > 0 ? w.ctx - p.window + w.n - w.key0 : INT_MIN, odd_from = w.ctx - w.key0 - K + 1;
       float m = -INFINITY, l = 0.f;
       int odd_n = 0;
       const bool both = Sh::kWide || w.two;
       const int mine = both ? w.nt : (w.nt + 1 - half) / 2;            // tiles of this warpgroup
       for (int i = 0; i < mine; ++i) {
-        const int j = both ? i : 2 * i + half, kbase = w.key0 + j * K;
+        const int j = both ? i : 2 * i + half, at0 = j * K, kbase = w.key0 + at0;
         const uint32_t c = made + i, buf = c & 1;
-        // tiles in which the nodes of the request may differ in what they see (need_mask: those of this warp do)
-        const bool odd_tile = kbase + K > w.ctx || (p.window > 0 && kbase < w.ctx - p.window + w.n);
-        const bool need_mask = kbase + K > w.ctx || kbase < low_most;
+        const bool odd_tile = at0 >= odd_from || at0 < odd_to;
         uint32_t seen[2] = {0xffffffffu, 0xffffffffu};
-        if (need_mask) {
+        if (odd_tile) {
           seen[0] = seen_word(kbase);
           seen[1] = seen_word(kbase + 32);
         }
@@ -580,7 +579,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1)
             for (int e = 0; e < 64; ++e) s[e] = __float_as_uint(tree_capped(__uint_as_float(s[e]) * sc, p.cap2, cap_in));
             sc = 1.f;
           }
-          if (need_mask) {
+          if (odd_tile) {
 #pragma unroll
             for (int e = 0; e < 64; ++e)
               if (!(seen[e >> 5] >> (e & 31) & 1)) s[e] = 0xff800000u;       // -inf
