@@ -29,6 +29,7 @@
 
 #include <algorithm>
 #include <mutex>
+#include <type_traits>
 #include <unordered_map>
 
 #include "api.h"
@@ -41,6 +42,7 @@ static constexpr int kTreeKeys = 64;          // keys of a tile
 static constexpr int kTreeStart = 6;          // what an item's start costs, in key tiles
 static constexpr int kTreeLeast = 3;          // tiles of a stretch at the least
 static constexpr int kTreePieces = 4;         // pieces that the TMA warp is ahead
+static constexpr float kTreeWideCap = 256.f;  // in log2 units
 
 struct TreeParams {
   const __nv_bfloat16* cache;
@@ -243,13 +245,35 @@ __device__ __forceinline__ float tree_ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-// cap tanh(x / cap) in log2 units, y = x / cap: 1 - 2 / (1 + e^(2 y)) is off by 2^-22 of the cap, which is too much of one far above the scores; small y
-// take y - y^3 / 3 + 2 y^5 / 15, off by 2^-28 of itself below 1 / 16.
-__device__ __forceinline__ float tree_capped(float x, float cap2, float to_2y) {
-  const float t = x * to_2y, y = t * 0.34657359f, yy = y * y;
+// cap tanh(x / cap) of four scores in log2 units, y = x / cap: 1 - 2 / (1 + e^(2 y)), where one reciprocal of a product of four does for all (special functions bound
+// the capped softmax: 64 dims, windows of 1024, 68 us with a reciprocal each). e^(2 y) stops at 2^30, past which the quotient is less than 2^-29. Off by 2^-21 of the
+// cap, which is too much of one far above the scores (WIDE): small y take y - y^3 / 3 + 2 y^5 / 15 there, off by 2^-28 of itself below 1 / 16. A NaN makes all
+// four one: hidden scores are 0 before.
+template <bool WIDE>
+__device__ __forceinline__ void tree_cap(uint32_t* s, float cap2, float to_2y) {
+  float t[4], d[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    t[e] = __uint_as_float(s[e]) * to_2y;
+    float x;
+    asm("min.NaN.f32 %0, %1, 0f41f00000;" : "=f"(x) : "f"(t[e]));
+    d[e] = 1.f + tree_ex2(x);
+  }
+  const float d01 = d[0] * d[1], d23 = d[2] * d[3];
   float r;
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.f + tree_ex2(t)));
-  return fabsf(y) < 0.0625f ? cap2 * y * fmaf(yy, fmaf(yy, 0.13333333f, -0.33333333f), 1.f) : fmaf(-2.f * cap2, r, cap2);
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(d01 * d23));
+  r *= -2.f * cap2;
+  const float r01 = r * d23, r23 = r * d01;
+  const float q[4] = {r01 * d[1], r01 * d[0], r23 * d[3], r23 * d[2]};
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    float c = cap2 + q[e];
+    if (WIDE) {
+      const float y = t[e] * 0.34657359f, yy = y * y;
+      if (fabsf(y) < 0.0625f) c = cap2 * y * fmaf(yy, fmaf(yy, 0.13333333f, -0.33333333f), 1.f);
+    }
+    s[e] = __float_as_uint(c);
+  }
 }
 __device__ __forceinline__ bool odd_bf16x2(uint32_t w) { return (w & 0x7f80u) == 0x7f80u || (w & 0x7f800000u) == 0x7f800000u; }
 
@@ -268,7 +292,8 @@ __device__ __forceinline__ uint32_t tree_seen(const uint64_t* mask, int words, i
   return v;
 }
 
-template <int D>
+// CAP: with capped scores (a kernel of its own: the others lose 2 % to its code)
+template <int D, bool CAP>
 __global__ void __launch_bounds__(kTreeThreads, 1)
     tree_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmKV, TreeParams p) {
   using Sh = TreeShape<D>;
@@ -524,7 +549,8 @@ __global__ void __launch_bounds__(kTreeThreads, 1)
     // ---------------- softmax and output: a thread a row (two where it is wide) ----------------
     const int half = warp >> 2, quarter = warp & 3, r = quarter * 32 + lane, t = Sh::kWide ? 0 : half;
     const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
-    const float cap_in = p.cap2 > 0.f ? fminf(2.8853900817779268f / p.cap2, 3.0e38f) : 0.f;
+    // scores as they come -> 2 y log2(e); finite, as a score of 0 times it is 0 however small the cap is
+    const float cap_in = CAP ? fminf(p.scale_log2 * fminf(2.8853900817779268f / p.cap2, 3.0e38f), 3.0e38f) : 0.f;
     const int row_node = r / p.G, row_head = r - row_node * p.G;
     uint32_t tiles0 = 0, piece = 0, made = 0, met = 0;       // tiles of V in the pieces before
     bool ok = true;
@@ -574,9 +600,19 @@ __global__ void __launch_bounds__(kTreeThreads, 1)
           tmem_ld_32x32b_x32(s_addr + 32, s + 32);
           tmem_ld_wait();
           float sc = p.scale_log2;
-          if (p.cap2 > 0.f) {
+          if constexpr (CAP) {
+            if (odd_tile) {
 #pragma unroll
-            for (int e = 0; e < 64; ++e) s[e] = __float_as_uint(tree_capped(__uint_as_float(s[e]) * sc, p.cap2, cap_in));
+              for (int e = 0; e < 64; ++e)
+                if (!(seen[e >> 5] >> (e & 31) & 1)) s[e] = 0;
+            }
+            if (p.cap2 <= kTreeWideCap) {
+#pragma unroll
+              for (int e = 0; e < 64; e += 4) tree_cap<false>(s + e, p.cap2, cap_in);
+            } else {
+#pragma unroll
+              for (int e = 0; e < 64; e += 4) tree_cap<true>(s + e, p.cap2, cap_in);
+            }
             sc = 1.f;
           }
           if (odd_tile) {
@@ -839,11 +875,11 @@ __global__ void __launch_bounds__(256)
     dst[warp + 8 * k] = make_uint2(pack_bf16x2(acc[k].x * inv, acc[k].y * inv), pack_bf16x2(acc[k].z * inv, acc[k].w * inv));
 }
 
-template <int D>
+template <int D, bool CAP>
 static int launch_tree(const CUtensorMap& tmQ, const CUtensorMap& tmKV, const TreeParams& p, int ctas, cudaStream_t stream) {
   static PerDeviceOnce once;
-  if (once.first()) cudaFuncSetAttribute(tree_attn_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, tree_smem<D>());
-  if (launch_pdl(tree_attn_kernel<D>, dim3(ctas), dim3(kTreeThreads), tree_smem<D>(), stream, tmQ, tmKV, p) != cudaSuccess) return -2;
+  if (once.first()) cudaFuncSetAttribute(tree_attn_kernel<D, CAP>, cudaFuncAttributeMaxDynamicSharedMemorySize, tree_smem<D>());
+  if (launch_pdl(tree_attn_kernel<D, CAP>, dim3(ctas), dim3(kTreeThreads), tree_smem<D>(), stream, tmQ, tmKV, p) != cudaSuccess) return -2;
   return launch_pdl(tree_join_kernel<D>, dim3(ctas, TreeShape<D>::kRows / 32), dim3(256), 0, stream, (const float*)p.parts, ctas, p.out, p.ldo,
                     p.G, p.nodes) == cudaSuccess ? 0 : -2;
 }
@@ -922,6 +958,9 @@ extern "C" int b200_tree_attn(const B200TreeAttn* a, cudaStream_t stream) {
     return -2;
   }
   const int ctas = b200_num_sms();
-  return D == 64 ? launch_tree<64>(tmQ, tmKV, p, ctas, stream) : D == 128 ? launch_tree<128>(tmQ, tmKV, p, ctas, stream)
-                                                                         : launch_tree<256>(tmQ, tmKV, p, ctas, stream);
+  const auto launch = [&](auto dim) {
+    constexpr int kD = decltype(dim)::value;
+    return p.cap2 > 0.f ? launch_tree<kD, true>(tmQ, tmKV, p, ctas, stream) : launch_tree<kD, false>(tmQ, tmKV, p, ctas, stream);
+  };
+  return D == 64 ? launch(std::integral_constant<int, 64>()) : D == 128 ? launch(std::integral_constant<int, 128>()) : launch(std::integral_constant<int, 256>());
 }
