@@ -39,8 +39,8 @@ namespace b200 {
 
 static constexpr int kTreeThreads = 384, kTreeReqs = 8192, kTreeNodes = 1024;       // (the last two: at most)
 static constexpr int kTreeKeys = 64;          // keys of a tile
-static constexpr int kTreeStart = 6;          // what an item's start costs, in key tiles
-static constexpr int kTreeLeast = 3;          // tiles of a stretch at the least
+static constexpr int kTreeStart = 6;          // what an item's start costs, in key tiles (48 ragged requests: 79 us, with 9 83; with 4 others lose 1 %)
+static constexpr int kTreeLeast = 5;          // tiles of a stretch at the least (one sequence of 1000 keys: 15.5 us, with 3 16.4, with 2 18.0)
 static constexpr int kTreePieces = 4;         // pieces that the TMA warp is ahead
 static constexpr float kTreeWideCap = 256.f;  // in log2 units
 
@@ -85,9 +85,10 @@ template <int D>
 __device__ __forceinline__ TreeReq tree_req(const TreeParams& p, int start, int end, int len) {
   TreeReq r;
   r.row0 = min(max(start, 0), p.total_q);
-  r.n = max(0, min(end, p.total_q) - r.row0);
+  const int rows = max(0, min(end, p.total_q) - r.row0);
+  r.n = min(rows, kTreeNodes);         // (more are left out)
   r.len = min(max(len, 0), p.max_len);
-  r.ctx = r.len - r.n;
+  r.ctx = r.len - rows;
   const int low = p.window > 0 ? max(0, r.ctx - p.window + 1) : 0;
   r.begin = min(low, max(r.len - 1, 0)) / kTreeKeys;
   r.tiles = max(1, (r.len + kTreeKeys - 1) / kTreeKeys - r.begin);     // (no keys: a tile that nobody sees)
@@ -106,6 +107,9 @@ struct TreePiece {
   int head, node0;                     // kv head, first node
   bool two, cut, whole;                // a second tile of rows; the item began before; the piece is all of it
 };
+struct TreeStart {
+  int req, off, begin, end, len;       // where a stretch starts: request, cells of it that are behind, its nodes and keys
+};
 template <int D>
 struct TreeWalk {
   const TreeParams& p;
@@ -113,11 +117,10 @@ struct TreeWalk {
   int b, off;                          // request, cells of it that are behind
   long long left;                      // cells of the stretch
   int end, next_end, next_len;         // where the request's nodes end; of the next request, on their way
-  __device__ __forceinline__ TreeWalk(const TreeParams& p_, int b_, int off_, long long left_) : p(p_), b(b_), off(off_), left(left_) {
+  __device__ __forceinline__ TreeWalk(const TreeParams& p_, const TreeStart& s, long long left_) : p(p_), b(s.req), off(s.off), left(left_), end(s.end) {
     if (left <= 0) return;
-    end = p.q_start[b + 1];
     ahead();
-    r = tree_req<D>(p, p.q_start[b], end, p.seq_lens[b]);
+    r = tree_req<D>(p, s.begin, s.end, s.len);
   }
   __device__ __forceinline__ void ahead() {
     const int nb = min(b + 1, p.num_reqs - 1);
@@ -171,7 +174,7 @@ struct alignas(8) TreeBars {
   TreePiece piece[kTreePieces];
   TreeCut cut;
   uint32_t tmem_base;
-  int start_req, start_off;
+  TreeStart start;
   union {
     long long sums[kTreeThreads / 32];
     float rows[2][128];                // what the two threads of a row tell one another
@@ -375,11 +378,11 @@ __global__ void __launch_bounds__(kTreeThreads, 1)
   if (lo < hi && upto - mine <= lo && lo < upto) {
     long long at = upto - mine;
     for (int b = b0; b < b1; ++b) {
-      const TreeReq r = tree_req<D>(p, b);
+      const TreeStart s{b, (int)(lo - at), p.q_start[b], p.q_start[b + 1], p.seq_lens[b]};
+      const TreeReq r = tree_req<D>(p, s.begin, s.end, s.len);
       const long long cells = (long long)r.items * (kTreeStart + r.tiles);
       if (lo < at + cells) {
-        bars.start_req = b;
-        bars.start_off = (int)(lo - at);
+        bars.start = s;
         break;
       }
       at += cells;
@@ -389,7 +392,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1)
 
   if (warp == 8) {
     // ---------------- pieces, queries and keys ----------------
-    TreeWalk<D> walk(p, lo < hi ? bars.start_req : 0, lo < hi ? bars.start_off : 0, hi - lo);
+    TreeWalk<D> walk(p, bars.start, hi - lo);
     TreeSlot<Sh::kKeySlots> slot;
     uint32_t queries = 0;
     bool ok = true;
@@ -699,8 +702,9 @@ __global__ void __launch_bounds__(kTreeThreads, 1)
           }
           fence_proxy_async_smem();
           const uint32_t who = __ballot_sync(0xffffffffu, odd);
-          if (who && lane == 0) {      // (rare: a note; room for every tile that can be looked at)
-            const int note = (both ? 0 : half * (kOdd / 2)) + odd_n;
+          const int most = both ? kOdd : kOdd / 2;                     // (notes that there is room for: all, but of requests with nodes that are left out)
+          if (who && lane == 0 && odd_n < most) {
+            const int note = (both ? 0 : half * most) + odd_n;
             bars.odd_tile[note] = kbase;
             atomicOr(&bars.odd[note][quarter & 1], who);
             atomicOr(&bars.odd_any, 1u);
@@ -841,6 +845,7 @@ __global__ void __launch_bounds__(256)
   using Sh = TreeShape<D>;
   constexpr int kQuads = D / 32;
   pdl_wait();
+  pdl_launch_dependents();
   const TreeCut cut = reinterpret_cast<const TreeCut*>(parts + 2 * (long long)ctas * Sh::kPartFloats)[blockIdx.x];
   if (cut.first < 0) return;
   const int warp = threadIdx.x >> 5, row = blockIdx.y * 32 + (threadIdx.x & 31), count = (int)blockIdx.x - cut.first + 1;
@@ -911,7 +916,7 @@ extern "C" int b200_tree_attn_takes(const B200TreeAttn* a) {
   if (a->num_blocks >= (1ll << 31) / (2 * bs) - 1) return -4;
   const int nodes = 128 / (a->Hq / a->Hkv);
   const long long tiles = ((long long)a->max_blocks * bs + keys - 1) / keys + kTreeStart;
-  const long long pairs = (std::min(a->total_q, 64 * a->words) + nodes - 1) / nodes + 1;
+  const long long pairs = (std::min(a->total_q, kTreeNodes) + nodes - 1) / nodes + 1;
   return tiles * pairs >= (1ll << 31) / a->Hkv || (long long)a->max_blocks * bs > (1ll << 31) - 4096 ? -4 : 0;
 }
 

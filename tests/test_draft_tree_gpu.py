@@ -102,9 +102,10 @@ def test_attention_in_a_window(d, window):
 
 
 @pytest.mark.parametrize("d", [64, 128, 256])
-@pytest.mark.parametrize("softcap", [0.5, 30.0, 20000.0])
-def test_attention_with_capped_scores(d, softcap):
-    case, scale = attention_case([9, 40], [77, 900], hq=6, hkv=2, d=d, page=16, seed=3, device=DEV)
+@pytest.mark.parametrize("softcap", [1e-38, 0.5, 30.0, 170.0, 200.0, 20000.0, 1e30])
+@pytest.mark.parametrize("n", [40, 70])
+def test_attention_with_capped_scores(d, softcap, n):
+    case, scale = attention_case([9, n], [77, 900], hq=6, hkv=2, d=d, page=16, seed=3, device=DEV)
     check_attention(case, scale, softcap=softcap)
     check_attention(case, scale, softcap=softcap, window=200)
 
@@ -181,6 +182,43 @@ def test_attention_keeps_out_what_lies_before_a_window(d):
     assert int(reached.sum()) == 10 and torch.equal(got[~reached], clean[~reached]) and bool(got[reached].isnan().all())
 
 
+def test_attention_of_keys_that_are_not_finite():
+    """A NaN among a seen key's dims reaches the rows that see it; one that is hidden does not, capped or not."""
+    case, scale = attention_case([12], [100], hq=8, hkv=2, d=128, page=16, seed=1, wide=3, device=DEV)
+    from vllm_cpp_b200.ops.draft_tree import seen_by
+    seen = seen_by(case["mask"], q_start=case["q_start"], seq_lens=case["seq_lens"])[0]
+    for softcap in (0.0, 30.0):
+        clean = run_attention(case, scale, softcap=softcap).clone()
+        for value in (math.nan, math.inf):
+            bad = dict(case, kv_cache=case["kv_cache"].clone())
+            bad["kv_cache"][int(case["block_table"][0, 110 // 16]), 0, 110 % 16] = value
+            got = run_attention(bad, scale, softcap=softcap)
+            assert torch.equal(got[~seen[:, 110]], clean[~seen[:, 110]])
+            if math.isnan(value):
+                assert bool(got[seen[:, 110]].isnan().all())
+
+
+def test_attention_of_nothing_and_of_short_lengths():
+    """Steps without rows or requests; lengths below a request's nodes, whose first cells lie before the cache's first: nobody sees them."""
+    case, scale = attention_case([12, 3], [100, 7], hq=8, hkv=2, d=128, page=16, seed=1, device=DEV)
+    assert run_attention(dict(case, q=case["q"][:0]), scale).shape == (0, 1024)
+    none = dict(case, q_start=case["q_start"][:1])
+    assert bool((run_attention(none, scale) == 7).all())
+    case["seq_lens"] = torch.tensor([5, 0], dtype=torch.int32, device=DEV)
+    got = run_attention(case, scale)
+    kv = case["kv_cache"][int(case["block_table"][0, 0])].double()
+    for node in range(12):
+        cells = [j - 7 for j in range(7, 12) if int(case["mask"][node, 0]) >> j & 1]
+        want = torch.zeros((8, 128), dtype=torch.float64, device=DEV)
+        if cells:
+            k, v = (kv[i, cells].repeat_interleave(4, 1) for i in (0, 1))
+            p = (torch.einsum("hd,khd->hk", case["q"][node].view(8, 128).double(), k) * scale).softmax(-1)
+            want = torch.einsum("hk,khd->hd", p, v)
+        # (weights and output rounded to bf16, 2^-8 of the largest value each, and as much again for scores in 32 bits)
+        assert float((got[node].view(8, 128).double() - want).abs().max()) <= 3 * 2.0 ** -8 * float(kv[1].abs().max())
+    assert bool((got[12:] == 0).all())
+
+
 def test_attention_over_pages_outside_the_cache():
     """They count as keys and values of zeros, and nothing else is read."""
     case, scale = attention_case([9], [300], hq=8, hkv=2, d=128, page=16, seed=3, device=DEV)
@@ -238,6 +276,15 @@ def test_attention_gives_the_same_bits_in_streams_and_graphs():
                 g.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(o, want) for o in outs)
+
+
+def test_attention_on_another_device_than_the_current_one():
+    if torch.cuda.device_count() < 2:
+        pytest.skip("one GPU")
+    case, scale = attention_case([9, 40, 3], [77, 900, 200], hq=8, hkv=2, d=128, page=16, seed=3, device="cuda:1")
+    got = draft_tree.attention(scale=scale, **case)
+    want = run_attention({k: v.to("cuda:0") for k, v in case.items()}, scale)
+    assert torch.equal(got.cpu(), want.cpu())
 
 
 # ------------------------------------------------------------------------------------------------ verify
@@ -364,6 +411,35 @@ def test_verify_keeps_the_targets_distribution(drawn, wide):
     got = torch.bincount(out[:, 0].cpu(), minlength=V).double()
     assert bool(((got - R * p).abs() <= 6 * (R * p * (1 - p)).sqrt()).all()), (got / R, p)
     assert int(count.max()) > 1
+
+
+def test_verify_of_steps_without_requests_or_rows():
+    case = on_gpu(verify_case([2, 3], 50, seed=1))
+    none = dict(case, q_start=case["q_start"][:1], seeds=case["seeds"][:0], steps=case["steps"][:0], temperature=None)
+    assert [tuple(t.shape) for t in draft_tree.verify(**none)] == [(0, 3), (0, 3), (0,)]
+    zero = torch.zeros(3, dtype=torch.int32, device=DEV)
+    empty = {k: case[k][:0] for k in ("logits", "tokens", "uniforms", "draft_probs")}
+    out, path, count = draft_tree.verify(**dict(case, q_start=zero, **empty))
+    assert count.tolist() == [0, 0] and bool((out == -1).all()) and bool((path == -1).all())
+
+
+@pytest.mark.parametrize("drawn", [True, False])
+def test_verify_of_rows_at_every_alignment(drawn):
+    """Rows that begin one, two or three columns off 16 bytes, and rows without a distance (the same logits for all nodes)."""
+    for shift in (1, 2, 3):
+        case = on_gpu(verify_case([4, 1, 6], 5003, wide=2, drawn=drawn, seed=shift))
+        want = [t.clone() for t in draft_tree.verify(**case)]
+        for name in ("logits", "draft_probs"):
+            if case[name] is not None:
+                flat = torch.full((case[name].numel() + 16,), 1e9, device=DEV)
+                at = flat[shift: shift + case[name].numel()].view(case[name].shape)
+                at.copy_(case[name])
+                case[name] = at
+        assert all(torch.equal(a, b) for a, b in zip(draft_tree.verify(**case), want))
+    case = on_gpu(verify_case([4, 1, 6], 5003, wide=2, drawn=drawn, seed=9))
+    case["logits"] = case["logits"][:1].expand(11, 5003)
+    got = draft_tree.verify(**case)
+    assert all(torch.equal(a, b) for a, b in zip(got, draft_tree.verify(**dict(case, logits=case["logits"].contiguous()))))
 
 
 def test_verify_in_a_graph():

@@ -17,7 +17,9 @@ touched. The ``ref_*`` functions restate the operators in plain PyTorch (any dev
 from __future__ import annotations
 
 import ctypes
+import functools
 import math
+import operator
 from typing import Optional, Sequence, Union
 
 import torch
@@ -49,6 +51,7 @@ class CompactArgs(ctypes.Structure):
                 ("cell_bytes", _L), ("num_caches", _I), ("max_blocks", _I), ("num_reqs", _I), ("total", _I), ("most", _I), ("block_size", _I)]
 
 
+_address, _contiguous, _kind = torch.Tensor.data_ptr, torch.Tensor.is_contiguous, operator.attrgetter("shape", "dtype", "device")
 _declared = False
 _attn = _mask = _verify = _compact = None
 
@@ -229,15 +232,14 @@ def compact(kv_caches: Union[torch.Tensor, Sequence[torch.Tensor]], *, block_tab
     caches = [kv_caches] if isinstance(kv_caches, torch.Tensor) else list(kv_caches)
     try:
         first = caches[0]
-        shape, dtype, dev = first.shape, first.dtype, first.get_device()
+        shape, dev = first.shape, first.get_device()
         (nb, two, bs, H, D), (treqs, pages), (ldt, t1), (reqs,), (prows, most) = shape, block_table.shape, block_table.stride(), q_start.shape, path.shape
         cell = H * D * first.element_size()
-        at = [c.data_ptr() for c in caches]
+        at = list(map(_address, caches))
         ok = (dev >= 0 and two == 2 and bs > 0 and cell > 0 and cell % 16 == 0 and pages > 0 and t1 == 1 and block_table.dtype is _I32 and block_table.get_device() == dev
               and treqs >= reqs - 1 and _ids(seq_lens, _I32, dev, reqs - 1) and _ids(q_start, _I32, dev, 1) and path.dtype is _I32
-              and path.get_device() == dev and path.is_contiguous() and prows == reqs - 1 and len(set(at)) == len(at))
-        for c, p in zip(caches, at):
-            ok = ok and p % 16 == 0 and c.is_contiguous() and c.shape == shape and c.dtype is dtype and c.get_device() == dev
+              and path.get_device() == dev and path.is_contiguous() and prows == reqs - 1 and len(set(at)) == len(at)
+              and not functools.reduce(operator.or_, at) % 16 and all(map(_contiguous, caches)) and len(set(map(_kind, caches))) == 1)
     except (TypeError, ValueError, AttributeError, IndexError):
         ok = False
     if not ok:
