@@ -28,9 +28,7 @@
 #include <limits.h>
 
 #include <algorithm>
-#include <mutex>
 #include <type_traits>
-#include <unordered_map>
 
 #include "api.h"
 #include "sm100.cuh"
@@ -889,18 +887,6 @@ static int launch_tree(const CUtensorMap& tmQ, const CUtensorMap& tmKV, const Tr
                     p.G, p.nodes) == cudaSuccess ? 0 : -2;
 }
 
-struct TreeMapKey {
-  const void* p;
-  uint64_t rows;
-  int hkv, d, box;
-  bool operator==(const TreeMapKey& o) const { return p == o.p && rows == o.rows && hkv == o.hkv && d == o.d && box == o.box; }
-};
-struct TreeMapHash {
-  size_t operator()(const TreeMapKey& k) const {
-    return reinterpret_cast<size_t>(k.p) ^ k.rows * 0x9e3779b97f4a7c15ull ^ (size_t)k.hkv << 40 ^ (size_t)k.d << 20 ^ (size_t)k.box;
-  }
-};
-
 }  // namespace b200
 
 using namespace b200;
@@ -936,32 +922,17 @@ extern "C" int b200_tree_attn(const B200TreeAttn* a, cudaStream_t stream) {
   p.seq_lens = (const int32_t*)a->seq_lens; p.q_start = (const int32_t*)a->q_start;
   p.positions = (const int64_t*)a->positions; p.mask = (const uint64_t*)a->mask; p.words = a->words;
   p.num_reqs = a->num_reqs; p.total_q = a->total_q; p.Hkv = a->Hkv; p.G = G; p.nodes = 128 / G;
-  p.block_size = bs; p.window = a->positions ? a->window : 0; p.max_len = a->max_blocks * bs;
+  p.block_size = bs; p.max_len = a->max_blocks * bs;
+  p.window = a->positions && a->window <= p.max_len ? a->window : 0;         // (one that holds any context is none)
   p.scale_log2 = a->scale * 1.4426950408889634f; p.cap2 = a->softcap * 1.4426950408889634f;
   p.parts = (float*)a->parts; p.status = device_status_word();
   CUtensorMap tmQ, tmKV;
   if (!encode_tmap_3d(&tmQ, a->q, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, (uint64_t)D, (uint64_t)a->Hq, (uint64_t)a->total_q, (uint64_t)D * 2,
                       (uint64_t)a->ldq * 2, 64, (uint32_t)G, (uint32_t)p.nodes, CU_TENSOR_MAP_SWIZZLE_128B))
     return -3;
-  static std::mutex mu;
-  static std::unordered_map<TreeMapKey, CUtensorMap, TreeMapHash> maps;
-  const uint64_t rows = (uint64_t)a->num_blocks * 2 * bs;
-  const TreeMapKey key{a->cache, rows, a->Hkv, D, std::min(bs, keys)};
-  try {
-    std::lock_guard<std::mutex> lock(mu);
-    auto it = maps.find(key);
-    if (it == maps.end()) {
-      if (maps.size() > 4096) maps.clear();          // scratch caches come and go
-      CUtensorMap m;
-      if (!encode_tmap_3d(&m, a->cache, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, (uint64_t)D, (uint64_t)a->Hkv, rows, (uint64_t)D * 2,
-                          (uint64_t)a->Hkv * D * 2, 64, 1, (uint32_t)key.box, CU_TENSOR_MAP_SWIZZLE_128B))
-        return -3;
-      it = maps.emplace(key, m).first;
-    }
-    tmKV = it->second;
-  } catch (...) {
-    return -2;
-  }
+  if (!encode_tmap_3d(&tmKV, a->cache, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, (uint64_t)D, (uint64_t)a->Hkv, (uint64_t)a->num_blocks * 2 * bs,
+                      (uint64_t)D * 2, (uint64_t)a->Hkv * D * 2, 64, 1, (uint32_t)std::min(bs, keys), CU_TENSOR_MAP_SWIZZLE_128B))
+    return -3;
   const int ctas = b200_num_sms();
   const auto launch = [&](auto dim) {
     constexpr int kD = decltype(dim)::value;

@@ -101,6 +101,15 @@ def test_attention_in_a_window(d, window):
     check_attention(case, scale, window=window)
 
 
+@pytest.mark.parametrize("window", [400, 2 ** 31 - 1])
+def test_attention_in_a_window_that_holds_everything(window):
+    """Lengths that are shorter than the request's nodes too."""
+    case, scale = attention_case([70, 9, 100], [0, 250, 30], hq=6, hkv=2, d=128, page=16, seed=3, wide=2, device=DEV)
+    for cut in (0, 5):
+        case["seq_lens"] -= cut
+        assert torch.equal(run_attention(case, scale, window=window), run_attention({**case}, scale))
+
+
 @pytest.mark.parametrize("d", [64, 128, 256])
 @pytest.mark.parametrize("softcap", [1e-38, 0.5, 30.0, 170.0, 200.0, 20000.0, 1e30])
 @pytest.mark.parametrize("n", [40, 70])
