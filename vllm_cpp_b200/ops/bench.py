@@ -258,6 +258,26 @@ def small_case(name: str):
             req, q0 = (torch.tensor(t, dtype=torch.int32, device=dev) for t in ref.build_prefill_tiles([new]))
             qs = torch.tensor([0, new], dtype=torch.int32, device=dev)
             fn = lambda: F4.prefill(q, cache, block_table=bt, seq_lens=sl, q_start=qs, tile_req=req, tile_q0=q0, scale=Dh ** -0.5)
+    elif name in ("tree_attn_small", "tree_verify_small"):
+        # 32 requests: trees of 60 nodes (two tiles of rows) after 4036 tokens, 32 query heads over 8 of 128 dims, 32-token pages; chains of 4 drafts over 128256 columns
+        from . import draft_tree as DT
+        B, n = (32, 60) if name == "tree_attn_small" else (32, 5)
+        starts = torch.arange(B + 1, device=dev, dtype=torch.int32) * n
+        if name == "tree_attn_small":
+            H, Hk, Dh, page, ctx = 32, 8, 128, 32, 4096
+            cache = torch.randn(B * ctx // page, 2, page, Hk, Dh, device=dev, dtype=torch.bfloat16)
+            bt = torch.randperm(B * ctx // page, device=dev).int().view(B, ctx // page)
+            sl = torch.full((B,), ctx, dtype=torch.int32, device=dev)
+            bits, _ = DT.mask(((torch.arange(n, device=dev) - 1) // 2).int().repeat(B), q_start=starts, seq_lens=sl)
+            q = torch.randn(B * n, H * Dh, device=dev, dtype=torch.bfloat16)
+            fn = lambda: DT.attention(q, cache, block_table=bt, seq_lens=sl, q_start=starts, mask=bits, scale=Dh ** -0.5)
+        else:
+            V = 128256
+            logits = torch.randn(B * n, V, device=dev) * 3
+            probs = torch.softmax(logits + torch.randn(B * n, V, device=dev), -1)
+            tokens = torch.multinomial(probs, 1).flatten().roll(1)
+            uniforms, ids = torch.rand(B * n, device=dev), torch.arange(B, device=dev)
+            fn = lambda: DT.verify(logits, tokens, q_start=starts, uniforms=uniforms, seeds=ids, steps=ids, max_tokens=n, draft_probs=probs)
     else:
         raise SystemExit(f"unknown case {name}")
     ms = _time(fn, iters=3, warmup=1)
@@ -275,7 +295,7 @@ def main():
                          "gdn_decode_small | moe_small | moe_few_small | moe_many_small | gemm_streamk_small | gemm_shared_small | gemm_gated_small | "
                          "gemm_fp8_small | gemm_w4a16_small | gemm_nvfp4_small | gemm_nvfp4_prefill_small | "
                          "decode_d256_small | mla_decode_small | bias_prefill_small | bias_decode_small | delta_small | "
-                         "fp4_append_small | fp4_decode_small | fp4_prefill_small")
+                         "fp4_append_small | fp4_decode_small | fp4_prefill_small | tree_attn_small | tree_verify_small")
     args = ap.parse_args()
     if args.case:
         return small_case(args.case)

@@ -16,6 +16,7 @@ touched. The ``ref_*`` functions restate the operators in plain PyTorch (any dev
 """
 from __future__ import annotations
 
+import array
 import ctypes
 import functools
 import math
@@ -51,7 +52,8 @@ class CompactArgs(ctypes.Structure):
                 ("cell_bytes", _L), ("num_caches", _I), ("max_blocks", _I), ("num_reqs", _I), ("total", _I), ("most", _I), ("block_size", _I)]
 
 
-_address, _contiguous, _kind = torch.Tensor.data_ptr, torch.Tensor.is_contiguous, operator.attrgetter("shape", "dtype", "device")
+_address, _contiguous, _device, _shape, _dtype = (torch.Tensor.data_ptr, torch.Tensor.is_contiguous, torch.Tensor.get_device,
+                                                  operator.attrgetter("shape"), operator.attrgetter("dtype"))
 _declared = False
 _attn = _mask = _verify = _compact = None
 
@@ -239,7 +241,8 @@ def compact(kv_caches: Union[torch.Tensor, Sequence[torch.Tensor]], *, block_tab
         ok = (dev >= 0 and two == 2 and bs > 0 and cell > 0 and cell % 16 == 0 and pages > 0 and t1 == 1 and block_table.dtype is _I32 and block_table.get_device() == dev
               and treqs >= reqs - 1 and _ids(seq_lens, _I32, dev, reqs - 1) and _ids(q_start, _I32, dev, 1) and path.dtype is _I32
               and path.get_device() == dev and path.is_contiguous() and prows == reqs - 1 and len(set(at)) == len(at)
-              and not functools.reduce(operator.or_, at) % 16 and all(map(_contiguous, caches)) and len(set(map(_kind, caches))) == 1)
+              and not functools.reduce(operator.or_, at) % 16 and all(map(_contiguous, caches))
+              and [*map(_device, caches)].count(dev) == [*map(_dtype, caches)].count(first.dtype) == [*map(_shape, caches)].count(shape) == len(at))
     except (TypeError, ValueError, AttributeError, IndexError):
         ok = False
     if not ok:
@@ -248,7 +251,8 @@ def compact(kv_caches: Union[torch.Tensor, Sequence[torch.Tensor]], *, block_tab
         cell, at = H * D * caches[0].element_size(), [c.data_ptr() for c in caches]
     _declare()
     a = CompactArgs()
-    a.caches, a.num_caches = ctypes.cast((_P * len(at))(*at), _P), len(at)
+    held = array.array("Q", at)
+    a.caches, a.num_caches = held.buffer_info()[0], len(at)
     a.block_table, a.ldt, a.max_blocks, a.seq_lens, a.q_start = block_table.data_ptr(), ldt, pages, seq_lens.data_ptr(), q_start.data_ptr()
     a.path, a.most, a.num_blocks, a.block_size, a.cell_bytes, a.num_reqs, a.total = path.data_ptr(), most, nb, bs, cell, reqs - 1, 2 ** 31 - 1
     _launch(caches[0], _compact, "tree_compact", a)
