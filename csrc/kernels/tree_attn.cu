@@ -24,7 +24,15 @@
 //
 // Warp roles (384 threads): warps 0..3 / 4..7 softmax and output; warp 8 keys by TMA, and the pieces of the stretch for the others; warp 9 values by TMA; warps
 // 10 / 11 MMA of either warpgroup, warp 10 TMEM owner. (One warp for both kinds of loads bounded the kernel by its instructions, 128 requests 300 us; one issuer
-// for both warpgroups made each wait for the other's turn.)
+// for both warpgroups made each wait for the other's turn: one context of 120000 keys 157 us, with two 146.)
+//
+// Measured (us on the device, in brackets what the bytes or products take at least; 32-token pages). One tile of rows is bound by memory where heads have 128 dims: 128
+// requests of 200 to 3800 keys with 32 nodes, 32 heads over 8, 203 (173), 5.6 TB/s; 16 of 8000 keys with 4 nodes 93 (80); 256 dims, 20 of 4000 121 (101). With 64 dims a
+// tile is half the bytes and as many exponentials: 33 of 4096 with 20 nodes, 24 heads over 8, 86 (43), soft-capped 139. Two tiles of rows are bound by the chain of a
+// warpgroup: one context of 120000 keys with 61 nodes 155 (75), 64 of 2000 with 60 nodes 186 (92), tensor pipe and special functions busy in 0.45 of the cycles each. A tile of 64
+// keys takes a warpgroup some 2500 cycles: its scores' wait 300 and load 150, the maximum 370, the exponentials 1050 (two warps a scheduler at once, 1024 by their rate), the
+// rest 400. Slower: turns at the exponentials (155 -> 197), tiles of 128 keys with one buffer of scores (174 to 187), weights checked by their own maximum instead of the scores'
+// (10 %); an eighth to a third of the exponentials as polynomials made that case 4 % faster and those with one tile of rows 5 to 10 % slower.
 #include <limits.h>
 
 #include <algorithm>

@@ -9,6 +9,7 @@ static constexpr int kCellNodes = 1024;        // of a request
 // Row i of a request's n nodes: the bits of i and of the nodes above it, and its position, what lies before the request's nodes plus its depth. A
 // thread walks from its node to the root, through shared memory; parents lie below their children, so that a word is whole before the next
 // is begun. (An entry that is not below its own node makes it a root: the walk ends whatever the entries are.)
+// Bound: the launch and two loads in a chain (bounds, parents). One tree of 60 nodes 2.4 us, 256 trees of 9 to 101 nodes 2.9.
 __global__ void __launch_bounds__(128)
     tree_mask_kernel(const int32_t* __restrict__ parents, const int32_t* __restrict__ q_start, const int32_t* __restrict__ seq_lens, int total,
                      int words, uint64_t* __restrict__ bits, int64_t* __restrict__ positions) {
@@ -44,7 +45,8 @@ __global__ void __launch_bounds__(128)
 
 // Cell context + path[i] of a request goes to cell context + i, i = 1, 2 .., in every cache. A thread moves the same 16 bytes of all cells, in that order
 // and several at a time: a source lies behind its own destination and all earlier ones, so that nothing is overwritten that is still to be
-// read. A block takes one request's keys or values in one cache.
+// read. A block takes one request's keys or values in one cache. Bound: the chain of bounds, path, table and cells for few paths (one of three drafts in 32 caches 3.0 us,
+// 0.16 by its bytes), bytes of scattered cells of 2 KB for many (64 of up to seven drafts in 16 caches 7.7 us, 3.3 TB/s).
 static constexpr int kCaches = 64;             // of a launch
 struct CompactCaches { uint8_t* at[kCaches]; };
 __global__ void __launch_bounds__(256)

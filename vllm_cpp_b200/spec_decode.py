@@ -5,6 +5,7 @@ the Qwen3.5/3.6 multi-token-prediction draft head and a separate draft model (mo
 The scheduler reserves look-ahead slots and rolls rejected tokens back; the loop is switched on
 with ``EngineArgs(speculative_config=...)`` or the server's ``--speculative-config`` (methods
 ngram, mtp and draft_model; the reference stops short of a user-facing switch).
+Operators for trees of drafts, and for drafts of requests that sample: ``vllm_cpp_b200.ops.draft_tree``.
 
 Reference: ``include/vllm/config/speculative.h``, ``include/vllm/v1/spec_decode/
 rejection_sampler.h:1-128``, ``src/vllm/model_executor/models/qwen3_5_mtp.cpp``.
