@@ -27,11 +27,11 @@
 // for both warpgroups made each wait for the other's turn: one context of 120000 keys 157 us, with two 146.)
 //
 // Measured (us on the device, in brackets what the bytes or products take at least; 32-token pages). One tile of rows is bound by memory where heads have 128 dims: 128
-// requests of 200 to 3800 keys with 32 nodes, 32 heads over 8, 203 (173), 5.6 TB/s; 16 of 8000 keys with 4 nodes 93 (80); 256 dims, 20 of 4000 121 (101). With 64 dims a
+// requests of 200 to 3800 keys with 32 nodes, 32 heads over 8, 195 to 202 by the card (173), 5.7 TB/s; 16 of 8000 keys with 4 nodes 91 (80); 256 dims, 20 of 4000 119 (101). With 64 dims a
 // tile is half the bytes and as many exponentials: 33 of 4096 with 20 nodes, 24 heads over 8, 86 (43), soft-capped 139. Two tiles of rows are bound by the chain of a
-// warpgroup: one context of 120000 keys with 61 nodes 155 (75), 64 of 2000 with 60 nodes 186 (92), tensor pipe and special functions busy in 0.45 of the cycles each. A tile of 64
-// keys takes a warpgroup some 2500 cycles: its scores' wait 300 and load 150, the maximum 370, the exponentials 1050 (two warps a scheduler at once, 1024 by their rate), the
-// rest 400. Slower: turns at the exponentials (155 -> 197), tiles of 128 keys with one buffer of scores (174 to 187), weights checked by their own maximum instead of the scores'
+// warpgroup: one context of 120000 keys with 61 nodes 147 to 156 (75), 64 of 2000 with 60 nodes 171 to 180 (92), tensor pipe and special functions busy in 0.45 of the cycles each. A tile of 64
+// keys takes a warpgroup some 2500 cycles: its scores' wait 300 and load 150, the maximum 370, the exponentials 1050 (as many where a warp has the scheduler to itself), the
+// rest 400. Slower: turns at the exponentials (155 -> 197 us), tiles of 128 keys with one buffer of scores (174 to 187), weights checked by their own maximum instead of the scores'
 // (10 %); an eighth to a third of the exponentials as polynomials made that case 4 % faster and those with one tile of rows 5 to 10 % slower.
 #include <limits.h>
 
@@ -45,7 +45,7 @@ namespace b200 {
 
 static constexpr int kTreeThreads = 384, kTreeReqs = 8192, kTreeNodes = 1024;       // (the last two: at most)
 static constexpr int kTreeKeys = 64;          // keys of a tile
-static constexpr int kTreeStart = 6;          // what an item's start costs, in key tiles (48 ragged requests: 79 us, with 9 83; with 4 others lose 1 %)
+static constexpr int kTreeStart = 4;          // what an item's start costs, in key tiles (48 ragged requests 72.7 us, with 6 74.3; 128 requests 195.3 and 193.8)
 static constexpr int kTreeLeast = 5;          // tiles of a stretch at the least (one sequence of 1000 keys: 15.5 us, with 3 16.4, with 2 18.0)
 static constexpr int kTreePieces = 4;         // pieces that the TMA warp is ahead
 static constexpr float kTreeWideCap = 256.f;  // in log2 units
@@ -284,7 +284,30 @@ __device__ __forceinline__ void tree_cap(uint32_t* s, float cap2, float to_2y) {
     s[e] = __float_as_uint(c);
   }
 }
-__device__ __forceinline__ bool odd_bf16x2(uint32_t w) { return (w & 0x7f80u) == 0x7f80u || (w & 0x7f800000u) == 0x7f800000u; }
+// Bits 15 and 31: which of two bf16 is not finite (an exponent of ones and one more passes into the sign's place).
+__device__ __forceinline__ uint32_t odd_bf16x2(uint32_t w) { return (w & 0x7f807f80u) + 0x00800080u; }
+// Of the four 16-byte pieces x of four neighbouring lanes, lane k gets the k-th of each: x[i] is lane i's.
+__device__ __forceinline__ void tree_quads(uint4 (&x)[4]) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int bit = 1; bit < 4; bit *= 2) {
+    const bool up = lane & bit;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (i & bit) continue;
+      uint4& a = x[i];
+      uint4& b = x[i | bit];
+      const uint4 give = up ? a : b;
+      uint4 get;
+      get.x = __shfl_xor_sync(0xffffffffu, give.x, bit);
+      get.y = __shfl_xor_sync(0xffffffffu, give.y, bit);
+      get.z = __shfl_xor_sync(0xffffffffu, give.z, bit);
+      get.w = __shfl_xor_sync(0xffffffffu, give.w, bit);
+      a = up ? get : a;
+      b = up ? b : get;
+    }
+  }
+}
 
 // Bits of the keys key .. key + 31 that a row sees.
 __device__ __forceinline__ uint32_t tree_seen(const uint64_t* mask, int words, int key, int ctx, int len, int low) {
@@ -689,21 +712,28 @@ __global__ void __launch_bounds__(kTreeThreads, 1)
           if (!(ok = __all_sync(0xffffffffu, mbar_wait(&bars.v_full[v % Sh::kValueSlots], (v / Sh::kValueSlots) & 1, p.status)))) break;
           const int key = r & 63;
           uint8_t* row = sV + (v % Sh::kValueSlots) * Sh::kSlot + key * 128;
-          bool odd = false;
+          const auto at16 = [&](int x) {
+            const int piece16 = (r >> 6) * (D / 16) + x;
+            return reinterpret_cast<uint4*>(row + (piece16 >> 3) * Sh::kPiece + (((piece16 & 7) ^ (key & 7)) << 4));
+          };
+          uint32_t any = 0;
 #pragma unroll
           for (int x = 0; x < D / 16; ++x) {
-            const int piece16 = (r >> 6) * (D / 16) + x;
-            uint4* at16 = reinterpret_cast<uint4*>(row + (piece16 >> 3) * Sh::kPiece + (((piece16 & 7) ^ (key & 7)) << 4));
-            const uint4 y = *at16;
-            if (odd_bf16x2(y.x) || odd_bf16x2(y.y) || odd_bf16x2(y.z) || odd_bf16x2(y.w)) {
+            const uint4 y = *at16(x);
+            any |= odd_bf16x2(y.x) | odd_bf16x2(y.y) | odd_bf16x2(y.z) | odd_bf16x2(y.w);
+          }
+          const bool odd = (any & 0x80008000u) != 0;
+          if (odd) {
+#pragma unroll 1
+            for (int x = 0; x < D / 16; ++x) {
+              const uint4 y = *at16(x);
               uint32_t e[4] = {y.x, y.y, y.z, y.w};
 #pragma unroll
               for (int g = 0; g < 4; ++g) {
                 if ((e[g] & 0x7f80u) == 0x7f80u) e[g] &= 0xffff0000u;
                 if ((e[g] & 0x7f800000u) == 0x7f800000u) e[g] &= 0xffffu;
               }
-              *at16 = make_uint4(e[0], e[1], e[2], e[3]);
-              odd = true;
+              *at16(x) = make_uint4(e[0], e[1], e[2], e[3]);
             }
           }
           fence_proxy_async_smem();
@@ -771,6 +801,13 @@ __global__ void __launch_bounds__(kTreeThreads, 1)
         const uint32_t o_addr = tmem + Sh::kO + lanes + (w.two ? half * D : 0);
         __nv_bfloat16* dst = p.out + (w.row0 + node) * p.ldo + (w.head * p.G + row_head) * D;
         float* part = p.parts + (2 * blockIdx.x + (w.cut ? 0 : 1)) * Sh::kPartFloats;
+        // (four lanes write 64 bytes of a row together: 16 bytes of 32 rows each would take the store unit four times as long)
+        __nv_bfloat16* quad[4];
+        if (w.whole) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            quad[i] = reinterpret_cast<__nv_bfloat16*>(__shfl_sync(0xffffffffu, there ? reinterpret_cast<unsigned long long>(dst) : 0ull, (lane & 28) + i));
+        }
 #pragma unroll 1
         for (int x = 0; x < cols; x += 32) {
           uint32_t rr[32], r1[32];
@@ -803,22 +840,24 @@ __global__ void __launch_bounds__(kTreeThreads, 1)
               }
             }
           }
-          if (there) {
-            if (w.whole) {
+          if (w.whole) {
+            uint4 o[4];
 #pragma unroll
-              for (int e = 0; e < 32; e += 8) {
-                uint4 o;
-                o.x = pack_bf16x2(__uint_as_float(rr[e + 0]), __uint_as_float(rr[e + 1]));
-                o.y = pack_bf16x2(__uint_as_float(rr[e + 2]), __uint_as_float(rr[e + 3]));
-                o.z = pack_bf16x2(__uint_as_float(rr[e + 4]), __uint_as_float(rr[e + 5]));
-                o.w = pack_bf16x2(__uint_as_float(rr[e + 6]), __uint_as_float(rr[e + 7]));
-                *reinterpret_cast<uint4*>(dst + col0 + x + e) = o;
-              }
-            } else {
-#pragma unroll
-              for (int e = 0; e < 32; e += 4)
-                *reinterpret_cast<uint4*>(part + ((size_t)((col0 + x + e) >> 2) * Sh::kRows + part_row) * 4) = make_uint4(rr[e], rr[e + 1], rr[e + 2], rr[e + 3]);
+            for (int g = 0; g < 4; ++g) {
+              const uint32_t* e = rr + 8 * g;
+              o[g].x = pack_bf16x2(__uint_as_float(e[0]), __uint_as_float(e[1]));
+              o[g].y = pack_bf16x2(__uint_as_float(e[2]), __uint_as_float(e[3]));
+              o[g].z = pack_bf16x2(__uint_as_float(e[4]), __uint_as_float(e[5]));
+              o[g].w = pack_bf16x2(__uint_as_float(e[6]), __uint_as_float(e[7]));
             }
+            tree_quads(o);
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              if (quad[i]) *reinterpret_cast<uint4*>(quad[i] + col0 + x + (lane & 3) * 8) = o[i];
+          } else if (there) {
+#pragma unroll
+            for (int e = 0; e < 32; e += 4)
+              *reinterpret_cast<uint4*>(part + ((size_t)((col0 + x + e) >> 2) * Sh::kRows + part_row) * 4) = make_uint4(rr[e], rr[e + 1], rr[e + 2], rr[e + 3]);
           }
         }
         if (!w.whole && there && (w.two || half == 0)) {
