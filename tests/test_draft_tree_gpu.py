@@ -251,6 +251,23 @@ def test_attention_of_chains_is_the_prefill_kernels():
     assert bool(((got.double() - other.double()).abs() <= 2 * bound).all())
 
 
+def test_cells_past_32_bits():
+    """Pages at the end of a cache of 2.6 G values: the same bits as at the beginning of a small one, values that are not finite included; moves too."""
+    case, scale = attention_case([9, 40], [300, 900], hq=16, hkv=8, d=128, page=256, seed=5, device=DEV)
+    small = case["kv_cache"]
+    end = int(case["seq_lens"][0]) - 1                           # (the last node, which the others do not see)
+    small[case["block_table"][0, end // 256].long(), 1, end % 256, :, 3] = math.inf
+    large = torch.empty((5000, *small.shape[1:]), dtype=torch.bfloat16, device=DEV)
+    large[-len(small):] = small
+    there = dict(case, kv_cache=large, block_table=case["block_table"] + (5000 - len(small)))
+    want = run_attention(case, scale)
+    assert torch.equal(run_attention(there, scale).view(torch.int16), want.view(torch.int16)) and bool(torch.isinf(want).any())
+    path = torch.tensor([[0, 2, 5, 8, -1], [0, 7, 8, 30, 39]], dtype=torch.int32, device=DEV)
+    for c in (case, there):
+        draft_tree.compact(c["kv_cache"], block_table=c["block_table"], seq_lens=c["seq_lens"], q_start=c["q_start"], path=path)
+    assert torch.equal(large[-len(small):].view(torch.int16), small.view(torch.int16))
+
+
 def ops_tiles(sizes):
     from vllm_cpp_b200.ops.reference import build_prefill_tiles
     req, q0 = build_prefill_tiles(sizes)
