@@ -92,19 +92,17 @@ __device__ __forceinline__ float verify_ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-// Weights e^(l - m) of a row whose largest logit is m: 0 for -inf and NaN, and 1 for m itself where it is infinite, or too large for log2 units. (In log2 units the
-// argument is off by 2^-24 of itself, which is 2^-20 of a weight that is 2^-16 of the largest, and all arguments by the same rounding of m.)
+// Weights e^(l - m) of a row whose largest logit is m: 0 for -inf and NaN, and 1 for m itself, where it is infinite too. l - m comes first, and near m it is exact: a row's
+// weights, and the factors that turn a warp's sum into a CTA's and a cluster's, are the same whatever all its logits have in common. (In log2 units l and m would each carry a
+// rounding of 2^-24 of themselves: one fused instruction a column less, and sums off by 2e-4 against the weights at logits of 3000, by 6 % at a million.) The difference
+// rounds by 2^-24 of itself, which is 2^-20 of a weight that is 2^-16 of the largest.
 struct Weights {
-  float m, m2;
-  bool far;
-  __device__ __forceinline__ Weights(float m_) : m(m_), m2(m_ * 1.4426950408889634f), far(!(fabsf(m_) < 1e38f)) {}
-  __device__ __forceinline__ float plain(float l) const { return verify_ex2(fmaf(l, 1.4426950408889634f, -m2)); }         // not far, not NaN
+  float m;
+  bool far;                            // m is infinite: the others of the row have no weight
+  __device__ __forceinline__ Weights(float m_) : m(m_), far(!(fabsf(m_) <= FLT_MAX)) {}
+  __device__ __forceinline__ float plain(float l) const { return verify_ex2((l - m) * 1.4426950408889634f); }             // not far, not NaN
   __device__ __forceinline__ float of(float l) const { return plain(logit_of(l)); }
-  __device__ __forceinline__ float any(float l) const {
-    if (!far) return of(l);
-    l = logit_of(l);
-    return l == -INFINITY ? 0.f : l == m ? 1.f : __expf(l - m);
-  }
+  __device__ __forceinline__ float any(float l) const { return !far ? of(l) : l == m && m > 0.f ? 1.f : 0.f; }
 };
 __device__ __forceinline__ float weight_of(float l, float m) { return Weights(m).any(l); }
 

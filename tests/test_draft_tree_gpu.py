@@ -410,6 +410,57 @@ def test_verify_of_odd_logits():
     check_verify(dict(case, temperature=torch.zeros(5)))
 
 
+@pytest.mark.parametrize("drawn", [True, False])
+@pytest.mark.parametrize("offset", [0.0, 100.0, 3e3, -3e3, 2e5, 1e6, 1e30])
+def test_verify_does_not_depend_on_what_all_logits_have_in_common(offset, drawn):
+    """Logits far from 0, rounded to 32 bits before the rule in 64 bits sees them; where they are rounded to whole numbers, many share the largest."""
+    for vocab, wide, whole in ((700, 1, False), (2500, 3, False), (2500, 3, True)):
+        case = verify_case([4, 2, 7] * 8, vocab, wide=wide, drawn=drawn, seed=int(math.log2(abs(offset) + 1)), cold=0.1)
+        case["logits"] = (case["logits"].round() if whole else case["logits"]) + offset
+        check_verify(case)
+
+
+@pytest.mark.parametrize("drawn", [True, False])
+@pytest.mark.parametrize("vocab", [700, 2500])
+@pytest.mark.parametrize("offset", [0.0, 100.0, 3e3, 2e5, 1e6])
+def test_verify_accepts_up_to_the_border(offset, vocab, drawn):
+    """One draft of each request, asked with numbers a little below and above what it is accepted with. Weights are off by 2^-20 at the most down to a 2^-16 of the
+    largest (their argument's rounding, an exponential of 2^-22), their sum by as much and by 24 roundings of 2^-24, q and the number by one each: 2^-17.5 in all."""
+    R = 200
+    gen = torch.Generator().manual_seed(vocab)
+    logits = torch.randn((R, vocab), generator=gen) * 1.5 + offset
+    p = torch.softmax(logits.double(), 1)
+    token = torch.where(torch.arange(R) % 2 == 0, logits.argmax(1), logits.topk(40, 1).indices[:, 39])
+    of_token = p.gather(1, token[:, None])[:, 0]
+    share = torch.rand(R, generator=gen) * 0.8 + 0.1                      # of the draws that are accepted
+    probs = torch.full((R, vocab), 0.5 / vocab)
+    border = of_token
+    if drawn:
+        probs.scatter_(1, token[:, None], (of_token / share).float()[:, None])
+        border = of_token / probs.gather(1, token[:, None])[:, 0].double()
+    for factor, accepted in ((1 - 2.0 ** -16, True), (1 + 2.0 ** -16, False)):
+        _, _, count = draft_tree.verify(
+            logits.repeat_interleave(2, 0).to(DEV), token.repeat_interleave(2).to(DEV), q_start=(torch.arange(R + 1) * 2).int().to(DEV),
+            uniforms=(border * factor).float().repeat_interleave(2).to(DEV), seeds=torch.arange(R, device=DEV), steps=torch.arange(R, device=DEV), max_tokens=2,
+            draft_probs=probs.repeat_interleave(2, 0).to(DEV) if drawn else None)
+        assert bool((count == (2 if accepted else 1)).all()), (factor, int((count != (2 if accepted else 1)).sum()))
+
+
+def test_verify_of_rows_with_one_likely_token():
+    """All of a row's weight on one token, which its draft is: whatever the logit, it is accepted with every number below one."""
+    R, V = 64, 2500
+    top = torch.linspace(130.0, 30000.0, R)
+    logits = torch.zeros((R, V))
+    logits[:, 7] = top
+    logits = logits.repeat_interleave(2, 0).to(DEV)
+    common = dict(q_start=(torch.arange(R + 1) * 2).int().to(DEV), uniforms=torch.full((2 * R,), 1 - 2.0 ** -24, device=DEV),
+                  seeds=torch.arange(R, device=DEV), steps=torch.arange(R, device=DEV), max_tokens=2)
+    tokens = torch.full((2 * R,), 7, device=DEV)
+    for probs in (None, torch.nn.functional.one_hot(tokens, V).float()):
+        out, _, count = draft_tree.verify(logits, tokens, draft_probs=probs, **common)
+        assert bool((count == 2).all()) and bool((out == 7).all())
+
+
 def test_verify_of_the_same_draft_twice():
     """The second of two chosen drafts alike has no weight left; drawn ones count each for itself."""
     case = verify_case([5] * 60, 6, wide=9, drawn=False, seed=7, cold=0.0, spread=1.0)
