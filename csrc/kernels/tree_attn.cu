@@ -972,6 +972,7 @@ extern "C" int b200_tree_attn(const B200TreeAttn* a, cudaStream_t stream) {
   p.block_size = bs; p.max_len = a->max_blocks * bs;
   p.window = a->positions && a->window <= p.max_len ? a->window : 0;         // (one that holds any context is none)
   p.scale_log2 = a->scale * 1.4426950408889634f; p.cap2 = a->softcap * 1.4426950408889634f;
+  if (!(p.scale_log2 > 0.f && p.scale_log2 < INFINITY && p.cap2 >= 0.f && p.cap2 < INFINITY)) return -1;
   p.parts = (float*)a->parts; p.status = device_status_word();
   CUtensorMap tmQ, tmKV;
   if (!encode_tmap_3d(&tmQ, a->q, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, (uint64_t)D, (uint64_t)a->Hq, (uint64_t)a->total_q, (uint64_t)D * 2,

@@ -135,6 +135,14 @@ def test_attention_refuses(what, change):
         draft_tree.attention(**args)
 
 
+@pytest.mark.parametrize("name", ["scale", "softcap"])
+@pytest.mark.parametrize("value", [1e-50, 2.0 ** -150, 2.36e38, 1e39, 1e300, math.nan])
+def test_attention_refuses_numbers_that_32_bits_do_not_hold(name, value):
+    """Below half the least number of 32 bits a cap would be none and a scale 0; above 2.35e38 they overflow in log2 units."""
+    with pytest.raises(OpArgumentError, match=f"{name} is|softcap not"):
+        draft_tree.attention(**{**attention_args(), name: value})
+
+
 def mask_args():
     return dict(parents=torch.tensor([-1, 0, 1], dtype=torch.int32), q_start=starts_of([3]), seq_lens=torch.tensor([7], dtype=torch.int32))
 

@@ -27,7 +27,7 @@ import torch
 
 from . import _lib, reference
 from ._lib import check, lib, stream_ptr
-from .validate import OpArgumentError, validate
+from .validate import LEAST_F32, MOST_LOG2_F32, OpArgumentError, validate
 
 MOST_NODES = 1024
 BF16, _I32, _I64, _F32 = torch.bfloat16, torch.int32, torch.int64, torch.float32
@@ -139,7 +139,8 @@ def attention(q: torch.Tensor, kv_cache: torch.Tensor, *, block_table: torch.Ten
     ``c + n - 1``; the bits alone say which nodes it sees). What a node does not see does not reach it, infinities and NaN among the values
     included. Entries of ``block_table`` outside the cache count as keys and values of zeros. ``out`` shares no memory with the rows of ``q``. ``tmp``:
     :func:`scratch`, allocated if not given. head_dim 64, 128 or 256, at most 128 query heads a kv head, pages that divide a tile of 64
-    tokens or are whole tiles; at most 8192 requests."""
+    tokens or are whole tiles; at most 8192 requests. ``scale`` and ``softcap`` are held in
+    32 bits: below 2.35e38, and not so small that they would be 0."""
     given = out is not None
     try:
         (T, cols), (nb, two, bs, H, D), (treqs, pages), (reqs,), (rows, words) = q.shape, kv_cache.shape, block_table.shape, q_start.shape, mask.shape
@@ -148,7 +149,8 @@ def attention(q: torch.Tensor, kv_cache: torch.Tensor, *, block_table: torch.Ten
               and kv_cache.dtype is BF16 and block_table.dtype is _I32 and mask.dtype is _I64 and two == 2 and H > 0 and cols > 0
               and (D == 128 or D == 64 or D == 256) and cols % (D * H) == 0 and kv_cache.is_contiguous() and q1 == t1 == 1 and pages > 0
               and treqs >= reqs - 1 and (qp | cp | 2 * ldq) % 16 == 0 and rows >= T and words > 0 and mask.is_contiguous()
-              and _ids(seq_lens, _I32, dev, reqs - 1) and _ids(q_start, _I32, dev, 1) and 0 < scale < math.inf and 0 <= softcap < math.inf
+              and _ids(seq_lens, _I32, dev, reqs - 1) and _ids(q_start, _I32, dev, 1)
+              and LEAST_F32 < scale <= MOST_LOG2_F32 and (softcap == 0 or LEAST_F32 < softcap <= MOST_LOG2_F32)
               and 0 <= window < 2 ** 31 and (window == 0 or _ids(positions, _I64, dev, T)))
         if ok and given:
             (orows, ocols), (ldo, o1), op_ = out.shape, out.stride(), out.data_ptr()

@@ -39,6 +39,8 @@ def _rows16(t: torch.Tensor) -> bool:
 
 
 BF16 = torch.bfloat16
+# Numbers that are 0 in 32 bits; the largest whose log2(e)-fold is finite there.
+LEAST_F32, MOST_LOG2_F32 = 2.0 ** -150, 2.35e38
 
 RULES: dict[str, list] = {
     "gemm": [
@@ -264,7 +266,8 @@ RULES.update({
         ("block_table is int32 [requests, pages], rows contiguous", lambda block_table, q_start, **_: _table(block_table, q_start.numel() - 1)),
         ("mask is int64 [T, words], contiguous", lambda q, mask, **_: mask.dtype == torch.int64 and mask.dim() == 2 and mask.shape[0] >= q.shape[0]
          and mask.shape[1] > 0 and mask.is_contiguous()),
-        ("scale is positive and finite, softcap finite and not negative", lambda scale, softcap, **_: 0 < scale < math.inf and 0 <= softcap < math.inf),
+        ("scale is positive, softcap not negative, both within 32 bits", lambda scale, softcap, **_: LEAST_F32 < scale <= MOST_LOG2_F32
+         and (softcap == 0 or LEAST_F32 < softcap <= MOST_LOG2_F32)),
         ("window is not negative and below 2^31, and has positions int64 [T]", lambda q, window, positions, **_: 0 <= window < 2 ** 31
          and (window == 0 or (positions is not None and _ids(positions, torch.int64, q.shape[0])))),
         ("tmp is fp32 and large enough", lambda kv_cache, tmp, **_: tmp is None or (tmp.dtype == torch.float32 and tmp.is_contiguous()
