@@ -220,7 +220,7 @@ typedef struct B200BiasAttn {
 
 // Attention of trees of drafted tokens over a paged bf16 cache [num_blocks, 2, block_size, Hkv, D] (tree_attn.cu). Request r has the nodes q_start[r] ..
 // q_start[r + 1] (int32, ascending), whose cells are the last of its seq_lens[r]; the cells before them are its context. A node sees the context and the
-// nodes whose bits are set in its row of mask. window > 0: of the context only what lies less than window before the node's position (int64; from the
+// nodes whose bits are set in its row of mask. window > 0: of both only what lies less than window before the node's position (int64; from the
 // context's length on, a node number more at most). Rows and cache lie on 16-byte boundaries. parts: b200_tree_attn_scratch floats, for this call alone until it
 // is done. At most 8192 requests, 1024 nodes a request; positions / 64 times kv heads times a request's tiles of 128 rows below 2^31 (-4).
 typedef struct B200TreeAttn {

@@ -2,8 +2,8 @@
 //
 //   o_i = sum_k p_ik v_k,  p_i = softmax over the keys k that node i sees of cap(scale q_i . k_k)
 //
-// A request has a context of c cells and n nodes whose keys and values lie behind it (node j at position c + j). Node i sees the context (its last
-// `window` positions, if there is a window) and the nodes whose bits are set in its mask. A node that sees nothing gives zeros.
+// A request has a context of c cells and n nodes whose keys and values lie behind it (node j in cell c + j). Node i sees the context and the nodes whose bits are
+// set in its mask; of either, if there is a window, only what lies less than `window` before its own position. A node that sees nothing gives zeros.
 //
 // Bound: a node's G query heads of a kv head share every key and value, so that rows = n G rows of scores read 4 D bytes a key once: with up to
 // 256 rows a request the cache's bytes are the floor, above it the products and exponentials. Rows are therefore the 128-row operand (a thread
@@ -309,8 +309,9 @@ __device__ __forceinline__ void tree_quads(uint4 (&x)[4]) {
   }
 }
 
-// Bits of the keys key .. key + 31 that a row sees.
-__device__ __forceinline__ uint32_t tree_seen(const uint64_t* mask, int words, int key, int ctx, int len, int low) {
+// Bits of the keys key .. key + 31 that a row sees. low: the first position in its window (INT_MIN: no window). The context's cells lie at their own positions, the
+// nodes of the request at `positions`, behind the context: a window ends among them only where it is shorter than the tree is deep.
+__device__ __forceinline__ uint32_t tree_seen(const uint64_t* mask, int words, const int64_t* positions, int key, int ctx, int len, int low) {
   const int rel = key - ctx;
   uint32_t v = 0xffffffffu;
   if (rel > -32) {
@@ -320,7 +321,13 @@ __device__ __forceinline__ uint32_t tree_seen(const uint64_t* mask, int words, i
     v = rel >= 0 ? (uint32_t)w : (uint32_t)w << -rel | ((1u << -rel) - 1);
   }
   if (len - key < 32) v &= len > key ? (1u << (len - key)) - 1 : 0;
-  if (key < low) v &= low - key < 32 ? ~((1u << (low - key)) - 1) : 0;
+  const int edge = min(low, ctx);
+  if (key < edge) v &= edge - key < 32 ? ~((1u << (edge - key)) - 1) : 0;
+  if (low > ctx && rel > -32) {        // (all of the context is hidden: what is left are nodes)
+#pragma unroll 1
+    for (uint32_t left = v; left; left &= left - 1)
+      if (positions[rel + __ffs(left) - 1] < low) v &= ~(left & -left);
+  }
   return v;
 }
 
@@ -602,12 +609,12 @@ __global__ void __launch_bounds__(kTreeThreads, 1)
       const bool there = row_node < p.nodes && node < w.n;
       const bool idle = !__any_sync(0xffffffffu, there);               // (its rows may hold anything: no other warp reads them)
       const uint64_t* bits = p.mask + (size_t)(w.row0 + (there ? node : 0)) * p.words;
-      int low = 0;
+      int low = INT_MIN;
       if (p.window > 0 && there) {     // (a node lies at most n - 1 positions behind the root)
         const long long depth = p.positions[w.row0 + node] - w.ctx;
-        low = min(w.ctx, w.ctx + (int)min(max(depth, 0ll), (long long)w.n - 1) - p.window + 1);
+        low = w.ctx + (int)min(max(depth, 0ll), (long long)w.n - 1) - p.window + 1;
       }
-      const auto seen_word = [&](int key) { return there ? tree_seen(bits, p.words, key, w.ctx, w.len, low) : 0u; };
+      const auto seen_word = [&](int key) { return there ? tree_seen(bits, p.words, p.positions + w.row0, key, w.ctx, w.len, low) : 0u; };
       // tiles in which the nodes of the request may differ in what they see: up to where a window begins for all of them, and from the context's end on
       const int odd_to = p.window > 0 ? w.ctx - p.window + w.n - w.key0 : INT_MIN, odd_from = w.ctx - w.key0 - K + 1;
       float m = -INFINITY, l = 0.f;

@@ -30,6 +30,27 @@ def test_the_attentions_restatement_of_a_chain_is_causal_attention(window, softc
     assert float((got - want).abs().max()) < 1e-4
 
 
+@pytest.mark.parametrize("window", [1, 2, 7, 30, 31])
+def test_the_attentions_restatement_of_a_chain_longer_than_its_window(window):
+    """A window ends among the nodes too: causal attention in that window."""
+    case, scale = attention_case([40, 1, 100], [50, 0, 0], hq=4, hkv=2, d=64, page=16, wide=1)
+    got = draft_tree.ref_attention(scale=scale, window=window, **case)
+    want = reference.paged_attention(case["q"].float(), case["kv_cache"], case["block_table"], case["seq_lens"], case["q_start"], 4, 2, 64, 16, scale, 0.0, window)
+    assert float((got - want).abs().max()) < 1e-4
+
+
+@pytest.mark.parametrize("window", [1, 2, 3, 20])
+def test_the_attentions_restatement_of_a_path_in_a_window(window):
+    """The last `window` of what its path, context and ancestors, holds."""
+    case, scale = attention_case([60], [10], hq=2, hkv=1, d=64, page=16, wide=2, seed=4)
+    got = draft_tree.ref_attention(scale=scale, dtype=torch.float64, window=window, **case)
+    for node in (59, 31, 0):
+        line = ([*range(10)] + [10 + j for j in range(60) if int(case["mask"][node, 0]) >> j & 1])[-window:]
+        kv = case["kv_cache"][case["block_table"][0].long()].transpose(1, 2).reshape(-1, 2, 1, 64)[line].double()
+        s = torch.einsum("hd,kd->hk", case["q"][node].view(2, 64).double(), kv[:, 0, 0]) * scale
+        assert torch.allclose(got[node].view(2, 64), s.softmax(-1) @ kv[:, 1, 0], atol=1e-12)
+
+
 def test_the_attentions_restatement_of_a_path_is_causal_attention_of_that_path():
     """A node of a tree sees what it would see if its ancestors stood alone behind the context."""
     case, scale = attention_case([17], [33], hq=2, hkv=1, d=64, page=16, wide=4, seed=4)

@@ -101,6 +101,43 @@ def test_attention_in_a_window(d, window):
     check_attention(case, scale, window=window)
 
 
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("window", [1, 2, 3, 8, 63, 130])
+def test_attention_in_a_window_that_ends_among_the_nodes(d, window):
+    """Trees and chains deeper than the window, capped and not; also where rows of no tree lie between them."""
+    for wide, sizes in ((1, [9, 200, 1, 70]), (2, [64, 0, 300, 33])):
+        case, scale = attention_case(sizes, [77, 20, 0, 500], hq=6, hkv=2, d=d, page=16, seed=window, wide=wide, device=DEV)
+        check_attention(case, scale, window=window)
+        check_attention(case, scale, window=window, softcap=20.0)
+
+
+@pytest.mark.parametrize("window", [5, 64, 200, 1000])
+def test_attention_of_chains_in_a_window_is_the_prefill_kernels(window):
+    """Chains longer than a window, a prompt's among them: what attn_prefill computes, within both kernels' roundings."""
+    sizes, contexts = [1000, 3, 130, 70], [0, 77, 1200, 3]
+    case, scale = attention_case(sizes, contexts, hq=8, hkv=2, d=128, page=16, wide=1, device=DEV)
+    got = run_attention(case, scale, window=window)
+    req, q0 = ops_tiles(sizes)
+    other = ops.attn_prefill(case["q"].contiguous(), case["kv_cache"], block_table=case["block_table"], seq_lens=case["seq_lens"], q_start=case["q_start"],
+                             tile_req=req, tile_q0=q0, num_q_heads=8, num_kv_heads=2, head_dim=128, block_size=16, scale=scale, window=window)
+    _, bound = attention_bound(case, scale, window=window)
+    assert bool(((got.double() - other.double()).abs() <= 2 * bound).all())
+
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_attention_keeps_out_nodes_before_a_window(d):
+    """NaN in an ancestor reaches the nodes below it that lie less than a window behind it, and no other."""
+    case, scale = attention_case([100], [40], hq=8, hkv=2, d=d, page=16, seed=d, wide=2, device=DEV)
+    clean = run_attention(case, scale, window=6).clone()
+    node = max((case["positions"] == 45).nonzero().flatten().tolist(), key=lambda j: int((case["mask"][:, j // 64] >> (j % 64) & 1).sum()))
+    bad = dict(case, kv_cache=case["kv_cache"].clone())
+    bad["kv_cache"][int(case["block_table"][0, (40 + node) // 16]), :, (40 + node) % 16] = math.nan
+    got = run_attention(bad, scale, window=6)
+    below = (case["mask"][:, node // 64] >> (node % 64) & 1).bool()
+    reached = below & (case["positions"] < 45 + 6)
+    assert bool((below & ~reached).any()) and torch.equal(got[~reached], clean[~reached]) and bool(got[reached].isnan().all())
+
+
 @pytest.mark.parametrize("window", [400, 2 ** 31 - 1])
 def test_attention_in_a_window_that_holds_everything(window):
     """Lengths that are shorter than the request's nodes too."""

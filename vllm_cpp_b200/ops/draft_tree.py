@@ -135,8 +135,8 @@ def attention(q: torch.Tensor, kv_cache: torch.Tensor, *, block_table: torch.Ten
               softcap: float = 0.0, window: int = 0, tmp: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Attention of the nodes ``q`` ``[T, Hq * D]`` (any row stride in steps of 8): each sees its request's context and the nodes whose bits
     are set in its row of ``mask`` (int64 ``[T, words]``, as :func:`mask` makes it, or any other); a node that sees nothing gives zeros. ``window``:
-    of the context a node sees only what lies less than ``window`` before it; that takes its ``positions`` (from ``c`` to
-    ``c + n - 1``; the bits alone say which nodes it sees). What a node does not see does not reach it, infinities and NaN among the values
+    of the context and of those nodes it sees only what lies less than ``window`` before it; that takes the nodes' ``positions``, as :func:`mask` makes
+    them (from ``c`` to ``c + n - 1``). What a node does not see does not reach it, infinities and NaN among the values
     included. Entries of ``block_table`` outside the cache count as keys and values of zeros. ``out`` shares no memory with the rows of ``q``. ``tmp``:
     :func:`scratch`, allocated if not given. head_dim 64, 128 or 256, at most 128 query heads a kv head, pages that divide a tile of 64
     tokens or are whole tiles; at most 8192 requests. ``scale`` and ``softcap`` are held in
@@ -300,7 +300,8 @@ def seen_by(mask, *, q_start, seq_lens, positions=None, window=0) -> list:
         seen = torch.where(key < c, torch.ones_like(bit), bit)
         if window > 0:
             at = positions[first: first + n].clamp(min=c, max=c + n - 1)
-            seen &= (key >= c) | (key > at[:, None] - window)
+            lies = torch.where(key < c, key, at[node.clamp(max=n - 1)]) if n else key
+            seen &= lies > at[:, None] - window
         out.append(seen)
     return out
 
