@@ -58,8 +58,8 @@ __global__ void __launch_bounds__(256)
   pdl_wait();
   pdl_launch_dependents();
   const int req = blockIdx.x;
-  const int row0 = min(max(q_start[req], 0), total), n = max(0, min(q_start[req + 1], total) - row0);
-  const long long context = (long long)min(max(seq_lens[req], 0), (int)min((long long)max_blocks * block_size, (1ll << 31) - 1)) - n;
+  const int row0 = min(max(q_start[req], 0), total), rows = max(0, min(q_start[req + 1], total) - row0), n = min(rows, kCellNodes);
+  const long long context = (long long)min(max(seq_lens[req], 0), (int)min((long long)max_blocks * block_size, (1ll << 31) - 1)) - rows;
   const int32_t* bt = block_table + req * ldt;
   const auto cell = [&](long long position) {
     const int blk = bt[position / block_size];
@@ -77,13 +77,13 @@ __global__ void __launch_bounds__(256)
       const bool is = a >= 0 && b >= 0;
       const uint32_t who = __ballot_sync(0xffffffffu, is);
       const int at = found + __popc(who & ((1u << threadIdx.x) - 1));
-      if (is && at < kCellNodes) {
+      if (is) {
         from[at] = a;
         to[at] = b;
       }
       found += __popc(who);
     }
-    if (threadIdx.x == 0) moves = min(found, kCellNodes);
+    if (threadIdx.x == 0) moves = found;
   }
   __syncthreads();
   const int count = moves;

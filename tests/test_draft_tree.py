@@ -21,6 +21,23 @@ def test_the_masks_restatement():
     assert bits[63].tolist() == [-1, 0, 0] and bits[129].tolist() == [-1, -1, 3]
 
 
+def test_the_restatements_of_more_than_1024_nodes():
+    """Nodes past the 1024th are left out, and lie behind the context all the same."""
+    n, c = 1030, 9
+    q_start, lens = starts_of([n]), torch.tensor([n + c], dtype=torch.int32)
+    bits, positions = draft_tree.ref_mask(torch.arange(-1, n - 1, dtype=torch.int32), q_start=q_start, seq_lens=lens, max_nodes=1024)
+    assert positions[:1024].tolist() == list(range(c, c + 1024)) and not bool(bits[1024:].any())
+    seen = draft_tree.seen_by(bits, q_start=q_start, seq_lens=lens)[0]
+    assert seen.sum(1).tolist() == list(range(c + 1, c + 1025)) and bool(seen[:, :c].all()) and not bool(seen[:, c + 1024:].any())
+    table, pages = page_table([n + c], 64, torch.Generator().manual_seed(1))
+    cache = torch.arange(pages * 2 * 64 * 4).view(pages, 2, 64, 1, 4).float()
+    before = cache.clone()
+    draft_tree.ref_compact(cache, block_table=table, seq_lens=lens, q_start=q_start, path=torch.tensor([[0, 3, 1023, 1024, 1029]]))
+    cell = lambda x, at: x[table[0, at // 64], :, at % 64]  # noqa: E731
+    assert torch.equal(cell(cache, c + 1), cell(before, c + 3)) and torch.equal(cell(cache, c + 2), cell(before, c + 1023))
+    assert all(torch.equal(cell(cache, c + j), cell(before, c + j)) for j in (0, 3, 4, 1023, 1024))
+
+
 @pytest.mark.parametrize("window,softcap", [(0, 0.0), (40, 0.0), (0, 20.0)])
 def test_the_attentions_restatement_of_a_chain_is_causal_attention(window, softcap):
     case, scale = attention_case([6, 1, 30], [50, 0, 77], hq=4, hkv=2, d=64, page=16, wide=1)

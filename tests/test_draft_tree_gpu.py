@@ -610,6 +610,40 @@ def test_compact_passes_over_what_is_not_a_path():
     assert torch.equal(got.cpu(), want) and not torch.equal(want, cache)
 
 
+# ------------------------------------------------------------------------------------------------ more nodes than a request has
+def test_nodes_past_the_1024th_are_left_out():
+    """Their rows stay as they are; the others are as the restatements have them, the request's context included."""
+    sizes, contexts = [1050, 3], [70, 9]
+    case, scale = attention_case(sizes, contexts, hq=4, hkv=2, d=64, page=16, seed=2, wide=3, words=16, device=DEV)
+    parents = torch.tensor([p for n in sizes for p in tree_parents(n, random.Random(1), 3)], dtype=torch.int32, device=DEV)
+    bits = torch.full((sum(sizes), 16), 77, dtype=torch.int64, device=DEV)
+    positions = torch.full((sum(sizes),), 78, dtype=torch.int64, device=DEV)
+    at = dict(q_start=case["q_start"], seq_lens=case["seq_lens"])
+    draft_tree.mask(parents, max_nodes=1024, bits=bits, positions=positions, **at)
+    want = draft_tree.ref_mask(parents, max_nodes=1024, **at)
+    node = torch.ones(sum(sizes), dtype=torch.bool, device=DEV)
+    node[1024: 1050] = False
+    assert torch.equal(bits[node], want[0][node]) and torch.equal(positions[node], want[1][node])
+    assert bool((bits[~node] == 77).all()) and bool((positions[~node] == 78).all())
+    case["mask"], case["positions"] = want
+    for window in (0, 40):
+        got = run_attention(case, scale, window=window)
+        o, bound = attention_bound(case, scale, window=window)
+        assert bool(((got.double() - o).abs() <= bound)[node].all()) and bool((got[~node] == 7).all())
+    gen = torch.Generator().manual_seed(1)
+    logits, ids = torch.randn((sum(sizes), 40), generator=gen), torch.tensor([5, 6])
+    tokens = torch.randint(0, 40, (sum(sizes),), generator=gen)
+    logits[torch.arange(1049), tokens[1: 1050]] = 60.0           # (a chain of drafts that are all accepted)
+    steps = dict(logits=logits, tokens=tokens, q_start=starts_of(sizes), uniforms=torch.full((sum(sizes),), 0.5), seeds=ids, steps=ids, max_tokens=1060)
+    out, path, count = draft_tree.verify(**on_gpu(steps))
+    assert all(torch.equal(a.cpu(), b) for a, b in zip((out, path, count), draft_tree.ref_verify(**steps))) and int(count[0]) == 1024
+    path = torch.tensor([[0, 3, 1023, 1024, 1049, -1], [0, 2, -1, -1, -1, -1]], dtype=torch.int32, device=DEV)
+    moved, kept = case["kv_cache"].clone(), case["kv_cache"].clone()
+    draft_tree.compact(moved, block_table=case["block_table"], path=path, **at)
+    draft_tree.ref_compact(kept, block_table=case["block_table"], path=path, **at)
+    assert torch.equal(moved, kept) and not torch.equal(moved, case["kv_cache"])
+
+
 # ------------------------------------------------------------------------------------------------ together
 def test_a_run_of_steps_with_trees():
     """A model of two layers decodes greedily with trees of drafts, some of them right, through the operators of a step: every token is the

@@ -10,7 +10,8 @@ context, node ``j`` at position ``c + j``, ``c = seq_lens[r] - n``; their rotary
 * ``tokens, path, count = verify(logits, ...)``;
 * ``compact(kv_caches, path=path, ...)``: the context is ``c + count`` cells now, and the last of ``tokens`` the next root.
 
-A chain of drafts is the tree whose parents count up; :func:`verify` takes ``parents=None`` for it. At most 1024 nodes a request.
+A chain of drafts is the tree whose parents count up; :func:`verify` takes ``parents=None`` for it. At most 1024 nodes a request: rows past them
+are left out (nothing sees, accepts or moves them, their outputs stay as they are), and count among the cells behind the context.
 bf16 queries and caches ``[num_blocks, 2, block_size, kv heads, head_dim]`` for the attention. Rows behind the last request are not
 touched. The ``ref_*`` functions restate the operators in plain PyTorch (any device).
 """
@@ -262,9 +263,9 @@ def compact(kv_caches: Union[torch.Tensor, Sequence[torch.Tensor]], *, block_tab
 
 # ------------------------------------------------------------------------------ restatements
 def _rows(q_start, T):
-    """(first row, nodes) of each request."""
+    """(first row, nodes, cells) of each request: those past the 1024th are no nodes, but their cells lie behind its context too."""
     at = [min(max(int(x), 0), T) for x in q_start.tolist()]
-    return [(a, min(max(0, b - a), MOST_NODES)) for a, b in zip(at, at[1:])]
+    return [(a, min(max(0, b - a), MOST_NODES), max(0, b - a)) for a, b in zip(at, at[1:])]
 
 
 def _signed(x: int) -> int:
@@ -276,7 +277,7 @@ def ref_mask(parents, *, q_start, seq_lens, max_nodes=64):
     bits = torch.zeros((parents.numel(), words), dtype=_I64, device=parents.device)
     positions = torch.zeros((parents.numel(),), dtype=_I64, device=parents.device)
     up = parents.tolist()
-    for r, (first, n) in enumerate(_rows(q_start, parents.numel())):
+    for r, (first, n, cells) in enumerate(_rows(q_start, parents.numel())):
         held, depth = [], []
         for j in range(n):
             p = up[first + j] if 0 <= up[first + j] < j else -1
@@ -284,16 +285,16 @@ def ref_mask(parents, *, q_start, seq_lens, max_nodes=64):
             depth.append(depth[p] + 1 if p >= 0 else 0)
             for w in range(words):
                 bits[first + j, w] = _signed(held[j] >> 64 * w & (1 << 64) - 1)
-            positions[first + j] = int(seq_lens[r]) - n + depth[j]
+            positions[first + j] = int(seq_lens[r]) - cells + depth[j]
     return bits, positions
 
 
 def seen_by(mask, *, q_start, seq_lens, positions=None, window=0) -> list:
     """For each request the truth values ``[n, seq_lens[r]]``: which positions its nodes see."""
     out = []
-    for r, (first, n) in enumerate(_rows(q_start, mask.shape[0])):
+    for r, (first, n, cells) in enumerate(_rows(q_start, mask.shape[0])):
         length = max(0, int(seq_lens[r]))
-        c, key = length - n, torch.arange(length, device=mask.device)
+        c, key = length - cells, torch.arange(length, device=mask.device)
         node = (key - c).clamp(min=0)
         word = mask[first: first + n][:, (node // 64).clamp(max=mask.shape[1] - 1)]
         bit = (word >> (node % 64) & 1).bool() & (node < 64 * mask.shape[1])
@@ -313,7 +314,7 @@ def ref_attention(q, kv_cache, *, block_table, seq_lens, q_start, mask, scale, p
     T, Hq = q.shape[0], q.shape[1] // D
     out = torch.zeros((T, Hq, D), dtype=dtype, device=q.device)
     seen_all = seen_by(mask, q_start=q_start, seq_lens=seq_lens, positions=positions, window=window)
-    for r, (first, n) in enumerate(_rows(q_start, T)):
+    for r, (first, n, _) in enumerate(_rows(q_start, T)):
         seen = seen_all[r]
         length = seen.shape[1]
         if not n or not length:
@@ -351,7 +352,7 @@ def ref_verify(logits, tokens, *, q_start, uniforms, seeds, steps, max_tokens, p
     rows = _rows(q_start, T)
     out = torch.full((len(rows), max_tokens), -1, dtype=_I64)
     path, count = torch.full((len(rows), max_tokens), -1, dtype=_I32), torch.zeros(len(rows), dtype=_I32)
-    for r, (first, n) in enumerate(rows):
+    for r, (first, n, _) in enumerate(rows):
         if not n:
             continue
         node, depth, greedy = 0, 0, temperature is not None and float(temperature[r]) < 1e-5
@@ -397,8 +398,8 @@ def ref_verify(logits, tokens, *, q_start, uniforms, seeds, steps, max_tokens, p
 def ref_compact(kv_caches, *, block_table, seq_lens, q_start, path) -> None:
     caches = [kv_caches] if isinstance(kv_caches, torch.Tensor) else list(kv_caches)
     nb, _, bs = caches[0].shape[:3]
-    for r, (first, n) in enumerate(_rows(q_start, 2 ** 31 - 1)):
-        c, held = int(seq_lens[r]) - n, []
+    for r, (first, n, cells) in enumerate(_rows(q_start, 2 ** 31 - 1)):
+        c, held = int(seq_lens[r]) - cells, []
 
         def cell(position):
             return int(block_table[r, position // bs]), position % bs
@@ -408,5 +409,5 @@ def ref_compact(kv_caches, *, block_table, seq_lens, q_start, path) -> None:
                 (b, o), to = cell(c + node), cell(c + i)
                 if 0 <= b < nb and 0 <= to[0] < nb:
                     held += [(x, to, x[b, :, o].clone()) for x in caches]
-        for x, (b, o), cells in held:
-            x[b, :, o] = cells
+        for x, (b, o), kv in held:
+            x[b, :, o] = kv
