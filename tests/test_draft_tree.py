@@ -155,6 +155,12 @@ def attention_args():
     ("block_table", lambda a: a.update(block_table=a["block_table"].long())),
     ("mask is", lambda a: a.update(mask=a["mask"][:5])),
     ("mask is", lambda a: a.update(mask=a["mask"].int())),
+    ("at most 16 words", lambda a: a.update(mask=torch.zeros((8, 17), dtype=torch.int64))),
+    ("at most 128 query heads", lambda a: a.update(q=torch.zeros((8, 2 * 129 * 64), dtype=torch.bfloat16))),
+    ("at most 8192 requests", lambda a: a.update(q_start=torch.zeros(8194, dtype=torch.int32), seq_lens=torch.zeros(8193, dtype=torch.int32),
+                                                 block_table=torch.zeros((8193, 1), dtype=torch.int32))),
+    ("block_size divides", lambda a: a.update(kv_cache=torch.zeros((3, 2, 48, 2, 64), dtype=torch.bfloat16))),
+    ("block_size divides", lambda a: a.update(kv_cache=torch.zeros((3, 2, 4, 2, 64), dtype=torch.bfloat16))),
     ("scale", lambda a: a.update(scale=0.0)),
     ("scale", lambda a: a.update(scale=math.inf)),
     ("softcap", lambda a: a.update(softcap=-1.0)),
@@ -191,6 +197,7 @@ def mask_args():
     ("seq_lens", lambda a: a.update(seq_lens=a["seq_lens"][:0])),
     ("max_nodes", lambda a: a.update(max_nodes=0)),
     ("max_nodes", lambda a: a.update(max_nodes=1025)),
+    ("max_nodes", lambda a: a.update(max_nodes=None)),
     ("bits", lambda a: a.update(bits=torch.zeros((3, 2), dtype=torch.int64))),
     ("positions", lambda a: a.update(positions=torch.zeros(3, dtype=torch.int32))),
     ("apart", lambda a: a.update(bits=(b := torch.zeros((3, 1), dtype=torch.int64)), positions=b[:, 0])),
@@ -211,6 +218,7 @@ def verify_args():
 @pytest.mark.parametrize("what,change", [
     ("logits", lambda a: a.update(logits=a["logits"].bfloat16())),
     ("logits", lambda a: a.update(logits=torch.zeros((9, 3)).t())),
+    ("778000 columns", lambda a: a.update(logits=torch.zeros((3, 778001)))),
     ("tokens", lambda a: a.update(tokens=a["tokens"].int())),
     ("uniforms", lambda a: a.update(uniforms=a["uniforms"][:2])),
     ("q_start", lambda a: a.update(q_start=a["q_start"].long())),

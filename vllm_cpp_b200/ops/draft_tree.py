@@ -30,7 +30,7 @@ from . import _lib, reference
 from ._lib import check, lib, stream_ptr
 from .validate import LEAST_F32, MOST_LOG2_F32, OpArgumentError, validate
 
-MOST_NODES = 1024
+MOST_NODES, MOST_COLUMNS = 1024, 778000
 BF16, _I32, _I64, _F32 = torch.bfloat16, torch.int32, torch.int64, torch.float32
 _P, _L, _I, _F = ctypes.c_void_p, ctypes.c_longlong, ctypes.c_int, ctypes.c_float
 
@@ -90,8 +90,8 @@ def mask(parents: torch.Tensor, *, q_start: torch.Tensor, seq_lens: torch.Tensor
          positions: Optional[torch.Tensor] = None) -> tuple[torch.Tensor, torch.Tensor]:
     """``parents`` int32 ``[T]``, a node's within its request (-1 and what is not below the node's own number: a root) ->
     ``bits`` int64 ``[T, ceil(max_nodes / 64)]``, bit ``j`` of a row (64 a word) set for the node itself and those above it, and ``positions`` int64 ``[T]``.
-    ``max_nodes``: of the largest tree; nodes past it have no bit."""
-    words = (max_nodes + 63) // 64
+    ``max_nodes``: of the largest tree. The trees' sizes are known on the device alone: in a larger one the nodes past it have no bit, and nothing sees them, they themselves
+    included."""
     try:
         (T,), (reqs,) = parents.shape, q_start.shape
         dev = parents.get_device()
@@ -102,6 +102,7 @@ def mask(parents: torch.Tensor, *, q_start: torch.Tensor, seq_lens: torch.Tensor
     if not ok:
         validate("tree_mask", parents=parents, q_start=q_start, seq_lens=seq_lens, max_nodes=max_nodes, bits=bits, positions=positions)
         T, reqs = parents.shape[0], q_start.shape[0]
+    words = (max_nodes + 63) // 64
     _declare()
     if bits is None:
         bits = parents.new_empty((T, words), dtype=_I64)
@@ -149,7 +150,8 @@ def attention(q: torch.Tensor, kv_cache: torch.Tensor, *, block_table: torch.Ten
         ok = (dev >= 0 and dev == kv_cache.get_device() == block_table.get_device() == mask.get_device() and q.dtype is BF16
               and kv_cache.dtype is BF16 and block_table.dtype is _I32 and mask.dtype is _I64 and two == 2 and H > 0 and cols > 0
               and (D == 128 or D == 64 or D == 256) and cols % (D * H) == 0 and kv_cache.is_contiguous() and q1 == t1 == 1 and pages > 0
-              and treqs >= reqs - 1 and (qp | cp | 2 * ldq) % 16 == 0 and rows >= T and words > 0 and mask.is_contiguous()
+              and treqs >= reqs - 1 and (qp | cp | 2 * ldq) % 16 == 0 and rows >= T and 0 < words <= 16 and mask.is_contiguous()
+              and cols <= 128 * D * H and (64 % bs == 0 and bs >= 8 or bs % 64 == 0) and reqs <= 8193
               and _ids(seq_lens, _I32, dev, reqs - 1) and _ids(q_start, _I32, dev, 1)
               and LEAST_F32 < scale <= MOST_LOG2_F32 and (softcap == 0 or LEAST_F32 < softcap <= MOST_LOG2_F32)
               and 0 <= window < 2 ** 31 and (window == 0 or _ids(positions, _I64, dev, T)))
@@ -202,7 +204,7 @@ def verify(logits: torch.Tensor, tokens: torch.Tensor, *, q_start: torch.Tensor,
         (T, V), (ld, one), dev, (reqs,) = logits.shape, logits.stride(), logits.get_device(), q_start.shape
         ok = (dev >= 0 and logits.dtype is _F32 and (one == 1 or V == 1) and V > 0 and _ids(tokens, _I64, dev, T) and _ids(q_start, _I32, dev, 1)
               and _ids(uniforms, _F32, dev, T) and _ids(seeds, _I64, dev, reqs - 1) and _ids(steps, _I64, dev, reqs - 1) and max_tokens > 0
-              and (parents is None or _ids(parents, _I32, dev, T)) and (temperature is None or _ids(temperature, _F32, dev, reqs - 1)))
+              and V <= MOST_COLUMNS and (parents is None or _ids(parents, _I32, dev, T)) and (temperature is None or _ids(temperature, _F32, dev, reqs - 1)))
         if ok and draft_probs is not None:
             ok = (draft_probs.shape == logits.shape and draft_probs.dtype is _F32 and draft_probs.get_device() == dev
                   and (draft_probs.stride(1) == 1 or V == 1))

@@ -258,14 +258,17 @@ RULES.update({
     "tree_attention": [
         ("kv_cache is bf16 [blocks, 2, block_size, kv heads, head_dim], contiguous, head_dim 64, 128 or 256", lambda kv_cache, **_:
          _paged_cache(kv_cache) and kv_cache.dtype == BF16 and kv_cache.shape[4] in (64, 128, 256)),
+        ("block_size divides 64, from 8 on, or is a multiple of it", lambda kv_cache, **_: kv_cache.shape[2] in (8, 16, 32) or kv_cache.shape[2] % 64 == 0),
         ("q is [T, Hq * head_dim] bf16 with rows on 16-byte boundaries, Hq a multiple of the kv heads", lambda q, kv_cache, **_: _bf16_rows(q)
          and q.shape[1] > 0 and q.shape[1] % (kv_cache.shape[3] * kv_cache.shape[4]) == 0),
+        ("there are at most 128 query heads a kv head", lambda q, kv_cache, **_: q.shape[1] <= 128 * kv_cache.shape[3] * kv_cache.shape[4]),
         ("out is like q and apart from it, its rows apart from one another", lambda q, out, **_: _bf16_rows(out) and out.shape == q.shape
          and _apart(out) and _apart_rows(q, out)),
         _TREE_REQS,
+        ("there are at most 8192 requests", lambda q_start, **_: q_start.numel() <= 8193),
         ("block_table is int32 [requests, pages], rows contiguous", lambda block_table, q_start, **_: _table(block_table, q_start.numel() - 1)),
-        ("mask is int64 [T, words], contiguous", lambda q, mask, **_: mask.dtype == torch.int64 and mask.dim() == 2 and mask.shape[0] >= q.shape[0]
-         and mask.shape[1] > 0 and mask.is_contiguous()),
+        ("mask is int64 [T, words], contiguous, at most 16 words", lambda q, mask, **_: mask.dtype == torch.int64 and mask.dim() == 2 and mask.shape[0] >= q.shape[0]
+         and 0 < mask.shape[1] <= 16 and mask.is_contiguous()),
         ("scale is positive, softcap not negative, both within 32 bits", lambda scale, softcap, **_: LEAST_F32 < scale <= MOST_LOG2_F32
          and (softcap == 0 or LEAST_F32 < softcap <= MOST_LOG2_F32)),
         ("window is not negative and below 2^31, and has positions int64 [T]", lambda q, window, positions, **_: 0 <= window < 2 ** 31
@@ -278,6 +281,7 @@ RULES.update({
     "tree_verify": [
         ("logits is fp32 [T, V], rows contiguous", lambda logits, **_: logits.dim() == 2 and logits.dtype == torch.float32 and logits.shape[1] > 0
          and (logits.shape[1] == 1 or logits.stride(1) == 1)),
+        ("logits has at most 778000 columns", lambda logits, **_: logits.shape[1] <= 778000),
         ("tokens is int64 [T], uniforms fp32 [T]", lambda logits, tokens, uniforms, **_: _ids(tokens, torch.int64, logits.shape[0])
          and _ids(uniforms, torch.float32, logits.shape[0])),
         ("q_start is int32 [requests + 1]", lambda q_start, **_: _ids(q_start, torch.int32, 1)),
