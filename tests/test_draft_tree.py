@@ -249,6 +249,7 @@ def compact_args():
     ("16-byte", lambda a: a.update(kv_caches=[torch.zeros((4, 2, 16, 1, 4), dtype=torch.bfloat16)])),
     ("alike", lambda a: a.update(kv_caches=[torch.zeros((4, 2, 3, 16, 64), dtype=torch.bfloat16).transpose(2, 3)])),
     ("twice", lambda a: a["kv_caches"].append(a["kv_caches"][0])),
+    ("share no memory", lambda a: a.update(kv_caches=[(b := torch.zeros((7, 2, 16, 1, 64), dtype=torch.bfloat16))[3:], b[:4]])),
     ("seq_lens", lambda a: a.update(seq_lens=a["seq_lens"].long())),
     ("block_table", lambda a: a.update(block_table=a["block_table"].t())),
     ("path", lambda a: a.update(path=torch.zeros((2, 3), dtype=torch.int32))),

@@ -234,7 +234,7 @@ def verify(logits: torch.Tensor, tokens: torch.Tensor, *, q_start: torch.Tensor,
 def compact(kv_caches: Union[torch.Tensor, Sequence[torch.Tensor]], *, block_table: torch.Tensor, seq_lens: torch.Tensor,
             q_start: torch.Tensor, path: torch.Tensor) -> None:
     """Keys and values of accepted nodes move behind their context, in place and in every one of the caches (``[num_blocks, 2, block_size, kv
-    heads, head_dim]``, alike, of any type): cell ``c + path[r, i]`` to cell ``c + i``. ``path`` int32 ``[requests, steps]`` as :func:`verify`
+    heads, head_dim]``, alike, of any type, apart from one another): cell ``c + path[r, i]`` to cell ``c + i``. ``path`` int32 ``[requests, steps]`` as :func:`verify`
     gives it; entries that are not behind their own place (padding too) move nothing. ``seq_lens`` still counts all nodes."""
     caches = [kv_caches] if isinstance(kv_caches, torch.Tensor) else list(kv_caches)
     try:
@@ -243,9 +243,11 @@ def compact(kv_caches: Union[torch.Tensor, Sequence[torch.Tensor]], *, block_tab
         (nb, two, bs, H, D), (treqs, pages), (ldt, t1), (reqs,), (prows, most) = shape, block_table.shape, block_table.stride(), q_start.shape, path.shape
         cell = H * D * first.element_size()
         at = list(map(_address, caches))
+        line = sorted(at)
         ok = (dev >= 0 and two == 2 and bs > 0 and cell > 0 and cell % 16 == 0 and pages > 0 and t1 == 1 and block_table.dtype is _I32 and block_table.get_device() == dev
               and treqs >= reqs - 1 and _ids(seq_lens, _I32, dev, reqs - 1) and _ids(q_start, _I32, dev, 1) and path.dtype is _I32
-              and path.get_device() == dev and path.is_contiguous() and prows == reqs - 1 and len(set(at)) == len(at)
+              and path.get_device() == dev and path.is_contiguous() and prows == reqs - 1
+              and min(map(operator.sub, line[1:], line), default=nb * 2 * bs * cell) >= nb * 2 * bs * cell
               and not functools.reduce(operator.or_, at) % 16 and all(map(_contiguous, caches))
               and [*map(_device, caches)].count(dev) == [*map(_dtype, caches)].count(first.dtype) == [*map(_shape, caches)].count(shape) == len(at))
     except (TypeError, ValueError, AttributeError, IndexError):

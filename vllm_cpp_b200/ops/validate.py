@@ -9,6 +9,7 @@ shape / dtype / layout errors in front of every backend).
 """
 from __future__ import annotations
 
+import itertools
 import math
 
 import torch
@@ -301,6 +302,8 @@ RULES.update({
             _paged_cache(c) and c.shape == caches[0].shape and c.dtype == caches[0].dtype
             and c.shape[3] * c.shape[4] * c.element_size() % 16 == 0 for c in caches)),
         ("no cache is there twice", lambda caches, **_: len({c.data_ptr() for c in caches}) == len(caches)),
+        ("the caches share no memory", lambda caches, **_: all(b - a >= caches[0].numel() * caches[0].element_size() for a, b in itertools.pairwise(
+            sorted(c.data_ptr() for c in caches)))),
         _TREE_REQS,
         ("block_table is int32 [requests, pages], rows contiguous", lambda block_table, q_start, **_: _table(block_table, q_start.numel() - 1)),
         ("path is int32 [requests, steps], contiguous", lambda path, q_start, **_: path.dtype == torch.int32 and path.dim() == 2
