@@ -119,6 +119,55 @@ def test_the_rule_keeps_the_targets_distribution(drawn):
     assert torch.allclose(total, p, atol=1e-12)
 
 
+@pytest.mark.parametrize("drawn", [True, False])
+def test_the_rules_restatement_keeps_the_targets_distribution(drawn):
+    """Two children of a root, all pairs of tokens: what each is accepted with is looked for among the random numbers (numbers below a border accept), and
+    what is drawn after both are refused is the residual's draw. Summed over what is drafted, the first token has the target's distribution."""
+    gen = torch.Generator().manual_seed(5)
+    logits = torch.randn(4, generator=gen)
+    p, q = torch.softmax(logits.double(), 0), torch.softmax(torch.randn(4, generator=gen).double(), 0)
+    ids = torch.arange(40)
+
+    def said(x, y, u, v):
+        """The first tokens of 40 requests with these children and numbers: (accepted node or -1, token)."""
+        n = len(ids)
+        out, path, count = draft_tree.ref_verify(
+            logits.expand(3 * n, 4), torch.tensor([0, x, y] * n), q_start=starts_of([3] * n), uniforms=torch.tensor([0.0, u, v] * n), seeds=ids, steps=ids * 7,
+            max_tokens=2, parents=torch.tensor([-1, 0, 0] * n, dtype=torch.int32), draft_probs=q.float().expand(3 * n, 4) if drawn else None)
+        return [(int(a[1]) if int(c) == 2 else -1, int(t[0])) for a, c, t in zip(path, count, out)]
+
+    def border(accepts):
+        low, high = 0.0, 1.0                                     # (numbers stay below one)
+        for _ in range(22):
+            mid = (low + high) / 2
+            low, high = (mid, high) if accepts(mid) else (low, mid)
+        return low
+    ids, many = ids[:1], ids
+    total, most = torch.zeros(4, dtype=torch.float64), 1 - 2.0 ** -23
+    for x in range(4):
+        for y in range(4):
+            if not drawn and (x, y) != (2, 0):
+                continue
+            ids = many[:1]
+            weight = q[x] * q[y] if drawn else 1.0
+            first = border(lambda u: said(x, y, u, most)[0][0] == 1)
+            total[x] += weight * first
+            if first >= 1 - 2.0 ** -21:
+                continue
+            second = border(lambda v: said(x, y, most, v)[0][0] == 2)
+            total[y] += weight * (1 - first) * second
+            left = p.clone()
+            for t in (x, y):
+                left = (left - (q if drawn else torch.eye(4, dtype=torch.float64)[t])).clamp(min=0)
+                left /= left.sum()
+            total += weight * (1 - first) * (1 - second) * left
+            if second < 1 - 2.0 ** -21:
+                ids = many
+                want = [int((left / draft_tree.race_numbers(i, 7 * i, 4)).argmax()) for i in range(len(many))]
+                assert said(x, y, most, most) == [(-1, t) for t in want]
+    assert torch.allclose(total, p, atol=2.0 ** -19)             # (borders to 2^-22, q in 32 bits)
+
+
 def test_the_draw_of_the_rule_is_the_samplers():
     p = torch.softmax(torch.randn(300, generator=torch.Generator().manual_seed(2)) * 2, 0)
     for seed, step in ((3, 0), (2 ** 63 + 5, 77)):

@@ -111,6 +111,16 @@ def test_attention_in_a_window_that_ends_among_the_nodes(d, window):
         check_attention(case, scale, window=window, softcap=20.0)
 
 
+@pytest.mark.parametrize("window", [1, 3, 40])
+def test_attention_in_a_window_of_lengths_below_the_nodes(window):
+    """The first nodes have no cells; positions run from before the cache's first one."""
+    for wide in (1, 2):
+        case, scale = attention_case([70, 9, 100], [0, 5, 30], hq=6, hkv=2, d=128, page=16, seed=3, wide=wide, device=DEV)
+        case["seq_lens"] -= 12
+        case["positions"] -= 12
+        check_attention(case, scale, window=window)
+
+
 @pytest.mark.parametrize("window", [5, 64, 200, 1000])
 def test_attention_of_chains_in_a_window_is_the_prefill_kernels(window):
     """Chains longer than a window, a prompt's among them: what attn_prefill computes, within both kernels' roundings."""
@@ -154,6 +164,42 @@ def test_attention_with_capped_scores(d, softcap, n):
     case, scale = attention_case([9, n], [77, 900], hq=6, hkv=2, d=d, page=16, seed=3, device=DEV)
     check_attention(case, scale, softcap=softcap)
     check_attention(case, scale, softcap=softcap, window=200)
+
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("softcap", [200.0, 1000.0, 20000.0, 1e30])
+def test_attention_with_caps_far_above_the_scores(d, softcap):
+    """A capped score is off by 2^-21 of its cap from a sixteenth of it on, and by some roundings of itself below: 2^-16 of the largest score either way. It counts twice
+    in a weight (the sum too); the rest is what uncapped scores are off by."""
+    case, scale = attention_case([9, 70], [77, 900], hq=6, hkv=2, d=d, page=16, seed=3, device=DEV)
+    got = run_attention(case, scale, softcap=softcap).double()
+    wide = {k: v.double() if v.dtype == torch.bfloat16 else v for k, v in case.items()}
+    want = draft_tree.ref_attention(scale=scale, softcap=softcap, dtype=torch.float64, **wide)
+    values = draft_tree.ref_attention(scale=scale, softcap=softcap, dtype=torch.float64, **dict(wide, kv_cache=torch.stack(
+        [wide["kv_cache"][:, 0], wide["kv_cache"][:, 1].abs()], 1)))
+    _, bound = attention_bound(case, scale)
+    top = float(wide["q"].reshape(-1, d).norm(dim=1).max()) * float(wide["kv_cache"][:, 0].norm(dim=-1).max()) * scale
+    assert bool(((got - want).abs() <= bound + 2 * 2.0 ** -16 * top * values).all())
+
+
+@pytest.mark.parametrize("group", [17, 20, 33, 64, 65, 100, 127, 128])
+def test_attention_of_many_query_heads_a_kv_head(group):
+    for d, hkv in ((64, 2), (128, 1), (256, 1)):
+        case, scale = attention_case([9, 0, 3, 1], [77, 5, 900, 0], hq=group * hkv, hkv=hkv, d=d, page=32, seed=group, device=DEV)
+        check_attention(case, scale)
+        check_attention(case, scale, window=50, softcap=25.0)
+
+
+def test_attention_of_as_many_requests_as_a_call_takes():
+    """8192 requests: 128 of them again and again."""
+    rng = random.Random(6)
+    sizes = [rng.randrange(0, 5) for _ in range(128)]
+    case, scale = attention_case(sizes, [rng.randrange(0, 200) for _ in sizes], hq=4, hkv=2, d=64, page=16, seed=6, device=DEV)
+    want, bound = attention_bound(case, scale)
+    many = dict(case, **{k: case[k].repeat(64, *[1] * (case[k].dim() - 1)) for k in ("q", "block_table", "seq_lens", "mask", "positions")},
+                q_start=starts_of(sizes * 64, DEV))
+    got = run_attention(many, scale).double().view(64, *want.shape)
+    assert bool(((got - want).abs() <= bound).all())
 
 
 def test_attention_of_many_requests():
@@ -305,6 +351,25 @@ def test_cells_past_32_bits():
     assert torch.equal(large[-len(small):].view(torch.int16), small.view(torch.int16))
 
 
+def test_cells_past_32_bits_of_values_and_31_of_pieces():
+    """Pages at the end of a cache of 19 G values, which are 2.4 G pieces of 16 bytes: attention (a value that is not finite is read again by its address) and moves."""
+    case, scale = attention_case([9, 40], [300, 900], hq=16, hkv=8, d=128, page=256, seed=5, device=DEV)
+    small = case["kv_cache"]
+    if torch.cuda.mem_get_info()[1] < 80 << 30:
+        pytest.skip("a cache of 38 GB")
+    end = int(case["seq_lens"][0]) - 1
+    small[case["block_table"][0, end // 256].long(), 1, end % 256, :, 3] = math.inf
+    large = torch.empty((36500, *small.shape[1:]), dtype=torch.bfloat16, device=DEV)
+    large[-len(small):] = small
+    there = dict(case, kv_cache=large, block_table=case["block_table"] + (36500 - len(small)))
+    want = run_attention(case, scale)
+    assert torch.equal(run_attention(there, scale).view(torch.int16), want.view(torch.int16)) and bool(torch.isinf(want).any())
+    path = torch.tensor([[0, 2, 5, 8, -1], [0, 7, 8, 30, 39]], dtype=torch.int32, device=DEV)
+    for c in (case, there):
+        draft_tree.compact(c["kv_cache"], block_table=c["block_table"], seq_lens=c["seq_lens"], q_start=c["q_start"], path=path)
+    assert torch.equal(large[-len(small):].view(torch.int16), small.view(torch.int16))
+
+
 def ops_tiles(sizes):
     from vllm_cpp_b200.ops.reference import build_prefill_tiles
     req, q0 = build_prefill_tiles(sizes)
@@ -405,6 +470,21 @@ def test_verify_of_long_rows_and_many_requests(drawn):
     check_verify(verify_case([4, 3], 33001, wide=2, drawn=drawn, seed=1))
     check_verify(verify_case([4], 220001, wide=2, drawn=drawn, seed=4, cold=0.0))
     check_verify(verify_case([3] * 150, 40, wide=2, drawn=drawn, seed=2))
+
+
+@pytest.mark.parametrize("drawn", [True, False])
+@pytest.mark.parametrize("wide", [1, 3])
+@pytest.mark.parametrize("requests,vocab", [(5, 60001), (13, 90000), (16, 128256)])
+def test_verify_of_long_rows_of_more_requests(requests, vocab, wide, drawn):
+    """Eight CTAs a request, one or two rows at a time; greedy requests among them."""
+    rng = random.Random(requests)
+    check_verify(verify_case([rng.randrange(1, 6) for _ in range(requests)], vocab, wide=wide, drawn=drawn, seed=wide, noise=0.3, spread=2.0 if drawn else 5.0))
+
+
+@pytest.mark.parametrize("drawn", [True, False])
+def test_verify_of_as_many_columns_as_a_call_takes(drawn):
+    check_verify(verify_case([3], 778000, wide=2, drawn=drawn, seed=1, cold=0.0))
+    check_verify(verify_case([2] * 6, 400001, drawn=drawn, seed=2))
 
 
 @pytest.mark.parametrize("drawn", [True, False])
@@ -727,3 +807,60 @@ def test_a_run_of_steps_with_trees():
                 odd += int(l.argmax()) != t
                 said[r].append(t)
     assert accepted > 50 and odd <= 5
+
+
+def test_a_run_of_steps_that_samples():
+    """A layer decodes with trees that a draft distribution drew: in every step masks, tokens, paths and cells are what the restatements make of the same
+    inputs, tokens by the rule in 64 bits, and outputs of the attention lie within its bound."""
+    gen, rng = torch.Generator().manual_seed(4), random.Random(2)
+    H, hq, hkv, D, V, page, R = 256, 8, 2, 64, 2104, 16, 4
+    w = lambda *s: (torch.randn(s, generator=gen) / math.sqrt(s[1])).to(torch.bfloat16).to(DEV)  # noqa: E731
+    emb, head, qkv_w, o_w = w(V, H) * 16, w(V, H) * 3, w((hq + 2 * hkv) * D, H), w(H, hq * D)
+    from vllm_cpp_b200.ops import reference
+    cos_sin = ops.rope_table(reference.rope_inv_freq(D, 10000.0).to(DEV), 400)
+    table, pages = page_table([200] * R, page, gen)
+    table = table.to(DEV)
+    cache = torch.zeros((pages, 2, page, hkv, D), dtype=torch.bfloat16, device=DEV)
+    temperature = torch.tensor([0.8, 1.0, 0.0, 0.5], device=DEV)
+    seeds = torch.tensor([3, 2 ** 40, 5, -9], device=DEV)
+    context, roots, accepted = [0] * R, [rng.randrange(V) for _ in range(R)], 0
+    for step in range(12):
+        sizes = [rng.randrange(2, 9) for _ in range(R)]
+        parents = torch.tensor([p for n in sizes for p in tree_parents(n, rng, 2)], dtype=torch.int32)
+        q_start, rows = starts_of(sizes), sum(sizes)
+        first = torch.repeat_interleave(q_start[:-1], q_start.diff()).long()
+        ids = torch.zeros(rows, dtype=torch.int64)
+        ids[q_start[:-1].long()] = torch.tensor(roots)
+        guess = torch.empty((rows, V))
+        for i in range(rows):                                    # (a draft of the next token by the last one alone)
+            if parents[i] >= 0:
+                ids[i] = torch.multinomial(guess[first[i] + parents[i]], 1, generator=gen)
+            guess[i] = torch.softmax(emb[ids[i]].float() @ head.float().t(), 0).cpu()
+        lens = torch.tensor([c + n for c, n in zip(context, sizes)], dtype=torch.int32)
+        where = dict(q_start=q_start.to(DEV), seq_lens=lens.to(DEV))
+        bits, positions = draft_tree.mask(parents.to(DEV), **where)
+        assert all(torch.equal(a, b) for a, b in zip((bits, positions), draft_tree.ref_mask(parents.to(DEV), **where)))
+        cell = torch.cat([torch.arange(c, c + n) for c, n in zip(context, sizes)]).to(DEV)
+        of = torch.repeat_interleave(torch.arange(R), torch.tensor(sizes)).to(DEV)
+        slots = table[of, cell // page].long() * page + cell % page
+        x = emb[ids.to(DEV)]
+        qkv = ops.gemm(x, qkv_w)
+        ops.rope_kv(qkv, positions, cos_sin, num_q_heads=hq, num_kv_heads=hkv, head_dim=D, slot_mapping=slots, kv_cache=cache, block_size=page)
+        case = dict(q=qkv[:, : hq * D], kv_cache=cache, block_table=table, mask=bits, positions=positions, **where)
+        a = check_attention(case, D ** -0.5)
+        logits = ops.gemm((x.float() + 0.3 * ops.gemm(a, o_w).float()).to(torch.bfloat16), head, out_dtype=torch.float32)
+        logits /= torch.where(temperature > 0, temperature, 1.0)[of, None]
+        given = dict(logits=logits, tokens=ids.to(DEV), parents=parents.to(DEV), draft_probs=guess.to(DEV), uniforms=torch.rand(rows, generator=gen).to(DEV),
+                     seeds=seeds, steps=torch.full((R,), step, device=DEV), temperature=temperature, q_start=where["q_start"], max_tokens=6)
+        got = draft_tree.verify(**given)
+        want = draft_tree.ref_verify(**{k: v.cpu() if isinstance(v, torch.Tensor) else v for k, v in given.items()})
+        assert all(torch.equal(g.cpu(), w) for g, w in zip(got, want))
+        moved = cache.clone()
+        draft_tree.compact(cache, block_table=table, path=got[1], **where)
+        draft_tree.ref_compact(moved, block_table=table, path=got[1], **where)
+        assert torch.equal(cache, moved)
+        counts = got[2].tolist()
+        roots = [int(got[0][r, k - 1]) for r, k in enumerate(counts)]
+        context = [c + k for c, k in zip(context, counts)]
+        accepted += sum(counts) - R
+    assert accepted >= 10
