@@ -24,10 +24,11 @@
 //
 // Warp roles (384 threads): warps 0..3 / 4..7 softmax and output; warp 8 keys by TMA, and the pieces of the stretch for the others; warp 9 values by TMA; warps
 // 10 / 11 MMA of either warpgroup, warp 10 TMEM owner. (One warp for both kinds of loads bounded the kernel by its instructions, 128 requests 300 us; one issuer
-// for both warpgroups made each wait for the other's turn: one context of 120000 keys 157 us, with two 146.)
+// for both warpgroups made each wait for the other's turn.)
 //
-// Measured (us on the device, in brackets what the bytes or products take at least; 32-token pages). One tile of rows is bound by memory where heads have 128 dims: 128
-// requests of 200 to 3800 keys with 32 nodes, 32 heads over 8, 195 to 202 by the card (173), 5.7 TB/s; 16 of 8000 keys with 4 nodes 91 (80); 256 dims, 20 of 4000 119 (101). With 64 dims a
+// Measured (us on the device after a pause, at 1965 MHz; in brackets what the bytes or products take at least; 32-token pages). One tile of rows is bound by memory at that
+// clock where heads have 128 dims: 128 requests of 200 to 3800 keys with 32 nodes, 32 heads over 8, 195 to 202 by the card (173), 5.7 TB/s; call after call the power limit takes the clock to
+// 1425 MHz: 243, 4.7 TB/s, as many cycles as memory and the softmax warps' chain bound together. 16 of 8000 keys with 4 nodes 91 (80); 256 dims, 20 of 4000 with 16 nodes 119 to 122 (101), with 100 nodes 243 (108). With 64 dims a
 // tile is half the bytes and as many exponentials: 33 of 4096 with 20 nodes, 24 heads over 8, 86 (43), soft-capped 139. Two tiles of rows are bound by the chain of a
 // warpgroup: one context of 120000 keys with 61 nodes 147 to 156 (75), 64 of 2000 with 60 nodes 171 to 180 (92), tensor pipe and special functions busy in 0.45 of the cycles each. A tile of 64
 // keys takes a warpgroup some 2500 cycles: its scores' wait 300 and load 150, the maximum 370, the exponentials 1050 (as many where a warp has the scheduler to itself), the

@@ -13,7 +13,7 @@
 // barrier. Bound: that chain where there are few requests, the rows' bytes and the draw's random numbers (some 60 instructions a column) where there are
 // many (there a stage reads one row: none in vain). Measured: a chain of four drafts, 128256 columns, drawn 17.8 us (0.8 by its rows' bytes; the first row's arrival, a stage's 4 us
 // and the draw); 64 chains of one to five over 151936 columns 81 us (33 by the rows that are visited; two waves of 33 clusters, issue 0.52, ALU 0.45); 24 trees of
-// 31 to 48 nodes over 128256 columns, chosen 39 us. Slower: rows streamed through registers a node at a time (one chain 24 to 60 us), q in a slot of its own.
+// 31 to 48 nodes over 128256 columns, chosen 39 us, drawn (up to three children a node) 56. Greedy requests, which have no sum and no draw: one chain 9.4 us, 64 chains 37. Slower: rows streamed through registers a node at a time (one chain 24 to 60 us), q in a slot of its own.
 #include <algorithm>
 #include <type_traits>
 
@@ -577,7 +577,11 @@ extern "C" int b200_tree_verify(const B200TreeVerify* a, cudaStream_t stream) {
   // its time, as do slices that leave room for one CTA an SM. us, 8 CTAs and 1 row / 8 and 2 / 16 and 2 / 16 and 4:
   //   chains of 3 to 6 nodes, 128256 columns: 1 request 20.8 / 20.2 / 15.3 / 13.8, 4: 24.0 / 21.9 / 17.0 / 15.6, 8: 24.3 / 22.4 / 22.2 / 26.9,
   //   16: 32 / 42 / 36 / 46, 64: 76 / 106 / 102 / 148; 32000 columns: 4: 17.8 / 15.4 / 14.8 / 13.3, 16: 19.6 / 17.6 / 26.8 / 25.1, 128: 75 / 69 / 136 / 130;
-  //   trees of 20 to 32 nodes, 128256 columns: 1 request 27.2 / 22.7 / 18.4 / 20.9, 8: 26.7 / 22.5 / 21.4 / 31.1, 64: 67 / 92 / 92 / 160
+  //   trees of 20 to 32 nodes, chosen, 128256 columns: 1 request 27.2 / 22.7 / 18.4 / 20.9, 8: 26.7 / 22.5 / 21.4 / 31.1, 64: 67 / 92 / 92 / 160;
+  //   drawn, up to three children a node: 1: 29.0 / 27.2 / 21.0 / 19.8, 8: 35 / 37 / 34 / 33, 16: 40 / 53 / 48 / 59, 64: 97 / 132 / 128 / 192;
+  //   4000 columns, chains: 1: 12.4 / 10.9 / 10.8 / 9.2, 16: 18.5 / 15.4 / 23.7 / 22.0, 128: 71 / 60 / 116 / 106; drawn trees: 16: 21.2 / 17.8 / 25.9 / 24.6
+  // Between the borders, chains of 128256 columns: 5: 23.2 / 22.4 / 17.3 / 15.8, 10: 26.3 / 25.1 / 24.1 / 28.9, 12: 26.2 / 25.3 / 23.8 / 32.8, 13: 29.3 / 27.2 / 24.1 / 30.7, 16: 31.1 / 41.4 / 35.8 / 45.9
+  // (from 5 to 8 requests of long rows sixteen CTAs would still be up to 5 us faster; 5 of 4000 columns 14.7 / 11.7 / 11.6 / 10.1, 8 of 32000 15.2 / 13.2 / 15.5 / 14.6)
   const bool few = a->num_reqs <= 4;
   const int ctas = a->V <= 2048 ? 1 : few || row_slice_cols(a->V, 8) * 4 + 16 > kVerifySmem ? 16 : 8;
   const int slot = row_slice_cols(a->V, ctas) * 4 + 16;
