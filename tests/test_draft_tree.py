@@ -210,6 +210,10 @@ def attention_args():
                                                  block_table=torch.zeros((8193, 1), dtype=torch.int32))),
     ("block_size divides", lambda a: a.update(kv_cache=torch.zeros((3, 2, 48, 2, 64), dtype=torch.bfloat16))),
     ("block_size divides", lambda a: a.update(kv_cache=torch.zeros((3, 2, 4, 2, 64), dtype=torch.bfloat16))),
+    ("kv_cache is bf16", lambda a: a.update(kv_cache=torch.zeros((3, 2, 0, 2, 64), dtype=torch.bfloat16))),
+    ("kv_cache is bf16", lambda a: a.update(kv_cache=torch.zeros((3, 2, 16, 0, 64), dtype=torch.bfloat16))),
+    ("kv_cache is bf16", lambda a: a.update(kv_cache=torch.zeros((3, 2, 16, 2, 0), dtype=torch.bfloat16))),
+    ("one GPU", lambda a: a.update(tmp=torch.zeros(10))),
     ("scale", lambda a: a.update(scale=0.0)),
     ("scale", lambda a: a.update(scale=math.inf)),
     ("softcap", lambda a: a.update(softcap=-1.0)),

@@ -9,6 +9,7 @@ import torch
 from draft_tree_cases import attention_bound, attention_case, page_table, starts_of, tree_parents
 from vllm_cpp_b200 import ops
 from vllm_cpp_b200.ops import draft_tree
+from vllm_cpp_b200.ops.validate import OpArgumentError
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -404,6 +405,23 @@ def test_attention_gives_the_same_bits_in_streams_and_graphs():
                 g.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(o, want) for o in outs)
+
+
+def test_attention_refuses_on_the_gpu_too():
+    """Refusals by the short checks of a call whose tensors are all on the GPU: nothing is launched."""
+    case, scale = attention_case([5, 3], [10, 4], hq=4, hkv=2, d=64, page=16, device=DEV)
+    zero = lambda *s, dtype=torch.bfloat16: torch.zeros(s, dtype=dtype, device=DEV)  # noqa: E731
+    for what, change in (("bf16", dict(kv_cache=zero(3, 2, 0, 2, 64))), ("bf16", dict(kv_cache=zero(3, 2, 16, 0, 64))), ("bf16", dict(kv_cache=zero(3, 2, 16, 2, 0))),
+                         ("block_size", dict(kv_cache=zero(3, 2, 48, 2, 64))), ("16 words", dict(mask=zero(8, 17, dtype=torch.int64))),
+                         ("128 query heads", dict(q=zero(8, 2 * 129 * 64))), ("tmp", dict(tmp=zero(10, dtype=torch.float32))), ("scale", dict(scale=1e-50)),
+                         ("softcap", dict(softcap=1e39)), ("window", dict(window=4, positions=None))):
+        with pytest.raises(OpArgumentError, match=what):
+            draft_tree.attention(**{**case, "scale": scale, **change})
+    caches = zero(7, 2, 16, 1, 64)
+    path = zero(2, 3, dtype=torch.int32)
+    with pytest.raises(OpArgumentError, match="share no memory"):
+        draft_tree.compact([caches[3:], caches[:4]], path=path, **{k: case[k] for k in ("block_table", "seq_lens", "q_start")})
+    assert ops.read_status() == 0
 
 
 def test_attention_on_another_device_than_the_current_one():

@@ -151,7 +151,7 @@ def attention(q: torch.Tensor, kv_cache: torch.Tensor, *, block_table: torch.Ten
               and kv_cache.dtype is BF16 and block_table.dtype is _I32 and mask.dtype is _I64 and two == 2 and H > 0 and cols > 0
               and (D == 128 or D == 64 or D == 256) and cols % (D * H) == 0 and kv_cache.is_contiguous() and q1 == t1 == 1 and pages > 0
               and treqs >= reqs - 1 and (qp | cp | 2 * ldq) % 16 == 0 and rows >= T and 0 < words <= 16 and mask.is_contiguous()
-              and cols <= 128 * D * H and (64 % bs == 0 and bs >= 8 or bs % 64 == 0) and reqs <= 8193
+              and cols <= 128 * D * H and bs >= 8 and (64 % bs == 0 or bs % 64 == 0) and reqs <= 8193
               and _ids(seq_lens, _I32, dev, reqs - 1) and _ids(q_start, _I32, dev, 1)
               and LEAST_F32 < scale <= MOST_LOG2_F32 and (softcap == 0 or LEAST_F32 < softcap <= MOST_LOG2_F32)
               and 0 <= window < 2 ** 31 and (window == 0 or _ids(positions, _I64, dev, T)))

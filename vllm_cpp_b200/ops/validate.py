@@ -321,7 +321,7 @@ def _all_apart(written, read) -> bool:
 
 def _tree_scratch(kv_cache) -> int:
     from .draft_tree import scratch_floats
-    return scratch_floats(kv_cache.device, kv_cache.shape[4])
+    return scratch_floats(kv_cache.device, kv_cache.shape[4]) if kv_cache.is_cuda else 0
 
 
 def validate(op: str, **args) -> None:
